@@ -200,7 +200,8 @@ int32_t bfvgpu_matrix_groups_device(bfvgpu_ctx *ctx, const uint64_t *in, uint64_
 
 /* Synchronises the context's device and returns (then clears) the error bits its kernels
  * recorded: bit 0 = a tensor-core product step whose completion wait expired (the block
- * freed its tensor memory and stopped; the output of that launch is incomplete).  Returns
+ * freed its tensor memory and stopped; the output of that launch is incomplete), bit 2 = a page
+ * number, row, length or start of the paged cache outside its range.  Returns
  * BFVGPU_E_CUDA when any bit was set.  No counterpart in the reference (its kernels have
  * no waits). */
 int32_t bfvgpu_ctx_check(bfvgpu_ctx *ctx, uint32_t *flags);
@@ -454,6 +455,74 @@ int32_t bfvgpu_token_finish_device(bfvgpu_ctx *ctx, const uint64_t *packed, uint
                                    uint64_t *c0_crt, void *stream);
 int32_t bfvgpu_token_close(bfvgpu_token *t, bfvgpu_cleanup *cleanup);
 int32_t bfvgpu_token_release(bfvgpu_token *t);
+
+/* ---- Paged key-value cache and its attention ----------------------------------------------
+ * What runs between the q/k/v call and the o call of a decoder layer, for the party that holds
+ * the decrypted projections.  No counterpart in the reference, whose attention is a two-party
+ * integer protocol.  All pointers are device memory; stream as for the other device entry points
+ * (NULL: the context stream; cudaStreamLegacy names the default stream).  Values on the device
+ * (tables, lengths, starts, page lists) cannot be checked by the host: the kernels check every
+ * page number, row and length against the cache, skip the access and set bit 2 (value 4) of
+ * bfvgpu_ctx_check's flags; the results of that sequence are then unspecified.
+ *
+ * K and V of one cache have the same shape [layers][pages][heads][page_tokens][dim] and the same
+ * strides (elements), dim innermost and contiguous, the other axes in any order; dim a multiple
+ * of 8 in [8, 128], page_tokens a power of two in [16, 256]; base pointers 16-byte aligned,
+ * strides multiples of 8 elements.  Token j of the sequence in row s of a table [rows][width]
+ * (int32, dense) lies in page table[s][j / page_tokens]; entries that no call reads may hold
+ * anything (-1 by convention).  Pages are numbered alike for all layers. */
+enum bfvgpu_kv_dtype { BFVGPU_KV_BF16 = 0, BFVGPU_KV_FP16 = 1, BFVGPU_KV_F32 = 2 /* append's source only */ };
+typedef struct bfvgpu_kv {
+  void *k, *v;
+  int32_t dtype; /* BFVGPU_KV_BF16 or BFVGPU_KV_FP16 */
+  int32_t layers, pages, heads, page_tokens, dim;
+  int64_t layer_stride, page_stride, head_stride, token_stride;
+} bfvgpu_kv;
+/* Writes the keys and values of new tokens into their pages, one layer.  k_new, v_new
+ * [tokens][heads][dim] with the given strides (elements; dim contiguous; rows 16-byte aligned), in
+ * the cache's type or in 32 bits (rounded to nearest).  starts [seqs + 1]: sequence s has the new
+ * tokens starts[s] .. starts[s + 1) - 1, the last ones of its lengths[s] tokens (lengths count
+ * them already); NULL: one new token each (tokens == seqs). */
+int32_t bfvgpu_kv_append_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t layer, const void *k_new,
+                                const void *v_new, int32_t source_dtype, int64_t token_stride, int64_t head_stride,
+                                uint64_t tokens, const int32_t *starts, const int32_t *table, uint64_t width,
+                                const int32_t *lengths, uint64_t seqs, void *stream);
+/* Row children[i] of the table becomes a continuation of row parents[i]: the same length and
+ * pages, but a partly filled last page is copied (all layers) to page fresh[i] (unread where the
+ * parent's length is a multiple of page_tokens).  No row is a child twice, or both parent and
+ * child. */
+int32_t bfvgpu_kv_fork_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, const int32_t *parents,
+                              const int32_t *children, const int32_t *fresh, uint64_t count, int32_t *table,
+                              uint64_t rows, uint64_t width, int32_t *lengths, void *stream);
+/* Copies pages src[i] to dst[i] (all layers) and rewrites every entry of the table (NULL: none)
+ * that names src[i] to dst[i].  src strictly increasing; no page is both in src and dst, or twice
+ * in dst. */
+int32_t bfvgpu_kv_move_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, const int32_t *src, const int32_t *dst,
+                              uint64_t count, int32_t *table, uint64_t rows, uint64_t width, void *stream);
+/* Attention of the newest token of every sequence: q [seqs][q_heads][dim] (strides in elements,
+ * 16-byte aligned rows), out [seqs][q_heads][dim] dense, both of the cache's type; query head h
+ * reads key head h / (q_heads / heads).  The query of sequence s stands at p = lengths[s] - 1 and
+ * sees key j if j <= p and (window == 0 or j > p - window or j < sinks):
+ *   out = sum_j softmax_j(scale q.k_j) v_j;  a sequence of length 0 gets zeros.
+ * scale > 0.  Sums and softmax statistics in 32 bits.  Keys that are not visible are not read.
+ * scratch: bfvgpu_kv_decode_scratch_words words (may be NULL when that is 0), free again when the
+ * call's work on the stream is done. */
+uint64_t bfvgpu_kv_decode_scratch_words(const bfvgpu_ctx *ctx, const bfvgpu_kv *cache, uint64_t q_heads,
+                                        uint64_t seqs, uint64_t width, int32_t window, int32_t sinks);
+int32_t bfvgpu_kv_decode_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t layer, const void *q,
+                                int64_t token_stride, int64_t head_stride, uint64_t q_heads, const int32_t *table,
+                                uint64_t width, const int32_t *lengths, uint64_t seqs, int32_t window, int32_t sinks,
+                                float scale, uint64_t *scratch, void *out, void *stream);
+/* The same for the new tokens of prompts (or of their next chunks): q [tokens][q_heads][dim], out
+ * dense; starts [seqs + 1] as for append; new token i of sequence s stands at
+ * p = lengths[s] - (starts[s + 1] - starts[s]) + i, and a row with p < 0 gets zeros. */
+uint64_t bfvgpu_kv_prompt_scratch_words(const bfvgpu_ctx *ctx, const bfvgpu_kv *cache, uint64_t q_heads,
+                                        uint64_t tokens, uint64_t seqs, uint64_t width, int32_t window, int32_t sinks);
+int32_t bfvgpu_kv_prompt_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t layer, const void *q,
+                                int64_t token_stride, int64_t head_stride, uint64_t q_heads, uint64_t tokens,
+                                const int32_t *starts, const int32_t *table, uint64_t width, const int32_t *lengths,
+                                uint64_t seqs, int32_t window, int32_t sinks, float scale, uint64_t *scratch,
+                                void *out, void *stream);
 
 #ifdef __cplusplus
 }

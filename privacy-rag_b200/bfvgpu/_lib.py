@@ -19,6 +19,8 @@ U64P = ctypes.POINTER(ctypes.c_uint64)
 U32 = ctypes.c_uint32
 U32P = ctypes.POINTER(ctypes.c_uint32)
 I32 = ctypes.c_int32
+I64 = ctypes.c_int64
+F32 = ctypes.c_float
 VP = ctypes.c_void_p
 
 ERROR_NAMES = {
@@ -53,6 +55,16 @@ class Cleanup(ctypes.Structure):
         return {"first_cuda_error": int(self.first_cuda_error), "closed": bool(self.closed),
                 "wiped": int(self.wiped), "freed": int(self.freed)}
 
+
+class KvDesc(ctypes.Structure):
+    """bfvgpu_kv: the pages of a key-value cache."""
+
+    _fields_ = [("k", VP), ("v", VP), ("dtype", I32), ("layers", I32), ("pages", I32), ("heads", I32),
+                ("page_tokens", I32), ("dim", I32), ("layer_stride", I64), ("page_stride", I64),
+                ("head_stride", I64), ("token_stride", I64)]
+
+
+_KV = ctypes.POINTER(KvDesc)
 
 _SIGNATURES = {
     "bfvgpu_version": (I32, []),
@@ -143,6 +155,14 @@ _SIGNATURES = {
     "bfvgpu_token_evaluate_finished": (I32, [VP, U64P, U64P, U64P]),
     "bfvgpu_token_close": (I32, [VP, ctypes.POINTER(Cleanup)]),
     "bfvgpu_token_release": (I32, [VP]),
+    "bfvgpu_kv_append_device": (I32, [VP, _KV, I32, VP, VP, I32, I64, I64, U64, VP, VP, U64, VP, U64, VP]),
+    "bfvgpu_kv_fork_device": (I32, [VP, _KV, VP, VP, VP, U64, VP, U64, U64, VP, VP]),
+    "bfvgpu_kv_move_device": (I32, [VP, _KV, VP, VP, U64, VP, U64, U64, VP]),
+    "bfvgpu_kv_decode_scratch_words": (U64, [VP, _KV, U64, U64, U64, I32, I32]),
+    "bfvgpu_kv_decode_device": (I32, [VP, _KV, I32, VP, I64, I64, U64, VP, U64, VP, U64, I32, I32, F32, VP, VP, VP]),
+    "bfvgpu_kv_prompt_scratch_words": (U64, [VP, _KV, U64, U64, U64, U64, I32, I32]),
+    "bfvgpu_kv_prompt_device": (I32, [VP, _KV, I32, VP, I64, I64, U64, U64, VP, VP, U64, VP, U64, I32, I32, F32, VP,
+                                      VP, VP]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

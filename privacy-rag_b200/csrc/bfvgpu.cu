@@ -22,6 +22,7 @@
 #include "bfvgpu.h"
 #include "ctx_internal.h"
 #include "kernels.cuh"
+#include "kv_common.cuh"
 #include "ntt_core.cuh"
 
 using u128 = unsigned __int128;
@@ -841,7 +842,8 @@ int32_t bfvgpu_ctx_check(bfvgpu_ctx* ctx, uint32_t* flags) {
     cuda_check(cudaDeviceSynchronize(), "ctx_check");
     cuda_check(cudaMemcpy(flags, ctx->c.P.err, 4, cudaMemcpyDeviceToHost), "ctx_check");
     cuda_check(cudaMemset(ctx->c.P.err, 0, 4), "ctx_check");
-    if (*flags) fail(BFVGPU_E_CUDA, "E_BFVGPU_KERNEL_TIMEOUT");
+    if (*flags & ~kv::kErrTable) fail(BFVGPU_E_CUDA, "E_BFVGPU_KERNEL_TIMEOUT");
+    if (*flags) fail(BFVGPU_E_CUDA, "E_KV_TABLE: a page number, row, length or start outside the cache");
   });
 }
 

@@ -1,0 +1,139 @@
+// Entry points of the attention over the paged cache: argument checks and the choice of kernel.
+#include "kv_attention.h"
+
+#include <algorithm>
+#include <atomic>
+
+#include "kv_host.h"
+
+namespace bfvgpu {
+namespace kv {
+namespace {
+
+constexpr uint64_t kMost = 0x7ffffffe;
+
+// Streaming multiprocessors of a device; the default of this GPU where there is none to ask.
+int sm_count(int device) {
+  constexpr int kDefault = 148, kDevices = 64;
+  static std::atomic<int> known[kDevices];
+  if (device < 0 || device >= kDevices) return kDefault;
+  int n = known[device].load();
+  if (!n) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) return kDefault;
+    known[device].store(n);
+  }
+  return n;
+}
+
+struct Call {
+  View view;
+  Batch batch;
+  Query query;
+};
+
+Call checked_call(const bfvgpu_kv* cache, int32_t layer, uint64_t q_heads, uint64_t tokens, uint64_t seqs,
+                  uint64_t width, int32_t window, int32_t sinks) {
+  Call c;
+  need(layer >= 0, BFVGPU_E_SHAPE, "E_KV_LAYER");
+  c.view = checked_view(cache, layer);
+  need(q_heads >= 1 && q_heads <= kMost && q_heads % c.view.heads == 0, BFVGPU_E_SHAPE, "E_KV_HEADS");
+  need(tokens <= kMost && seqs <= kMost && width <= kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+  need(q_heads / c.view.heads <= 1024 && tokens * (q_heads / c.view.heads) <= kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+  // positions and their sums with the window stay in 32 bits
+  need((width << c.view.page_log) <= (uint64_t(1) << 30), BFVGPU_E_SHAPE, "E_KV_WIDTH");
+  need(window >= 0 && sinks >= 0, BFVGPU_E_ARGUMENT, "E_KV_WINDOW");
+  const int32_t top = 1 << 30;
+  c.query.group = (int32_t)(q_heads / c.view.heads);
+  c.query.tokens = (int32_t)tokens;
+  c.query.window = window < top ? window : 0;  // a window past every position hides nothing
+  c.query.sinks = std::min(sinks, top);
+  c.batch.seqs = (int32_t)seqs;
+  c.batch.width = (int32_t)width;
+  return c;
+}
+
+void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int64_t token_stride, int64_t head_stride,
+            const int32_t* starts, const int32_t* table, const int32_t* lengths, float scale, uint64_t* scratch,
+            void* out, void* stream) {
+  need(std::isfinite(scale) && scale > 0, BFVGPU_E_ARGUMENT, "E_KV_SCALE");
+  const Place at = checked_place(ctx, stream);
+  if (!c.query.tokens) return;
+  need(c.batch.seqs && q && table && c.batch.width && lengths && out, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
+  need(aligned16(q) && aligned16(out) && token_stride % 8 == 0 && head_stride % 8 == 0, BFVGPU_E_ARGUMENT,
+       "E_KV_ALIGNMENT");
+  OnDevice scope(at.device);
+  c.batch.table = table;
+  c.batch.lengths = lengths;
+  c.batch.starts = starts;
+  c.batch.err = at.err;
+  c.query.q = static_cast<const uint16_t*>(q);
+  c.query.token_stride = token_stride;
+  c.query.head_stride = head_stride;
+  c.query.out = static_cast<uint16_t*>(out);
+  c.query.scale_log2 = scale * 1.4426950408889634f;
+  const RowSplit sp = plan_rows(c.view, c.batch, c.query, sm_count(at.device));
+  need(sp.scratch_floats() == 0 || scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
+  need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
+  need(sp.blocks16 * sp.parts <= (int64_t)(kMost / sp.cluster), BFVGPU_E_SHAPE, "E_KV_SHAPE");
+  int launches = 0;
+  cuda_need(launch_rows(c.view, c.batch, c.query, cache->dtype, sp, reinterpret_cast<float*>(scratch), at.stream,
+                        &launches),
+            "kv attention");
+  internal_count_launch(launches);
+}
+
+// Words of scratch; 0 for arguments that the call itself refuses.
+uint64_t scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q_heads, uint64_t tokens, bool ragged,
+                       uint64_t seqs, uint64_t width, int32_t window, int32_t sinks) {
+  uint64_t words = 0;
+  guarded([&] {
+    Call c = checked_call(cache, 0, q_heads, tokens, seqs, width, window, sinks);
+    static const int32_t some = 0;
+    if (ragged) c.batch.starts = &some;  // only asked whether there is one
+    int device = -1;
+    internal_params(ctx, &device, nullptr);
+    words = (plan_rows(c.view, c.batch, c.query, sm_count(device)).scratch_floats() + 1) / 2;
+  });
+  return words;
+}
+
+}  // namespace
+}  // namespace kv
+}  // namespace bfvgpu
+
+using namespace bfvgpu;
+using namespace bfvgpu::kv;
+
+extern "C" uint64_t bfvgpu_kv_decode_scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q_heads,
+                                                   uint64_t seqs, uint64_t width, int32_t window, int32_t sinks) {
+  return scratch_words(ctx, cache, q_heads, seqs, false, seqs, width, window, sinks);
+}
+
+extern "C" int32_t bfvgpu_kv_decode_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, int32_t layer, const void* q,
+                                           int64_t token_stride, int64_t head_stride, uint64_t q_heads,
+                                           const int32_t* table, uint64_t width, const int32_t* lengths, uint64_t seqs,
+                                           int32_t window, int32_t sinks, float scale, uint64_t* scratch, void* out,
+                                           void* stream) {
+  return guarded([&] {
+    Call c = checked_call(cache, layer, q_heads, seqs, seqs, width, window, sinks);
+    attend(ctx, cache, c, q, token_stride, head_stride, nullptr, table, lengths, scale, scratch, out, stream);
+  });
+}
+
+extern "C" uint64_t bfvgpu_kv_prompt_scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q_heads,
+                                                   uint64_t tokens, uint64_t seqs, uint64_t width, int32_t window,
+                                                   int32_t sinks) {
+  return scratch_words(ctx, cache, q_heads, tokens, true, seqs, width, window, sinks);
+}
+
+extern "C" int32_t bfvgpu_kv_prompt_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, int32_t layer, const void* q,
+                                           int64_t token_stride, int64_t head_stride, uint64_t q_heads,
+                                           uint64_t tokens, const int32_t* starts, const int32_t* table,
+                                           uint64_t width, const int32_t* lengths, uint64_t seqs, int32_t window,
+                                           int32_t sinks, float scale, uint64_t* scratch, void* out, void* stream) {
+  return guarded([&] {
+    need(starts || !tokens, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
+    Call c = checked_call(cache, layer, q_heads, tokens, seqs, width, window, sinks);
+    attend(ctx, cache, c, q, token_stride, head_stride, starts, table, lengths, scale, scratch, out, stream);
+  });
+}

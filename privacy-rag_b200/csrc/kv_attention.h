@@ -1,0 +1,37 @@
+// Internal launch API of the attention kernels over the paged cache.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "kv_common.cuh"
+
+namespace bfvgpu {
+namespace kv {
+
+// Queries and results.  Row R of a (sequence, key head) is query head (key head * group + R % group)
+// of the sequence's new token R / group: all rows of one key head read the same keys.
+struct Query {
+  const uint16_t* q = nullptr;
+  int64_t token_stride = 0, head_stride = 0;  // elements
+  uint16_t* out = nullptr;                    // [tokens][heads * group][dim]
+  int32_t tokens = 0;                         // new tokens of the batch
+  int32_t group = 1;                          // query heads per key head
+  int32_t window = 0, sinks = 0;              // window 0: every earlier key
+  float scale_log2 = 0;                       // scale * log2(e)
+};
+
+// Split of one launch of the row kernel.
+struct RowSplit {
+  int32_t cluster = 1;     // blocks that share a unit and join in shared memory
+  int32_t parts = 1;       // clusters per unit, joined by a second kernel
+  int64_t blocks16 = 0;    // units: (16-row block, key head)
+  uint64_t scratch_floats() const;
+  int32_t dim_padded = 128;
+};
+RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int sms);
+cudaError_t launch_rows(const View& kv, const Batch& bt, const Query& q, int dtype, const RowSplit& split,
+                        float* scratch, cudaStream_t st, int* launches);
+
+}  // namespace kv
+}  // namespace bfvgpu

@@ -1,0 +1,302 @@
+// Pages of the key-value cache: new tokens written, sequences forked, pages moved.
+//
+// All three only move bytes; their floor is each byte read once and written once.  The copies move
+// 16 bytes per thread and access, four accesses in flight per thread, all layers in one launch.
+#include "kv_host.h"
+
+namespace bfvgpu {
+namespace kv {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kInFlight = 4;  // 16-byte accesses in flight per thread
+
+struct Source {
+  const void* k = nullptr;
+  const void* v = nullptr;
+  int64_t token_stride = 0, head_stride = 0;
+  int32_t tokens = 0;
+};
+
+// Eight elements of the source, rounded to nearest into the cache's type.
+template <class T, int SRC>
+__device__ __forceinline__ uint4 eight(const void* base, int64_t at) {
+  if constexpr (SRC == 2) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+    const float4 a = __ldg(p), b = __ldg(p + 1);
+    return make_uint4(T::pack(a.x, a.y), T::pack(a.z, a.w), T::pack(b.x, b.y), T::pack(b.z, b.w));
+  } else {
+    return __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
+  }
+}
+
+// One warp per new token: it finds the token's sequence and page once, then moves the K and V rows
+// of every head.
+template <class T, int SRC>
+__global__ void __launch_bounds__(kThreads) k_kv_append(View kv, Batch bt, Source s) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t64 = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (t64 >= s.tokens) return;
+  const int32_t t = (int32_t)t64;
+  int32_t b = t, first = t, next = t + 1;
+  if (bt.starts) {
+    b = sequence_of_token(bt, t);
+    first = bt.starts[b];
+    next = bt.starts[b + 1];
+  }
+  const int64_t pos = (int64_t)sequence_length(bt, kv, b) - next + t;
+  const int64_t slot = pos >> kv.page_log;
+  const int32_t page = t >= first && t < next && pos >= 0 && slot < bt.width ? bt.table[(int64_t)b * bt.width + slot] : -1;
+  if (page < 0 || page >= kv.pages) {
+    if (lane == 0) flag_error(bt.err, kErrTable);
+    return;
+  }
+  const int64_t to = page * kv.page_stride + (pos & ((1 << kv.page_log) - 1)) * kv.token_stride;
+  const int64_t from = t * s.token_stride;
+  const int32_t row = kv.dim / 8, chunks = kv.heads * row;
+  for (int32_t c0 = lane; c0 < chunks; c0 += 32 * kInFlight) {
+    uint4 kk[kInFlight], vv[kInFlight];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+      const int32_t c = c0 + 32 * i, h = c / row;
+      if (c < chunks) {
+        const int64_t at = from + h * s.head_stride + (c - h * row) * 8;
+        kk[i] = eight<T, SRC>(s.k, at);
+        vv[i] = eight<T, SRC>(s.v, at);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+      const int32_t c = c0 + 32 * i, h = c / row;
+      if (c < chunks) {
+        const int64_t at = to + h * kv.head_stride + (c - h * row) * 8;
+        *reinterpret_cast<uint4*>(kv.k + at) = kk[i];
+        *reinterpret_cast<uint4*>(kv.v + at) = vv[i];
+      }
+    }
+  }
+}
+
+// A page as rows of contiguous 16-byte chunks: the whole page where its strides leave no gap, else
+// one row per (head, token).
+struct PageShape {
+  int32_t rows = 1, inner = 1, row_chunks = 0;
+  int64_t outer_stride = 0, inner_stride = 0;  // row = outer * inner + i
+  int64_t chunks() const { return (int64_t)rows * row_chunks; }
+};
+
+PageShape page_shape(const View& w) {
+  const int64_t tokens = int64_t(1) << w.page_log;
+  PageShape s;
+  const bool hnd = w.token_stride == w.dim && (w.heads == 1 || w.head_stride == tokens * w.dim);
+  const bool nhd = (w.heads == 1 || w.head_stride == w.dim) && w.token_stride == (int64_t)w.heads * w.dim;
+  if (hnd || nhd) {
+    s.row_chunks = (int32_t)(w.heads * tokens * w.dim / 8);
+    return s;
+  }
+  s.rows = w.heads << w.page_log;
+  s.inner = (int32_t)tokens;
+  s.row_chunks = w.dim / 8;
+  s.outer_stride = w.head_stride;
+  s.inner_stride = w.token_stride;
+  return s;
+}
+
+// The block's share `part` of page `from` -> page `to` of one layer's K or V.
+__device__ __forceinline__ void copy_share(uint16_t* base, int64_t page_stride, int32_t from, int32_t to,
+                                           const PageShape& s, int32_t part) {
+  const uint16_t* src = base + from * page_stride;
+  uint16_t* dst = base + to * page_stride;
+  const int32_t chunks = s.rows * s.row_chunks, c0 = part * (kThreads * kInFlight) + threadIdx.x;
+  uint4 x[kInFlight];
+  int64_t at[kInFlight];
+#pragma unroll
+  for (int i = 0; i < kInFlight; ++i) {
+    const int32_t c = c0 + i * kThreads;
+    if (c >= chunks) continue;
+    const int32_t row = c / s.row_chunks, o = row / s.inner;
+    at[i] = o * s.outer_stride + (row - o * s.inner) * s.inner_stride + (int64_t)(c - row * s.row_chunks) * 8;
+    x[i] = *reinterpret_cast<const uint4*>(src + at[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kInFlight; ++i)
+    if (c0 + i * kThreads < chunks) *reinterpret_cast<uint4*>(dst + at[i]) = x[i];
+}
+
+struct Copies {
+  PageShape shape;
+  int64_t layer_stride = 0;
+  int32_t layers = 0, parts = 0, count = 0;
+};
+
+// Blocks [copy c][layer][K, V][part of the page], part fastest.
+__device__ __forceinline__ void copy_block(const View& kv, const Copies& cp, int64_t block, int32_t from, int32_t to) {
+  const int32_t part = (int32_t)(block % cp.parts);
+  const int64_t rest = block / cp.parts;
+  uint16_t* base = ((rest & 1) ? kv.v : kv.k) + ((rest >> 1) % cp.layers) * cp.layer_stride;
+  copy_share(base, kv.page_stride, from, to, cp.shape, part);
+}
+
+__global__ void __launch_bounds__(kThreads)
+    k_kv_move(View kv, Copies cp, const int32_t* src, const int32_t* dst, int32_t* table, int64_t entries,
+              int64_t copy_blocks, uint32_t* err) {
+  if (blockIdx.x < copy_blocks) {
+    const int64_t c = blockIdx.x / (2ll * cp.layers * cp.parts);
+    const int32_t from = src[c], to = dst[c];
+    if ((uint32_t)from >= (uint32_t)kv.pages || (uint32_t)to >= (uint32_t)kv.pages) {
+      if (threadIdx.x == 0) flag_error(err, kErrTable);
+      return;
+    }
+    copy_block(kv, cp, blockIdx.x, from, to);
+    return;
+  }
+  // table entries: a binary search in src, which is strictly increasing
+  const int64_t e = (blockIdx.x - copy_blocks) * kThreads + threadIdx.x;
+  if (e >= entries) return;
+  const int32_t page = table[e];
+  if (page < 0) return;
+  int32_t lo = 0, hi = cp.count;
+  while (lo < hi) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (src[mid] < page) lo = mid + 1;
+    else hi = mid;
+  }
+  if (lo < cp.count && src[lo] == page && (uint32_t)dst[lo] < (uint32_t)kv.pages) table[e] = dst[lo];
+}
+
+__global__ void __launch_bounds__(kThreads)
+    k_kv_fork(View kv, Copies cp, const int32_t* parents, const int32_t* children, const int32_t* fresh,
+              int32_t* table, int32_t rows, int32_t width, int32_t* lengths, uint32_t* err) {
+  const int64_t per = 2ll * cp.layers * cp.parts;
+  const int64_t c = blockIdx.x / per, share = blockIdx.x % per;
+  const int32_t p = parents[c], child = children[c];
+  if ((uint32_t)p >= (uint32_t)rows || (uint32_t)child >= (uint32_t)rows || p == child) {
+    if (threadIdx.x == 0) flag_error(err, kErrTable);
+    return;
+  }
+  const int32_t n = lengths[p], tokens = 1 << kv.page_log;
+  const int32_t last = n >> kv.page_log;
+  const bool part = n & (tokens - 1);
+  const int32_t to = part ? fresh[c] : -1;
+  bool ok = n >= 0 && last + part <= width;
+  int32_t from = -1;
+  if (ok && part) {
+    from = table[(int64_t)p * width + last];
+    ok = (uint32_t)from < (uint32_t)kv.pages && (uint32_t)to < (uint32_t)kv.pages;
+  }
+  if (!ok) {
+    if (threadIdx.x == 0) flag_error(err, kErrTable);
+    return;
+  }
+  if (share == 0) {
+    const int32_t* row = table + (int64_t)p * width;
+    int32_t* out = table + (int64_t)child * width;
+    for (int32_t i = threadIdx.x; i < width; i += kThreads) out[i] = part && i == last ? to : row[i];
+    if (threadIdx.x == 0) lengths[child] = n;
+  }
+  if (part && from != to) copy_block(kv, cp, share, from, to);
+}
+
+Copies copies_of(const View& w, const bfvgpu_kv* c, uint64_t count) {
+  Copies cp;
+  cp.shape = page_shape(w);
+  cp.layers = c->layers;
+  cp.layer_stride = c->layers > 1 ? c->layer_stride : 0;
+  cp.count = (int32_t)count;
+  const int64_t per = (int64_t)kThreads * kInFlight;
+  cp.parts = (int32_t)((cp.shape.chunks() + per - 1) / per);
+  return cp;
+}
+
+constexpr int64_t kMostBlocks = 0x7fffffff;
+
+}  // namespace
+}  // namespace kv
+}  // namespace bfvgpu
+
+using namespace bfvgpu;
+using namespace bfvgpu::kv;
+
+extern "C" int32_t bfvgpu_kv_append_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, int32_t layer, const void* k_new,
+                                           const void* v_new, int32_t source_dtype, int64_t token_stride,
+                                           int64_t head_stride, uint64_t tokens, const int32_t* starts,
+                                           const int32_t* table, uint64_t width, const int32_t* lengths, uint64_t seqs,
+                                           void* stream) {
+  return guarded([&] {
+    need(layer >= 0, BFVGPU_E_SHAPE, "E_KV_LAYER");
+    const View w = checked_view(cache, layer);
+    need(source_dtype == cache->dtype || source_dtype == BFVGPU_KV_F32, BFVGPU_E_ARGUMENT, "E_KV_SOURCE_DTYPE");
+    need(tokens <= 0x7fffffff && seqs <= 0x7ffffffe && width <= 0x7fffffff, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    need(starts || tokens == seqs, BFVGPU_E_SHAPE, "E_KV_STARTS");
+    const Place at = checked_place(ctx, stream);
+    if (!tokens) return;
+    need(seqs && k_new && v_new && table && width && lengths, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
+    const int64_t unit = source_dtype == BFVGPU_KV_F32 ? 4 : 8;
+    need(aligned16(k_new) && aligned16(v_new) && token_stride % unit == 0 && head_stride % unit == 0, BFVGPU_E_ARGUMENT,
+         "E_KV_ALIGNMENT");
+    OnDevice scope(at.device);
+    Batch bt;
+    bt.table = table;
+    bt.lengths = lengths;
+    bt.starts = starts;
+    bt.seqs = (int32_t)seqs;
+    bt.width = (int32_t)width;
+    bt.err = at.err;
+    Source s;
+    s.k = k_new;
+    s.v = v_new;
+    s.token_stride = token_stride;
+    s.head_stride = head_stride;
+    s.tokens = (int32_t)tokens;
+    const unsigned grid = (unsigned)((tokens + kThreads / 32 - 1) / (kThreads / 32));
+    if (source_dtype != BFVGPU_KV_F32)
+      k_kv_append<Bf16, 0><<<grid, kThreads, 0, at.stream>>>(w, bt, s);
+    else if (cache->dtype == BFVGPU_KV_BF16)
+      k_kv_append<Bf16, 2><<<grid, kThreads, 0, at.stream>>>(w, bt, s);
+    else
+      k_kv_append<Fp16, 2><<<grid, kThreads, 0, at.stream>>>(w, bt, s);
+    cuda_need(cudaGetLastError(), "kv append");
+    internal_count_launch(1);
+  });
+}
+
+extern "C" int32_t bfvgpu_kv_fork_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, const int32_t* parents,
+                                         const int32_t* children, const int32_t* fresh, uint64_t count, int32_t* table,
+                                         uint64_t rows, uint64_t width, int32_t* lengths, void* stream) {
+  return guarded([&] {
+    const View w = checked_view(cache, -1);
+    need(rows <= 0x7fffffff && width <= 0x7fffffff && count <= rows, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    const Place at = checked_place(ctx, stream);
+    if (!count) return;
+    need(parents && children && fresh && table && width && lengths, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
+    const Copies cp = copies_of(w, cache, count);
+    const int64_t blocks = (int64_t)count * 2 * cp.layers * cp.parts;
+    need(blocks <= kMostBlocks, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    OnDevice scope(at.device);
+    k_kv_fork<<<(unsigned)blocks, kThreads, 0, at.stream>>>(w, cp, parents, children, fresh, table, (int32_t)rows,
+                                                            (int32_t)width, lengths, at.err);
+    cuda_need(cudaGetLastError(), "kv fork");
+    internal_count_launch(1);
+  });
+}
+
+extern "C" int32_t bfvgpu_kv_move_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, const int32_t* src,
+                                         const int32_t* dst, uint64_t count, int32_t* table, uint64_t rows,
+                                         uint64_t width, void* stream) {
+  return guarded([&] {
+    const View w = checked_view(cache, -1);
+    need(count <= (uint64_t)w.pages && rows <= 0x7fffffff && width <= 0x7fffffff, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    const Place at = checked_place(ctx, stream);
+    if (!count) return;
+    need(src && dst && (table || !rows || !width), BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
+    const Copies cp = copies_of(w, cache, count);
+    const int64_t entries = table ? (int64_t)rows * (int64_t)width : 0;
+    const int64_t copy_blocks = (int64_t)count * 2 * cp.layers * cp.parts;
+    const int64_t blocks = copy_blocks + (entries + kThreads - 1) / kThreads;
+    need(blocks <= kMostBlocks, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    OnDevice scope(at.device);
+    k_kv_move<<<(unsigned)blocks, kThreads, 0, at.stream>>>(w, cp, src, dst, table, entries, copy_blocks, at.err);
+    cuda_need(cudaGetLastError(), "kv move");
+    internal_count_launch(1);
+  });
+}

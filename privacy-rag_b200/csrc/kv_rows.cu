@@ -1,0 +1,541 @@
+// Attention of a few query rows per key head over the paged cache: the single-token form, and the
+// form for prompts of few tokens.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c (q.k_j) - m),  c = scale log2(e),
+// in one pass over the visible keys: a block keeps the running maximum m of the exponents, the
+// running sum and the running o, and rescales the last two when m grows.  Partial results (m, sum, o)
+// of disjoint key sets join by the same rule.
+//
+// Bound by HBM: per visible key and key head 4 dim bytes are read for 4 dim group operations (group
+// query heads per key head), about one byte per operation at group 1.  So the layout serves the
+// loads.  A warp owns its own ring of 16-key stages in shared memory, filled by 16-byte asynchronous
+// copies that follow the page table row by row, and no block-wide barrier stands in the loop.  The
+// rows of a key head share each key, as the 16 rows of mma.m16n8k16 (K and V fragments by ldmatrix
+// from a ring swizzled by 16-byte chunks): two m16n8k16 products per key and 128 dims, a fifth of
+// the time that the key's bytes take to arrive, so the wide tensor path, whose smallest tile is 64
+// rows and which would need the keys of all warps in one tile, has nothing to give here.
+//
+// The length is split: the blocks of a thread-block cluster take equal runs of the visible keys and
+// join through distributed shared memory in rank order, which needs no workspace, no atomics and no
+// second launch, and adapts to the lengths on the device.  Only where units x 8 blocks cannot fill
+// the GPU (few sequences and key heads, long context) does a unit take several clusters, whose
+// partial results a second kernel joins, in order too: results do not depend on timing.
+//
+// Keys that no row sees (before the window, past the length) are never read: the loop runs over the
+// visible keys, counted through: first tokens, then the window.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "kv_attention.h"
+
+namespace cg = cooperative_groups;
+
+namespace bfvgpu {
+namespace kv {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kKeys = 16;   // keys per stage
+constexpr int kRows = 16;   // query rows per unit
+constexpr int kMaxCluster = 8;
+
+template <int DP>
+struct Ring {
+  static constexpr int kStages = 3;
+  static constexpr int kRowBytes = DP * 2;
+  static constexpr int kTile = kKeys * kRowBytes;       // K or V of one stage
+  static constexpr int kWarpBytes = kStages * 2 * kTile;
+  static constexpr int kBytes = kWarps * kWarpBytes;
+  // after the loop the same memory holds the warps' results, then the block's
+  static constexpr int kMergeFloats = kWarps * kRows * (DP + 2) + kRows * (DP + 2);
+  static_assert(kMergeFloats * 4 <= kBytes, "results fit the ring");
+};
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool take) {
+  const uint32_t n = take ? 16 : 0;  // 0: the 16 bytes are filled with zeros and nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <class T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (T::kind == 0)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// What p loses in 16 bits, as a second pair: hi + lo holds p to about 16 bits more.
+template <class T>
+__device__ __forceinline__ uint32_t pack_rest(float x, float y, uint32_t hi) {
+  const float2 h = T::unpack(hi);
+  return T::pack(x - h.x, y - h.y);
+}
+
+// The rows of one unit: 16 rows of one (sequence, key head), and the keys that any of them sees.
+struct Unit {
+  int32_t b = 0, g = 0;
+  int32_t row0 = 0, rows = 0;    // first row of the (sequence, key head), rows in this unit (0: none)
+  int32_t token0 = 0;            // the sequence's first new token in q and out
+  int32_t pos0 = 0;              // its position in the sequence
+  int32_t sinks = 0, begin = 0;  // visible keys: [0, sinks) and [begin, begin + n - sinks)
+  int32_t n = 0;
+  __device__ __forceinline__ int32_t token(int32_t i) const { return i < sinks ? i : i - sinks + begin; }
+};
+
+// Units are numbered [16-row block of the batch][key head]; surplus numbers find no rows.
+__device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const Query& q, int64_t u) {
+  Unit un;
+  un.g = (int32_t)(u % kv.heads);
+  const int64_t block = u / kv.heads;
+  int32_t first = 0, tokens = 1;
+  int64_t at = 0;  // the 16-row block within the sequence
+  if (bt.starts) {
+    // blocks of the sequences before this one, 32 sequences a step
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    bool found = false;
+    for (int32_t b0 = 0; b0 < bt.seqs && !found; b0 += 32) {
+      int64_t mine = 0;
+      int32_t s = 0, e = 0;
+      if (b0 + lane < bt.seqs) {
+        s = bt.starts[b0 + lane];
+        e = bt.starts[b0 + lane + 1];
+        if (s < 0 || e < s || e > q.tokens) {
+          flag_error(bt.err, kErrTable);
+          s = e = 0;
+        }
+        mine = ((int64_t)(e - s) * q.group + kRows - 1) / kRows;
+      }
+      int64_t upto = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += o;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, block < before + upto);
+      if (hit) {
+        const int from = __ffs(hit) - 1;
+        un.b = b0 + from;
+        at = block - before - __shfl_sync(0xffffffffu, upto - mine, from);
+        first = __shfl_sync(0xffffffffu, s, from);
+        tokens = __shfl_sync(0xffffffffu, e, from) - first;
+        found = true;
+      } else {
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (!found) return un;
+  } else {
+    const int32_t per = (q.group + kRows - 1) / kRows;
+    un.b = (int32_t)(block / per);
+    at = block % per;
+    first = un.b;
+    if (un.b >= bt.seqs) return un;
+  }
+  const int64_t all = (int64_t)tokens * q.group;
+  un.row0 = (int32_t)(at * kRows);
+  un.rows = (int32_t)(all - un.row0 < kRows ? all - un.row0 : kRows);
+  un.token0 = first;
+  const int32_t length = sequence_length(bt, kv, un.b);
+  un.pos0 = length - tokens;
+  // positions of the unit's first and last row
+  const int32_t lo = un.pos0 + un.row0 / q.group, hi = un.pos0 + (un.row0 + un.rows - 1) / q.group;
+  if (hi >= 0) {
+    un.begin = q.window && lo + 1 > q.window ? lo + 1 - q.window : 0;
+    un.sinks = q.sinks < un.begin ? q.sinks : un.begin;
+    if (!q.window) un.sinks = 0;
+    un.n = un.sinks + hi + 1 - un.begin;
+  }
+  return un;
+}
+
+// PAIR: at most 8 rows.  The upper 8 rows of the products then carry what p loses in 16 bits (p = hi
+// + lo), so o keeps about 16 bits of p at no cost; with more rows a second product does the same.
+template <class T, int DP, bool PAIR>
+__global__ void __launch_bounds__(kThreads)
+    k_kv_rows(View kv, Batch bt, Query q, int32_t cluster, int32_t parts, float* scratch) {
+  using R = Ring<DP>;
+  extern __shared__ __align__(1024) uint8_t ring[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int32_t rank = (int32_t)(blockIdx.x % cluster);
+  const int64_t at_part = blockIdx.x / cluster;
+  const int32_t part = (int32_t)(at_part % parts);
+  const int64_t u = at_part / parts;
+  const Unit un = find_unit(kv, bt, q, u);
+  const int32_t quad = lane >> 2, pair = (lane & 3) * 2;
+
+  // stages of the unit -> this block's run of them
+  const int32_t stages = (un.n + kKeys - 1) / kKeys;
+  const int32_t shares = cluster * parts, share = part * cluster + rank;
+  const int32_t s0 = (int32_t)((int64_t)stages * share / shares), s1 = (int32_t)((int64_t)stages * (share + 1) / shares);
+
+  // query fragments (rows past the unit's and dims past the head's are 0)
+  uint32_t qa[DP / 16][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int32_t row = un.row0 + quad + 8 * h;
+    const bool in = quad + 8 * h < un.rows;
+    const int32_t tok = row / q.group;
+    const uint16_t* p = q.q + (int64_t)(un.token0 + tok) * q.token_stride +
+                        (int64_t)(un.g * q.group + row - tok * q.group) * q.head_stride;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int32_t d = ks * 16 + c * 8 + pair;
+        qa[ks][h + 2 * c] = in && d < kv.dim ? __ldg(reinterpret_cast<const uint32_t*>(p + d)) : 0;
+      }
+  }
+
+  const uint32_t base = smem_addr(ring) + warp * R::kWarpBytes;
+  if (kv.dim != DP) {  // the chunks past the head's dims are never copied: zeros
+    for (int i = lane; i < R::kWarpBytes / 16; i += 32)
+      *reinterpret_cast<uint4*>(ring + warp * R::kWarpBytes + i * 16) = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  }
+
+  // lane l looks up the page of key l % 16 of a stage, one stage ahead of its copies
+  const int32_t* row_of_table = bt.table + (int64_t)un.b * bt.width;
+  const int32_t page_mask = (1 << kv.page_log) - 1;
+  const int64_t head_at = un.g * kv.head_stride;
+  auto entry_of = [&](int32_t s) {
+    const int32_t i = s * kKeys + (lane & 15);
+    return s < s1 && i < un.n ? __ldg(row_of_table + (un.token(i) >> kv.page_log)) : 0;
+  };
+  int32_t entry = entry_of(s0 + warp);
+  auto issue = [&](int32_t s, int32_t slot) {
+    if (s < s1) {
+      const int32_t i = s * kKeys + (lane & 15);
+      const bool in = i < un.n, good = (uint32_t)entry < (uint32_t)kv.pages;
+      if (in && !good) flag_error(bt.err, kErrTable);
+      const int64_t off = in && good ? entry * kv.page_stride + head_at + (int64_t)(un.token(i) & page_mask) * kv.token_stride : -1;
+      entry = entry_of(s + kWarps);
+      constexpr int kChunks = DP / 8, kPer = 32 / kChunks;  // chunks a row, rows an access
+      const int chunk = lane % kChunks;
+      const uint32_t to = base + slot * 2 * R::kTile;
+#pragma unroll
+      for (int it = 0; it < kKeys / kPer; ++it) {
+        const int r = it * kPer + lane / kChunks;
+        const int64_t o = __shfl_sync(0xffffffffu, off, r);
+        const uint32_t dst = to + r * R::kRowBytes + ((chunk ^ (r & 7)) << 4);
+        if (chunk * 8 < kv.dim) {
+          const bool take = o >= 0;
+          const int64_t from = take ? o + chunk * 8 : 0;
+          copy16(dst, kv.k + from, take);
+          copy16(dst + R::kTile, kv.v + from, take);
+        }
+      }
+    }
+    copies_commit();
+  };
+
+  float o[DP / 8][4];
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[i][c] = 0;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
+  // positions of this thread's two rows
+  int32_t pos[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) pos[h] = un.pos0 + (un.row0 + quad + 8 * h) / q.group;
+  const bool one_token = un.rows > 0 && un.row0 / q.group == (un.row0 + un.rows - 1) / q.group;
+
+#pragma unroll
+  for (int i = 0; i < R::kStages - 1; ++i) issue(s0 + warp + i * kWarps, i);
+  int slot = 0;
+  for (int32_t s = s0 + warp; s < s1; s += kWarps) {
+    // the slot filled next was read in the last step
+    issue(s + (R::kStages - 1) * kWarps, slot == 0 ? R::kStages - 1 : slot - 1);
+    copies_wait<R::kStages - 1>();
+    __syncwarp();
+    const uint32_t kt = base + slot * 2 * R::kTile, vt = kt + R::kTile;
+    float c[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[t][i] = 0;
+    const int mat = lane >> 3, r8 = lane & 7;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      uint32_t b[4];
+      ldsm4(b, kt + ((mat >> 1) * 8 + r8) * R::kRowBytes + (((ks * 2 + (mat & 1)) ^ r8) << 4));
+      mma<T>(c[0], qa[ks], b[0], b[1]);
+      mma<T>(c[1], qa[ks], b[2], b[3]);
+    }
+    // exponents; keys past the visible ones and, with several tokens, those a row does not see: -inf
+    float x[2][4], top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (PAIR && i >= 2) continue;
+        const int h = i >> 1;
+        const int32_t key = s * kKeys + t * 8 + pair + (i & 1);
+        bool seen = key < un.n;
+        if (!one_token) {
+          const int32_t tok = un.token(key);
+          seen = seen && tok <= pos[h] && (!q.window || tok > pos[h] - q.window || tok < q.sinks);
+        }
+        x[t][i] = seen ? c[t][i] * q.scale_log2 : -INFINITY;
+        top[h] = fmaxf(top[h], x[t][i]);
+      }
+#pragma unroll
+    for (int h = 0; h < (PAIR ? 1 : 2); ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+    }
+    float use[2];
+    bool grew = false;
+#pragma unroll
+    for (int h = 0; h < (PAIR ? 1 : 2); ++h) {
+      grew |= top[h] > m[h];
+      top[h] = fmaxf(m[h], top[h]);
+      use[h] = top[h] == -INFINITY ? 0.f : top[h];  // nothing seen yet: every p is 0
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+      float f[2];
+#pragma unroll
+      for (int h = 0; h < (PAIR ? 1 : 2); ++h) {
+        f[h] = exp2_fast(m[h] - use[h]);
+        l[h] *= f[h];
+        m[h] = top[h];
+      }
+      if (PAIR) f[1] = f[0];
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) {
+        o[i][0] *= f[0];
+        o[i][1] *= f[0];
+        o[i][2] *= f[1];
+        o[i][3] *= f[1];
+      }
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int h = 0; h < (PAIR ? 1 : 2); ++h) {
+        const float p0 = exp2_fast(x[t][2 * h] - use[h]), p1 = exp2_fast(x[t][2 * h + 1] - use[h]);
+        l[h] += p0 + p1;
+        hi[2 * t + h] = T::pack(p0, p1);
+        lo[2 * t + h] = pack_rest<T>(p0, p1, hi[2 * t + h]);
+        if (PAIR) hi[2 * t + 1] = lo[2 * t];
+      }
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      uint32_t b[4];
+      ldsm4t(b, vt + ((mat & 1) * 8 + r8) * R::kRowBytes + (((ks * 2 + (mat >> 1)) ^ r8) << 4));
+      mma<T>(o[2 * ks], hi, b[0], b[1]);
+      mma<T>(o[2 * ks + 1], hi, b[2], b[3]);
+      if (!PAIR) {
+        mma<T>(o[2 * ks], lo, b[0], b[1]);
+        mma<T>(o[2 * ks + 1], lo, b[2], b[3]);
+      }
+    }
+    __syncwarp();
+    slot = slot + 1 == R::kStages ? 0 : slot + 1;
+  }
+  copies_wait<0>();
+  __syncthreads();
+
+  // ---- join: the block's warps, then the cluster's blocks, each in a fixed order ----
+  float* res = reinterpret_cast<float*>(ring);             // [warp][row][DP], then [warp][row][m, l]
+  float* ml = res + kWarps * kRows * DP;
+  float* own = ml + kWarps * kRows * 2;                    // the block's [row][DP], [row][m, l]
+  float* own_ml = own + kRows * DP;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (PAIR && h) break;
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    const int row = quad + 8 * h;
+    float* to = res + (warp * kRows + row) * DP;
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+      const float a = PAIR ? o[i][0] + o[i][2] : o[i][2 * h], b = PAIR ? o[i][1] + o[i][3] : o[i][2 * h + 1];
+      *reinterpret_cast<float2*>(to + i * 8 + pair) = make_float2(a, b);
+    }
+    if (pair == 0) {
+      ml[(warp * kRows + row) * 2] = m[h];
+      ml[(warp * kRows + row) * 2 + 1] = l[h];
+    }
+  }
+  __syncthreads();
+  const int32_t live = un.rows * DP;
+  for (int32_t e = threadIdx.x; e < live; e += kThreads) {
+    const int32_t row = e / DP;
+    float top = -INFINITY, sum = 0, val = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[(w * kRows + row) * 2]);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2_fast(ml[(w * kRows + row) * 2] - ref);
+      sum += f * ml[(w * kRows + row) * 2 + 1];
+      val += f * res[w * kRows * DP + e];
+    }
+    own[e] = val;
+    if (e % DP == 0) {
+      own_ml[row * 2] = top;
+      own_ml[row * 2 + 1] = sum;
+    }
+  }
+  cg::cluster_group cl = cg::this_cluster();
+  if (cluster > 1) cl.sync();
+  else __syncthreads();
+  for (int32_t e = (rank * kThreads + threadIdx.x) * 2; e < live; e += cluster * kThreads * 2) {
+    const int32_t row = e / DP, d = e % DP;
+    float top = -INFINITY, sum = 0, v0 = 0, v1 = 0;
+    for (int32_t c = 0; c < cluster; ++c) {
+      const float* other = cluster > 1 ? cl.map_shared_rank(own, c) : own;
+      const float* other_ml = other + kRows * DP;
+      const float mc = other_ml[row * 2], lc = other_ml[row * 2 + 1];
+      const float2 vc = *reinterpret_cast<const float2*>(other + e);
+      const float now = fmaxf(top, mc), ref = now == -INFINITY ? 0.f : now;
+      const float fo = exp2_fast(top - ref), fc = exp2_fast(mc - ref);
+      sum = sum * fo + lc * fc;
+      v0 = v0 * fo + vc.x * fc;
+      v1 = v1 * fo + vc.y * fc;
+      top = now;
+    }
+    if (parts == 1) {
+      if (d < kv.dim) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key seen: zeros
+        const int32_t r = un.row0 + row, tok = r / q.group;
+        const int64_t to = ((int64_t)(un.token0 + tok) * kv.heads * q.group + un.g * q.group + r - tok * q.group) * kv.dim + d;
+        *reinterpret_cast<uint32_t*>(q.out + to) = T::pack(v0 * inv, v1 * inv);
+      }
+    } else {
+      float* to = scratch + (u * parts + part) * (kRows * (DP + 2));
+      *reinterpret_cast<float2*>(to + e) = make_float2(v0, v1);
+      if (d == 0) *reinterpret_cast<float2*>(to + kRows * DP + row * 2) = make_float2(top, sum);
+    }
+  }
+  if (cluster > 1) cl.sync();  // no block leaves while another reads its shared memory
+}
+
+// Joins the parts of each unit, in order.
+template <class T, int DP>
+__global__ void __launch_bounds__(kThreads)
+    k_kv_rows_join(View kv, Batch bt, Query q, int32_t parts, const float* scratch) {
+  const Unit un = find_unit(kv, bt, q, blockIdx.x);
+  const float* from = scratch + (int64_t)blockIdx.x * parts * (kRows * (DP + 2));
+  for (int32_t e = threadIdx.x * 2; e < un.rows * DP; e += kThreads * 2) {
+    const int32_t row = e / DP, d = e % DP;
+    if (d >= kv.dim) continue;
+    float top = -INFINITY, sum = 0, v0 = 0, v1 = 0;
+    for (int32_t c = 0; c < parts; ++c) {
+      const float* other = from + (int64_t)c * (kRows * (DP + 2));
+      const float2 mlc = *reinterpret_cast<const float2*>(other + kRows * DP + row * 2);
+      const float2 vc = *reinterpret_cast<const float2*>(other + e);
+      const float now = fmaxf(top, mlc.x), ref = now == -INFINITY ? 0.f : now;
+      const float fo = exp2_fast(top - ref), fc = exp2_fast(mlc.x - ref);
+      sum = sum * fo + mlc.y * fc;
+      v0 = v0 * fo + vc.x * fc;
+      v1 = v1 * fo + vc.y * fc;
+      top = now;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int32_t r = un.row0 + row, tok = r / q.group;
+    const int64_t to = ((int64_t)(un.token0 + tok) * kv.heads * q.group + un.g * q.group + r - tok * q.group) * kv.dim + d;
+    *reinterpret_cast<uint32_t*>(q.out + to) = T::pack(v0 * inv, v1 * inv);
+  }
+}
+
+template <class T, int DP, bool PAIR>
+cudaError_t launch(const View& kv, const Batch& bt, const Query& q, const RowSplit& sp, float* scratch, cudaStream_t st,
+                   int* launches) {
+  // the shared-memory limit is an attribute of the function on a device
+  static std::atomic<uint64_t> allowed{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device >= 64 || !(allowed.load() >> device & 1)) {
+    e = cudaFuncSetAttribute(k_kv_rows<T, DP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DP>::kBytes);
+    if (e != cudaSuccess) return e;
+    if (device < 64) allowed.fetch_or(uint64_t(1) << device);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(sp.blocks16 * sp.parts * sp.cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Ring<DP>::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = sp.cluster;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, k_kv_rows<T, DP, PAIR>, kv, bt, q, sp.cluster, sp.parts, scratch);
+  if (e != cudaSuccess) return e;
+  *launches += 1;
+  if (sp.parts > 1) {
+    k_kv_rows_join<T, DP><<<(unsigned)sp.blocks16, kThreads, 0, st>>>(kv, bt, q, sp.parts, scratch);
+    *launches += 1;
+  }
+  return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch_typed(const View& kv, const Batch& bt, const Query& q, const RowSplit& sp, float* scratch,
+                         cudaStream_t st, int* launches) {
+  const bool pair = !bt.starts && q.group <= 8;
+  if (sp.dim_padded == 64)
+    return pair ? launch<T, 64, true>(kv, bt, q, sp, scratch, st, launches)
+                : launch<T, 64, false>(kv, bt, q, sp, scratch, st, launches);
+  return pair ? launch<T, 128, true>(kv, bt, q, sp, scratch, st, launches)
+              : launch<T, 128, false>(kv, bt, q, sp, scratch, st, launches);
+}
+
+}  // namespace
+
+uint64_t RowSplit::scratch_floats() const {
+  return parts > 1 ? (uint64_t)blocks16 * parts * kRows * (dim_padded + 2) : 0;
+}
+
+RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int sms) {
+  RowSplit sp;
+  sp.dim_padded = kv.dim <= 64 ? 64 : 128;
+  const int64_t per = (q.group + kRows - 1) / kRows;
+  // at most ceil(rows / 16) blocks per sequence
+  const int64_t row_blocks = bt.starts ? (int64_t)q.tokens * q.group / kRows + bt.seqs : bt.seqs * per;
+  sp.blocks16 = row_blocks * kv.heads;
+  // what a unit can have to read, from the width of the table
+  int64_t keys = (int64_t)bt.width << kv.page_log;
+  if (q.window) keys = std::min<int64_t>(keys, (int64_t)q.window + q.sinks + kRows);
+  const int64_t resident = (int64_t)sms * (sp.dim_padded == 64 ? 4 : 2);
+  // split until the GPU is filled twice over, while a block keeps at least two stages per warp
+  int64_t split = std::max<int64_t>(1, (2 * resident + sp.blocks16 - 1) / std::max<int64_t>(1, sp.blocks16));
+  split = std::min<int64_t>(split, std::max<int64_t>(1, keys / (2 * kKeys * kWarps)));
+  while (sp.cluster < split && sp.cluster < kMaxCluster) sp.cluster *= 2;
+  if (split > kMaxCluster) sp.parts = (int32_t)((split + kMaxCluster - 1) / kMaxCluster);
+  return sp;
+}
+
+cudaError_t launch_rows(const View& kv, const Batch& bt, const Query& q, int dtype, const RowSplit& sp, float* scratch,
+                        cudaStream_t st, int* launches) {
+  return dtype == 0 ? launch_typed<Bf16>(kv, bt, q, sp, scratch, st, launches)
+                    : launch_typed<Fp16>(kv, bt, q, sp, scratch, st, launches);
+}
+
+}  // namespace kv
+}  // namespace bfvgpu

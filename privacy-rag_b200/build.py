@@ -15,7 +15,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "lib", "libbfvgpu.so")
-SOURCES = ["kernels.cu", "bfvgpu.cu", "noalloc.cu", "peak.cu", "kv_pages.cu", "kv_rows.cu", "kv_attention.cu"]
+SOURCES = ["kernels.cu", "bfvgpu.cu", "noalloc.cu", "peak.cu", "kv_pages.cu", "kv_rows.cu", "kv_prompt.cu", "kv_attention.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

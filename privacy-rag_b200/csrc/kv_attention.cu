@@ -25,6 +25,12 @@ int sm_count(int device) {
   return n;
 }
 
+// Prompts of more rows than this per sequence and key head, on average, go to the tile kernel.
+constexpr int64_t kFewRows = 32;
+bool few_rows(const Batch& bt, const Query& q, bool ragged) {
+  return !ragged || (int64_t)q.tokens * q.group <= kFewRows * bt.seqs;
+}
+
 struct Call {
   View view;
   Batch batch;
@@ -71,6 +77,12 @@ void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int
   c.query.head_stride = head_stride;
   c.query.out = static_cast<uint16_t*>(out);
   c.query.scale_log2 = scale * 1.4426950408889634f;
+  if (!few_rows(c.batch, c.query, starts)) {
+    need(prompt_units(c.view, c.batch, c.query) <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    cuda_need(launch_prompt(c.view, c.batch, c.query, cache->dtype, at.stream), "kv prompt");
+    internal_count_launch(1);
+    return;
+  }
   const RowSplit sp = plan_rows(c.view, c.batch, c.query, sm_count(at.device));
   need(sp.scratch_floats() == 0 || scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
   need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
@@ -90,6 +102,7 @@ uint64_t scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q
     Call c = checked_call(cache, 0, q_heads, tokens, seqs, width, window, sinks);
     static const int32_t some = 0;
     if (ragged) c.batch.starts = &some;  // only asked whether there is one
+    if (!few_rows(c.batch, c.query, ragged)) return;
     int device = -1;
     internal_params(ctx, &device, nullptr);
     words = (plan_rows(c.view, c.batch, c.query, sm_count(device)).scratch_floats() + 1) / 2;

@@ -33,5 +33,10 @@ RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int sms);
 cudaError_t launch_rows(const View& kv, const Batch& bt, const Query& q, int dtype, const RowSplit& split,
                         float* scratch, cudaStream_t st, int* launches);
 
+
+// Blocks of the prompt kernel (256 rows of one key head each, or none).
+int64_t prompt_units(const View& kv, const Batch& bt, const Query& q);
+cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int dtype, cudaStream_t st);
+
 }  // namespace kv
 }  // namespace bfvgpu

@@ -1,0 +1,89 @@
+// Which rows and keys a block of the attention kernels works on.
+#pragma once
+#include "kv_attention.h"
+
+namespace bfvgpu {
+namespace kv {
+
+// The rows of one unit: ROWS consecutive rows of one (sequence, key head), and the keys that any of them sees.
+struct Unit {
+  int32_t b = 0, g = 0;
+  int32_t row0 = 0, rows = 0;    // first row of the (sequence, key head), rows in this unit (0: none)
+  int32_t token0 = 0;            // the sequence's first new token in q and out
+  int32_t pos0 = 0;              // its position in the sequence
+  int32_t sinks = 0, begin = 0;  // visible keys: [0, sinks) and [begin, begin + n - sinks)
+  int32_t n = 0;
+  __device__ __forceinline__ int32_t token(int32_t i) const { return i < sinks ? i : i - sinks + begin; }
+};
+
+// Units are numbered [block of ROWS rows of the batch][key head]; surplus numbers find no rows.  Every
+// warp of a block finds its unit by itself.
+template <int ROWS>
+__device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const Query& q, int64_t u) {
+  Unit un;
+  un.g = (int32_t)(u % kv.heads);
+  const int64_t block = u / kv.heads;
+  int32_t first = 0, tokens = 1;
+  int64_t at = 0;  // the block of rows within the sequence
+  if (bt.starts) {
+    // blocks of the sequences before this one, 32 sequences a step
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    bool found = false;
+    for (int32_t b0 = 0; b0 < bt.seqs && !found; b0 += 32) {
+      int64_t mine = 0;
+      int32_t s = 0, e = 0;
+      if (b0 + lane < bt.seqs) {
+        s = bt.starts[b0 + lane];
+        e = bt.starts[b0 + lane + 1];
+        if (s < 0 || e < s || e > q.tokens) {
+          flag_error(bt.err, kErrTable);
+          s = e = 0;
+        }
+        mine = ((int64_t)(e - s) * q.group + ROWS - 1) / ROWS;
+      }
+      int64_t upto = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += o;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, block < before + upto);
+      if (hit) {
+        const int from = __ffs(hit) - 1;
+        un.b = b0 + from;
+        at = block - before - __shfl_sync(0xffffffffu, upto - mine, from);
+        first = __shfl_sync(0xffffffffu, s, from);
+        tokens = __shfl_sync(0xffffffffu, e, from) - first;
+        found = true;
+      } else {
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (!found) return un;
+  } else {
+    const int32_t per = (q.group + ROWS - 1) / ROWS;
+    un.b = (int32_t)(block / per);
+    at = block % per;
+    first = un.b;
+    if (un.b >= bt.seqs) return un;
+  }
+  const int64_t all = (int64_t)tokens * q.group;
+  un.row0 = (int32_t)(at * ROWS);
+  un.rows = (int32_t)(all - un.row0 < ROWS ? all - un.row0 : ROWS);
+  un.token0 = first;
+  const int32_t length = sequence_length(bt, kv, un.b);
+  un.pos0 = length - tokens;
+  // positions of the unit's first and last row
+  const int32_t lo = un.pos0 + un.row0 / q.group, hi = un.pos0 + (un.row0 + un.rows - 1) / q.group;
+  if (hi >= 0) {
+    un.begin = q.window && lo + 1 > q.window ? lo + 1 - q.window : 0;
+    un.sinks = q.sinks < un.begin ? q.sinks : un.begin;
+    if (un.sinks == un.begin) un.sinks = un.begin = 0;  // nothing is left out between them
+    un.n = un.sinks + hi + 1 - un.begin;
+  }
+  return un;
+}
+
+}  // namespace kv
+}  // namespace bfvgpu

@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kv_attention.h"
 #include "kv_units.cuh"
@@ -32,8 +33,11 @@ namespace {
 constexpr int kTileRows = 128;
 constexpr int kBlockRows = 2 * kTileRows;
 constexpr int kTileKeys = 128;
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;         // two warpgroups of rows, one of the issuing warps (two of its warps idle)
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
+// Registers a thread: launched with 168 (384 x 168 of the SM's 65536); the issuing warpgroup keeps 64 and
+// the rows take 216: 128 x 64 + 256 x 216 <= 384 x 168.
+constexpr int kIssueRegs = 64, kRowRegs = 216;
 constexpr float kLag = 8.f;           // how far m may stay behind the running maximum
 constexpr uint32_t kPolls = 1u << 22; // of a wait before it gives up
 
@@ -86,6 +90,14 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
   flag_error(err, kErrWait);
   return false;
 }
+// One thread of a converged warp, always the same.
+__device__ __forceinline__ bool elected() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes;
+}
+// The same value in every lane, known to the compiler as such.
+__device__ __forceinline__ int32_t same(int32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 __device__ __forceinline__ void tma_box(uint32_t to, const CUtensorMap* map, int32_t x, int32_t token, int32_t head,
                                         int32_t page, uint32_t bar) {
   asm volatile(
@@ -122,7 +134,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
 }
-#define KV_R8(x, i) x[i], x[i + 1], x[i + 2], x[i + 3], x[i + 4], x[i + 5], x[i + 6], x[i + 7]
 // 32 consecutive columns of this thread's lane.
 __device__ __forceinline__ void tmem_load(uint32_t at, float* x) {
   uint32_t* r = reinterpret_cast<uint32_t*>(x);
@@ -155,27 +166,25 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- which key tiles the block and each of its row tiles need ------------------------------------
+// The block's key tiles are numbered 0 .. n-1: `first` tiles of first tokens, then the window's from tile
+// `from` on.  A row tile needs [0, first) and [begin, end).  It may take part in a tile that it sees
+// nothing of; every tile is needed by one row tile.
 struct Span {
-  int32_t lo = 0, hi = -1;  // positions of the rows (hi < 0: no row sees a key)
+  int32_t lo = 0, hi = -1;        // positions of the rows (hi < 0: no row sees a key)
+  int32_t begin = 0, end = 0;
 };
 struct Plan {
-  int32_t tiles = 0;          // row tiles with rows
-  int32_t n = 0;              // key tiles of the block: `first` from the front, then from `from` on
-  int32_t first = 0, from = 0;
-  int32_t end = 0;            // keys the block sees: [0, sinks) and [begin, end)
-  Span span[2];
+  int32_t n = 0, first = 0, from = 0;
+  int32_t end = 0;                // keys the block sees: [0, sinks) and [begin, end)
   __device__ __forceinline__ int32_t key0(int32_t i) const { return (i < first ? i : i - first + from) * kTileKeys; }
+  // the row tile's first key tile from i on; n: none
+  __device__ __forceinline__ int32_t at_or_after(const Span& s, int32_t i) const {
+    i = i < first ? i : max(i, s.begin);
+    return i < s.end ? i : n;
+  }
 };
-__device__ __forceinline__ Plan make_plan(const Unit& un, const Query& q) {
+__device__ __forceinline__ Plan make_plan(const Unit& un) {
   Plan p;
-  p.tiles = (un.rows + kTileRows - 1) / kTileRows;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-    if (t < p.tiles) {
-      const int32_t r1 = min(un.rows, (t + 1) * kTileRows) - 1;
-      p.span[t].lo = un.pos0 + (un.row0 + t * kTileRows) / q.group;
-      p.span[t].hi = un.pos0 + (un.row0 + r1) / q.group;
-    }
   if (un.n > 0) {
     p.end = un.begin + un.n - un.sinks;
     p.from = un.begin / kTileKeys;
@@ -184,11 +193,17 @@ __device__ __forceinline__ Plan make_plan(const Unit& un, const Query& q) {
   }
   return p;
 }
-// Whether a row tile sees anything of the key tile.  Every key tile of the block is seen by one.
-__device__ __forceinline__ bool sees(const Span& s, const Query& q, int32_t key0) {
-  if (key0 > s.hi) return false;
-  if (!q.window) return true;
-  return key0 + kTileKeys - 1 > max(s.lo, 0) - q.window || key0 < q.sinks;
+__device__ __forceinline__ Span make_span(const Unit& un, const Query& q, const Plan& p, int t) {
+  Span s;
+  if (t * kTileRows >= un.rows) return s;
+  s.lo = un.pos0 + (un.row0 + t * kTileRows) / q.group;
+  s.hi = un.pos0 + (un.row0 + min(un.rows, (t + 1) * kTileRows) - 1) / q.group;
+  if (s.hi < 0) return s;
+  s.end = p.first + s.hi / kTileKeys - p.from + 1;
+  s.begin = p.first;
+  // the block's window tiles before the row tile's own, unless first tokens reach into them
+  if (un.begin > 0 && un.sinks <= p.from * kTileKeys) s.begin += max(0, (s.lo + 1 - q.window) / kTileKeys - p.from);
+  return s;
 }
 
 template <class T, int DP>
@@ -198,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
   uint8_t* sm = raw + (base - smem_addr(raw));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = same(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t bars = base + S::kBar;
   const uint32_t q_full = bars, k_full = bars + 16, k_empty = k_full + 8 * S::kStages, v_full = k_empty + 8 * S::kStages,
                  v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages, p_full = s_full + 16,
@@ -209,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the blocks with the most keys first
   const Unit un = find_unit<kBlockRows>(kv, bt, q, units - 1 - blockIdx.x);
   if (un.rows == 0) return;
-  const Plan plan = make_plan(un, q);
+  const Plan plan = make_plan(un);
 
   if (threadIdx.x == 0) {
     bar_init(q_full, kTileRows);
@@ -236,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto s_col = [&](int t) { return tmem + t * kTileKeys; };
   auto o_col = [&](int t) { return tmem + 2 * kTileKeys + t * DP; };
 
+  if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
   if (warp == kLoadWarp) {
     // ---- loads: lane j has the j-th page of a key tile ----
     const int32_t page_tokens = 1 << kv.page_log, box = min(page_tokens, kTileKeys), boxes = kTileKeys / box;
@@ -304,74 +320,96 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      // ---- products ----
-      bool ok = true;
-      int32_t next[2] = {0, 0}, released = 0, done_s[2] = {0, 0}, done_p[2] = {0, 0};
-      bool first_o[2] = {true, true};
-      auto following = [&](int t, int32_t i) {
-        while (i < plan.n && !(t < plan.tiles && sees(plan.span[t], q, plan.key0(i)))) ++i;
-        return i;
-      };
-      auto issue_s = [&](int t) {  // scores of the tile's next key tile
-        const int32_t i = next[t];
-        if (i >= plan.n) return;
-        const int st = i % S::kStages;
-        ok = ok && bar_wait(k_full + 8 * st, (i / S::kStages) & 1, abort, bt.err);
-        if (done_s[t] == 0) ok = ok && bar_wait(q_full + 8 * t, 0, abort, bt.err);
-        if (!ok) return;
-        fence_after();
-        const uint32_t qb = base + S::kQ + t * S::kTileBytes, kb = base + S::kK + st * S::kTileBytes;
+    // ---- products: S of a tile as soon as its P is used up, so that the two tiles take turns.  The
+    // whole warp runs the loop and one thread issues: descriptors in uniform registers go to the
+    // tensor core at once (from inside a one-thread branch each product took about 100 cycles to issue) ----
+    Plan pl = plan;
+    pl.n = same(pl.n);
+    pl.first = same(pl.first);
+    Span s0 = make_span(un, q, plan, 0), s1 = make_span(un, q, plan, 1);
+    s0.begin = same(s0.begin);
+    s0.end = same(s0.end);
+    s1.begin = same(s1.begin);
+    s1.end = same(s1.end);
+    const uint32_t tm = same(tmem);
+    bool ok = true;
+    // next key tile of each row tile's S, and of its P; key tiles whose K is given back
+    int32_t s_next[2] = {pl.at_or_after(s0, 0), pl.at_or_after(s1, 0)};
+    int32_t p_next[2] = {s_next[0], s_next[1]}, released = 0;
+    uint32_t p_turn[2] = {0, 0};
+    const uint64_t q_desc = operand(base + S::kQ, 16), k_desc = operand(base + S::kK, 16),
+                   v_desc = operand(base + S::kV, S::kHalfBytes);
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      ok = ok && __all_sync(0xffffffffu, bar_wait(bar, parity, abort, bt.err));
+    };
+    auto issue_s = [&](auto tile) {
+      constexpr int t = decltype(tile)::value;
+      const int32_t i = s_next[t];
+      if (i >= pl.n) return;
+      const int st = i % S::kStages;
+      wait(k_full + 8 * st, (i / S::kStages) & 1);
+      if (!ok) return;
+      s_next[t] = pl.at_or_after(t ? s1 : s0, i + 1);
+      const int32_t free = min(s_next[0], s_next[1]);
+      fence_after();
+      const uint64_t qd = q_desc + t * (S::kTileBytes >> 4), kd = k_desc + st * (S::kTileBytes >> 4);
+      if (elected()) {
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * S::kHalfBytes + (ks & 3) * 32;
-          mma_ss(s_col(t), operand(qb + off, 16), operand(kb + off, 16), instruction<T>(kTileKeys, false), ks > 0);
+          constexpr uint32_t kHalf = S::kHalfBytes >> 4;
+          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 2;
+          mma_ss(tm + t * kTileKeys, qd + off, kd + off, instruction<T>(kTileKeys, false), ks > 0);
         }
         mma_commit(s_full + 8 * t);
-        ++done_s[t];
-        next[t] = following(t, i + 1);
-        while (released < min(next[0], next[1])) {
-          mma_commit(k_empty + 8 * (released % S::kStages));
-          ++released;
-        }
-      };
-      next[0] = following(0, 0);
-      next[1] = following(1, 0);
-      int32_t at_p[2] = {next[0], next[1]};  // the key tile whose P comes next
-      issue_s(0);
-      issue_s(1);
-      for (int32_t i = 0; i < plan.n && ok; ++i) {
-        const int st = i % S::kStages;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (at_p[t] != i) continue;
-          ok = bar_wait(v_full + 8 * st, (i / S::kStages) & 1, abort, bt.err) &&
-               bar_wait(p_full + 8 * t, done_p[t] & 1, abort, bt.err);
-          if (!ok) break;
-          fence_after();
-          const uint32_t vb = base + S::kV + st * S::kTileBytes;
+        for (int32_t r = released; r < free; ++r) mma_commit(k_empty + 8 * (r % S::kStages));
+      }
+      __syncwarp();
+      released = max(released, free);
+    };
+    auto issue_o = [&](auto tile, int32_t i) {
+      constexpr int t = decltype(tile)::value;
+      if (!ok || p_next[t] != i) return;
+      const int st = i % S::kStages;
+      wait(v_full + 8 * st, (i / S::kStages) & 1);
+      wait(p_full + 8 * t, p_turn[t] & 1);
+      if (!ok) return;
+      p_next[t] = pl.at_or_after(t ? s1 : s0, i + 1);
+      fence_after();
+      const uint64_t vd = v_desc + st * (S::kTileBytes >> 4);
+      if (elected()) {
 #pragma unroll
-          for (int ks = 0; ks < kTileKeys / 16; ++ks)
-            mma_ts(o_col(t), s_col(t) + ks * 8, operand(vb + ks * 2048, S::kHalfBytes), instruction<T>(DP, true),
-                   !(first_o[t] && ks == 0));
-          first_o[t] = false;
-          ++done_p[t];
-          at_p[t] = following(t, i + 1);
-          if (at_p[t] >= plan.n) mma_commit(o_full + 8 * t);
-          issue_s(t);
-        }
-        if (ok) mma_commit(v_empty + 8 * st);
+        for (int ks = 0; ks < kTileKeys / 16; ++ks)
+          mma_ts(tm + 2 * kTileKeys + t * DP, tm + t * kTileKeys + ks * 8, vd + ks * 128, instruction<T>(DP, true),
+                 ks > 0 || p_turn[t] > 0);
+        if (p_next[t] >= pl.n) mma_commit(o_full + 8 * t);
       }
-      if (!ok) {  // products in flight end before the tensor memory is given back
-        mma_commit(drain);
-        for (uint32_t n = 0; n < kPolls && !bar_try(drain, 0); ++n) {
-        }
-      }
+      __syncwarp();
+      ++p_turn[t];
+      issue_s(tile);
+    };
+    const std::integral_constant<int, 0> tile0;
+    const std::integral_constant<int, 1> tile1;
+    if (s0.end) wait(q_full, 0);
+    issue_s(tile0);
+    if (s1.end) wait(q_full + 8, 0);
+    issue_s(tile1);
+    for (int32_t i = 0; i < pl.n && ok; ++i) {
+      issue_o(tile0, i);
+      issue_o(tile1, i);
+      if (ok && elected()) mma_commit(v_empty + 8 * (i % S::kStages));
+      __syncwarp();
     }
-    __syncwarp();
-  } else {
+    if (!ok) {  // products in flight end before the tensor memory is given back
+      if (elected()) mma_commit(drain);
+      for (uint32_t n = 0; n < kPolls && !bar_try(drain, 0); ++n) {
+      }
+      __syncwarp();
+    }
+  } else if (warp < kMmaWarp) {
     // ---- rows ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
     const int t = warp >> 2;
-    if (t < plan.tiles) {
+    if (t * kTileRows < un.rows) {
       const int tid = threadIdx.x & 127, row = tid;
       uint8_t* qs = sm + S::kQ + t * S::kTileBytes;
       constexpr int kChunks = DP / 8;
@@ -387,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_arrive(q_full + 8 * t);
 
-      const Span span = plan.span[t];
+      const Span span = make_span(un, q, plan, t);
       const int32_t last_row = min(un.rows, (t + 1) * kTileRows) - 1;
       const int32_t my_row = min(t * kTileRows + row, last_row);  // rows past the last do its work again
       const int32_t pos = un.pos0 + (un.row0 + my_row) / q.group;
@@ -397,9 +435,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0;
       int32_t done = 0;
       bool ok = true;
-      for (int32_t i = 0; i < plan.n; ++i) {
+      for (int32_t i = plan.at_or_after(span, 0); i < plan.n; i = plan.at_or_after(span, i + 1)) {
         const int32_t key0 = plan.key0(i);
-        if (!sees(span, q, key0)) continue;
         ok = bar_wait(s_full + 8 * t, done & 1, abort, bt.err);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
@@ -425,7 +462,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int j = 4; j < kTileKeys; ++j) top[j & 3] = fmaxf(top[j & 3], x[j]);
+        for (int j = 4; j + 8 <= kTileKeys + 4; j += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            top[e] = fmaxf(fmaxf(top[e], x[j + e]), j + 4 + e < kTileKeys ? x[j + 4 + e] : -INFINITY);
         const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
         if (done == 0) {
           m = now;
@@ -445,20 +485,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        float sum[2] = {0, 0};
+        float sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < kTileKeys; j += 32) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float p0 = exp2_fast(fmaf(x[j + e], c, -ref)), p1 = exp2_fast(fmaf(x[j + e + 1], c, -ref));
-            sum[0] += p0;
-            sum[1] += p1;
+            sum[e & 2] += p0;
+            sum[(e & 2) + 1] += p1;
             p[e / 2] = T::pack(p0, p1);
           }
           tmem_store16(s_at + j / 2, p);
         }
-        l += sum[0] + sum[1];
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tmem_store_wait();
         fence_before();
         bar_arrive(p_full + 8 * t);

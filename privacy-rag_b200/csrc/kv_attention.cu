@@ -44,12 +44,13 @@ Call checked_call(const bfvgpu_kv* cache, int32_t layer, uint64_t q_heads, uint6
   c.view = checked_view(cache, layer);
   need(q_heads >= 1 && q_heads <= kMost && q_heads % c.view.heads == 0, BFVGPU_E_SHAPE, "E_KV_HEADS");
   need(tokens <= kMost && seqs <= kMost && width <= kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
-  need(q_heads / c.view.heads <= 1024 && tokens * (q_heads / c.view.heads) <= kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+  need(q_heads / c.view.heads <= kMaxGroup && tokens * (q_heads / c.view.heads) <= kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
   // positions and their sums with the window stay in 32 bits
   need((width << c.view.page_log) <= (uint64_t(1) << 30), BFVGPU_E_SHAPE, "E_KV_WIDTH");
   need(window >= 0 && sinks >= 0, BFVGPU_E_ARGUMENT, "E_KV_WINDOW");
   const int32_t top = 1 << 30;
   c.query.group = (int32_t)(q_heads / c.view.heads);
+  c.query.group_inverse = ((1u << kGroupShift) + c.query.group - 1) / c.query.group;
   c.query.tokens = (int32_t)tokens;
   c.query.window = window < top ? window : 0;  // a window past every position hides nothing
   c.query.sinks = std::min(sinks, top);

@@ -9,6 +9,10 @@
 namespace bfvgpu {
 namespace kv {
 
+// Largest group and rows of a block: x / group = (x group_inverse) >> 21 for x < kMaxGroup + kMaxRows
+// (x group_inverse < 2^32, and x (group group_inverse - 2^21) < 1280 x 1024 < 2^21).
+constexpr int kMaxGroup = 1024, kMaxRows = 256, kGroupShift = 21;
+
 // Queries and results.  Row R of a (sequence, key head) is query head (key head * group + R % group)
 // of the sequence's new token R / group: all rows of one key head read the same keys.
 struct Query {
@@ -16,7 +20,8 @@ struct Query {
   int64_t token_stride = 0, head_stride = 0;  // elements
   uint16_t* out = nullptr;                    // [tokens][heads * group][dim]
   int32_t tokens = 0;                         // new tokens of the batch
-  int32_t group = 1;                          // query heads per key head
+  int32_t group = 1;                          // query heads per key head (at most kMaxGroup)
+  uint32_t group_inverse = 0;                 // ceil(2^21 / group)
   int32_t window = 0, sinks = 0;              // window 0: every earlier key
   float scale_log2 = 0;                       // scale * log2(e)
 };

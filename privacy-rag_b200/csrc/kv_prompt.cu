@@ -196,8 +196,8 @@ __device__ __forceinline__ Plan make_plan(const Unit& un) {
 __device__ __forceinline__ Span make_span(const Unit& un, const Query& q, const Plan& p, int t) {
   Span s;
   if (t * kTileRows >= un.rows) return s;
-  s.lo = un.pos0 + (un.row0 + t * kTileRows) / q.group;
-  s.hi = un.pos0 + (un.row0 + min(un.rows, (t + 1) * kTileRows) - 1) / q.group;
+  s.lo = un.position(q, t * kTileRows);
+  s.hi = un.position(q, min(un.rows, (t + 1) * kTileRows) - 1);
   if (s.hi < 0) return s;
   s.end = p.first + s.hi / kTileKeys - p.from + 1;
   s.begin = p.first;
@@ -221,11 +221,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::kBar + S::kBars * 8);
   volatile uint32_t* abort = tmem_slot + 1;
 
-  // the blocks with the most keys first
-  const Unit un = find_unit<kBlockRows>(kv, bt, q, units - 1 - blockIdx.x);
-  if (un.rows == 0) return;
-  const Plan plan = make_plan(un);
-
   if (threadIdx.x == 0) {
     bar_init(q_full, kTileRows);
     bar_init(q_full + 8, kTileRows);
@@ -243,6 +238,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  // the blocks with the most keys first
+  const Unit un = find_unit<kBlockRows>(kv, bt, q, units - 1 - blockIdx.x);
+  const Plan plan = make_plan(un);
+
   fence_before();
   __syncthreads();
   fence_after();
@@ -413,14 +412,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tid = threadIdx.x & 127, row = tid;
       uint8_t* qs = sm + S::kQ + t * S::kTileBytes;
       constexpr int kChunks = DP / 8;
-      for (int r = tid / kChunks; r < kTileRows; r += kTileRows / kChunks) {
-        const int chunk = tid % kChunks;
-        const int32_t ri = un.row0 + t * kTileRows + r, tok = ri / q.group;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (t * kTileRows + r < un.rows && chunk * 8 < kv.dim)
-          x = __ldg(reinterpret_cast<const uint4*>(q.q + (int64_t)(un.token0 + tok) * q.token_stride +
-                                                   (int64_t)(un.g * q.group + ri - tok * q.group) * q.head_stride + chunk * 8));
-        *reinterpret_cast<uint4*>(qs + (chunk >> 3) * S::kHalfBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = x;
+      constexpr int kLoads = kTileRows * kChunks / 128, kStep = 128 / kChunks;
+      {
+        const int chunk = tid % kChunks, r0 = tid / kChunks;
+        uint4 x[kLoads];  // all in flight together
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+          const int r = r0 + n * kStep;
+          x[n] = make_uint4(0, 0, 0, 0);
+          if (t * kTileRows + r < un.rows && chunk * 8 < kv.dim)
+            x[n] = __ldg(reinterpret_cast<const uint4*>(un.query(q, t * kTileRows + r) + chunk * 8));
+        }
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+          const int r = r0 + n * kStep;
+          *reinterpret_cast<uint4*>(qs + (chunk >> 3) * S::kHalfBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = x[n];
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_arrive(q_full + 8 * t);
@@ -428,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Span span = make_span(un, q, plan, t);
       const int32_t last_row = min(un.rows, (t + 1) * kTileRows) - 1;
       const int32_t my_row = min(t * kTileRows + row, last_row);  // rows past the last do its work again
-      const int32_t pos = un.pos0 + (un.row0 + my_row) / q.group;
+      const int32_t pos = un.position(q, my_row);
       const uint32_t quadrant = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4) ..
       const uint32_t s_at = s_col(t) + quadrant, o_at = o_col(t) + quadrant;
       const float c = q.scale_log2;
@@ -450,10 +457,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool cut_end = key0 + kTileKeys - 1 > span.lo;
         const bool cut_begin = q.window && key0 <= span.hi - q.window && key0 + kTileKeys > q.sinks;
         if (cut_begin) {
-          const int32_t hi = pos - key0, lo = hi - q.window, sk = q.sinks - key0;
+          // keys lo .. hi of the tile are seen, and those below sk
+          const int32_t hi = pos - key0, sk = q.sinks - key0;
+          const uint32_t lo = (uint32_t)max(hi - q.window + 1, 0), n = (uint32_t)max(hi - (int32_t)lo + 1, 0);
+          if (sk > 0) {
 #pragma unroll
-          for (int j = 0; j < kTileKeys; ++j)
-            if (j > hi || (j <= lo && j >= sk)) x[j] = -INFINITY;
+            for (int j = 0; j < kTileKeys; ++j)
+              if ((uint32_t)j - lo >= n && (j >= sk || j > hi)) x[j] = -INFINITY;
+          } else {
+#pragma unroll
+            for (int j = 0; j < kTileKeys; ++j)
+              if ((uint32_t)j - lo >= n) x[j] = -INFINITY;
+          }
         } else if (cut_end) {
           const int32_t hi = pos - key0;
 #pragma unroll
@@ -508,13 +523,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && done) ok = bar_wait(o_full + 8 * t, 0, abort, bt.err);
       ok = __all_sync(0xffffffffu, ok);
       if (ok && !done) {  // no row of the tile sees a key
-        for (int32_t r = tid / kChunks; r < kTileRows; r += kTileRows / kChunks) {
-          const int chunk = tid % kChunks;
-          const int32_t ri = un.row0 + t * kTileRows + r, tok = ri / q.group;
-          if (t * kTileRows + r < un.rows && chunk * 8 < kv.dim)
-            *reinterpret_cast<uint4*>(q.out + ((int64_t)(un.token0 + tok) * kv.heads * q.group + un.g * q.group + ri -
-                                               tok * q.group) * kv.dim + chunk * 8) = make_uint4(0, 0, 0, 0);
-        }
+        for (int r = tid / kChunks; r < kTileRows && t * kTileRows + r < un.rows; r += kStep)
+          if (tid % kChunks * 8 < kv.dim)
+            *reinterpret_cast<uint4*>(un.result(kv, q, t * kTileRows + r) + tid % kChunks * 8) = make_uint4(0, 0, 0, 0);
       } else if (ok) {
         fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -533,12 +544,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         __syncwarp();  // a warp writes out its own 32 rows
-        for (int r = lane / kChunks; r < 32; r += 32 / kChunks) {
-          const int chunk = lane % kChunks, rr = (warp & 3) * 32 + r;
-          const int32_t ri = un.row0 + t * kTileRows + rr, tok = ri / q.group;
+        const int chunk = lane % kChunks;
+#pragma unroll
+        for (int n = 0; n < kChunks; ++n) {
+          const int rr = (warp & 3) * 32 + lane / kChunks + n * (32 / kChunks);
           if (t * kTileRows + rr < un.rows && chunk * 8 < kv.dim)
-            *reinterpret_cast<uint4*>(q.out + ((int64_t)(un.token0 + tok) * kv.heads * q.group + un.g * q.group + ri -
-                                               tok * q.group) * kv.dim + chunk * 8) =
+            *reinterpret_cast<uint4*>(un.result(kv, q, t * kTileRows + rr) + chunk * 8) =
                 *reinterpret_cast<const uint4*>(qs + rr * DP * 2 + ((chunk ^ (rr & 7)) << 4));
         }
       }

@@ -115,11 +115,8 @@ __global__ void __launch_bounds__(kThreads)
   uint32_t qa[DP / 16][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int32_t row = un.row0 + quad + 8 * h;
     const bool in = quad + 8 * h < un.rows;
-    const int32_t tok = row / q.group;
-    const uint16_t* p = q.q + (int64_t)(un.token0 + tok) * q.token_stride +
-                        (int64_t)(un.g * q.group + row - tok * q.group) * q.head_stride;
+    const uint16_t* p = un.query(q, quad + 8 * h);
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
@@ -180,8 +177,8 @@ __global__ void __launch_bounds__(kThreads)
   // positions of this thread's two rows
   int32_t pos[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) pos[h] = un.pos0 + (un.row0 + quad + 8 * h) / q.group;
-  const bool one_token = un.rows > 0 && un.row0 / q.group == (un.row0 + un.rows - 1) / q.group;
+  for (int h = 0; h < 2; ++h) pos[h] = un.position(q, quad + 8 * h);
+  const bool one_token = un.token_of(q, un.rows - 1) == 0;
 
 #pragma unroll
   for (int i = 0; i < R::kStages - 1; ++i) issue(s0 + warp + i * kWarps, i);
@@ -343,9 +340,7 @@ __global__ void __launch_bounds__(kThreads)
     if (parts == 1) {
       if (d < kv.dim) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key seen: zeros
-        const int32_t r = un.row0 + row, tok = r / q.group;
-        const int64_t to = ((int64_t)(un.token0 + tok) * kv.heads * q.group + un.g * q.group + r - tok * q.group) * kv.dim + d;
-        *reinterpret_cast<uint32_t*>(q.out + to) = T::pack(v0 * inv, v1 * inv);
+        *reinterpret_cast<uint32_t*>(un.result(kv, q, row) + d) = T::pack(v0 * inv, v1 * inv);
       }
     } else {
       float* to = scratch + (u * parts + part) * (kRows * (DP + 2));
@@ -378,9 +373,7 @@ __global__ void __launch_bounds__(kThreads)
       top = now;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int32_t r = un.row0 + row, tok = r / q.group;
-    const int64_t to = ((int64_t)(un.token0 + tok) * kv.heads * q.group + un.g * q.group + r - tok * q.group) * kv.dim + d;
-    *reinterpret_cast<uint32_t*>(q.out + to) = T::pack(v0 * inv, v1 * inv);
+    *reinterpret_cast<uint32_t*>(un.result(kv, q, row) + d) = T::pack(v0 * inv, v1 * inv);
   }
 }
 

@@ -8,12 +8,28 @@ namespace kv {
 // The rows of one unit: ROWS consecutive rows of one (sequence, key head), and the keys that any of them sees.
 struct Unit {
   int32_t b = 0, g = 0;
-  int32_t row0 = 0, rows = 0;    // first row of the (sequence, key head), rows in this unit (0: none)
-  int32_t token0 = 0;            // the sequence's first new token in q and out
-  int32_t pos0 = 0;              // its position in the sequence
+  int32_t rows = 0;              // 0: none
+  int32_t token0 = 0;            // the token of the first row in q and out,
+  int32_t pos0 = 0;              // its position in the sequence,
+  int32_t head0 = 0;             // and the first row's query head within the group
   int32_t sinks = 0, begin = 0;  // visible keys: [0, sinks) and [begin, begin + n - sinks)
   int32_t n = 0;
   __device__ __forceinline__ int32_t token(int32_t i) const { return i < sinks ? i : i - sinks + begin; }
+  // tokens from the first row's to row r's
+  __device__ __forceinline__ int32_t token_of(const Query& q, int32_t r) const {
+    return (int32_t)(((uint32_t)(head0 + r) * q.group_inverse) >> kGroupShift);
+  }
+  // position of row r's token
+  __device__ __forceinline__ int32_t position(const Query& q, int32_t r) const { return pos0 + token_of(q, r); }
+  // row r's query, and its place in out
+  __device__ __forceinline__ const uint16_t* query(const Query& q, int32_t r) const {
+    const int32_t t = token_of(q, r);
+    return q.q + (int64_t)(token0 + t) * q.token_stride + (int64_t)(g * q.group + head0 + r - t * q.group) * q.head_stride;
+  }
+  __device__ __forceinline__ uint16_t* result(const View& kv, const Query& q, int32_t r) const {
+    const int32_t t = token_of(q, r);
+    return q.out + ((int64_t)(token0 + t) * kv.heads * q.group + g * q.group + head0 + r - t * q.group) * kv.dim;
+  }
 };
 
 // Units are numbered [block of ROWS rows of the batch][key head]; surplus numbers find no rows.  Every
@@ -68,14 +84,14 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
     first = un.b;
     if (un.b >= bt.seqs) return un;
   }
-  const int64_t all = (int64_t)tokens * q.group;
-  un.row0 = (int32_t)(at * ROWS);
-  un.rows = (int32_t)(all - un.row0 < ROWS ? all - un.row0 : ROWS);
-  un.token0 = first;
-  const int32_t length = sequence_length(bt, kv, un.b);
-  un.pos0 = length - tokens;
+  const int64_t all = (int64_t)tokens * q.group, row0 = at * ROWS;
+  un.rows = (int32_t)(all - row0 < ROWS ? all - row0 : ROWS);
+  const int32_t before = (int32_t)(row0 / q.group);
+  un.head0 = (int32_t)(row0 - (int64_t)before * q.group);
+  un.token0 = first + before;
+  un.pos0 = sequence_length(bt, kv, un.b) - tokens + before;
   // positions of the unit's first and last row
-  const int32_t lo = un.pos0 + un.row0 / q.group, hi = un.pos0 + (un.row0 + un.rows - 1) / q.group;
+  const int32_t lo = un.pos0, hi = un.position(q, un.rows - 1);
   if (hi >= 0) {
     un.begin = q.window && lo + 1 > q.window ? lo + 1 - q.window : 0;
     un.sinks = q.sinks < un.begin ? q.sinks : un.begin;

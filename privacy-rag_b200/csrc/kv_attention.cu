@@ -78,20 +78,23 @@ void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int
   c.query.head_stride = head_stride;
   c.query.out = static_cast<uint16_t*>(out);
   c.query.scale_log2 = scale * 1.4426950408889634f;
-  if (!few_rows(c.batch, c.query, starts)) {
-    need(prompt_units(c.view, c.batch, c.query) <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
-    cuda_need(launch_prompt(c.view, c.batch, c.query, cache->dtype, at.stream), "kv prompt");
-    internal_count_launch(1);
-    return;
-  }
-  const RowSplit sp = plan_rows(c.view, c.batch, c.query, sm_count(at.device));
-  need(sp.scratch_floats() == 0 || scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
-  need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
-  need(sp.blocks16 * sp.parts <= (int64_t)(kMost / sp.cluster), BFVGPU_E_SHAPE, "E_KV_SHAPE");
+  float* work = reinterpret_cast<float*>(scratch);
+  auto need_scratch = [&](uint64_t floats) {
+    need(floats == 0 || scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
+    need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
+  };
   int launches = 0;
-  cuda_need(launch_rows(c.view, c.batch, c.query, cache->dtype, sp, reinterpret_cast<float*>(scratch), at.stream,
-                        &launches),
-            "kv attention");
+  if (few_rows(c.batch, c.query, starts)) {
+    const RowSplit sp = plan_rows(c.view, c.batch, c.query, sm_count(at.device));
+    need_scratch(sp.scratch_floats());
+    need(sp.blocks16 * sp.parts <= (int64_t)(kMost / sp.cluster), BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    cuda_need(launch_rows(c.view, c.batch, c.query, cache->dtype, sp, work, at.stream, &launches), "kv attention");
+  } else {
+    const PromptSplit sp = plan_prompt(c.view, c.batch, c.query, sm_count(at.device));
+    need_scratch(sp.scratch_floats());
+    need(sp.units * sp.parts <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    cuda_need(launch_prompt(c.view, c.batch, c.query, cache->dtype, sp, work, at.stream, &launches), "kv attention");
+  }
   internal_count_launch(launches);
 }
 
@@ -103,10 +106,11 @@ uint64_t scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q
     Call c = checked_call(cache, 0, q_heads, tokens, seqs, width, window, sinks);
     static const int32_t some = 0;
     if (ragged) c.batch.starts = &some;  // only asked whether there is one
-    if (!few_rows(c.batch, c.query, ragged)) return;
     int device = -1;
     internal_params(ctx, &device, nullptr);
-    words = (plan_rows(c.view, c.batch, c.query, sm_count(device)).scratch_floats() + 1) / 2;
+    const int sms = sm_count(device);
+    words = ((few_rows(c.batch, c.query, ragged) ? plan_rows(c.view, c.batch, c.query, sms).scratch_floats()
+                                                 : plan_prompt(c.view, c.batch, c.query, sms).scratch_floats()) + 1) / 2;
   });
   return words;
 }

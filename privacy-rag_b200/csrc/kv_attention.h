@@ -39,9 +39,15 @@ cudaError_t launch_rows(const View& kv, const Batch& bt, const Query& q, int dty
                         float* scratch, cudaStream_t st, int* launches);
 
 
-// Blocks of the prompt kernel (256 rows of one key head each, or none).
-int64_t prompt_units(const View& kv, const Batch& bt, const Query& q);
-cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int dtype, cudaStream_t st);
+// Launch of the prompt kernel: units of 256 rows of one key head, each in so many parts of its keys.
+struct PromptSplit {
+  int64_t units = 0;
+  int32_t parts = 1, dim_padded = 128;
+  uint64_t scratch_floats() const;
+};
+PromptSplit plan_prompt(const View& kv, const Batch& bt, const Query& q, int sms);
+cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& split,
+                          float* scratch, cudaStream_t st, int* launches);
 
 }  // namespace kv
 }  // namespace bfvgpu

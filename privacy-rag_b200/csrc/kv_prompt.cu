@@ -10,12 +10,18 @@
 // and the 32-bit sums, and O need not be rescaled.  The sum of the weights is kept in 32 bits, from
 // the weights before they are rounded to 16 bits for the product.
 //
-// Roles: warps 0-3 and 4-7 hold the rows of tile 0 and 1, one thread of warp 8 issues the products,
-// warp 9 the loads.  While one tile's rows are in their exponentials, the other tile's products run.
+// Roles: warps 0-3 and 4-7 hold the rows of tile 0 and 1, warp 8 issues the products, warp 9 the loads of K
+// and V, warps 10 and 11 load the queries of tile 0 and 1.  While one tile's rows are in their
+// exponentials, the other tile's products run.  A block is resident on its SM for the whole launch and
+// takes over the blocks that have not started yet (cluster launch control), so that the loads of the
+// next rows and the results of the last ones run under the products in between.
 // K and V arrive by TMA page by page as the table names them, in the 128-byte swizzle (K as K-major,
 // V as MN-major operand).  Only visible tokens of V are loaded: what no row of the block sees may
 // hold NaN (unwritten rest of a page, pages given up), and 0 x NaN would reach every row.  Such
 // pages are read row by row, the other rows filled with zeros.
+//
+// Where there are too few rows to fill the GPU, the key tiles of a block's rows are dealt to several
+// blocks, which leave (m, sum, O) in 32 bits for a second kernel to join in a fixed order.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -33,13 +39,26 @@ namespace {
 constexpr int kTileRows = 128;
 constexpr int kBlockRows = 2 * kTileRows;
 constexpr int kTileKeys = 128;
-constexpr int kThreads = 384;         // two warpgroups of rows, one of the issuing warps (two of its warps idle)
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kThreads = 384;         // two warpgroups of rows, one of the issuing warps
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kQueryWarp = 10;
+constexpr int kReaders = 11;          // warps that are told of the next rows: all but the loads' own
 // Registers a thread: launched with 168 (384 x 168 of the SM's 65536); the issuing warpgroup keeps 64 and
 // the rows take 216: 128 x 64 + 256 x 216 <= 384 x 168.
 constexpr int kIssueRegs = 64, kRowRegs = 216;
 constexpr float kLag = 8.f;           // how far m may stay behind the running maximum
-constexpr uint32_t kPolls = 1u << 22; // of a wait before it gives up
+constexpr uint32_t kPolls = 1u << 20;     // of a wait for the next step before it gives up
+constexpr uint32_t kLongPolls = 1u << 27; // of a wait that may span all keys of other rows
+constexpr int kPartTiles = 8;         // key tiles that a part has at least
+constexpr int kMaxParts = 16;
+
+// What the loading warp tells the others: the rows, and which of their key tiles.
+struct Item {
+  Unit un;
+  int32_t begin = 0, end = 0;  // key tiles
+  int32_t parts = 1;           // of the unit; 1: the rows' results are final
+  int32_t slot = 0;            // of the partial results
+  int32_t more = 0;            // 0: no further rows
+};
 
 template <int DP>
 struct Smem {
@@ -50,9 +69,11 @@ struct Smem {
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
-  static constexpr int kBar = kV + kStages * kTileBytes;
-  // barriers: Q of tile 0/1; K full, K empty, V full, V empty per stage; S, P, O of tile 0/1; drain
-  static constexpr int kBars = 2 + 4 * kStages + 6 + 1;
+  static constexpr int kOut = kV + kStages * kTileBytes;  // 128 bytes of each row, per warp
+  static constexpr int kAnswer = kOut + 8 * 32 * 128;     // of the launch control, 16 bytes
+  static constexpr int kItems = kAnswer + 16;             // two
+  static constexpr int kBar = kItems + ((2 * (int)sizeof(Item) + 7) & ~7);
+  static constexpr int kBars = 4 + 4 * kStages + 2 + 4 + 4 + 4 + 2;
   static constexpr int kBytes = kBar + kBars * 8 + 16;    // + tensor memory address, abort flag
   static constexpr int kLaunch = kBytes + 1024;           // slack for the 1024-byte alignment
   static_assert(kLaunch > 115 * 1024 && kLaunch <= 227 * 1024, "one block, and its tensor memory, per SM");
@@ -81,14 +102,31 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   return done;
 }
 // Bounded; gives up early when another role has.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t* err) {
-  for (uint32_t i = 0; i < kPolls; ++i) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t* err,
+                                         uint32_t polls = kPolls) {
+  for (uint32_t i = 0; i < polls; ++i) {
     if (bar_try(bar, parity)) return true;
     if ((i & 1023) == 1023 && *abort) return false;
   }
   *abort = 1;
   flag_error(err, kErrWait);
   return false;
+}
+// Asks the launch control for a block of this grid that has not started; the answer (16 bytes) arrives on
+// the barrier.  Not to be asked again after a refusal.
+__device__ __forceinline__ void ask_for_block(uint32_t answer, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(answer), "r"(bar) : "memory");
+}
+// The block of an answer; -1: none is left.
+__device__ __forceinline__ int64_t answered_block(uint32_t answer) {
+  uint32_t yes, x;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\tld.shared.b128 a, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\tselp.b32 %0, 1, 0, p;\n\tmov.b32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, a;\n\t}"
+      : "=r"(yes), "=r"(x) : "r"(answer) : "memory");
+  return yes ? (int64_t)x : -1;
 }
 // One thread of a converged warp, always the same.
 __device__ __forceinline__ bool elected() {
@@ -165,23 +203,14 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// ---- which key tiles the block and each of its row tiles need ------------------------------------
-// The block's key tiles are numbered 0 .. n-1: `first` tiles of first tokens, then the window's from tile
+// ---- which key tiles the rows and each of their row tiles need -----------------------------------
+// The rows' key tiles are numbered 0 .. n-1: `first` tiles of first tokens, then the window's from tile
 // `from` on.  A row tile needs [0, first) and [begin, end).  It may take part in a tile that it sees
 // nothing of; every tile is needed by one row tile.
-struct Span {
-  int32_t lo = 0, hi = -1;        // positions of the rows (hi < 0: no row sees a key)
-  int32_t begin = 0, end = 0;
-};
 struct Plan {
   int32_t n = 0, first = 0, from = 0;
-  int32_t end = 0;                // keys the block sees: [0, sinks) and [begin, end)
+  int32_t end = 0;                // keys the rows see: [0, sinks) and [begin, end)
   __device__ __forceinline__ int32_t key0(int32_t i) const { return (i < first ? i : i - first + from) * kTileKeys; }
-  // the row tile's first key tile from i on; n: none
-  __device__ __forceinline__ int32_t at_or_after(const Span& s, int32_t i) const {
-    i = i < first ? i : max(i, s.begin);
-    return i < s.end ? i : n;
-  }
 };
 __device__ __forceinline__ Plan make_plan(const Unit& un) {
   Plan p;
@@ -193,43 +222,91 @@ __device__ __forceinline__ Plan make_plan(const Unit& un) {
   }
   return p;
 }
-__device__ __forceinline__ Span make_span(const Unit& un, const Query& q, const Plan& p, int t) {
+struct Span {
+  int32_t lo = 0, hi = -1;  // positions of the rows (hi < 0: no row sees a key)
+  // the item's key tiles that the row tile needs: [from, first) and [begin, end), in the item's [from, to)
+  int32_t first = 0, begin = 0, end = 0, from = 0, to = 0;
+  __device__ __forceinline__ int32_t at_or_after(int32_t i) const {  // to: none
+    i = i < first ? i : max(i, begin);
+    return i < end ? i : to;
+  }
+  __device__ __forceinline__ int32_t start() const { return at_or_after(from); }
+  __device__ __forceinline__ bool active() const { return start() < to; }
+};
+__device__ __forceinline__ Span make_span(const Item& it, const Query& q, const Plan& p, int t) {
+  const Unit& un = it.un;
   Span s;
+  s.from = it.begin;
+  s.to = it.end;
   if (t * kTileRows >= un.rows) return s;
   s.lo = un.position(q, t * kTileRows);
   s.hi = un.position(q, min(un.rows, (t + 1) * kTileRows) - 1);
   if (s.hi < 0) return s;
-  s.end = p.first + s.hi / kTileKeys - p.from + 1;
+  s.first = p.first;
+  s.end = min(it.end, p.first + s.hi / kTileKeys - p.from + 1);
   s.begin = p.first;
-  // the block's window tiles before the row tile's own, unless first tokens reach into them
+  // the window tiles before the row tile's own, unless first tokens reach into them
   if (un.begin > 0 && un.sinks <= p.from * kTileKeys) s.begin += max(0, (s.lo + 1 - q.window) / kTileKeys - p.from);
   return s;
+}
+// Parts of a unit of n key tiles where the launch has `most`.
+__device__ __forceinline__ int32_t parts_of(int32_t n, int32_t most) {
+  return max(1, min(most, (n + kPartTiles - 1) / kPartTiles));
+}
+// Partial results: per slot [row][DP] O, then [row][m, sum].
+template <int DP>
+constexpr int64_t kSlotFloats = (int64_t)kBlockRows * (DP + 2);
+
+// 128 bytes of each of the warp's 32 rows: every lane has its own row's; stored by whole rows.
+template <class To>
+__device__ __forceinline__ void store_rows(uint8_t* stage, const uint32_t* w, int lane, int rows, int bytes, To to) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+        make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  __syncwarp();
+  const int c = lane & 7;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const int r = n * 4 + (lane >> 3);
+    if (r < rows && c * 16 < bytes)
+      *reinterpret_cast<uint4*>(to(r) + c * 16) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+  }
+  __syncwarp();
 }
 
 template <class T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_kv_prompt(const __grid_constant__ Maps maps, View kv, Batch bt, Query q, int64_t units) {
+    k_kv_prompt(const __grid_constant__ Maps maps, View kv, Batch bt, Query q, int64_t units, int32_t most_parts,
+                float* scratch) {
   using S = Smem<DP>;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
   uint8_t* sm = raw + (base - smem_addr(raw));
   const int warp = same(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t bars = base + S::kBar;
-  const uint32_t q_full = bars, k_full = bars + 16, k_empty = k_full + 8 * S::kStages, v_full = k_empty + 8 * S::kStages,
-                 v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages, p_full = s_full + 16,
-                 o_full = p_full + 16, drain = o_full + 16;
+  const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * S::kStages,
+                 v_full = k_empty + 8 * S::kStages, v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages,
+                 p_half = s_full + 16, o_full = p_half + 32, o_empty = o_full + 16, item_full = o_empty + 16,
+                 item_empty = item_full + 16, answered = item_empty + 16, drain = answered + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::kBar + S::kBars * 8);
   volatile uint32_t* abort = tmem_slot + 1;
+  Item* items = reinterpret_cast<Item*>(sm + S::kItems);
 
   if (threadIdx.x == 0) {
-    bar_init(q_full, kTileRows);
-    bar_init(q_full + 8, kTileRows);
-    for (int i = 0; i < 4 * S::kStages; ++i) bar_init(k_full + 8 * i, 1);
     for (int t = 0; t < 2; ++t) {
+      bar_init(q_full + 8 * t, 32);
+      bar_init(q_empty + 8 * t, 1);
       bar_init(s_full + 8 * t, 1);
-      bar_init(p_full + 8 * t, kTileRows);
+      bar_init(p_half + 16 * t, kTileRows);
+      bar_init(p_half + 16 * t + 8, kTileRows);
       bar_init(o_full + 8 * t, 1);
+      bar_init(o_empty + 8 * t, kTileRows);
+      bar_init(item_full + 8 * t, 1);
+      bar_init(item_empty + 8 * t, kReaders);
     }
+    for (int i = 0; i < 4 * S::kStages; ++i) bar_init(k_full + 8 * i, 1);
+    bar_init(answered, 1);
     bar_init(drain, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -238,165 +315,240 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // the blocks with the most keys first
-  const Unit un = find_unit<kBlockRows>(kv, bt, q, units - 1 - blockIdx.x);
-  const Plan plan = make_plan(un);
-
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = *tmem_slot;
-  // tensor memory columns: S (and P over it) of tile 0 and 1, O of tile 0 and 1
-  auto s_col = [&](int t) { return tmem + t * kTileKeys; };
-  auto o_col = [&](int t) { return tmem + 2 * kTileKeys + t * DP; };
+  const uint32_t tmem = *tmem_slot;  // columns: S (and P over it) of tile 0 and 1, O of tile 0 and 1
+
+  // the next item, for every warp but the loads'; false: no more (or given up)
+  uint32_t item_turn = 0;
+  bool ok = true;
+  auto next_item = [&](Item& it) {
+    const uint32_t at = item_turn & 1;
+    ok = __all_sync(0xffffffffu, bar_wait(item_full + 8 * at, (item_turn >> 1) & 1, abort, bt.err, kLongPolls));
+    if (!ok) return false;
+    it = items[at];
+    __syncwarp();
+    if (lane == 0) bar_arrive(item_empty + 8 * at);
+    ++item_turn;
+    return it.more != 0;
+  };
 
   if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
   if (warp == kLoadWarp) {
-    // ---- loads: lane j has the j-th page of a key tile ----
+    // ---- items, and loads of K and V: lane j has the j-th page of a key tile ----
     const int32_t page_tokens = 1 << kv.page_log, box = min(page_tokens, kTileKeys), boxes = kTileKeys / box;
-    const int32_t* row = bt.table + (int64_t)un.b * bt.width;
-    bool ok = true;
-    int32_t i = 0;
-    for (; i < plan.n; ++i) {
-      const int st = i % S::kStages;
-      const uint32_t turn = (i / S::kStages) & 1;
-      const int32_t t0 = plan.key0(i) + lane * box, t1 = t0 + box;
-      int32_t page = kv.pages;  // a box outside the pages reads zeros
-      bool whole = true;
-      if (lane < boxes) {
-        const bool in = t0 < un.sinks || (t0 < plan.end && t1 > un.begin);
-        whole = !in || t1 <= un.sinks || (t0 >= un.begin && t1 <= plan.end);
-        if (in) {
-          page = __ldg(row + (t0 >> kv.page_log));
-          if ((uint32_t)page >= (uint32_t)kv.pages) {
-            flag_error(bt.err, kErrTable);
-            page = kv.pages;
+    int64_t block = blockIdx.x;
+    uint32_t turn = 0, answers = 0, k_issued = 0, v_issued = 0;
+    bool asked = false;
+    auto tell = [&](const Item& it) {
+      const uint32_t at = item_turn & 1;
+      ok = __all_sync(0xffffffffu, bar_wait(item_empty + 8 * at, ((item_turn >> 1) & 1) ^ 1, abort, bt.err, kLongPolls));
+      if (!ok) return;
+      if (lane == 0) {
+        items[at] = it;
+        bar_arrive(item_full + 8 * at);
+      }
+      __syncwarp();
+      ++item_turn;
+    };
+    auto ask = [&] {
+      if (asked) return;
+      asked = true;
+      if (lane == 0) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the last answer has been read
+        bar_expect(answered, 16);
+        ask_for_block(base + S::kAnswer, answered);
+      }
+      __syncwarp();
+    };
+    while (ok && block >= 0) {
+      // the blocks with the most keys come first
+      const int64_t u = units - 1 - block / most_parts;
+      const int32_t part = (int32_t)(block % most_parts);
+      Item it;
+      it.un = find_unit<kBlockRows>(kv, bt, q, u);
+      const Unit& un = it.un;
+      const Plan plan = make_plan(un);
+      it.parts = parts_of(plan.n, most_parts);
+      it.begin = (int32_t)((int64_t)plan.n * part / it.parts);
+      it.end = (int32_t)((int64_t)plan.n * (part + 1) / it.parts);
+      it.slot = (int32_t)(u * most_parts + part);
+      it.more = 1;
+      if (un.rows > 0 && part < it.parts) {
+        tell(it);
+        const int32_t* row = bt.table + (int64_t)un.b * bt.width;
+        for (int32_t i = it.begin; i < it.end && ok; ++i, ++turn) {
+          const int st = turn % S::kStages;
+          const uint32_t parity = ((turn / S::kStages) & 1) ^ 1;
+          const int32_t t0 = plan.key0(i) + lane * box, t1 = t0 + box;
+          int32_t page = kv.pages;  // a box outside the pages reads zeros
+          bool whole = true;
+          if (lane < boxes) {
+            const bool in = t0 < un.sinks || (t0 < plan.end && t1 > un.begin);
+            whole = !in || t1 <= un.sinks || (t0 >= un.begin && t1 <= plan.end);
+            if (in) {
+              page = __ldg(row + (t0 >> kv.page_log));
+              if ((uint32_t)page >= (uint32_t)kv.pages) {
+                flag_error(bt.err, kErrTable);
+                page = kv.pages;
+              }
+            }
           }
+          const int32_t at = t0 & (page_tokens - 1);
+          const uint32_t kb = base + S::kK + st * S::kTileBytes, vb = base + S::kV + st * S::kTileBytes;
+          ok = __all_sync(0xffffffffu, bar_wait(k_empty + 8 * st, parity, abort, bt.err));
+          if (!ok) break;
+          if (lane == 0) bar_expect(k_full + 8 * st, S::kTileBytes);
+          __syncwarp();
+          if (lane < boxes)
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)
+              tma_box(kb + h * S::kHalfBytes + lane * box * 128, &maps.k, h * 64, at, un.g, page, k_full + 8 * st);
+          k_issued = turn + 1;
+          if (i + 1 == it.end) ask();
+          ok = __all_sync(0xffffffffu, bar_wait(v_empty + 8 * st, parity, abort, bt.err));
+          if (!ok) break;
+          if (lane == 0) bar_expect(v_full + 8 * st, S::kTileBytes);
+          __syncwarp();
+          if (lane < boxes && whole)
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)
+              tma_box(vb + h * S::kHalfBytes + lane * box * 128, &maps.v, h * 64, at, un.g, page, v_full + 8 * st);
+          for (uint32_t left = __ballot_sync(0xffffffffu, !whole); left; left &= left - 1) {
+            const int j = __ffs(left) - 1;
+            const int32_t pj = __shfl_sync(0xffffffffu, page, j), tj = __shfl_sync(0xffffffffu, t0, j);
+            const int32_t aj = __shfl_sync(0xffffffffu, at, j);
+            for (int32_t r = lane; r < box; r += 32) {
+              const int32_t tok = tj + r;
+              const bool seen = tok < un.sinks || (tok >= un.begin && tok < plan.end);
+#pragma unroll
+              for (int h = 0; h < S::kHalves; ++h)
+                tma_box(vb + h * S::kHalfBytes + (j * box + r) * 128, &maps.v_row, h * 64, aj + r, un.g,
+                        seen ? pj : kv.pages, v_full + 8 * st);
+            }
+          }
+          v_issued = turn + 1;
         }
       }
-      const int32_t at = t0 & (page_tokens - 1);
-      const uint32_t kb = base + S::kK + st * S::kTileBytes, vb = base + S::kV + st * S::kTileBytes;
-      ok = bar_wait(k_empty + 8 * st, turn ^ 1, abort, bt.err);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane == 0) bar_expect(k_full + 8 * st, S::kTileBytes);
+      if (!ok) break;
+      ask();
+      ok = __all_sync(0xffffffffu, bar_wait(answered, answers & 1, abort, bt.err));
+      if (!ok) break;
+      block = answered_block(base + S::kAnswer);
       __syncwarp();
-      if (lane < boxes)
-#pragma unroll
-        for (int h = 0; h < S::kHalves; ++h)
-          tma_box(kb + h * S::kHalfBytes + lane * box * 128, &maps.k, h * 64, at, un.g, page, k_full + 8 * st);
-      ok = bar_wait(v_empty + 8 * st, turn ^ 1, abort, bt.err);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane == 0) bar_expect(v_full + 8 * st, S::kTileBytes);
-      __syncwarp();
-      if (lane < boxes && whole)
-#pragma unroll
-        for (int h = 0; h < S::kHalves; ++h)
-          tma_box(vb + h * S::kHalfBytes + lane * box * 128, &maps.v, h * 64, at, un.g, page, v_full + 8 * st);
-      for (uint32_t left = __ballot_sync(0xffffffffu, !whole); left; left &= left - 1) {
-        const int j = __ffs(left) - 1;
-        const int32_t pj = __shfl_sync(0xffffffffu, page, j), tj = __shfl_sync(0xffffffffu, t0, j);
-        const int32_t aj = __shfl_sync(0xffffffffu, at, j);
-        for (int32_t r = lane; r < box; r += 32) {
-          const int32_t tok = tj + r;
-          const bool seen = tok < un.sinks || (tok >= un.begin && tok < plan.end);
-#pragma unroll
-          for (int h = 0; h < S::kHalves; ++h)
-            tma_box(vb + h * S::kHalfBytes + (j * box + r) * 128, &maps.v_row, h * 64, aj + r, un.g,
-                    seen ? pj : kv.pages, v_full + 8 * st);
-        }
-      }
+      ++answers;
+      asked = false;
     }
-    if (i < plan.n) {
+    if (ok) tell(Item{});
+    if (!ok) {
       // given up: what is in flight into shared memory lands before the block ends
-      for (int32_t j = max(0, i - S::kStages); j <= i; ++j) {
-        if (j < plan.n)
-          for (uint32_t n = 0; n < kPolls && !bar_try(k_full + 8 * (j % S::kStages), (j / S::kStages) & 1); ++n) {
-            if (j == i && n > 1024) break;  // perhaps never issued
+      auto land = [&](uint32_t full, uint32_t issued) {
+        for (uint32_t j = issued > S::kStages ? issued - S::kStages : 0; j < issued; ++j)
+          for (uint32_t n = 0; n < kPolls && !bar_try(full + 8 * (j % S::kStages), (j / S::kStages) & 1); ++n) {
           }
-        if (j < i)
-          for (uint32_t n = 0; n < kPolls && !bar_try(v_full + 8 * (j % S::kStages), (j / S::kStages) & 1); ++n) {
-          }
+      };
+      land(k_full, k_issued);
+      land(v_full, v_issued);
+      for (uint32_t n = 0; asked && n < kPolls && !bar_try(answered, answers & 1); ++n) {
       }
     }
   } else if (warp == kMmaWarp) {
     // ---- products: S of a tile as soon as its P is used up, so that the two tiles take turns.  The
     // whole warp runs the loop and one thread issues: descriptors in uniform registers go to the
     // tensor core at once (from inside a one-thread branch each product took about 100 cycles to issue) ----
-    Plan pl = plan;
-    pl.n = same(pl.n);
-    pl.first = same(pl.first);
-    Span s0 = make_span(un, q, plan, 0), s1 = make_span(un, q, plan, 1);
-    s0.begin = same(s0.begin);
-    s0.end = same(s0.end);
-    s1.begin = same(s1.begin);
-    s1.end = same(s1.end);
     const uint32_t tm = same(tmem);
-    bool ok = true;
-    // next key tile of each row tile's S, and of its P; key tiles whose K is given back
-    int32_t s_next[2] = {pl.at_or_after(s0, 0), pl.at_or_after(s1, 0)};
-    int32_t p_next[2] = {s_next[0], s_next[1]}, released = 0;
-    uint32_t p_turn[2] = {0, 0};
     const uint64_t q_desc = operand(base + S::kQ, 16), k_desc = operand(base + S::kK, 16),
                    v_desc = operand(base + S::kV, S::kHalfBytes);
+    uint32_t turn0 = 0;                   // the ring's turn of the item's first key tile
+    uint32_t p_turn[2] = {0, 0}, active[2] = {0, 0};
     auto wait = [&](uint32_t bar, uint32_t parity) {
       ok = ok && __all_sync(0xffffffffu, bar_wait(bar, parity, abort, bt.err));
     };
-    auto issue_s = [&](auto tile) {
-      constexpr int t = decltype(tile)::value;
-      const int32_t i = s_next[t];
-      if (i >= pl.n) return;
-      const int st = i % S::kStages;
-      wait(k_full + 8 * st, (i / S::kStages) & 1);
-      if (!ok) return;
-      s_next[t] = pl.at_or_after(t ? s1 : s0, i + 1);
-      const int32_t free = min(s_next[0], s_next[1]);
-      fence_after();
-      const uint64_t qd = q_desc + t * (S::kTileBytes >> 4), kd = k_desc + st * (S::kTileBytes >> 4);
-      if (elected()) {
+    Item it;
+    while (next_item(it)) {
+      const Plan plan = make_plan(it.un);
+      Span span[2];
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          constexpr uint32_t kHalf = S::kHalfBytes >> 4;
-          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 2;
-          mma_ss(tm + t * kTileKeys, qd + off, kd + off, instruction<T>(kTileKeys, false), ks > 0);
+      for (int t = 0; t < 2; ++t) {
+        span[t] = make_span(it, q, plan, t);
+        span[t].first = same(span[t].first);
+        span[t].begin = same(span[t].begin);
+        span[t].end = same(span[t].end);
+        span[t].from = same(span[t].from);
+        span[t].to = same(span[t].to);
+      }
+      const int32_t from = span[0].from, to = span[0].to;
+      // next key tile of each row tile's S, and of its P; key tiles whose K is given back
+      int32_t s_next[2] = {span[0].start(), span[1].start()}, p_next[2] = {s_next[0], s_next[1]}, released = from;
+      auto issue_s = [&](auto tile) {
+        constexpr int t = decltype(tile)::value;
+        const int32_t i = s_next[t];
+        if (i >= to || !ok) return;
+        const uint32_t turn = turn0 + (uint32_t)(i - from);
+        const int st = turn % S::kStages;
+        wait(k_full + 8 * st, (turn / S::kStages) & 1);
+        if (!ok) return;
+        s_next[t] = span[t].at_or_after(i + 1);
+        const int32_t free = min(s_next[0], s_next[1]);
+        fence_after();
+        const uint64_t qd = q_desc + t * (S::kTileBytes >> 4), kd = k_desc + st * (S::kTileBytes >> 4);
+        if (elected()) {
+#pragma unroll
+          for (int ks = 0; ks < DP / 16; ++ks) {
+            constexpr uint32_t kHalf = S::kHalfBytes >> 4;
+            const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 2;
+            mma_ss(tm + t * kTileKeys, qd + off, kd + off, instruction<T>(kTileKeys, false), ks > 0);
+          }
+          mma_commit(s_full + 8 * t);
+          if (s_next[t] >= to) mma_commit(q_empty + 8 * t);
+          for (int32_t r = released; r < free; ++r) mma_commit(k_empty + 8 * ((turn0 + (uint32_t)(r - from)) % S::kStages));
         }
-        mma_commit(s_full + 8 * t);
-        for (int32_t r = released; r < free; ++r) mma_commit(k_empty + 8 * (r % S::kStages));
-      }
-      __syncwarp();
-      released = max(released, free);
-    };
-    auto issue_o = [&](auto tile, int32_t i) {
-      constexpr int t = decltype(tile)::value;
-      if (!ok || p_next[t] != i) return;
-      const int st = i % S::kStages;
-      wait(v_full + 8 * st, (i / S::kStages) & 1);
-      wait(p_full + 8 * t, p_turn[t] & 1);
-      if (!ok) return;
-      p_next[t] = pl.at_or_after(t ? s1 : s0, i + 1);
-      fence_after();
-      const uint64_t vd = v_desc + st * (S::kTileBytes >> 4);
-      if (elected()) {
+        __syncwarp();
+        released = max(released, free);
+      };
+      auto issue_o = [&](auto tile, int32_t i) {
+        constexpr int t = decltype(tile)::value;
+        if (!ok || p_next[t] != i) return;
+        const bool first = i == span[t].start();
+        const uint32_t turn = turn0 + (uint32_t)(i - from);
+        const int st = turn % S::kStages;
+        wait(v_full + 8 * st, (turn / S::kStages) & 1);
+        if (first) wait(o_empty + 8 * t, (active[t] & 1) ^ 1);
+        p_next[t] = span[t].at_or_after(i + 1);
+        const uint64_t vd = v_desc + st * (S::kTileBytes >> 4);
 #pragma unroll
-        for (int ks = 0; ks < kTileKeys / 16; ++ks)
-          mma_ts(tm + 2 * kTileKeys + t * DP, tm + t * kTileKeys + ks * 8, vd + ks * 128, instruction<T>(DP, true),
-                 ks > 0 || p_turn[t] > 0);
-        if (p_next[t] >= pl.n) mma_commit(o_full + 8 * t);
+        for (int h = 0; h < 2; ++h) {
+          wait(p_half + 16 * t + 8 * h, p_turn[t] & 1);
+          if (!ok) return;
+          fence_after();
+          if (elected()) {
+#pragma unroll
+            for (int ks = h * (kTileKeys / 32); ks < (h + 1) * (kTileKeys / 32); ++ks)
+              mma_ts(tm + 2 * kTileKeys + t * DP, tm + t * kTileKeys + ks * 8, vd + ks * 128, instruction<T>(DP, true),
+                     ks > 0 || !first);
+            if (h && p_next[t] >= to) mma_commit(o_full + 8 * t);
+          }
+          __syncwarp();
+        }
+        ++p_turn[t];
+        if (first) ++active[t];
+        issue_s(tile);
+      };
+      const std::integral_constant<int, 0> tile0;
+      const std::integral_constant<int, 1> tile1;
+      if (s_next[0] < to) wait(q_full, active[0] & 1);
+      issue_s(tile0);
+      if (s_next[1] < to) wait(q_full + 8, active[1] & 1);
+      issue_s(tile1);
+      for (int32_t i = from; i < to && ok; ++i) {
+        issue_o(tile0, i);
+        issue_o(tile1, i);
+        if (ok && elected()) mma_commit(v_empty + 8 * ((turn0 + (uint32_t)(i - from)) % S::kStages));
+        __syncwarp();
       }
-      __syncwarp();
-      ++p_turn[t];
-      issue_s(tile);
-    };
-    const std::integral_constant<int, 0> tile0;
-    const std::integral_constant<int, 1> tile1;
-    if (s0.end) wait(q_full, 0);
-    issue_s(tile0);
-    if (s1.end) wait(q_full + 8, 0);
-    issue_s(tile1);
-    for (int32_t i = 0; i < pl.n && ok; ++i) {
-      issue_o(tile0, i);
-      issue_o(tile1, i);
-      if (ok && elected()) mma_commit(v_empty + 8 * (i % S::kStages));
-      __syncwarp();
+      if (!ok) break;
+      turn0 += (uint32_t)(to - from);
     }
     if (!ok) {  // products in flight end before the tensor memory is given back
       if (elected()) mma_commit(drain);
@@ -404,51 +556,70 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-  } else if (warp < kMmaWarp) {
-    // ---- rows ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
-    const int t = warp >> 2;
-    if (t * kTileRows < un.rows) {
-      const int tid = threadIdx.x & 127, row = tid;
-      uint8_t* qs = sm + S::kQ + t * S::kTileBytes;
-      constexpr int kChunks = DP / 8;
-      constexpr int kLoads = kTileRows * kChunks / 128, kStep = 128 / kChunks;
-      {
-        const int chunk = tid % kChunks, r0 = tid / kChunks;
-        uint4 x[kLoads];  // all in flight together
-#pragma unroll
-        for (int n = 0; n < kLoads; ++n) {
-          const int r = r0 + n * kStep;
-          x[n] = make_uint4(0, 0, 0, 0);
-          if (t * kTileRows + r < un.rows && chunk * 8 < kv.dim)
-            x[n] = __ldg(reinterpret_cast<const uint4*>(un.query(q, t * kTileRows + r) + chunk * 8));
-        }
-#pragma unroll
-        for (int n = 0; n < kLoads; ++n) {
-          const int r = r0 + n * kStep;
-          *reinterpret_cast<uint4*>(qs + (chunk >> 3) * S::kHalfBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = x[n];
+  } else if (warp >= kQueryWarp) {
+    // ---- queries of one row tile, as soon as the products have used up the last ones ----
+    const int t = warp - kQueryWarp;
+    const uint32_t qs = base + S::kQ + t * S::kTileBytes;
+    constexpr int kChunks = DP / 8;
+    const int chunk = lane % kChunks;
+    uint32_t turn = 0;
+    Item it;
+    while (next_item(it)) {
+      const Plan plan = make_plan(it.un);
+      if (!make_span(it, q, plan, t).active()) continue;
+      ok = __all_sync(0xffffffffu, bar_wait(q_empty + 8 * t, (turn & 1) ^ 1, abort, bt.err, kLongPolls));
+      if (!ok) break;
+      // row lane / kChunks and every kStep-th after it; the query's place moves by a constant, and by another
+      // where the heads of the group start over
+      constexpr int kStep = 32 / kChunks;
+      const int r0 = lane / kChunks, rows = it.un.rows - t * kTileRows;
+      const int32_t dt = it.un.token_of(q, t * kTileRows + r0);
+      int32_t head = it.un.head0 + t * kTileRows + r0 - dt * q.group;
+      const uint16_t* from = it.un.query(q, t * kTileRows + r0) + chunk * 8;
+      const int32_t tokens = kStep / q.group, heads = kStep - tokens * q.group;
+      const int64_t step = tokens * q.token_stride + heads * q.head_stride, over = q.token_stride - q.group * q.head_stride;
+#pragma unroll 8
+      for (int r = r0; r < kTileRows; r += kStep) {
+        const uint32_t n = r < rows && chunk * 8 < kv.dim ? 16 : 0;  // 0: zeros
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     ::"r"(qs + (chunk >> 3) * S::kHalfBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)),
+                     "l"(n ? from : q.q), "r"(n) : "memory");
+        from += step;
+        head += heads;
+        if (head >= q.group) {
+          head -= q.group;
+          from += over;
         }
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_arrive(q_full + 8 * t);
-
-      const Span span = make_span(un, q, plan, t);
-      const int32_t last_row = min(un.rows, (t + 1) * kTileRows) - 1;
-      const int32_t my_row = min(t * kTileRows + row, last_row);  // rows past the last do its work again
-      const int32_t pos = un.position(q, my_row);
-      const uint32_t quadrant = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4) ..
-      const uint32_t s_at = s_col(t) + quadrant, o_at = o_col(t) + quadrant;
-      const float c = q.scale_log2;
+      ++turn;
+    }
+  } else {
+    // ---- rows ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
+    const int t = warp >> 2, row = threadIdx.x & 127;
+    uint8_t* stage = sm + S::kOut + warp * 32 * 128;
+    const uint32_t quadrant = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4) ..
+    const uint32_t s_at = tmem + t * kTileKeys + quadrant, o_at = tmem + 2 * kTileKeys + t * DP + quadrant;
+    const float c = q.scale_log2;
+    uint32_t s_turn = 0, active = 0;
+    Item it;
+    while (next_item(it)) {
+      const Unit& un = it.un;
+      const int32_t row0 = t * kTileRows + (warp & 3) * 32, rows = un.rows - row0;  // the warp's
+      if (t * kTileRows >= un.rows) continue;
+      const Plan plan = make_plan(un);
+      const Span span = make_span(it, q, plan, t);
+      const int32_t pos = un.position(q, min(t * kTileRows + row, un.rows - 1));  // rows past the last do its work again
       float m = -INFINITY, l = 0;
-      int32_t done = 0;
-      bool ok = true;
-      for (int32_t i = plan.at_or_after(span, 0); i < plan.n; i = plan.at_or_after(span, i + 1)) {
+      bool fresh = true;
+      for (int32_t i = span.start(); i < it.end; i = span.at_or_after(i + 1)) {
         const int32_t key0 = plan.key0(i);
-        ok = bar_wait(s_full + 8 * t, done & 1, abort, bt.err);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+        ok = __all_sync(0xffffffffu, bar_wait(s_full + 8 * t, s_turn & 1, abort, bt.err));
+        if (!ok) break;
+        ++s_turn;
         fence_after();
         float x[kTileKeys];
 #pragma unroll
@@ -482,7 +653,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 4; ++e)
             top[e] = fmaxf(fmaxf(top[e], x[j + e]), j + 4 + e < kTileKeys ? x[j + 4 + e] : -INFINITY);
         const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
-        if (done == 0) {
+        if (fresh) {
+          fresh = false;
           m = now;
         } else if (__any_sync(0xffffffffu, now > m + kLag)) {
           // O is at rest: the scores just read were issued after the last product into it
@@ -512,54 +684,92 @@ __global__ void __launch_bounds__(kThreads, 1)
             p[e / 2] = T::pack(p0, p1);
           }
           tmem_store16(s_at + j / 2, p);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_store_wait();
-        fence_before();
-        bar_arrive(p_full + 8 * t);
-        ++done;
-      }
-      // ---- results: through the tile's Q in shared memory, for whole rows ----
-      if (ok && done) ok = bar_wait(o_full + 8 * t, 0, abort, bt.err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok && !done) {  // no row of the tile sees a key
-        for (int r = tid / kChunks; r < kTileRows && t * kTileRows + r < un.rows; r += kStep)
-          if (tid % kChunks * 8 < kv.dim)
-            *reinterpret_cast<uint4*>(un.result(kv, q, t * kTileRows + r) + tid % kChunks * 8) = make_uint4(0, 0, 0, 0);
-      } else if (ok) {
-        fence_after();
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int j = 0; j < DP; j += 32) {
-          float o[32];
-          tmem_load(o_at + j, o);
-          tmem_load_wait();
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int h = 0; h < 4; ++h) w[h] = l == 0.f ? 0 : T::pack(o[e + 2 * h] * inv, o[e + 2 * h + 1] * inv);
-            const int chunk = (j + e) / 8;
-            *reinterpret_cast<uint4*>(qs + row * DP * 2 + ((chunk ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (j == kTileKeys / 2 - 32 || j == kTileKeys - 32) {  // the product of a half can begin
+            tmem_store_wait();
+            fence_before();
+            bar_arrive(p_half + 16 * t + (j == kTileKeys - 32 ? 8 : 0));
           }
         }
-        __syncwarp();  // a warp writes out its own 32 rows
-        const int chunk = lane % kChunks;
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      }
+      if (!ok) break;
+      // ---- results ----
+      const int32_t whole = min(rows, 32);
+      float* slot = scratch + it.slot * kSlotFloats<DP>;
+      if (it.parts > 1 && lane < rows)
+        *reinterpret_cast<float2*>(slot + kBlockRows * DP + (row0 + lane) * 2) = make_float2(m, l);
+      if (fresh) {  // no row of the tile sees a key of the item
+        if (it.parts == 1)
+          for (int r = 0; r < whole; ++r)
+            if (lane * 8 < kv.dim) *reinterpret_cast<uint4*>(un.result(kv, q, row0 + r) + lane * 8) = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      ok = __all_sync(0xffffffffu, bar_wait(o_full + 8 * t, active & 1, abort, bt.err));
+      if (!ok) break;
+      ++active;
+      fence_after();
+      float o[DP];
 #pragma unroll
-        for (int n = 0; n < kChunks; ++n) {
-          const int rr = (warp & 3) * 32 + lane / kChunks + n * (32 / kChunks);
-          if (t * kTileRows + rr < un.rows && chunk * 8 < kv.dim)
-            *reinterpret_cast<uint4*>(un.result(kv, q, t * kTileRows + rr) + chunk * 8) =
-                *reinterpret_cast<const uint4*>(qs + rr * DP * 2 + ((chunk ^ (rr & 7)) << 4));
+      for (int j = 0; j < DP; j += 32) tmem_load(o_at + j, o + j);
+      tmem_load_wait();
+      fence_before();
+      bar_arrive(o_empty + 8 * t);
+      if (it.parts == 1) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int h = 0; h < S::kHalves; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) w[e] = l == 0.f ? 0 : T::pack(o[h * 64 + 2 * e] * inv, o[h * 64 + 2 * e + 1] * inv);
+          store_rows(stage, w, lane, whole, (kv.dim - h * 64) * 2,
+                     [&](int r) { return reinterpret_cast<uint8_t*>(un.result(kv, q, row0 + r) + h * 64); });
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < DP; j += 32)
+          store_rows(stage, reinterpret_cast<const uint32_t*>(o + j), lane, whole, 128,
+                     [&](int r) { return reinterpret_cast<uint8_t*>(slot + (row0 + r) * DP + j); });
       }
     }
   }
+  __syncwarp();
   fence_before();
   __syncthreads();
   if (warp == kMmaWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// Joins the parts of 32 rows of a unit, in order.
+template <class T, int DP>
+__global__ void __launch_bounds__(256)
+    k_kv_prompt_join(View kv, Batch bt, Query q, int32_t most_parts, const float* scratch) {
+  const Unit un = find_unit<kBlockRows>(kv, bt, q, blockIdx.x);
+  const int32_t parts = parts_of(make_plan(un).n, most_parts);
+  if (parts == 1) return;
+  const float* from = scratch + (int64_t)blockIdx.x * most_parts * kSlotFloats<DP>;
+  for (int32_t e = threadIdx.x * 4; e < 32 * DP; e += 256 * 4) {
+    const int32_t row = blockIdx.y * 32 + e / DP, d = e % DP;
+    if (row >= un.rows || d >= kv.dim) continue;
+    float top = -INFINITY;
+    for (int32_t p = 0; p < parts; ++p) top = fmaxf(top, from[p * kSlotFloats<DP> + kBlockRows * DP + row * 2]);
+    float sum = 0, v[4] = {0, 0, 0, 0};
+    for (int32_t p = 0; p < parts; ++p) {
+      const float* slot = from + p * kSlotFloats<DP>;
+      const float2 ml = *reinterpret_cast<const float2*>(slot + kBlockRows * DP + row * 2);
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // nothing seen: no O was stored
+      const float f = exp2_fast(ml.x - top);
+      const float4 x = *reinterpret_cast<const float4*>(slot + (int64_t)row * DP + d);
+      sum += f * ml.y;
+      v[0] += f * x.x;
+      v[1] += f * x.y;
+      v[2] += f * x.z;
+      v[3] += f * x.w;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint2*>(un.result(kv, q, row) + d) =
+        make_uint2(T::pack(v[0] * inv, v[1] * inv), T::pack(v[2] * inv, v[3] * inv));
   }
 }
 
@@ -590,7 +800,8 @@ bool encode(CUtensorMap* map, const View& kv, int dtype, uint16_t* pages, uint32
 }
 
 template <class T, int DP>
-cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, cudaStream_t st) {
+cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& sp, float* scratch,
+                   cudaStream_t st, int* launches) {
   static std::atomic<uint64_t> allowed{0};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -605,21 +816,42 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, c
   if (!encode(&maps.k, kv, dtype, kv.k, box) || !encode(&maps.v, kv, dtype, kv.v, box) ||
       !encode(&maps.v_row, kv, dtype, kv.v, 1))
     return cudaErrorInvalidValue;
-  const int64_t units = prompt_units(kv, bt, q);
-  k_kv_prompt<T, DP><<<(unsigned)units, kThreads, Smem<DP>::kLaunch, st>>>(maps, kv, bt, q, units);
+  k_kv_prompt<T, DP><<<(unsigned)(sp.units * sp.parts), kThreads, Smem<DP>::kLaunch, st>>>(maps, kv, bt, q, sp.units,
+                                                                                           sp.parts, scratch);
+  *launches += 1;
+  if (sp.parts > 1) {
+    k_kv_prompt_join<T, DP><<<dim3((unsigned)sp.units, kBlockRows / 32), 256, 0, st>>>(kv, bt, q, sp.parts, scratch);
+    *launches += 1;
+  }
   return cudaGetLastError();
 }
 
 }  // namespace
 
-int64_t prompt_units(const View& kv, const Batch& bt, const Query& q) {
-  return ((int64_t)q.tokens * q.group / kBlockRows + bt.seqs) * kv.heads;
+uint64_t PromptSplit::scratch_floats() const {
+  return parts > 1 ? (uint64_t)units * parts * kBlockRows * (dim_padded + 2) : 0;
 }
 
-cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int dtype, cudaStream_t st) {
-  const bool small = kv.dim <= 64;
-  if (dtype == 0) return small ? launch<Bf16, 64>(kv, bt, q, dtype, st) : launch<Bf16, 128>(kv, bt, q, dtype, st);
-  return small ? launch<Fp16, 64>(kv, bt, q, dtype, st) : launch<Fp16, 128>(kv, bt, q, dtype, st);
+PromptSplit plan_prompt(const View& kv, const Batch& bt, const Query& q, int sms) {
+  PromptSplit sp;
+  sp.dim_padded = kv.dim <= 64 ? 64 : 128;
+  // at most ceil(rows / 256) units per sequence and key head
+  sp.units = ((int64_t)q.tokens * q.group / kBlockRows + bt.seqs) * kv.heads;
+  int64_t keys = (int64_t)bt.width << kv.page_log;
+  if (q.window) keys = std::min<int64_t>(keys, (int64_t)q.window + q.sinks + 2 * kTileKeys + kBlockRows);
+  const int64_t most = std::min<int64_t>(kMaxParts, keys / (kPartTiles * kTileKeys));
+  sp.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(most, 3 * sms / std::max<int64_t>(1, sp.units)));
+  return sp;
+}
+
+cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& sp,
+                          float* scratch, cudaStream_t st, int* launches) {
+  const bool small = sp.dim_padded == 64;
+  if (dtype == 0)
+    return small ? launch<Bf16, 64>(kv, bt, q, dtype, sp, scratch, st, launches)
+                 : launch<Bf16, 128>(kv, bt, q, dtype, sp, scratch, st, launches);
+  return small ? launch<Fp16, 64>(kv, bt, q, dtype, sp, scratch, st, launches)
+               : launch<Fp16, 128>(kv, bt, q, dtype, sp, scratch, st, launches);
 }
 
 }  // namespace kv

@@ -3,7 +3,7 @@
 // Rows of one (sequence, key head) are packed token by token, the query heads of the group side by
 // side, so that a block's 256 rows (two tiles of 128) share every key it loads.  Per tile of 128 keys:
 //   S = Q K^T            tcgen05.mma 128 x 128 x dim, Q and K from shared memory, S in tensor memory
-//   P = 2^(c S - m)      one thread per row, the row's 128 scores in registers; P in 16 bits over S
+//   P = 2^(c S - m)      one thread per row, the row's 128 scores in registers; P in 16 bits
 //   O += P V             tcgen05.mma 128 x dim x 128, P from tensor memory, V from shared memory
 // m is the row's reference exponent.  It starts as the running maximum and follows it only when the
 // maximum has grown by more than 8: until then weights of up to 2^8 stay far inside both 16-bit types
@@ -48,6 +48,7 @@ constexpr int kIssueRegs = 64, kRowRegs = 216;
 constexpr float kLag = 8.f;           // how far m may stay behind the running maximum
 constexpr uint32_t kPolls = 1u << 20;     // of a wait for the next step before it gives up
 constexpr uint32_t kLongPolls = 1u << 27; // of a wait that may span all keys of other rows
+constexpr int kPolynomial = 6;             // of every 8 weights, the two from this one on go by polynomial
 constexpr int kPartTiles = 8;         // key tiles that a part has at least
 constexpr int kMaxParts = 16;
 
@@ -66,6 +67,12 @@ struct Smem {
   static constexpr int kHalfBytes = kTileKeys * 128;
   static constexpr int kTileBytes = kHalves * kHalfBytes; // Q, K or V tile
   static constexpr int kStages = DP == 128 ? 2 : 4;
+  // Tensor memory columns: S of tile 0 and 1, O of tile 0 and 1, and with 64 dims P of tile 0 and 1.  With 128
+  // there is no room for P but over its own S, so the next S waits until P is used up; with 64 it
+  // follows as soon as S has been read.
+  static constexpr bool kOwnP = DP == 64;
+  static constexpr int kColO = 2 * kTileKeys, kColP = kOwnP ? kColO + 2 * DP : 0;
+  static constexpr int kPitchP = kOwnP ? kTileKeys / 2 : kTileKeys;
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
@@ -73,7 +80,7 @@ struct Smem {
   static constexpr int kAnswer = kOut + 8 * 32 * 128;     // of the launch control, 16 bytes
   static constexpr int kItems = kAnswer + 16;             // two
   static constexpr int kBar = kItems + ((2 * (int)sizeof(Item) + 7) & ~7);
-  static constexpr int kBars = 4 + 4 * kStages + 2 + 4 + 4 + 4 + 2;
+  static constexpr int kBars = 4 + 4 * kStages + 4 + 4 + 4 + 2 + 4 + 2;
   static constexpr int kBytes = kBar + kBars * 8 + 16;    // + tensor memory address, abort flag
   static constexpr int kLaunch = kBytes + 1024;           // slack for the 1024-byte alignment
   static_assert(kLaunch > 115 * 1024 && kLaunch <= 227 * 1024, "one block, and its tensor memory, per SM");
@@ -136,6 +143,12 @@ __device__ __forceinline__ bool elected() {
 }
 // The same value in every lane, known to the compiler as such.
 __device__ __forceinline__ int32_t same(int32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+// The same in one place for the issuing warps, which read their instructions through caches that the rows'
+// long loops keep sweeping: what counts for them is how little code they run.
+__device__ __noinline__ bool bar_wait_shared(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t* err,
+                                             uint32_t polls) {
+  return __all_sync(0xffffffffu, bar_wait(bar, parity, abort, err, polls));
+}
 __device__ __forceinline__ void tma_box(uint32_t to, const CUtensorMap* map, int32_t x, int32_t token, int32_t head,
                                         int32_t page, uint32_t bar) {
   asm volatile(
@@ -151,9 +164,10 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 // Shared-memory operand descriptor, 128-byte swizzle: start address, leading and stride byte offset in
 // 16-byte units, version 1, layout 2.  K-major: rows of 128 bytes, 8-row groups `stride` apart (1024).
 // MN-major: chunks of 64 MN elements `leading` apart, groups of 8 K rows `stride` apart (1024).
-__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t leading) {
-  return (uint64_t)((at >> 4) & 0x3fff) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// The upper word is the same for all; the lower one is what moves.
+constexpr uint32_t kOperandHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t operand(uint32_t at, uint32_t leading) {
+  return ((at >> 4) & 0x3fff) | ((leading >> 4) << 16);
 }
 // Instruction descriptor, kind::f16: D 32-bit float, A and B of type T, A K-major, B K-major or
 // MN-major, M = 128.
@@ -162,15 +176,17 @@ constexpr uint32_t instruction(int n, bool b_mn) {
   const uint32_t type = T::kind == 0 ? 1 : 0;
   return (1u << 4) | (type << 7) | (type << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "n"(kOperandHigh) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "n"(kOperandHigh) : "memory");
 }
 // 32 consecutive columns of this thread's lane.
 __device__ __forceinline__ void tmem_load(uint32_t at, float* x) {
@@ -202,6 +218,60 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- two floats at a time, and weights without the special-function unit --------------------------
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^x for two x <= 8 on the multiply-add pipes: x = n + f, n the nearest integer (Cody and Waite's reduction,
+// by adding and subtracting 1.5 2^23), 2^f by a degree-5 polynomial on [-1/2, 1/2] (Remez exchange on the
+// relative error: 2^-22), times 2^n from the bits.  x below -127 gives 0, NaN gives NaN.
+__device__ __forceinline__ uint64_t exp2_two(uint64_t x) {
+  constexpr float kShift = 12582912.f;
+  float a, b;
+  split(x, a, b);
+  x = two(max_or_nan(a, -127.f), max_or_nan(b, -127.f));
+  const uint64_t n = add2(x, two(kShift, kShift));
+  const uint64_t f = add2(x, mul2(add2(n, two(-kShift, -kShift)), two(-1.f, -1.f)));
+  uint64_t p = two(1.3276472454890609e-3f, 1.3276472454890609e-3f);
+  p = fma2(p, f, two(9.675540961325169e-3f, 9.675540961325169e-3f));
+  p = fma2(p, f, two(5.550713092088699e-2f, 5.550713092088699e-2f));
+  p = fma2(p, f, two(2.4022120237350464e-1f, 2.4022120237350464e-1f));
+  p = fma2(p, f, two(6.931469440460205e-1f, 6.931469440460205e-1f));
+  p = fma2(p, f, two(1.f, 1.f));
+  split(n, a, b);
+  return mul2(p, two(__int_as_float((__float_as_int(a) + 127) << 23), __int_as_float((__float_as_int(b) + 127) << 23)));
+}
+// Bits first .. last of a word whose bits stand for the numbers from `base` on.
+__device__ __forceinline__ uint32_t bits_of(int32_t first, int32_t last, int32_t base) {
+  const int32_t a = max(first - base, 0), b = min(last - base, 31);
+  return a > b ? 0 : (0xffffffffu >> (31 - b)) & (0xffffffffu << a);
+}
 
 // ---- which key tiles the rows and each of their row tiles need -----------------------------------
 // The rows' key tiles are numbered 0 .. n-1: `first` tiles of first tokens, then the window's from tile
@@ -287,7 +357,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t bars = base + S::kBar;
   const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * S::kStages,
                  v_full = k_empty + 8 * S::kStages, v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages,
-                 p_half = s_full + 16, o_full = p_half + 32, o_empty = o_full + 16, item_full = o_empty + 16,
+                 s_read = s_full + 16, p_half = s_read + 16, o_done = p_half + 32, o_empty = o_done + 32,
+                 item_full = o_empty + 16,
                  item_empty = item_full + 16, answered = item_empty + 16, drain = answered + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::kBar + S::kBars * 8);
   volatile uint32_t* abort = tmem_slot + 1;
@@ -300,7 +371,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(s_full + 8 * t, 1);
       bar_init(p_half + 16 * t, kTileRows);
       bar_init(p_half + 16 * t + 8, kTileRows);
-      bar_init(o_full + 8 * t, 1);
+      bar_init(s_read + 8 * t, kTileRows);
+      bar_init(o_done + 16 * t, 1);
+      bar_init(o_done + 16 * t + 8, 1);
       bar_init(o_empty + 8 * t, kTileRows);
       bar_init(item_full + 8 * t, 1);
       bar_init(item_empty + 8 * t, kReaders);
@@ -318,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = *tmem_slot;  // columns: S (and P over it) of tile 0 and 1, O of tile 0 and 1
+  const uint32_t tmem = *tmem_slot;
 
   // the next item, for every warp but the loads'; false: no more (or given up)
   uint32_t item_turn = 0;
@@ -454,98 +527,121 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    // ---- products: S of a tile as soon as its P is used up, so that the two tiles take turns.  The
-    // whole warp runs the loop and one thread issues: descriptors in uniform registers go to the
-    // tensor core at once (from inside a one-thread branch each product took about 100 cycles to issue) ----
+    // ---- products.  The whole warp runs the loop and one thread issues: descriptors in uniform registers
+    // go to the tensor core at once (from inside a one-thread branch each product took about 100 cycles
+    // to issue).  One copy of the code serves both row tiles, which take turns as `x`: unrolled for the two,
+    // the loop spent most of its time fetching instructions. ----
+    struct Tile {
+      uint32_t t = 0;                   // 0, 1
+      Span span;
+      int32_t s_next = 0, p_next = 0;   // next key tile of its S, and of its P
+      uint32_t s_turn = 0, p_turn = 0, active = 0;
+    };
+    Tile x, y;
+    y.t = 1;
     const uint32_t tm = same(tmem);
-    const uint64_t q_desc = operand(base + S::kQ, 16), k_desc = operand(base + S::kK, 16),
+    const uint32_t q_desc = operand(base + S::kQ, 16), k_desc = operand(base + S::kK, 16),
                    v_desc = operand(base + S::kV, S::kHalfBytes);
-    uint32_t turn0 = 0;                   // the ring's turn of the item's first key tile
-    uint32_t p_turn[2] = {0, 0}, active[2] = {0, 0};
+    uint32_t turn0 = 0;  // the ring's turn of the item's first key tile
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      ok = ok && __all_sync(0xffffffffu, bar_wait(bar, parity, abort, bt.err));
+      ok = ok && (bar_try(bar, parity) || bar_wait_shared(bar, parity, abort, bt.err, kPolls));
+      ok = __all_sync(0xffffffffu, ok);
     };
     Item it;
     while (next_item(it)) {
       const Plan plan = make_plan(it.un);
-      Span span[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        span[t] = make_span(it, q, plan, t);
-        span[t].first = same(span[t].first);
-        span[t].begin = same(span[t].begin);
-        span[t].end = same(span[t].end);
-        span[t].from = same(span[t].from);
-        span[t].to = same(span[t].to);
-      }
-      const int32_t from = span[0].from, to = span[0].to;
-      // next key tile of each row tile's S, and of its P; key tiles whose K is given back
-      int32_t s_next[2] = {span[0].start(), span[1].start()}, p_next[2] = {s_next[0], s_next[1]}, released = from;
-      auto issue_s = [&](auto tile) {
-        constexpr int t = decltype(tile)::value;
-        const int32_t i = s_next[t];
-        if (i >= to || !ok) return;
-        const uint32_t turn = turn0 + (uint32_t)(i - from);
-        const int st = turn % S::kStages;
+      x.span = make_span(it, q, plan, 0);
+      y.span = make_span(it, q, plan, 1);
+      const int32_t from = same(x.span.from), to = same(x.span.to);
+      x.s_next = x.p_next = x.span.start();
+      y.s_next = y.p_next = y.span.start();
+      // key tiles whose K and V are given back: as soon as both row tiles are past them, before this warp
+      // waits for later ones
+      int32_t k_free = from, v_free = from;
+      auto turn_of = [&](int32_t i) { return turn0 + (uint32_t)(i - from); };
+      auto give_back = [&](uint32_t empty, int32_t& done, int32_t free) {
+#pragma unroll 1
+        for (; done < free; ++done)
+          if (elected()) mma_commit(empty + 8 * (turn_of(done) % S::kStages));
+        __syncwarp();
+      };
+      auto product_s = [&](bool first) {
+        const int32_t i = x.s_next;
+        const uint32_t turn = turn_of(i), st = turn % S::kStages;
+        if (first) wait(q_full + 8 * x.t, x.active & 1);
+        if (S::kOwnP) wait(s_read + 8 * x.t, (x.s_turn & 1) ^ 1);  // the last S has been read
         wait(k_full + 8 * st, (turn / S::kStages) & 1);
         if (!ok) return;
-        s_next[t] = span[t].at_or_after(i + 1);
-        const int32_t free = min(s_next[0], s_next[1]);
+        x.s_next = x.span.at_or_after(i + 1);
         fence_after();
-        const uint64_t qd = q_desc + t * (S::kTileBytes >> 4), kd = k_desc + st * (S::kTileBytes >> 4);
+        const bool last = x.s_next >= to;
+        const uint32_t d = same(tm + x.t * kTileKeys), full = s_full + 8 * x.t, empty = q_empty + 8 * x.t;
+        uint32_t a = same(q_desc + x.t * (S::kTileBytes >> 4)), b = same(k_desc + st * (S::kTileBytes >> 4));
         if (elected()) {
+#pragma unroll 1
+          for (uint32_t h = 0; h < S::kHalves; ++h) {
 #pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) {
-            constexpr uint32_t kHalf = S::kHalfBytes >> 4;
-            const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 2;
-            mma_ss(tm + t * kTileKeys, qd + off, kd + off, instruction<T>(kTileKeys, false), ks > 0);
+            for (uint32_t ks = 0; ks < 4; ++ks)
+              mma_ss(d, a + 2 * ks, b + 2 * ks, instruction<T>(kTileKeys, false), ks > 0 ? 1 : h);
+            a += S::kHalfBytes >> 4;
+            b += S::kHalfBytes >> 4;
           }
-          mma_commit(s_full + 8 * t);
-          if (s_next[t] >= to) mma_commit(q_empty + 8 * t);
-          for (int32_t r = released; r < free; ++r) mma_commit(k_empty + 8 * ((turn0 + (uint32_t)(r - from)) % S::kStages));
+          mma_commit(full);
+          if (last) mma_commit(empty);
         }
         __syncwarp();
-        released = max(released, free);
+        ++x.s_turn;
+        give_back(k_empty, k_free, min(x.s_next, y.s_next));
       };
-      auto issue_o = [&](auto tile, int32_t i) {
-        constexpr int t = decltype(tile)::value;
-        if (!ok || p_next[t] != i) return;
-        const bool first = i == span[t].start();
-        const uint32_t turn = turn0 + (uint32_t)(i - from);
-        const int st = turn % S::kStages;
+      auto product_o = [&](int32_t i) {
+        const uint32_t turn = turn_of(i), st = turn % S::kStages;
+        const bool first = i == x.span.start();
         wait(v_full + 8 * st, (turn / S::kStages) & 1);
-        if (first) wait(o_empty + 8 * t, (active[t] & 1) ^ 1);
-        p_next[t] = span[t].at_or_after(i + 1);
-        const uint64_t vd = v_desc + st * (S::kTileBytes >> 4);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          wait(p_half + 16 * t + 8 * h, p_turn[t] & 1);
+        if (first) wait(o_empty + 8 * x.t, (x.active & 1) ^ 1);
+        x.p_next = x.span.at_or_after(i + 1);
+        uint32_t add = same(first ? 0 : 1);
+        const uint32_t d = same(tm + S::kColO + x.t * DP), done = o_done + 16 * x.t + 8 * (x.p_turn & 1);
+        uint32_t a = same(tm + S::kColP + x.t * S::kPitchP), b = same(v_desc + st * (S::kTileBytes >> 4));
+#pragma unroll 1
+        for (uint32_t h = 0; h < 2; ++h) {
+          wait(p_half + 16 * x.t + 8 * h, x.p_turn & 1);
           if (!ok) return;
           fence_after();
           if (elected()) {
 #pragma unroll
-            for (int ks = h * (kTileKeys / 32); ks < (h + 1) * (kTileKeys / 32); ++ks)
-              mma_ts(tm + 2 * kTileKeys + t * DP, tm + t * kTileKeys + ks * 8, vd + ks * 128, instruction<T>(DP, true),
-                     ks > 0 || !first);
-            if (h && p_next[t] >= to) mma_commit(o_full + 8 * t);
+            for (int ks = 0; ks < kTileKeys / 32; ++ks)
+              mma_ts(d, a + ks * 8, b + ks * 128, instruction<T>(DP, true), ks > 0 ? 1 : add);
+            if (h) mma_commit(done);
           }
           __syncwarp();
+          add = 1;
+          a += kTileKeys / 4;
+          b += kTileKeys * 4;
         }
-        ++p_turn[t];
-        if (first) ++active[t];
-        issue_s(tile);
+        ++x.p_turn;
+        if (first) ++x.active;
+        give_back(v_empty, v_free, min(x.p_next, y.p_next));
       };
-      const std::integral_constant<int, 0> tile0;
-      const std::integral_constant<int, 1> tile1;
-      if (s_next[0] < to) wait(q_full, active[0] & 1);
-      issue_s(tile0);
-      if (s_next[1] < to) wait(q_full + 8, active[1] & 1);
-      issue_s(tile1);
-      for (int32_t i = from; i < to && ok; ++i) {
-        issue_o(tile0, i);
-        issue_o(tile1, i);
-        if (ok && elected()) mma_commit(v_empty + 8 * ((turn0 + (uint32_t)(i - from)) % S::kStages));
-        __syncwarp();
+      // before the first P: the first S of both; then P of both in turn, and the S that can follow
+#pragma unroll 1
+      for (int32_t i = from - 1; i < to && ok; ++i) {
+#pragma unroll 1
+        for (int n = 0; n < 2 && ok; ++n) {
+          const bool mine = i < from || x.p_next == i;
+          if (!S::kOwnP && mine && i >= from) product_o(i);
+          if (mine && ok && x.s_next < to) product_s(i < from);
+          const Tile other = y;
+          y = x;
+          x = other;
+        }
+        if (S::kOwnP && i >= from)
+#pragma unroll 1
+          for (int n = 0; n < 2 && ok; ++n) {
+            if (x.p_next == i) product_o(i);
+            const Tile other = y;
+            y = x;
+            x = other;
+          }
       }
       if (!ok) break;
       turn0 += (uint32_t)(to - from);
@@ -602,9 +698,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = warp >> 2, row = threadIdx.x & 127;
     uint8_t* stage = sm + S::kOut + warp * 32 * 128;
     const uint32_t quadrant = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4) ..
-    const uint32_t s_at = tmem + t * kTileKeys + quadrant, o_at = tmem + 2 * kTileKeys + t * DP + quadrant;
+    const uint32_t s_at = tmem + t * kTileKeys + quadrant, o_at = tmem + S::kColO + t * DP + quadrant;
+    const uint32_t p_at = tmem + S::kColP + t * S::kPitchP + quadrant;
     const float c = q.scale_log2;
-    uint32_t s_turn = 0, active = 0;
+    uint32_t turn = 0;  // key tiles of the row tile so far
+    // The n-th product into O.  Two barriers in turn: the product n - 2 is done when S of n arrives, so a
+    // parity is that of n's own phase or of the one before.
+    auto added = [&](uint32_t n) { return bar_wait(o_done + 16 * t + 8 * (n & 1), (n >> 1) & 1, abort, bt.err); };
     Item it;
     while (next_item(it)) {
       const Unit& un = it.un;
@@ -617,34 +717,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool fresh = true;
       for (int32_t i = span.start(); i < it.end; i = span.at_or_after(i + 1)) {
         const int32_t key0 = plan.key0(i);
-        ok = __all_sync(0xffffffffu, bar_wait(s_full + 8 * t, s_turn & 1, abort, bt.err));
+        ok = __all_sync(0xffffffffu, bar_wait(s_full + 8 * t, turn & 1, abort, bt.err));
         if (!ok) break;
-        ++s_turn;
         fence_after();
         float x[kTileKeys];
 #pragma unroll
         for (int j = 0; j < kTileKeys; j += 32) tmem_load(s_at + j, x + j);
         tmem_load_wait();
+        if (S::kOwnP) {
+          fence_before();
+          bar_arrive(s_read + 8 * t);
+        }
         const bool cut_end = key0 + kTileKeys - 1 > span.lo;
         const bool cut_begin = q.window && key0 <= span.hi - q.window && key0 + kTileKeys > q.sinks;
-        if (cut_begin) {
-          // keys lo .. hi of the tile are seen, and those below sk
-          const int32_t hi = pos - key0, sk = q.sinks - key0;
-          const uint32_t lo = (uint32_t)max(hi - q.window + 1, 0), n = (uint32_t)max(hi - (int32_t)lo + 1, 0);
-          if (sk > 0) {
+        if (cut_end || cut_begin) {
+          const int32_t hi = pos - key0, lo = q.window ? hi - q.window + 1 : 0, sk = min(q.sinks - 1 - key0, hi);
 #pragma unroll
-            for (int j = 0; j < kTileKeys; ++j)
-              if ((uint32_t)j - lo >= n && (j >= sk || j > hi)) x[j] = -INFINITY;
-          } else {
+          for (int j = 0; j < kTileKeys; j += 32) {
+            const uint32_t seen = bits_of(lo, hi, j) | bits_of(0, sk, j);
 #pragma unroll
-            for (int j = 0; j < kTileKeys; ++j)
-              if ((uint32_t)j - lo >= n) x[j] = -INFINITY;
+            for (int e = 0; e < 32; ++e)
+              if (!(seen >> e & 1)) x[j + e] = -INFINITY;
           }
-        } else if (cut_end) {
-          const int32_t hi = pos - key0;
-#pragma unroll
-          for (int j = 0; j < kTileKeys; ++j)
-            if (j > hi) x[j] = -INFINITY;
         }
         float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
@@ -657,7 +751,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           fresh = false;
           m = now;
         } else if (__any_sync(0xffffffffu, now > m + kLag)) {
-          // O is at rest: the scores just read were issued after the last product into it
+          ok = __all_sync(0xffffffffu, added(turn - 1));  // O is at rest
+          if (!ok) break;
+          fence_after();
           const float f = exp2_fast(m - (now == -INFINITY ? 0.f : now));
           l *= f;
           m = now;
@@ -672,25 +768,44 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0, 0, 0, 0};
+        const uint64_t scale = two(c, c), shift = two(-ref, -ref);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int j = 0; j < kTileKeys; j += 32) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float p0 = exp2_fast(fmaf(x[j + e], c, -ref)), p1 = exp2_fast(fmaf(x[j + e + 1], c, -ref));
-            sum[e & 2] += p0;
-            sum[(e & 2) + 1] += p1;
+            uint64_t y = fma2(two(x[j + e], x[j + e + 1]), scale, shift);
+            float p0, p1;
+            if (e % 8 == kPolynomial) {
+              y = exp2_two(y);
+              split(y, p0, p1);
+            } else {
+              split(y, p0, p1);
+              p0 = exp2_fast(p0);
+              p1 = exp2_fast(p1);
+              y = two(p0, p1);
+            }
+            sum[e / 2 & 1] = add2(sum[e / 2 & 1], y);
             p[e / 2] = T::pack(p0, p1);
           }
-          tmem_store16(s_at + j / 2, p);
+          if (S::kOwnP && j == 0 && turn > 0) {  // the last P has been used up
+            ok = __all_sync(0xffffffffu, added(turn - 1));
+            if (!ok) break;
+            fence_after();
+          }
+          tmem_store16(p_at + j / 2, p);
           if (j == kTileKeys / 2 - 32 || j == kTileKeys - 32) {  // the product of a half can begin
             tmem_store_wait();
             fence_before();
             bar_arrive(p_half + 16 * t + (j == kTileKeys - 32 ? 8 : 0));
           }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (!ok) break;
+        ++turn;
+        float l0, l1;
+        split(add2(sum[0], sum[1]), l0, l1);
+        l += l0 + l1;
       }
       if (!ok) break;
       // ---- results ----
@@ -704,9 +819,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane * 8 < kv.dim) *reinterpret_cast<uint4*>(un.result(kv, q, row0 + r) + lane * 8) = make_uint4(0, 0, 0, 0);
         continue;
       }
-      ok = __all_sync(0xffffffffu, bar_wait(o_full + 8 * t, active & 1, abort, bt.err));
+      ok = __all_sync(0xffffffffu, added(turn - 1));
       if (!ok) break;
-      ++active;
       fence_after();
       float o[DP];
 #pragma unroll
@@ -716,13 +830,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_arrive(o_empty + 8 * t);
       if (it.parts == 1) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t* out = un.results(kv, q);
 #pragma unroll
         for (int h = 0; h < S::kHalves; ++h) {
           uint32_t w[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) w[e] = l == 0.f ? 0 : T::pack(o[h * 64 + 2 * e] * inv, o[h * 64 + 2 * e + 1] * inv);
-          store_rows(stage, w, lane, whole, (kv.dim - h * 64) * 2,
-                     [&](int r) { return reinterpret_cast<uint8_t*>(un.result(kv, q, row0 + r) + h * 64); });
+          store_rows(stage, w, lane, whole, (kv.dim - h * 64) * 2, [&](int r) {
+            return reinterpret_cast<uint8_t*>(out + (int64_t)un.result_row(kv, q, row0 + r) * kv.dim + h * 64);
+          });
         }
       } else {
 #pragma unroll

@@ -26,9 +26,15 @@ struct Unit {
     const int32_t t = token_of(q, r);
     return q.q + (int64_t)(token0 + t) * q.token_stride + (int64_t)(g * q.group + head0 + r - t * q.group) * q.head_stride;
   }
+  // (results: of the first row's token; result_row: dense rows from there to row r's)
+  __device__ __forceinline__ uint16_t* results(const View& kv, const Query& q) const {
+    return q.out + ((int64_t)token0 * kv.heads + g) * q.group * kv.dim;
+  }
+  __device__ __forceinline__ int32_t result_row(const View& kv, const Query& q, int32_t r) const {
+    return token_of(q, r) * (kv.heads - 1) * q.group + head0 + r;
+  }
   __device__ __forceinline__ uint16_t* result(const View& kv, const Query& q, int32_t r) const {
-    const int32_t t = token_of(q, r);
-    return q.out + ((int64_t)(token0 + t) * kv.heads * q.group + g * q.group + head0 + r - t * q.group) * kv.dim;
+    return results(kv, q) + (int64_t)result_row(kv, q, r) * kv.dim;
   }
 };
 

@@ -84,7 +84,7 @@ void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int
     need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
   };
   int launches = 0;
-  if (few_rows(c.batch, c.query, starts)) {
+  if (few_rows(c.batch, c.query, starts) || !prompt_strides(c.view, c.query)) {
     const RowSplit sp = plan_rows(c.view, c.batch, c.query, sm_count(at.device));
     need_scratch(sp.scratch_floats());
     need(sp.blocks16 * sp.parts <= (int64_t)(kMost / sp.cluster), BFVGPU_E_SHAPE, "E_KV_SHAPE");
@@ -109,8 +109,11 @@ uint64_t scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q
     int device = -1;
     internal_params(ctx, &device, nullptr);
     const int sms = sm_count(device);
-    words = ((few_rows(c.batch, c.query, ragged) ? plan_rows(c.view, c.batch, c.query, sms).scratch_floats()
-                                                 : plan_prompt(c.view, c.batch, c.query, sms).scratch_floats()) + 1) / 2;
+    // the row kernel's too where the strides of the queries, not known here, may send them there
+    uint64_t floats = plan_rows(c.view, c.batch, c.query, sms).scratch_floats();
+    if (!few_rows(c.batch, c.query, ragged))
+      floats = std::max(floats, plan_prompt(c.view, c.batch, c.query, sms).scratch_floats());
+    words = (floats + 1) / 2;
   });
   return words;
 }

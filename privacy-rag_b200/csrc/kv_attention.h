@@ -45,6 +45,8 @@ struct PromptSplit {
   int32_t parts = 1, dim_padded = 128;
   uint64_t scratch_floats() const;
 };
+// Whether the queries' strides suit the prompt kernel's loads (no broadcast, no reversed axis).
+bool prompt_strides(const View& kv, const Query& q);
 PromptSplit plan_prompt(const View& kv, const Batch& bt, const Query& q, int sms);
 cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& split,
                           float* scratch, cudaStream_t st, int* launches);

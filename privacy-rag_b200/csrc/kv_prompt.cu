@@ -3,15 +3,16 @@
 // Rows of one (sequence, key head) are packed token by token, the query heads of the group side by
 // side, so that a block's 256 rows (two tiles of 128) share every key it loads.  Per tile of 128 keys:
 //   S = Q K^T            tcgen05.mma 128 x 128 x dim, Q and K from shared memory, S in tensor memory
-//   P = 2^(c S - m)      one thread per row, the row's 128 scores in registers; P in 16 bits
+//   P = 2^(c S - m)      two threads per row, its scores in registers; P in 16 bits
 //   O += P V             tcgen05.mma 128 x dim x 128, P from tensor memory, V from shared memory
 // m is the row's reference exponent.  It starts as the running maximum and follows it only when the
 // maximum has grown by more than 8: until then weights of up to 2^8 stay far inside both 16-bit types
 // and the 32-bit sums, and O need not be rescaled.  The sum of the weights is kept in 32 bits, from
 // the weights before they are rounded to 16 bits for the product.
 //
-// Roles: warps 0-3 and 4-7 hold the rows of tile 0 and 1, warp 8 issues the products, warp 9 the loads of K
-// and V, warps 10 and 11 load the queries of tile 0 and 1.  While one tile's rows are in their
+// Roles: warps 0-7 and 8-15 hold the rows of tile 0 and 1, the first four of each the first 64 keys' scores,
+// warp 16 issues the products, warp 17 the loads of K and V, warps 18 and 19 load the queries of tile 0
+// and 1.  While one tile's rows are in their
 // exponentials, the other tile's products run.  A block is resident on its SM for the whole launch and
 // takes over the blocks that have not started yet (cluster launch control), so that the loads of the
 // next rows and the results of the last ones run under the products in between.
@@ -39,23 +40,50 @@ namespace {
 constexpr int kTileRows = 128;
 constexpr int kBlockRows = 2 * kTileRows;
 constexpr int kTileKeys = 128;
-constexpr int kThreads = 384;         // two warpgroups of rows, one of the issuing warps
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kQueryWarp = 10;
-constexpr int kReaders = 11;          // warps that are told of the next rows: all but the loads' own
-// Registers a thread: launched with 168 (384 x 168 of the SM's 65536); the issuing warpgroup keeps 64 and
-// the rows take 216: 128 x 64 + 256 x 216 <= 384 x 168.
-constexpr int kIssueRegs = 64, kRowRegs = 216;
+// Two warpgroups per row tile (each thread has half a row's scores: with one, the time of a row's
+// exponentials and of the products that wait for them added up, and two warps per scheduler could not
+// fill it), and one of the issuing warps.
+constexpr int kThreads = 640;
+constexpr int kScoreWarp = 16, kValueWarp = 17, kLoadWarp = 18, kQueryWarp = 19;
+constexpr int kReaders = 19;          // warps that are told of the next rows: all but the loads' own
+// Registers a thread: launched with 96 (640 x 96 of the SM's 65536); the issuing warpgroup keeps 56 and the
+// rows take 104: 128 x 56 + 512 x 104 <= 640 x 96.
+constexpr int kIssueRegs = 56, kRowRegs = 104;
+constexpr int kHalfKeys = kTileKeys / 2;  // of a thread
 constexpr float kLag = 8.f;           // how far m may stay behind the running maximum
 constexpr uint32_t kPolls = 1u << 20;     // of a wait for the next step before it gives up
 constexpr uint32_t kLongPolls = 1u << 27; // of a wait that may span all keys of other rows
-constexpr int kPolynomial = 6;             // of every 8 weights, the two from this one on go by polynomial
 constexpr int kPartTiles = 8;         // key tiles that a part has at least
 constexpr int kMaxParts = 16;
+
+// A row tile's part of an item.
+struct Span {
+  int32_t lo = 0, hi = -1;  // positions of the rows (hi < 0: no row sees a key)
+  // the key tiles that it needs: [from, first) and [begin, end), none from `to` on
+  int32_t first = 0, begin = 0, end = 0, from = 0, to = 0;
+  __device__ __forceinline__ int32_t at_or_after(int32_t i) const {  // to: none
+    i = i < first ? i : max(i, begin);
+    return i < end ? i : to;
+  }
+  __device__ __forceinline__ bool needs(int32_t i) const { return i < end && (i < first || i >= begin); }
+  __device__ __forceinline__ int32_t start() const { return at_or_after(from); }
+  __device__ __forceinline__ bool active() const { return start() < to; }
+};
+
+// Key tiles of the rows, numbered 0 .. n-1: `first` tiles of first tokens, then the window's from tile `from`
+// on.  A row tile may take part in a tile that it sees nothing of; every tile is needed by one row tile.
+struct Plan {
+  int32_t n = 0, first = 0, from = 0;
+  int32_t end = 0;                // keys the rows see: [0, sinks) and [begin, end)
+  __device__ __forceinline__ int32_t key0(int32_t i) const { return (i < first ? i : i - first + from) * kTileKeys; }
+};
 
 // What the loading warp tells the others: the rows, and which of their key tiles.
 struct Item {
   Unit un;
+  Plan plan;
   int32_t begin = 0, end = 0;  // key tiles
+  Span span[2];
   int32_t parts = 1;           // of the unit; 1: the rows' results are final
   int32_t slot = 0;            // of the partial results
   int32_t more = 0;            // 0: no further rows
@@ -67,26 +95,28 @@ struct Smem {
   static constexpr int kHalfBytes = kTileKeys * 128;
   static constexpr int kTileBytes = kHalves * kHalfBytes; // Q, K or V tile
   static constexpr int kStages = DP == 128 ? 2 : 4;
-  // Tensor memory columns: S of tile 0 and 1, O of tile 0 and 1, and with 64 dims P of tile 0 and 1.  With 128
-  // there is no room for P but over its own S, so the next S waits until P is used up; with 64 it
-  // follows as soon as S has been read.
-  static constexpr bool kOwnP = DP == 64;
-  static constexpr int kColO = 2 * kTileKeys, kColP = kOwnP ? kColO + 2 * DP : 0;
-  static constexpr int kPitchP = kOwnP ? kTileKeys / 2 : kTileKeys;
+  // Tensor memory columns: S, P of tile 0 and 1, O of tile 0 and 1.  With 64 dims there is room for an S of each
+  // row tile; with 128 they share one, which is free again as soon as the rows have read it.
+  static constexpr bool kTwoS = DP == 64;
+  static constexpr int kColP = kTwoS ? 2 * kTileKeys : kTileKeys, kColO = kColP + kTileKeys;
+  static_assert(kColO + 2 * DP <= 512, "tensor memory");
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
-  static constexpr int kOut = kV + kStages * kTileBytes;  // 128 bytes of each row, per warp
-  static constexpr int kAnswer = kOut + 8 * 32 * 128;     // of the launch control, 16 bytes
+  static constexpr int kOut = kV + kStages * kTileBytes;  // 32 bytes of each row, per warp
+  static constexpr int kMax = kOut + 16 * 32 * 32;        // two turns: a number of each thread for the row's other
+  static constexpr int kAnswer = kMax + 2 * 512 * 4;      // of the launch control, 16 bytes
   static constexpr int kItems = kAnswer + 16;             // two
   static constexpr int kBar = kItems + ((2 * (int)sizeof(Item) + 7) & ~7);
-  static constexpr int kBars = 4 + 4 * kStages + 4 + 4 + 4 + 2 + 4 + 2;
+  static constexpr int kBars = 4 + 4 * kStages + 2 + 2 + 4 + 4 + 2 + 2 + 4 + 1 + 2;
   static constexpr int kBytes = kBar + kBars * 8 + 16;    // + tensor memory address, abort flag
   static constexpr int kLaunch = kBytes + 1024;           // slack for the 1024-byte alignment
   static_assert(kLaunch > 115 * 1024 && kLaunch <= 227 * 1024, "one block, and its tensor memory, per SM");
 };
 
 struct Maps {
+  CUtensorMap q;         // 64 dims of a token's heads that share a key head; of 128 rows where they fill them
+  CUtensorMap q_row;     // 64 dims of one row
   CUtensorMap k, v;      // one page (or 128 tokens of it) x 64 dims
   CUtensorMap v_row;     // one token x 64 dims
 };
@@ -143,17 +173,17 @@ __device__ __forceinline__ bool elected() {
 }
 // The same value in every lane, known to the compiler as such.
 __device__ __forceinline__ int32_t same(int32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-// The same in one place for the issuing warps, which read their instructions through caches that the rows'
-// long loops keep sweeping: what counts for them is how little code they run.
-__device__ __noinline__ bool bar_wait_shared(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t* err,
-                                             uint32_t polls) {
-  return __all_sync(0xffffffffu, bar_wait(bar, parity, abort, err, polls));
-}
 __device__ __forceinline__ void tma_box(uint32_t to, const CUtensorMap* map, int32_t x, int32_t token, int32_t head,
                                         int32_t page, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
       ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(token), "r"(head), "r"(page), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_rows(uint32_t to, const CUtensorMap* map, int32_t x, int32_t head, int32_t token,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -200,6 +230,15 @@ __device__ __forceinline__ void tmem_load(uint32_t at, float* x) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(at));
 }
+// 16 columns.
+__device__ __forceinline__ void tmem_load16(uint32_t at, float* x) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(x);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
 __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_store32(uint32_t at, const float* x) {
   const uint32_t* r = reinterpret_cast<const uint32_t*>(x);
@@ -219,7 +258,7 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// ---- two floats at a time, and weights without the special-function unit --------------------------
+// ---- two floats at a time --------------------------------------------------------------------------
 __device__ __forceinline__ uint64_t two(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -238,35 +277,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-// 2^x for two x <= 8 on the multiply-add pipes: x = n + f, n the nearest integer (Cody and Waite's reduction,
-// by adding and subtracting 1.5 2^23), 2^f by a degree-5 polynomial on [-1/2, 1/2] (Remez exchange on the
-// relative error: 2^-22), times 2^n from the bits.  x below -127 gives 0, NaN gives NaN.
-__device__ __forceinline__ uint64_t exp2_two(uint64_t x) {
-  constexpr float kShift = 12582912.f;
-  float a, b;
-  split(x, a, b);
-  x = two(max_or_nan(a, -127.f), max_or_nan(b, -127.f));
-  const uint64_t n = add2(x, two(kShift, kShift));
-  const uint64_t f = add2(x, mul2(add2(n, two(-kShift, -kShift)), two(-1.f, -1.f)));
-  uint64_t p = two(1.3276472454890609e-3f, 1.3276472454890609e-3f);
-  p = fma2(p, f, two(9.675540961325169e-3f, 9.675540961325169e-3f));
-  p = fma2(p, f, two(5.550713092088699e-2f, 5.550713092088699e-2f));
-  p = fma2(p, f, two(2.4022120237350464e-1f, 2.4022120237350464e-1f));
-  p = fma2(p, f, two(6.931469440460205e-1f, 6.931469440460205e-1f));
-  p = fma2(p, f, two(1.f, 1.f));
-  split(n, a, b);
-  return mul2(p, two(__int_as_float((__float_as_int(a) + 127) << 23), __int_as_float((__float_as_int(b) + 127) << 23)));
-}
 // Bits first .. last of a word whose bits stand for the numbers from `base` on.
 __device__ __forceinline__ uint32_t bits_of(int32_t first, int32_t last, int32_t base) {
   const int32_t a = max(first - base, 0), b = min(last - base, 31);
@@ -274,14 +284,6 @@ __device__ __forceinline__ uint32_t bits_of(int32_t first, int32_t last, int32_t
 }
 
 // ---- which key tiles the rows and each of their row tiles need -----------------------------------
-// The rows' key tiles are numbered 0 .. n-1: `first` tiles of first tokens, then the window's from tile
-// `from` on.  A row tile needs [0, first) and [begin, end).  It may take part in a tile that it sees
-// nothing of; every tile is needed by one row tile.
-struct Plan {
-  int32_t n = 0, first = 0, from = 0;
-  int32_t end = 0;                // keys the rows see: [0, sinks) and [begin, end)
-  __device__ __forceinline__ int32_t key0(int32_t i) const { return (i < first ? i : i - first + from) * kTileKeys; }
-};
 __device__ __forceinline__ Plan make_plan(const Unit& un) {
   Plan p;
   if (un.n > 0) {
@@ -292,19 +294,9 @@ __device__ __forceinline__ Plan make_plan(const Unit& un) {
   }
   return p;
 }
-struct Span {
-  int32_t lo = 0, hi = -1;  // positions of the rows (hi < 0: no row sees a key)
-  // the item's key tiles that the row tile needs: [from, first) and [begin, end), in the item's [from, to)
-  int32_t first = 0, begin = 0, end = 0, from = 0, to = 0;
-  __device__ __forceinline__ int32_t at_or_after(int32_t i) const {  // to: none
-    i = i < first ? i : max(i, begin);
-    return i < end ? i : to;
-  }
-  __device__ __forceinline__ int32_t start() const { return at_or_after(from); }
-  __device__ __forceinline__ bool active() const { return start() < to; }
-};
-__device__ __forceinline__ Span make_span(const Item& it, const Query& q, const Plan& p, int t) {
+__device__ __forceinline__ Span make_span(const Item& it, const Query& q, int t) {
   const Unit& un = it.un;
+  const Plan& p = it.plan;
   Span s;
   s.from = it.begin;
   s.to = it.end;
@@ -327,20 +319,19 @@ __device__ __forceinline__ int32_t parts_of(int32_t n, int32_t most) {
 template <int DP>
 constexpr int64_t kSlotFloats = (int64_t)kBlockRows * (DP + 2);
 
-// 128 bytes of each of the warp's 32 rows: every lane has its own row's; stored by whole rows.
+// 32 bytes of each of the warp's 32 rows: every lane has its own row's; stored by whole sectors.
 template <class To>
-__device__ __forceinline__ void store_rows(uint8_t* stage, const uint32_t* w, int lane, int rows, int bytes, To to) {
-#pragma unroll
-  for (int c = 0; c < 8; ++c)
-    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-        make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+__device__ __forceinline__ void store_rows(uint8_t* stage, uint4 a, uint4 b, int lane, int rows, int bytes, To to) {
+  const int turn = (lane >> 2 & 1) << 4;
+  *reinterpret_cast<uint4*>(stage + lane * 32 + turn) = a;
+  *reinterpret_cast<uint4*>(stage + lane * 32 + (16 - turn)) = b;
   __syncwarp();
-  const int c = lane & 7;
+  const int c = lane & 1;
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const int r = n * 4 + (lane >> 3);
+  for (int n = 0; n < 2; ++n) {
+    const int r = n * 16 + (lane >> 1);
     if (r < rows && c * 16 < bytes)
-      *reinterpret_cast<uint4*>(to(r) + c * 16) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+      *reinterpret_cast<uint4*>(to(r) + c * 16) = *reinterpret_cast<const uint4*>(stage + r * 32 + ((c ^ (r >> 2 & 1)) << 4));
   }
   __syncwarp();
 }
@@ -348,7 +339,7 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, const uint32_t* w, in
 template <class T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     k_kv_prompt(const __grid_constant__ Maps maps, View kv, Batch bt, Query q, int64_t units, int32_t most_parts,
-                float* scratch) {
+                float* scratch, uint32_t q_tokens) {
   using S = Smem<DP>;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
@@ -358,33 +349,34 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * S::kStages,
                  v_full = k_empty + 8 * S::kStages, v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages,
                  s_read = s_full + 16, p_half = s_read + 16, o_done = p_half + 32, o_empty = o_done + 32,
-                 item_full = o_empty + 16,
-                 item_empty = item_full + 16, answered = item_empty + 16, drain = answered + 8;
+                 met = o_empty + 16, item_full = met + 16,
+                 item_empty = item_full + 16, drain = item_empty + 16, answered = drain + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::kBar + S::kBars * 8);
   volatile uint32_t* abort = tmem_slot + 1;
   Item* items = reinterpret_cast<Item*>(sm + S::kItems);
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
-      bar_init(q_full + 8 * t, 32);
+      bar_init(q_full + 8 * t, 1);
       bar_init(q_empty + 8 * t, 1);
       bar_init(s_full + 8 * t, 1);
-      bar_init(p_half + 16 * t, kTileRows);
-      bar_init(p_half + 16 * t + 8, kTileRows);
-      bar_init(s_read + 8 * t, kTileRows);
-      bar_init(o_done + 16 * t, 1);
-      bar_init(o_done + 16 * t + 8, 1);
-      bar_init(o_empty + 8 * t, kTileRows);
+      bar_init(s_read + 8 * t, 2 * kTileRows);
+      for (int b = 0; b < 2; ++b) {
+        bar_init(p_half + 16 * t + 8 * b, kTileRows);
+        bar_init(o_done + 16 * t + 8 * b, 1);
+      }
+      bar_init(o_empty + 8 * t, 2 * kTileRows);
+      bar_init(met + 8 * t, 2 * kTileRows);
       bar_init(item_full + 8 * t, 1);
       bar_init(item_empty + 8 * t, kReaders);
+      bar_init(drain + 8 * t, 1);
     }
     for (int i = 0; i < 4 * S::kStages; ++i) bar_init(k_full + 8 * i, 1);
     bar_init(answered, 1);
-    bar_init(drain, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -393,21 +385,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // the next item, for every warp but the loads'; false: no more (or given up)
+  // the next item, for every warp but the loads'; false: no more (or given up).  It stays where it is until
+  // the warp gives its place back.
   uint32_t item_turn = 0;
   bool ok = true;
-  auto next_item = [&](Item& it) {
+  auto next_item = [&] {
     const uint32_t at = item_turn & 1;
     ok = __all_sync(0xffffffffu, bar_wait(item_full + 8 * at, (item_turn >> 1) & 1, abort, bt.err, kLongPolls));
-    if (!ok) return false;
-    it = items[at];
+    return ok && items[at].more != 0;
+  };
+  auto end_item = [&] {
     __syncwarp();
-    if (lane == 0) bar_arrive(item_empty + 8 * at);
+    if (lane == 0) bar_arrive(item_empty + 8 * (item_turn & 1));
     ++item_turn;
-    return it.more != 0;
   };
 
-  if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+  if (warp >= kScoreWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
   if (warp == kLoadWarp) {
     // ---- items, and loads of K and V: lane j has the j-th page of a key tile ----
     const int32_t page_tokens = 1 << kv.page_log, box = min(page_tokens, kTileKeys), boxes = kTileKeys / box;
@@ -442,10 +435,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item it;
       it.un = find_unit<kBlockRows>(kv, bt, q, u);
       const Unit& un = it.un;
-      const Plan plan = make_plan(un);
+      const Plan& plan = it.plan;
+      it.plan = make_plan(un);
       it.parts = parts_of(plan.n, most_parts);
       it.begin = (int32_t)((int64_t)plan.n * part / it.parts);
       it.end = (int32_t)((int64_t)plan.n * (part + 1) / it.parts);
+      it.span[0] = make_span(it, q, 0);
+      it.span[1] = make_span(it, q, 1);
       it.slot = (int32_t)(u * most_parts + part);
       it.more = 1;
       if (un.rows > 0 && part < it.parts) {
@@ -526,214 +522,212 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t n = 0; asked && n < kPolls && !bar_try(answered, answers & 1); ++n) {
       }
     }
-  } else if (warp == kMmaWarp) {
-    // ---- products.  The whole warp runs the loop and one thread issues: descriptors in uniform registers
-    // go to the tensor core at once (from inside a one-thread branch each product took about 100 cycles
-    // to issue).  One copy of the code serves both row tiles, which take turns as `x`: unrolled for the two,
-    // the loop spent most of its time fetching instructions. ----
-    struct Tile {
-      uint32_t t = 0;                   // 0, 1
-      Span span;
-      int32_t s_next = 0, p_next = 0;   // next key tile of its S, and of its P
-      uint32_t s_turn = 0, p_turn = 0, active = 0;
-    };
-    Tile x, y;
-    y.t = 1;
+  } else if (warp == kScoreWarp) {
+    // ---- S of both row tiles in turn, ahead of the rows.  The whole warp runs the loop and one thread
+    // issues: descriptors in uniform registers go to the tensor core at once (from inside a one-thread
+    // branch each product took about 100 cycles to issue).  Beside the rows' warps every instruction here
+    // takes many cycles, so the rows must not have to wait for them: S of the next key tile follows as
+    // soon as its columns have been read, not when this tile's weights are used up. ----
     const uint32_t tm = same(tmem);
-    const uint32_t q_desc = operand(base + S::kQ, 16), k_desc = operand(base + S::kK, 16),
-                   v_desc = operand(base + S::kV, S::kHalfBytes);
-    uint32_t turn0 = 0;  // the ring's turn of the item's first key tile
+    const uint32_t q_desc = same(operand(base + S::kQ, 16)), k_desc = operand(base + S::kK, 16);
+    uint32_t turn = 0, q_turn = 0;                 // key tiles so far; bit t: turns of tile t's queries
+    uint32_t read_turn = 0x3, last = 0;            // bit t: parity of the last phase of s_read[t]; tile of the last S
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      ok = ok && (bar_try(bar, parity) || bar_wait_shared(bar, parity, abort, bt.err, kPolls));
-      ok = __all_sync(0xffffffffu, ok);
+      ok = ok && __all_sync(0xffffffffu, bar_wait(bar, parity, abort, bt.err));
     };
-    Item it;
-    while (next_item(it)) {
-      const Plan plan = make_plan(it.un);
-      x.span = make_span(it, q, plan, 0);
-      y.span = make_span(it, q, plan, 1);
-      const int32_t from = same(x.span.from), to = same(x.span.to);
-      x.s_next = x.p_next = x.span.start();
-      y.s_next = y.p_next = y.span.start();
-      // key tiles whose K and V are given back: as soon as both row tiles are past them, before this warp
-      // waits for later ones
-      int32_t k_free = from, v_free = from;
-      auto turn_of = [&](int32_t i) { return turn0 + (uint32_t)(i - from); };
-      auto give_back = [&](uint32_t empty, int32_t& done, int32_t free) {
+    while (next_item()) {
+      const Item& it = items[item_turn & 1];
+      const int32_t to = same(it.end);
 #pragma unroll 1
-        for (; done < free; ++done)
-          if (elected()) mma_commit(empty + 8 * (turn_of(done) % S::kStages));
-        __syncwarp();
-      };
-      auto product_s = [&](bool first) {
-        const int32_t i = x.s_next;
-        const uint32_t turn = turn_of(i), st = turn % S::kStages;
-        if (first) wait(q_full + 8 * x.t, x.active & 1);
-        if (S::kOwnP) wait(s_read + 8 * x.t, (x.s_turn & 1) ^ 1);  // the last S has been read
+      for (int32_t i = same(it.begin); i < to && ok; ++i, ++turn) {
+        const uint32_t st = turn % S::kStages;
         wait(k_full + 8 * st, (turn / S::kStages) & 1);
-        if (!ok) return;
-        x.s_next = x.span.at_or_after(i + 1);
-        fence_after();
-        const bool last = x.s_next >= to;
-        const uint32_t d = same(tm + x.t * kTileKeys), full = s_full + 8 * x.t, empty = q_empty + 8 * x.t;
-        uint32_t a = same(q_desc + x.t * (S::kTileBytes >> 4)), b = same(k_desc + st * (S::kTileBytes >> 4));
-        if (elected()) {
+        const uint32_t b = same(k_desc + st * (S::kTileBytes >> 4));
 #pragma unroll 1
-          for (uint32_t h = 0; h < S::kHalves; ++h) {
-#pragma unroll
-            for (uint32_t ks = 0; ks < 4; ++ks)
-              mma_ss(d, a + 2 * ks, b + 2 * ks, instruction<T>(kTileKeys, false), ks > 0 ? 1 : h);
-            a += S::kHalfBytes >> 4;
-            b += S::kHalfBytes >> 4;
-          }
-          mma_commit(full);
-          if (last) mma_commit(empty);
-        }
-        __syncwarp();
-        ++x.s_turn;
-        give_back(k_empty, k_free, min(x.s_next, y.s_next));
-      };
-      auto product_o = [&](int32_t i) {
-        const uint32_t turn = turn_of(i), st = turn % S::kStages;
-        const bool first = i == x.span.start();
-        wait(v_full + 8 * st, (turn / S::kStages) & 1);
-        if (first) wait(o_empty + 8 * x.t, (x.active & 1) ^ 1);
-        x.p_next = x.span.at_or_after(i + 1);
-        uint32_t add = same(first ? 0 : 1);
-        const uint32_t d = same(tm + S::kColO + x.t * DP), done = o_done + 16 * x.t + 8 * (x.p_turn & 1);
-        uint32_t a = same(tm + S::kColP + x.t * S::kPitchP), b = same(v_desc + st * (S::kTileBytes >> 4));
-#pragma unroll 1
-        for (uint32_t h = 0; h < 2; ++h) {
-          wait(p_half + 16 * x.t + 8 * h, x.p_turn & 1);
-          if (!ok) return;
+        for (uint32_t t = 0; t < 2; ++t) {
+          const Span& span = it.span[t];
+          if (!same(span.needs(i))) continue;
+          if (same(i == span.start())) wait(q_full + 8 * t, q_turn >> t & 1);
+          const uint32_t of = S::kTwoS ? t : last;   // whose S was there before
+          wait(s_read + 8 * of, read_turn >> of & 1);
+          if (!ok) break;
+          last = t;
+          read_turn ^= 1u << t;
+          const bool end = same(span.at_or_after(i + 1) >= to);
+          if (end) q_turn ^= 1u << t;
+          const uint32_t a = same(q_desc + t * (S::kTileBytes >> 4)), d = same(tm + (S::kTwoS ? t * kTileKeys : 0));
           fence_after();
           if (elected()) {
 #pragma unroll
-            for (int ks = 0; ks < kTileKeys / 32; ++ks)
-              mma_ts(d, a + ks * 8, b + ks * 128, instruction<T>(DP, true), ks > 0 ? 1 : add);
-            if (h) mma_commit(done);
+            for (uint32_t ks = 0; ks < DP / 16; ++ks) {
+              const uint32_t off = (ks >> 2) * (S::kHalfBytes >> 4) + (ks & 3) * 2;
+              mma_ss(d, a + off, b + off, instruction<T>(kTileKeys, false), ks > 0);
+            }
+            mma_commit(s_full + 8 * t);
+            if (end) mma_commit(q_empty + 8 * t);
           }
           __syncwarp();
-          add = 1;
-          a += kTileKeys / 4;
-          b += kTileKeys * 4;
         }
-        ++x.p_turn;
-        if (first) ++x.active;
-        give_back(v_empty, v_free, min(x.p_next, y.p_next));
-      };
-      // before the first P: the first S of both; then P of both in turn, and the S that can follow
-#pragma unroll 1
-      for (int32_t i = from - 1; i < to && ok; ++i) {
-#pragma unroll 1
-        for (int n = 0; n < 2 && ok; ++n) {
-          const bool mine = i < from || x.p_next == i;
-          if (!S::kOwnP && mine && i >= from) product_o(i);
-          if (mine && ok && x.s_next < to) product_s(i < from);
-          const Tile other = y;
-          y = x;
-          x = other;
-        }
-        if (S::kOwnP && i >= from)
-#pragma unroll 1
-          for (int n = 0; n < 2 && ok; ++n) {
-            if (x.p_next == i) product_o(i);
-            const Tile other = y;
-            y = x;
-            x = other;
-          }
+        if (ok && elected()) mma_commit(k_empty + 8 * st);
+        __syncwarp();
       }
       if (!ok) break;
-      turn0 += (uint32_t)(to - from);
+      end_item();
     }
     if (!ok) {  // products in flight end before the tensor memory is given back
       if (elected()) mma_commit(drain);
       for (uint32_t n = 0; n < kPolls && !bar_try(drain, 0); ++n) {
       }
-      __syncwarp();
     }
-  } else if (warp >= kQueryWarp) {
-    // ---- queries of one row tile, as soon as the products have used up the last ones ----
-    const int t = warp - kQueryWarp;
-    const uint32_t qs = base + S::kQ + t * S::kTileBytes;
-    constexpr int kChunks = DP / 8;
-    const int chunk = lane % kChunks;
-    uint32_t turn = 0;
-    Item it;
-    while (next_item(it)) {
-      const Plan plan = make_plan(it.un);
-      if (!make_span(it, q, plan, t).active()) continue;
-      ok = __all_sync(0xffffffffu, bar_wait(q_empty + 8 * t, (turn & 1) ^ 1, abort, bt.err, kLongPolls));
-      if (!ok) break;
-      // row lane / kChunks and every kStep-th after it; the query's place moves by a constant, and by another
-      // where the heads of the group start over
-      constexpr int kStep = 32 / kChunks;
-      const int r0 = lane / kChunks, rows = it.un.rows - t * kTileRows;
-      const int32_t dt = it.un.token_of(q, t * kTileRows + r0);
-      int32_t head = it.un.head0 + t * kTileRows + r0 - dt * q.group;
-      const uint16_t* from = it.un.query(q, t * kTileRows + r0) + chunk * 8;
-      const int32_t tokens = kStep / q.group, heads = kStep - tokens * q.group;
-      const int64_t step = tokens * q.token_stride + heads * q.head_stride, over = q.token_stride - q.group * q.head_stride;
-#pragma unroll 8
-      for (int r = r0; r < kTileRows; r += kStep) {
-        const uint32_t n = r < rows && chunk * 8 < kv.dim ? 16 : 0;  // 0: zeros
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                     ::"r"(qs + (chunk >> 3) * S::kHalfBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)),
-                     "l"(n ? from : q.q), "r"(n) : "memory");
-        from += step;
-        head += heads;
-        if (head >= q.group) {
-          head -= q.group;
-          from += over;
+    __syncwarp();
+  } else if (warp == kValueWarp) {
+    // ---- O += P V of both row tiles in turn ----
+    const uint32_t tm = same(tmem), v_desc = operand(base + S::kV, S::kHalfBytes);
+    uint32_t turn = 0, p_turn[2] = {0, 0}, active = 0;  // bit t of active: items of tile t
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      ok = ok && __all_sync(0xffffffffu, bar_wait(bar, parity, abort, bt.err));
+    };
+    while (next_item()) {
+      const Item& it = items[item_turn & 1];
+      const int32_t to = same(it.end);
+#pragma unroll 1
+      for (int32_t i = same(it.begin); i < to && ok; ++i, ++turn) {
+        const uint32_t st = turn % S::kStages;
+        wait(v_full + 8 * st, (turn / S::kStages) & 1);
+        const uint32_t b = same(v_desc + st * (S::kTileBytes >> 4));
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t) {
+          const Span& span = it.span[t];
+          if (!same(span.needs(i))) continue;
+          const uint32_t add = same(i == span.start() ? 0 : 1);
+          if (!add) {
+            wait(o_empty + 8 * t, (active >> t & 1) ^ 1);  // the last O has been read
+            active ^= 1u << t;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            wait(p_half + 16 * t + 8 * h, p_turn[t] & 1);
+            if (!ok) break;
+            fence_after();
+            if (elected()) {
+#pragma unroll
+              for (int ks = h * (kTileKeys / 32); ks < (h + 1) * (kTileKeys / 32); ++ks)
+                mma_ts(tm + S::kColO + t * DP, tm + S::kColP + t * (kTileKeys / 2) + ks * 8, b + ks * 128,
+                       instruction<T>(DP, true), ks > 0 ? 1 : add);
+              if (h) mma_commit(o_done + 16 * t + 8 * (p_turn[t] & 1));
+            }
+            __syncwarp();
+          }
+          ++p_turn[t];
         }
+        if (ok && elected()) mma_commit(v_empty + 8 * st);
+        __syncwarp();
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(q_full + 8 * t);
-      ++turn;
+      if (!ok) break;
+      end_item();
+    }
+    if (!ok) {
+      if (elected()) mma_commit(drain + 8);
+      for (uint32_t n = 0; n < kPolls && !bar_try(drain + 8, 0); ++n) {
+      }
+    }
+    __syncwarp();
+  } else if (warp == kQueryWarp) {
+    // ---- queries, as soon as the products have used up the last ones: one box where the heads of whole
+    // tokens fill the 128 rows (q_tokens of them), else a box per token, and a row at a time what is
+    // cut off at either end ----
+    uint32_t turn = 0;  // bit t: of tile t
+    for (; next_item(); end_item()) {
+      const Item& it = items[item_turn & 1];
+      const Unit& un = it.un;
+#pragma unroll 1
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (!it.span[t].active()) continue;
+        ok = __all_sync(0xffffffffu, bar_wait(q_empty + 8 * t, (turn >> t & 1) ^ 1, abort, bt.err, kLongPolls));
+        if (!ok) break;
+        turn ^= 1u << t;
+        const uint32_t to = base + S::kQ + t * S::kTileBytes, bar = q_full + 8 * t;
+        const int32_t rows = q_tokens ? kTileRows : min(un.rows - t * kTileRows, kTileRows);
+        if (lane == 0) bar_expect(bar, rows * 128 * S::kHalves);
+        __syncwarp();
+        const int32_t token0 = un.token_of(q, t * kTileRows);
+        if (q_tokens) {
+          if (lane < S::kHalves)
+            tma_rows(to + lane * S::kHalfBytes, &maps.q, lane * 64, un.g * q.group, un.token0 + token0, bar);
+          continue;
+        }
+        for (int32_t k = token0 + lane;; k += 32) {
+          const int32_t r0 = k * q.group - un.head0 - t * kTileRows, r1 = r0 + q.group;  // rows of token k
+          if (r0 >= rows) break;
+          const bool whole = r0 >= 0 && r1 <= rows;
+          for (int32_t r = max(r0, 0); r < min(r1, rows); r += whole ? q.group : 1)
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)
+              tma_rows(to + h * S::kHalfBytes + r * 128, whole ? &maps.q : &maps.q_row, h * 64, un.g * q.group + r - r0,
+                       un.token0 + k, bar);
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+    }
+    if (!ok) {
+      // what is in flight lands before the block ends
+      for (int t = 0; t < 2; ++t)
+        for (uint32_t n = 0; n < kPolls && !bar_try(q_full + 8 * t, (turn >> t & 1) ^ 1); ++n) {
+        }
     }
   } else {
     // ---- rows ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
-    const int t = warp >> 2, row = threadIdx.x & 127;
-    uint8_t* stage = sm + S::kOut + warp * 32 * 128;
+    const int t = warp >> 3, half = warp >> 2 & 1, row = threadIdx.x & 127;
+    uint8_t* stage = sm + S::kOut + warp * 32 * 32;
+    // a number for the thread that has the other half of the row, and that thread's
+    float* mine = reinterpret_cast<float*>(sm + S::kMax) + threadIdx.x;
+    const float* others = reinterpret_cast<float*>(sm + S::kMax) + (threadIdx.x ^ kTileRows);
+    uint32_t exchanges = 0;
+    auto exchange = [&](float v) {
+      const uint32_t turn = exchanges++ & 1;
+      mine[turn * 512] = v;
+      bar_arrive(met + 8 * t);
+      ok = __all_sync(0xffffffffu, bar_wait(met + 8 * t, turn, abort, bt.err));
+      return others[turn * 512];
+    };
     const uint32_t quadrant = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4) ..
-    const uint32_t s_at = tmem + t * kTileKeys + quadrant, o_at = tmem + S::kColO + t * DP + quadrant;
-    const uint32_t p_at = tmem + S::kColP + t * S::kPitchP + quadrant;
+    const uint32_t s_at = tmem + (S::kTwoS ? t * kTileKeys : 0) + half * kHalfKeys + quadrant;
+    const uint32_t o_at = tmem + S::kColO + t * DP + half * (DP / 2) + quadrant;  // each half rescales half of O
+    const uint32_t p_at = tmem + S::kColP + t * (kTileKeys / 2) + half * (kHalfKeys / 2) + quadrant;
     const float c = q.scale_log2;
     uint32_t turn = 0;  // key tiles of the row tile so far
     // The n-th product into O.  Two barriers in turn: the product n - 2 is done when S of n arrives, so a
     // parity is that of n's own phase or of the one before.
     auto added = [&](uint32_t n) { return bar_wait(o_done + 16 * t + 8 * (n & 1), (n >> 1) & 1, abort, bt.err); };
-    Item it;
-    while (next_item(it)) {
+    for (; next_item(); end_item()) {
+      const Item& it = items[item_turn & 1];
       const Unit& un = it.un;
-      const int32_t row0 = t * kTileRows + (warp & 3) * 32, rows = un.rows - row0;  // the warp's
       if (t * kTileRows >= un.rows) continue;
-      const Plan plan = make_plan(un);
-      const Span span = make_span(it, q, plan, t);
+      const Plan plan = it.plan;
+      const Span span = it.span[t];
       const int32_t pos = un.position(q, min(t * kTileRows + row, un.rows - 1));  // rows past the last do its work again
       float m = -INFINITY, l = 0;
       bool fresh = true;
-      for (int32_t i = span.start(); i < it.end; i = span.at_or_after(i + 1)) {
+      for (int32_t i = span.start(); i < span.end; i = span.at_or_after(i + 1)) {
         const int32_t key0 = plan.key0(i);
         ok = __all_sync(0xffffffffu, bar_wait(s_full + 8 * t, turn & 1, abort, bt.err));
         if (!ok) break;
         fence_after();
-        float x[kTileKeys];
+        float x[kHalfKeys];
 #pragma unroll
-        for (int j = 0; j < kTileKeys; j += 32) tmem_load(s_at + j, x + j);
+        for (int j = 0; j < kHalfKeys; j += 32) tmem_load(s_at + j, x + j);
         tmem_load_wait();
-        if (S::kOwnP) {
-          fence_before();
-          bar_arrive(s_read + 8 * t);
-        }
+        fence_before();
+        bar_arrive(s_read + 8 * t);
+        const int32_t my_key0 = key0 + half * kHalfKeys;
         const bool cut_end = key0 + kTileKeys - 1 > span.lo;
         const bool cut_begin = q.window && key0 <= span.hi - q.window && key0 + kTileKeys > q.sinks;
         if (cut_end || cut_begin) {
-          const int32_t hi = pos - key0, lo = q.window ? hi - q.window + 1 : 0, sk = min(q.sinks - 1 - key0, hi);
+          const int32_t hi = pos - my_key0, lo = q.window ? hi - q.window + 1 : 0, sk = min(q.sinks - 1 - my_key0, hi);
 #pragma unroll
-          for (int j = 0; j < kTileKeys; j += 32) {
+          for (int j = 0; j < kHalfKeys; j += 32) {
             const uint32_t seen = bits_of(lo, hi, j) | bits_of(0, sk, j);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
@@ -742,23 +736,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int j = 4; j + 8 <= kTileKeys + 4; j += 8)
+        for (int j = 4; j < kHalfKeys; j += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            top[e] = fmaxf(fmaxf(top[e], x[j + e]), j + 4 + e < kTileKeys ? x[j + 4 + e] : -INFINITY);
-        const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
+            top[e] = fmaxf(fmaxf(top[e], x[j + e]), j + 4 + e < kHalfKeys ? x[j + 4 + e] : -INFINITY);
+        // over both halves of the row
+        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const float now = fmaxf(m, fmaxf(best, exchange(best)) * c);
+        if (!ok) break;
+        if (turn > 0) {  // the last P has been used up, and O is at rest
+          ok = __all_sync(0xffffffffu, added(turn - 1));
+          if (!ok) break;
+        }
         if (fresh) {
           fresh = false;
           m = now;
-        } else if (__any_sync(0xffffffffu, now > m + kLag)) {
-          ok = __all_sync(0xffffffffu, added(turn - 1));  // O is at rest
-          if (!ok) break;
+        } else if (__any_sync(0xffffffffu, now > m + kLag)) {  // the same in the warp of the other half
           fence_after();
           const float f = exp2_fast(m - (now == -INFINITY ? 0.f : now));
           l *= f;
           m = now;
-#pragma unroll
-          for (int j = 0; j < DP; j += 32) {
+#pragma unroll 1
+          for (int j = 0; j < DP / 2; j += 32) {
             float o[32];
             tmem_load(o_at + j, o);
             tmem_load_wait();
@@ -767,41 +766,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_store32(o_at + j, o);
           }
         }
+        fence_after();
         const float ref = m == -INFINITY ? 0.f : m;
         const uint64_t scale = two(c, c), shift = two(-ref, -ref);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < kTileKeys; j += 32) {
+        for (int j = 0; j < kHalfKeys; j += 32) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             uint64_t y = fma2(two(x[j + e], x[j + e + 1]), scale, shift);
             float p0, p1;
-            if (e % 8 == kPolynomial) {
-              y = exp2_two(y);
-              split(y, p0, p1);
-            } else {
-              split(y, p0, p1);
-              p0 = exp2_fast(p0);
-              p1 = exp2_fast(p1);
-              y = two(p0, p1);
-            }
+            split(y, p0, p1);
+            p0 = exp2_fast(p0);
+            p1 = exp2_fast(p1);
+            y = two(p0, p1);
             sum[e / 2 & 1] = add2(sum[e / 2 & 1], y);
             p[e / 2] = T::pack(p0, p1);
           }
-          if (S::kOwnP && j == 0 && turn > 0) {  // the last P has been used up
-            ok = __all_sync(0xffffffffu, added(turn - 1));
-            if (!ok) break;
-            fence_after();
-          }
           tmem_store16(p_at + j / 2, p);
-          if (j == kTileKeys / 2 - 32 || j == kTileKeys - 32) {  // the product of a half can begin
-            tmem_store_wait();
-            fence_before();
-            bar_arrive(p_half + 16 * t + (j == kTileKeys - 32 ? 8 : 0));
-          }
         }
-        if (!ok) break;
+        tmem_store_wait();
+        fence_before();
+        bar_arrive(p_half + 16 * t + 8 * half);  // the product of this half can begin
         ++turn;
         float l0, l1;
         split(add2(sum[0], sum[1]), l0, l1);
@@ -809,49 +796,58 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // ---- results ----
-      const int32_t whole = min(rows, 32);
+      const int32_t row0 = t * kTileRows + (warp & 3) * 32, rows = un.rows - row0, whole = min(rows, 32);  // the warp's
       float* slot = scratch + it.slot * kSlotFloats<DP>;
-      if (it.parts > 1 && lane < rows)
-        *reinterpret_cast<float2*>(slot + kBlockRows * DP + (row0 + lane) * 2) = make_float2(m, l);
       if (fresh) {  // no row of the tile sees a key of the item
-        if (it.parts == 1)
+        if (it.parts > 1 && half == 0 && lane < rows)
+          *reinterpret_cast<float2*>(slot + kBlockRows * DP + (row0 + lane) * 2) = make_float2(m, l);
+        if (it.parts == 1 && half == 0)
           for (int r = 0; r < whole; ++r)
             if (lane * 8 < kv.dim) *reinterpret_cast<uint4*>(un.result(kv, q, row0 + r) + lane * 8) = make_uint4(0, 0, 0, 0);
         continue;
       }
+      l += exchange(l);
+      if (!ok) break;
+      if (it.parts > 1 && half == 0 && lane < rows)
+        *reinterpret_cast<float2*>(slot + kBlockRows * DP + (row0 + lane) * 2) = make_float2(m, l);
       ok = __all_sync(0xffffffffu, added(turn - 1));
       if (!ok) break;
       fence_after();
-      float o[DP];
-#pragma unroll
-      for (int j = 0; j < DP; j += 32) tmem_load(o_at + j, o + j);
-      tmem_load_wait();
-      fence_before();
-      bar_arrive(o_empty + 8 * t);
-      if (it.parts == 1) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* out = un.results(kv, q);
-#pragma unroll
-        for (int h = 0; h < S::kHalves; ++h) {
-          uint32_t w[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) w[e] = l == 0.f ? 0 : T::pack(o[h * 64 + 2 * e] * inv, o[h * 64 + 2 * e + 1] * inv);
-          store_rows(stage, w, lane, whole, (kv.dim - h * 64) * 2, [&](int r) {
-            return reinterpret_cast<uint8_t*>(out + (int64_t)un.result_row(kv, q, row0 + r) * kv.dim + h * 64);
-          });
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      uint16_t* out = un.results(kv, q) + half * (DP / 2);
+      float* part = slot + half * (DP / 2);
+#pragma unroll 1
+      for (int j = 0; j < DP / 2; j += 16) {  // a loop: code that runs once an item waits for its instructions
+        float o[16];
+        tmem_load16(o_at + j, o);
+        tmem_load_wait();
+        if (j == DP / 2 - 16) {
+          fence_before();
+          bar_arrive(o_empty + 8 * t);
         }
-      } else {
+        if (it.parts == 1) {
+          uint32_t w[8];
 #pragma unroll
-        for (int j = 0; j < DP; j += 32)
-          store_rows(stage, reinterpret_cast<const uint32_t*>(o + j), lane, whole, 128,
-                     [&](int r) { return reinterpret_cast<uint8_t*>(slot + (row0 + r) * DP + j); });
+          for (int e = 0; e < 8; ++e) w[e] = l == 0.f ? 0 : T::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
+          store_rows(stage, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]), lane, whole,
+                     (kv.dim - half * (DP / 2) - j) * 2, [&](int r) {
+                       return reinterpret_cast<uint8_t*>(out + (int64_t)un.result_row(kv, q, row0 + r) * kv.dim + j);
+                     });
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; e += 8) {
+            const uint4* w = reinterpret_cast<const uint4*>(o + e);
+            store_rows(stage, w[0], w[1], lane, whole, 32,
+                       [&](int r) { return reinterpret_cast<uint8_t*>(part + (row0 + r) * DP + j + e); });
+          }
+        }
       }
     }
   }
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
@@ -902,6 +898,22 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
 }
 
+CUtensorMapDataType type_of(int dtype) {
+  return dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// Queries: boxes of 64 dims x heads x tokens.
+bool encode_q(CUtensorMap* map, const View& kv, const Query& q, int dtype, uint32_t heads, uint32_t tokens) {
+  const auto enc = encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)kv.dim, (cuuint64_t)kv.heads * q.group, (cuuint64_t)q.tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)std::max<int64_t>(q.head_stride, 8) * 2,
+                                 (cuuint64_t)std::max<int64_t>(q.token_stride, 8) * 2};
+  const cuuint32_t box[3] = {64, heads, tokens}, ones[3] = {1, 1, 1};
+  return enc(map, type_of(dtype), 3, const_cast<uint16_t*>(q.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool encode(CUtensorMap* map, const View& kv, int dtype, uint16_t* pages, uint32_t tokens) {
   const auto enc = encoder();
   if (!enc) return false;
@@ -910,7 +922,7 @@ bool encode(CUtensorMap* map, const View& kv, int dtype, uint16_t* pages, uint32
   const cuuint64_t strides[3] = {(cuuint64_t)kv.token_stride * 2, (cuuint64_t)std::max<int64_t>(kv.head_stride, 8) * 2,
                                  (cuuint64_t)std::max<int64_t>(kv.page_stride, 8) * 2};
   const cuuint32_t box[4] = {64, tokens, 1, 1}, ones[4] = {1, 1, 1, 1};
-  return enc(map, dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, pages, dims, strides,
+  return enc(map, type_of(dtype), 4, pages, dims, strides,
              box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -929,11 +941,16 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, c
   }
   Maps maps;
   const uint32_t box = (uint32_t)std::min(1 << kv.page_log, kTileKeys);
+  // whole tokens fill a row tile where the group divides it (units begin at multiples of 256 rows)
+  const uint32_t q_tokens = q.group <= kTileRows && kTileRows % q.group == 0 ? kTileRows / q.group : 0;
+  if (!encode_q(&maps.q, kv, q, dtype, q.group <= kTileRows ? q.group : 1, std::max(q_tokens, 1u)) ||
+      !encode_q(&maps.q_row, kv, q, dtype, 1, 1))
+    return cudaErrorInvalidValue;
   if (!encode(&maps.k, kv, dtype, kv.k, box) || !encode(&maps.v, kv, dtype, kv.v, box) ||
       !encode(&maps.v_row, kv, dtype, kv.v, 1))
     return cudaErrorInvalidValue;
   k_kv_prompt<T, DP><<<(unsigned)(sp.units * sp.parts), kThreads, Smem<DP>::kLaunch, st>>>(maps, kv, bt, q, sp.units,
-                                                                                           sp.parts, scratch);
+                                                                                           sp.parts, scratch, q_tokens);
   *launches += 1;
   if (sp.parts > 1) {
     k_kv_prompt_join<T, DP><<<dim3((unsigned)sp.units, kBlockRows / 32), 256, 0, st>>>(kv, bt, q, sp.parts, scratch);
@@ -946,6 +963,12 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, c
 
 uint64_t PromptSplit::scratch_floats() const {
   return parts > 1 ? (uint64_t)units * parts * kBlockRows * (dim_padded + 2) : 0;
+}
+
+bool prompt_strides(const View& kv, const Query& q) {
+  const int64_t most = int64_t(1) << 38;
+  return (kv.heads * q.group == 1 || (q.head_stride >= 8 && q.head_stride < most)) &&
+         (q.tokens == 1 || (q.token_stride >= 8 && q.token_stride < most));
 }
 
 PromptSplit plan_prompt(const View& kv, const Batch& bt, const Query& q, int sms) {

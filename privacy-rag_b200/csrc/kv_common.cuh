@@ -66,9 +66,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 __device__ __forceinline__ void flag_error(uint32_t* err, uint32_t bit) { atomicOr(err, bit); }
 
-// Length of sequence b, held to what its row of the table can name.
-__device__ __forceinline__ int32_t sequence_length(const Batch& bt, const View& kv, int32_t b) {
-  int32_t n = bt.lengths[b];
+// A sequence's length, held to what its row of the table can name.
+__device__ __forceinline__ int32_t checked_length(const Batch& bt, const View& kv, int32_t n) {
   const int64_t most = (int64_t)bt.width << kv.page_log;
   if (n < 0 || n > most) {
     flag_error(bt.err, kErrTable);

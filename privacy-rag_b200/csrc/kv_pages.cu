@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_append(View kv, Batch bt, Sourc
     first = bt.starts[b];
     next = bt.starts[b + 1];
   }
-  const int64_t pos = (int64_t)sequence_length(bt, kv, b) - next + t;
+  const int64_t pos = (int64_t)checked_length(bt, kv, bt.lengths[b]) - next + t;
   const int64_t slot = pos >> kv.page_log;
   const int32_t page = t >= first && t < next && pos >= 0 && slot < bt.width ? bt.table[(int64_t)b * bt.width + slot] : -1;
   if (page < 0 || page >= kv.pages) {

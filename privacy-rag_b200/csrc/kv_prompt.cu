@@ -103,8 +103,7 @@ struct Smem {
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
-  static constexpr int kOut = kV + kStages * kTileBytes;  // 32 bytes of each row, per warp
-  static constexpr int kMax = kOut + 16 * 32 * 32;        // two turns: a number of each thread for the row's other
+  static constexpr int kMax = kV + kStages * kTileBytes;  // two turns: a number of each thread for the row's other
   static constexpr int kAnswer = kMax + 2 * 512 * 4;      // of the launch control, 16 bytes
   static constexpr int kItems = kAnswer + 16;             // two
   static constexpr int kBar = kItems + ((2 * (int)sizeof(Item) + 7) & ~7);
@@ -319,21 +318,15 @@ __device__ __forceinline__ int32_t parts_of(int32_t n, int32_t most) {
 template <int DP>
 constexpr int64_t kSlotFloats = (int64_t)kBlockRows * (DP + 2);
 
-// 32 bytes of each of the warp's 32 rows: every lane has its own row's; stored by whole sectors.
-template <class To>
-__device__ __forceinline__ void store_rows(uint8_t* stage, uint4 a, uint4 b, int lane, int rows, int bytes, To to) {
-  const int turn = (lane >> 2 & 1) << 4;
-  *reinterpret_cast<uint4*>(stage + lane * 32 + turn) = a;
-  *reinterpret_cast<uint4*>(stage + lane * 32 + (16 - turn)) = b;
-  __syncwarp();
-  const int c = lane & 1;
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int r = n * 16 + (lane >> 1);
-    if (r < rows && c * 16 < bytes)
-      *reinterpret_cast<uint4*>(to(r) + c * 16) = *reinterpret_cast<const uint4*>(stage + r * 32 + ((c ^ (r >> 2 & 1)) << 4));
+// 32 bytes to a 16-byte aligned place.
+__device__ __forceinline__ void store32(void* to, const uint32_t* w, bool whole, int32_t bytes) {
+  if (whole) {  // 32-byte aligned, all 32 wanted
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+  } else {
+    if (bytes > 0) *static_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (bytes > 16) *(static_cast<uint4*>(to) + 1) = make_uint4(w[4], w[5], w[6], w[7]);
   }
-  __syncwarp();
 }
 
 template <class T, int DP>
@@ -376,6 +369,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == kLoadWarp && lane < 5)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.q) + lane * sizeof(CUtensorMap)) : "memory");
   if (warp == kScoreWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -447,21 +442,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (un.rows > 0 && part < it.parts) {
         tell(it);
         const int32_t* row = bt.table + (int64_t)un.b * bt.width;
+        // lane j's box of a key tile; its page is looked up one tile ahead
+        auto box_at = [&](int32_t i) { return plan.key0(i) + lane * box; };
+        auto seen = [&](int32_t k) { return k < un.sinks || (k < plan.end && k + box > un.begin); };
+        auto look_up = [&](int32_t i) {
+          const int32_t k = box_at(i);
+          return i < it.end && lane < boxes && seen(k) ? __ldg(row + (k >> kv.page_log)) : kv.pages;
+        };
+        int32_t ahead = look_up(it.begin);
         for (int32_t i = it.begin; i < it.end && ok; ++i, ++turn) {
           const int st = turn % S::kStages;
           const uint32_t parity = ((turn / S::kStages) & 1) ^ 1;
-          const int32_t t0 = plan.key0(i) + lane * box, t1 = t0 + box;
-          int32_t page = kv.pages;  // a box outside the pages reads zeros
+          const int32_t t0 = box_at(i), t1 = t0 + box;
+          int32_t page = ahead;  // a box outside the pages reads zeros
+          ahead = look_up(i + 1);
           bool whole = true;
-          if (lane < boxes) {
-            const bool in = t0 < un.sinks || (t0 < plan.end && t1 > un.begin);
-            whole = !in || t1 <= un.sinks || (t0 >= un.begin && t1 <= plan.end);
-            if (in) {
-              page = __ldg(row + (t0 >> kv.page_log));
-              if ((uint32_t)page >= (uint32_t)kv.pages) {
-                flag_error(bt.err, kErrTable);
-                page = kv.pages;
-              }
+          if (lane < boxes && seen(t0)) {
+            whole = t1 <= un.sinks || (t0 >= un.begin && t1 <= plan.end);
+            if ((uint32_t)page >= (uint32_t)kv.pages) {
+              flag_error(bt.err, kErrTable);
+              page = kv.pages;
             }
           }
           const int32_t at = t0 & (page_tokens - 1);
@@ -680,7 +680,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- rows ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
     const int t = warp >> 3, half = warp >> 2 & 1, row = threadIdx.x & 127;
-    uint8_t* stage = sm + S::kOut + warp * 32 * 32;
     // a number for the thread that has the other half of the row, and that thread's
     float* mine = reinterpret_cast<float*>(sm + S::kMax) + threadIdx.x;
     const float* others = reinterpret_cast<float*>(sm + S::kMax) + (threadIdx.x ^ kTileRows);
@@ -715,33 +714,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, bar_wait(s_full + 8 * t, turn & 1, abort, bt.err));
         if (!ok) break;
         fence_after();
+        const int32_t my_key0 = key0 + half * kHalfKeys;
+        // whether any row sees any of this half's keys
+        const bool empty = my_key0 > span.hi || (q.window && my_key0 >= q.sinks && my_key0 + kHalfKeys <= max(span.lo, 0) - q.window + 1);
         float x[kHalfKeys];
+        if (!empty) {
 #pragma unroll
-        for (int j = 0; j < kHalfKeys; j += 32) tmem_load(s_at + j, x + j);
-        tmem_load_wait();
+          for (int j = 0; j < kHalfKeys; j += 32) tmem_load(s_at + j, x + j);
+          tmem_load_wait();
+        }
         fence_before();
         bar_arrive(s_read + 8 * t);
-        const int32_t my_key0 = key0 + half * kHalfKeys;
-        const bool cut_end = key0 + kTileKeys - 1 > span.lo;
-        const bool cut_begin = q.window && key0 <= span.hi - q.window && key0 + kTileKeys > q.sinks;
-        if (cut_end || cut_begin) {
-          const int32_t hi = pos - my_key0, lo = q.window ? hi - q.window + 1 : 0, sk = min(q.sinks - 1 - my_key0, hi);
+        float best = -INFINITY;
+        if (!empty) {
+          const bool cut_end = my_key0 + kHalfKeys - 1 > span.lo;
+          const bool cut_begin = q.window && my_key0 <= span.hi - q.window && my_key0 + kHalfKeys > q.sinks;
+          if (cut_end || cut_begin) {
+            const int32_t hi = pos - my_key0, lo = q.window ? hi - q.window + 1 : 0, sk = min(q.sinks - 1 - my_key0, hi);
 #pragma unroll
-          for (int j = 0; j < kHalfKeys; j += 32) {
-            const uint32_t seen = bits_of(lo, hi, j) | bits_of(0, sk, j);
+            for (int j = 0; j < kHalfKeys; j += 32) {
+              const uint32_t in = bits_of(lo, hi, j) | bits_of(0, sk, j);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(seen >> e & 1)) x[j + e] = -INFINITY;
+              for (int e = 0; e < 32; ++e)
+                if (!(in >> e & 1)) x[j + e] = -INFINITY;
+            }
           }
+          float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int j = 4; j < kHalfKeys; j += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              top[e] = fmaxf(fmaxf(top[e], x[j + e]), j + 4 + e < kHalfKeys ? x[j + 4 + e] : -INFINITY);
+          best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         }
-        float top[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int j = 4; j < kHalfKeys; j += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            top[e] = fmaxf(fmaxf(top[e], x[j + e]), j + 4 + e < kHalfKeys ? x[j + 4 + e] : -INFINITY);
         // over both halves of the row
-        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         const float now = fmaxf(m, fmaxf(best, exchange(best)) * c);
         if (!ok) break;
         if (turn > 0) {  // the last P has been used up, and O is at rest
@@ -770,6 +776,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float ref = m == -INFINITY ? 0.f : m;
         const uint64_t scale = two(c, c), shift = two(-ref, -ref);
         uint64_t sum[2] = {0, 0};
+        if (empty) {
+          const uint32_t zeros[16] = {};
+          tmem_store16(p_at, zeros);
+          tmem_store16(p_at + 16, zeros);
+        } else {
 #pragma unroll
         for (int j = 0; j < kHalfKeys; j += 32) {
           uint32_t p[16];
@@ -786,6 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tmem_store16(p_at + j / 2, p);
         }
+        }
         tmem_store_wait();
         fence_before();
         bar_arrive(p_half + 16 * t + 8 * half);  // the product of this half can begin
@@ -796,26 +808,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // ---- results ----
-      const int32_t row0 = t * kTileRows + (warp & 3) * 32, rows = un.rows - row0, whole = min(rows, 32);  // the warp's
+      const int32_t at_row = t * kTileRows + row;
+      const bool mine_live = at_row < un.rows;
       float* slot = scratch + it.slot * kSlotFloats<DP>;
+      if (it.parts > 1 && fresh && half == 0 && mine_live)
+        *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = make_float2(m, l);
       if (fresh) {  // no row of the tile sees a key of the item
-        if (it.parts > 1 && half == 0 && lane < rows)
-          *reinterpret_cast<float2*>(slot + kBlockRows * DP + (row0 + lane) * 2) = make_float2(m, l);
-        if (it.parts == 1 && half == 0)
-          for (int r = 0; r < whole; ++r)
-            if (lane * 8 < kv.dim) *reinterpret_cast<uint4*>(un.result(kv, q, row0 + r) + lane * 8) = make_uint4(0, 0, 0, 0);
+        if (it.parts == 1 && half == 0 && mine_live)
+          for (int32_t d = 0; d < kv.dim; d += 8) *reinterpret_cast<uint4*>(un.result(kv, q, at_row) + d) = make_uint4(0, 0, 0, 0);
         continue;
       }
       l += exchange(l);
       if (!ok) break;
-      if (it.parts > 1 && half == 0 && lane < rows)
-        *reinterpret_cast<float2*>(slot + kBlockRows * DP + (row0 + lane) * 2) = make_float2(m, l);
+      if (it.parts > 1 && half == 0 && mine_live)
+        *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = make_float2(m, l);
       ok = __all_sync(0xffffffffu, added(turn - 1));
       if (!ok) break;
       fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint16_t* out = un.results(kv, q) + half * (DP / 2);
-      float* part = slot + half * (DP / 2);
+      const int32_t d0 = half * (DP / 2);
+      uint16_t* out = un.result(kv, q, at_row) + d0;
+      float* part = slot + (int64_t)at_row * DP + d0;
+      const bool sectors = ((reinterpret_cast<uintptr_t>(out) | (uint32_t)kv.dim * 2) & 31) == 0;
 #pragma unroll 1
       for (int j = 0; j < DP / 2; j += 16) {  // a loop: code that runs once an item waits for its instructions
         float o[16];
@@ -825,21 +839,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_before();
           bar_arrive(o_empty + 8 * t);
         }
+        if (!mine_live) continue;
         if (it.parts == 1) {
           uint32_t w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = l == 0.f ? 0 : T::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
-          store_rows(stage, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]), lane, whole,
-                     (kv.dim - half * (DP / 2) - j) * 2, [&](int r) {
-                       return reinterpret_cast<uint8_t*>(out + (int64_t)un.result_row(kv, q, row0 + r) * kv.dim + j);
-                     });
+          const int32_t bytes = (kv.dim - d0 - j) * 2;
+          store32(out + j, w, sectors && bytes >= 32, bytes);
         } else {
-#pragma unroll
-          for (int e = 0; e < 16; e += 8) {
-            const uint4* w = reinterpret_cast<const uint4*>(o + e);
-            store_rows(stage, w[0], w[1], lane, whole, 32,
-                       [&](int r) { return reinterpret_cast<uint8_t*>(part + (row0 + r) * DP + j + e); });
-          }
+          const bool sectors = (reinterpret_cast<uintptr_t>(part) & 31) == 0;
+          store32(part + j, reinterpret_cast<const uint32_t*>(o), sectors, 32);
+          store32(part + j + 8, reinterpret_cast<const uint32_t*>(o) + 8, sectors, 32);
         }
       }
     }

@@ -45,7 +45,7 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
   Unit un;
   un.g = (int32_t)(u % kv.heads);
   const int64_t block = u / kv.heads;
-  int32_t first = 0, tokens = 1;
+  int32_t first = 0, tokens = 1, length = 0;
   int64_t at = 0;  // the block of rows within the sequence
   if (bt.starts) {
     // blocks of the sequences before this one, 32 sequences a step
@@ -54,8 +54,9 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
     bool found = false;
     for (int32_t b0 = 0; b0 < bt.seqs && !found; b0 += 32) {
       int64_t mine = 0;
-      int32_t s = 0, e = 0;
+      int32_t s = 0, e = 0, held = 0;
       if (b0 + lane < bt.seqs) {
+        held = bt.lengths[b0 + lane];  // in one round trip with the starts
         s = bt.starts[b0 + lane];
         e = bt.starts[b0 + lane + 1];
         if (s < 0 || e < s || e > q.tokens) {
@@ -77,6 +78,7 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
         at = block - before - __shfl_sync(0xffffffffu, upto - mine, from);
         first = __shfl_sync(0xffffffffu, s, from);
         tokens = __shfl_sync(0xffffffffu, e, from) - first;
+        length = __shfl_sync(0xffffffffu, held, from);
         found = true;
       } else {
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -89,13 +91,14 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
     at = block % per;
     first = un.b;
     if (un.b >= bt.seqs) return un;
+    length = bt.lengths[un.b];
   }
   const int64_t all = (int64_t)tokens * q.group, row0 = at * ROWS;
   un.rows = (int32_t)(all - row0 < ROWS ? all - row0 : ROWS);
   const int32_t before = (int32_t)(row0 / q.group);
   un.head0 = (int32_t)(row0 - (int64_t)before * q.group);
   un.token0 = first + before;
-  un.pos0 = sequence_length(bt, kv, un.b) - tokens + before;
+  un.pos0 = checked_length(bt, kv, length) - tokens + before;
   // positions of the unit's first and last row
   const int32_t lo = un.pos0, hi = un.position(q, un.rows - 1);
   if (hi >= 0) {

@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <optional>
 
 #include "kv_host.h"
 
@@ -85,7 +86,7 @@ void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int
   };
   int launches = 0;
   if (few_rows(c.batch, c.query, starts) || !prompt_strides(c.view, c.query)) {
-    const RowSplit sp = plan_rows(c.view, c.batch, c.query, sm_count(at.device));
+    const RowSplit sp = plan_rows(c.view, c.batch, c.query, at.device);
     need_scratch(sp.scratch_floats());
     need(sp.blocks16 * sp.parts <= (int64_t)(kMost / sp.cluster), BFVGPU_E_SHAPE, "E_KV_SHAPE");
     cuda_need(launch_rows(c.view, c.batch, c.query, cache->dtype, sp, work, at.stream, &launches), "kv attention");
@@ -108,11 +109,12 @@ uint64_t scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q
     if (ragged) c.batch.starts = &some;  // only asked whether there is one
     int device = -1;
     internal_params(ctx, &device, nullptr);
-    const int sms = sm_count(device);
+    std::optional<OnDevice> scope;
+    if (device >= 0) scope.emplace(device);
     // the row kernel's too where the strides of the queries, not known here, may send them there
-    uint64_t floats = plan_rows(c.view, c.batch, c.query, sms).scratch_floats();
+    uint64_t floats = plan_rows(c.view, c.batch, c.query, device).scratch_floats();
     if (!few_rows(c.batch, c.query, ragged))
-      floats = std::max(floats, plan_prompt(c.view, c.batch, c.query, sms).scratch_floats());
+      floats = std::max(floats, plan_prompt(c.view, c.batch, c.query, sm_count(device)).scratch_floats());
     words = (floats + 1) / 2;
   });
   return words;

@@ -34,7 +34,7 @@ struct RowSplit {
   uint64_t scratch_floats() const;
   int32_t dim_padded = 128;
 };
-RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int sms);
+RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int device);  // device: current, or -1
 cudaError_t launch_rows(const View& kv, const Batch& bt, const Query& q, int dtype, const RowSplit& split,
                         float* scratch, cudaStream_t st, int* launches);
 

@@ -27,6 +27,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "kv_attention.h"
 #include "kv_units.cuh"
@@ -355,6 +356,7 @@ __global__ void __launch_bounds__(kThreads)
 template <class T, int DP>
 __global__ void __launch_bounds__(kThreads)
     k_kv_rows_join(View kv, Batch bt, Query q, int32_t parts, const float* scratch) {
+  cudaGridDependencySynchronize();
   const Unit un = find_unit<kRows>(kv, bt, q, blockIdx.x);
   const float* from = scratch + (int64_t)blockIdx.x * parts * (kRows * (DP + 2));
   for (int32_t e = threadIdx.x * 2; e < un.rows * DP; e += kThreads * 2) {
@@ -377,38 +379,80 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+constexpr int kDevices = 64;
+
+// The shared-memory limit is an attribute of the function on a device.
+template <class T, int DP, bool PAIR>
+cudaError_t allow_ring(int device) {
+  static std::atomic<uint64_t> allowed{0};
+  if (device < kDevices && (allowed.load() >> device & 1)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(k_kv_rows<T, DP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DP>::kBytes);
+  if (e == cudaSuccess && device < kDevices) allowed.fetch_or(uint64_t(1) << device);
+  return e;
+}
+
+template <int DP>
+void configure(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* at, int64_t blocks, int cluster, cudaStream_t st) {
+  cfg->gridDim = dim3((unsigned)blocks);
+  cfg->blockDim = dim3(kThreads);
+  cfg->dynamicSmemBytes = Ring<DP>::kBytes;
+  cfg->stream = st;
+  at->id = cudaLaunchAttributeClusterDimension;
+  at->val.clusterDim.x = cluster;
+  at->val.clusterDim.y = at->val.clusterDim.z = 1;
+  cfg->attrs = at;
+  cfg->numAttrs = 1;
+}
+
 template <class T, int DP, bool PAIR>
 cudaError_t launch(const View& kv, const Batch& bt, const Query& q, const RowSplit& sp, float* scratch, cudaStream_t st,
                    int* launches) {
-  // the shared-memory limit is an attribute of the function on a device
-  static std::atomic<uint64_t> allowed{0};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = allow_ring<T, DP, PAIR>(device);
   if (e != cudaSuccess) return e;
-  if (device >= 64 || !(allowed.load() >> device & 1)) {
-    e = cudaFuncSetAttribute(k_kv_rows<T, DP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DP>::kBytes);
-    if (e != cudaSuccess) return e;
-    if (device < 64) allowed.fetch_or(uint64_t(1) << device);
-  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(sp.blocks16 * sp.parts * sp.cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Ring<DP>::kBytes;
-  cfg.stream = st;
   cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = sp.cluster;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  configure<DP>(&cfg, &at, sp.blocks16 * sp.parts * sp.cluster, sp.cluster, st);
+  if (sp.cluster == 1) cfg.numAttrs = 0;
   e = cudaLaunchKernelEx(&cfg, k_kv_rows<T, DP, PAIR>, kv, bt, q, sp.cluster, sp.parts, scratch);
   if (e != cudaSuccess) return e;
   *launches += 1;
   if (sp.parts > 1) {
-    k_kv_rows_join<T, DP><<<(unsigned)sp.blocks16, kThreads, 0, st>>>(kv, bt, q, sp.parts, scratch);
+    // its blocks may start while the last ones above are still running, and wait for them there
+    cfg.gridDim = dim3((unsigned)sp.blocks16);
+    cfg.dynamicSmemBytes = 0;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, k_kv_rows_join<T, DP>, kv, bt, q, sp.parts, (const float*)scratch);
+    if (e != cudaSuccess) return e;
     *launches += 1;
   }
   return cudaGetLastError();
+}
+
+// How many clusters of 2^log blocks a device holds at once (a cluster lies within one of its processor
+// groups, so that large ones leave processors idle); without a device, what this GPU gives.
+template <int DP>
+int64_t resident_clusters(int device, int log) {
+  constexpr int kPerSm = DP == 64 ? 4 : 2;
+  static const int given[4] = {148 * kPerSm, 74 * kPerSm, DP == 64 ? 142 : 71, DP == 64 ? 71 : 33};
+  static std::atomic<int> known[kDevices][4];
+  if (device < 0 || device >= kDevices) return given[log];
+  int n = known[device][log].load();
+  if (!n) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at{};
+    configure<DP>(&cfg, &at, 1 << log, 1 << log, nullptr);
+    if (allow_ring<Bf16, DP, true>(device) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_kv_rows<Bf16, DP, true>, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = given[log];
+    }
+    known[device][log].store(n);
+  }
+  return n;
 }
 
 template <class T>
@@ -428,7 +472,14 @@ uint64_t RowSplit::scratch_floats() const {
   return parts > 1 ? (uint64_t)blocks16 * parts * kRows * (dim_padded + 2) : 0;
 }
 
-RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int sms) {
+// Shares of the keys, by an estimate in keys that one block streams while all are busy: a block costs its
+// share plus kStart (start, first loads, joins: 6 us against 23 ns a key, measured with 2048 units of
+// 2048 keys in 1 to 8 shares: 167, 195, 269, 444 us), and blocks run in waves of what is resident
+// (whole waves up to two, after that they mix).  One unit's further parts cost a second kernel, kJoin.
+// 16 sequences of 1024 keys and 8 key heads: 20, 17, 22 us in 1, 2, 4 shares; 131071 keys and 4 key heads:
+// 55 us in 8 x 8 shares, which are resident together, 82 us in 8 x 9, which are not.
+RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int device) {
+  constexpr double kStart = 270, kJoin = 170;
   RowSplit sp;
   sp.dim_padded = kv.dim <= 64 ? 64 : 128;
   const int64_t per = (q.group + kRows - 1) / kRows;
@@ -438,12 +489,21 @@ RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int sms) {
   // what a unit can have to read, from the width of the table
   int64_t keys = (int64_t)bt.width << kv.page_log;
   if (q.window) keys = std::min<int64_t>(keys, (int64_t)q.window + q.sinks + kRows);
-  const int64_t resident = (int64_t)sms * (sp.dim_padded == 64 ? 4 : 2);
-  // split until the GPU is filled twice over, while a block keeps at least two stages per warp
-  int64_t split = std::max<int64_t>(1, (2 * resident + sp.blocks16 - 1) / std::max<int64_t>(1, sp.blocks16));
-  split = std::min<int64_t>(split, std::max<int64_t>(1, keys / (2 * kKeys * kWarps)));
-  while (sp.cluster < split && sp.cluster < kMaxCluster) sp.cluster *= 2;
-  if (split > kMaxCluster) sp.parts = (int32_t)((split + kMaxCluster - 1) / kMaxCluster);
+  auto resident = [&](int log) {
+    return sp.dim_padded == 64 ? resident_clusters<64>(device, log) : resident_clusters<128>(device, log);
+  };
+  double best = 0;
+  for (int log = 0; 1 << log <= kMaxCluster; ++log) {
+    const double fill = (double)sp.blocks16 / resident(log);
+    const double time = (fill < 2 ? std::ceil(fill) : fill) * ((double)keys / (1 << log) + kStart);
+    if (log && time >= best) continue;
+    best = time;
+    sp.cluster = 1 << log;
+  }
+  if (sp.cluster == kMaxCluster) {
+    const int64_t most = std::min<int64_t>(resident(3) / std::max<int64_t>(1, sp.blocks16), keys / (kKeys * kWarps * kMaxCluster));
+    if (most > 1 && (double)keys / kMaxCluster * (1 - 1.0 / most) > kJoin) sp.parts = (int32_t)most;
+  }
   return sp;
 }
 

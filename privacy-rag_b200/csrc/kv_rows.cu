@@ -325,18 +325,27 @@ __global__ void __launch_bounds__(kThreads)
   else __syncthreads();
   for (int32_t e = (rank * kThreads + threadIdx.x) * 2; e < live; e += cluster * kThreads * 2) {
     const int32_t row = e / DP, d = e % DP;
-    float top = -INFINITY, sum = 0, v0 = 0, v1 = 0;
-    for (int32_t c = 0; c < cluster; ++c) {
+    // all blocks' numbers asked for together: each is a round trip to another processor
+    float2 mlc[kMaxCluster], vc[kMaxCluster];
+#pragma unroll
+    for (int32_t c = 0; c < kMaxCluster; ++c) {
+      if (c >= cluster) break;
       const float* other = cluster > 1 ? cl.map_shared_rank(own, c) : own;
-      const float* other_ml = other + kRows * DP;
-      const float mc = other_ml[row * 2], lc = other_ml[row * 2 + 1];
-      const float2 vc = *reinterpret_cast<const float2*>(other + e);
-      const float now = fmaxf(top, mc), ref = now == -INFINITY ? 0.f : now;
-      const float fo = exp2_fast(top - ref), fc = exp2_fast(mc - ref);
-      sum = sum * fo + lc * fc;
-      v0 = v0 * fo + vc.x * fc;
-      v1 = v1 * fo + vc.y * fc;
-      top = now;
+      mlc[c] = *reinterpret_cast<const float2*>(other + kRows * DP + row * 2);
+      vc[c] = *reinterpret_cast<const float2*>(other + e);
+    }
+    float top = -INFINITY, sum = 0, v0 = 0, v1 = 0;
+#pragma unroll
+    for (int32_t c = 0; c < kMaxCluster; ++c)
+      if (c < cluster) top = fmaxf(top, mlc[c].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int32_t c = 0; c < kMaxCluster; ++c) {
+      if (c >= cluster) break;
+      const float f = exp2_fast(mlc[c].x - ref);
+      sum += f * mlc[c].y;
+      v0 += f * vc[c].x;
+      v1 += f * vc[c].y;
     }
     if (parts == 1) {
       if (d < kv.dim) {
@@ -352,31 +361,55 @@ __global__ void __launch_bounds__(kThreads)
   if (cluster > 1) cl.sync();  // no block leaves while another reads its shared memory
 }
 
-// Joins the parts of each unit, in order.
+// Joins the parts of a unit's rows, in order: a warp per row, four rows a block.
 template <class T, int DP>
 __global__ void __launch_bounds__(kThreads)
     k_kv_rows_join(View kv, Batch bt, Query q, int32_t parts, const float* scratch) {
   cudaGridDependencySynchronize();
-  const Unit un = find_unit<kRows>(kv, bt, q, blockIdx.x);
-  const float* from = scratch + (int64_t)blockIdx.x * parts * (kRows * (DP + 2));
-  for (int32_t e = threadIdx.x * 2; e < un.rows * DP; e += kThreads * 2) {
-    const int32_t row = e / DP, d = e % DP;
-    if (d >= kv.dim) continue;
-    float top = -INFINITY, sum = 0, v0 = 0, v1 = 0;
-    for (int32_t c = 0; c < parts; ++c) {
-      const float* other = from + (int64_t)c * (kRows * (DP + 2));
-      const float2 mlc = *reinterpret_cast<const float2*>(other + kRows * DP + row * 2);
-      const float2 vc = *reinterpret_cast<const float2*>(other + e);
-      const float now = fmaxf(top, mlc.x), ref = now == -INFINITY ? 0.f : now;
-      const float fo = exp2_fast(top - ref), fc = exp2_fast(mlc.x - ref);
-      sum = sum * fo + mlc.y * fc;
-      v0 = v0 * fo + vc.x * fc;
-      v1 = v1 * fo + vc.y * fc;
-      top = now;
+  constexpr int kPer = DP / 32;  // dims a lane
+  const int64_t u = blockIdx.x / (kRows / kWarps);
+  const int32_t row = (blockIdx.x % (kRows / kWarps)) * kWarps + (threadIdx.x >> 5), d = (threadIdx.x & 31) * kPer;
+  const Unit un = find_unit<kRows>(kv, bt, q, u);
+  if (row >= un.rows || d >= kv.dim) return;
+  const float* from = scratch + u * parts * (kRows * (DP + 2));
+  float top = -INFINITY, sum = 0, v[kPer] = {};
+  constexpr int kTogether = 8;  // parts whose numbers are asked for together
+  for (int32_t c0 = 0; c0 < parts; c0 += kTogether) {
+    float2 mlc[kTogether];
+    float vc[kTogether][kPer];
+#pragma unroll
+    for (int c = 0; c < kTogether; ++c) {
+      const float* other = from + (int64_t)(c0 + c) * (kRows * (DP + 2));
+      mlc[c] = make_float2(-INFINITY, 0.f);
+      if (c0 + c < parts) mlc[c] = *reinterpret_cast<const float2*>(other + kRows * DP + row * 2);
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        float2 x = make_float2(0.f, 0.f);
+        if (c0 + c < parts) x = *reinterpret_cast<const float2*>(other + row * DP + d + e);
+        vc[c][e] = x.x;
+        vc[c][e + 1] = x.y;
+      }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint32_t*>(un.result(kv, q, row) + d) = T::pack(v0 * inv, v1 * inv);
+    float now = top;
+#pragma unroll
+    for (int c = 0; c < kTogether; ++c) now = fmaxf(now, mlc[c].x);
+    const float ref = now == -INFINITY ? 0.f : now, fo = exp2_fast(top - ref);
+    sum *= fo;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) v[e] *= fo;
+#pragma unroll
+    for (int c = 0; c < kTogether; ++c) {
+      const float f = exp2_fast(mlc[c].x - ref);
+      sum += f * mlc[c].y;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[e] += f * vc[c][e];
+    }
+    top = now;
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* out = un.result(kv, q, row) + d;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(out + e) = T::pack(v[e] * inv, v[e + 1] * inv);
 }
 
 constexpr int kDevices = 64;
@@ -420,7 +453,7 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, const RowSpl
   *launches += 1;
   if (sp.parts > 1) {
     // its blocks may start while the last ones above are still running, and wait for them there
-    cfg.gridDim = dim3((unsigned)sp.blocks16);
+    cfg.gridDim = dim3((unsigned)(sp.blocks16 * (kRows / kWarps)));
     cfg.dynamicSmemBytes = 0;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;

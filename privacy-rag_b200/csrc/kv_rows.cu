@@ -358,7 +358,12 @@ __global__ void __launch_bounds__(kThreads)
       if (d == 0) *reinterpret_cast<float2*>(to + kRows * DP + row * 2) = make_float2(top, sum);
     }
   }
-  if (cluster > 1) cl.sync();  // no block leaves while another reads its shared memory
+  if (cluster > 1) {
+    // No block leaves while another reads its shared memory.  What was read has been used in the stores
+    // above; relaxed, because the barrier need not wait for the stores themselves.
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  }
 }
 
 // Joins the parts of a unit's rows, in order: a warp per row, four rows a block.

@@ -26,10 +26,19 @@ int sm_count(int device) {
   return n;
 }
 
-// Prompts of more rows than this per sequence and key head, on average, go to the tile kernel.
-constexpr int64_t kFewRows = 32;
-bool few_rows(const Batch& bt, const Query& q, bool ragged) {
-  return !ragged || (int64_t)q.tokens * q.group <= kFewRows * bt.seqs;
+// Single tokens go to the row kernel, which reads a sequence's keys once per 16 query rows; so do prompts of
+// up to 16 rows per sequence and key head on average (64 sequences of 4096 tokens, 2 to 16 rows each: 184 to
+// 205 us, the prompt kernel 218 to 221), and those whose rows times keys are few, where the prompt kernel's
+// start counts.  At 512 keys, 32, 64, 128 and 256 rows: 9, 10, 13 and 15 us against 13, 13, 13 and 16; at 8192
+// keys, 16 and 32 rows: 23 and 33 against 26 and 30; with 64 dims, 64 rows: 24 against 24.
+constexpr int64_t kFewRows = 16;
+constexpr double kFewProducts = 20e6;  // 16-row blocks x keys x padded dims
+bool few_rows(const View& kv, const Batch& bt, const Query& q, bool ragged) {
+  if (!ragged || (int64_t)q.tokens * q.group <= kFewRows * bt.seqs) return true;
+  int64_t keys = (int64_t)bt.width << kv.page_log;
+  if (q.window) keys = std::min<int64_t>(keys, (int64_t)q.window + q.sinks);
+  const int64_t blocks = ((int64_t)q.tokens * q.group / 16 + bt.seqs) * kv.heads;
+  return (double)blocks * (double)keys * (kv.dim <= 64 ? 64 : 128) <= kFewProducts;
 }
 
 struct Call {
@@ -85,7 +94,7 @@ void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int
     need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
   };
   int launches = 0;
-  if (few_rows(c.batch, c.query, starts) || !prompt_strides(c.view, c.query)) {
+  if (few_rows(c.view, c.batch, c.query, starts) || !prompt_strides(c.view, c.query)) {
     const RowSplit sp = plan_rows(c.view, c.batch, c.query, at.device);
     need_scratch(sp.scratch_floats());
     need(sp.blocks16 * sp.parts <= (int64_t)(kMost / sp.cluster), BFVGPU_E_SHAPE, "E_KV_SHAPE");
@@ -113,7 +122,7 @@ uint64_t scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q
     if (device >= 0) scope.emplace(device);
     // the row kernel's too where the strides of the queries, not known here, may send them there
     uint64_t floats = plan_rows(c.view, c.batch, c.query, device).scratch_floats();
-    if (!few_rows(c.batch, c.query, ragged))
+    if (!few_rows(c.view, c.batch, c.query, ragged))
       floats = std::max(floats, plan_prompt(c.view, c.batch, c.query, sm_count(device)).scratch_floats());
     words = (floats + 1) / 2;
   });

@@ -95,10 +95,11 @@ struct Smem {
   static constexpr int kHalfBytes = kTileKeys * 128;
   static constexpr int kTileBytes = kHalves * kHalfBytes; // Q, K or V tile
   static constexpr int kStages = DP == 128 ? 2 : 4;
-  // Tensor memory columns: S, P of tile 0 and 1, O of tile 0 and 1.  With 64 dims there is room for an S of each
-  // row tile; with 128 they share one, which is free again as soon as the rows have read it.
-  static constexpr bool kTwoS = DP == 64;
-  static constexpr int kColP = kTwoS ? 2 * kTileKeys : kTileKeys, kColO = kColP + kTileKeys;
+  // Tensor memory columns: S, P of tile 0 and 1, O of tile 0 and 1.  The row tiles share one S, which is free
+  // again as soon as the rows have read it: there is no room for two with 128 dims, and with 64, where there
+  // is, taking turns keeps one tile's exponentials beside the other's maxima and exchanges (16384 tokens
+  // causal: 686 us, with an S each 807).
+  static constexpr int kColP = kTileKeys, kColO = kColP + kTileKeys;
   static_assert(kColO + 2 * DP <= 512, "tensor memory");
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + 2 * kTileBytes;
@@ -425,16 +426,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     while (ok && block >= 0) {
       // the blocks with the most keys come first
-      const int64_t u = units - 1 - block / most_parts;
-      const int32_t part = (int32_t)(block % most_parts);
+      const uint32_t from_end = (uint32_t)block / (uint32_t)most_parts, u = (uint32_t)units - 1 - from_end;
+      const int32_t part = (int32_t)((uint32_t)block - from_end * most_parts);
       Item it;
       it.un = find_unit<kBlockRows>(kv, bt, q, u);
       const Unit& un = it.un;
       const Plan& plan = it.plan;
       it.plan = make_plan(un);
       it.parts = parts_of(plan.n, most_parts);
-      it.begin = (int32_t)((int64_t)plan.n * part / it.parts);
-      it.end = (int32_t)((int64_t)plan.n * (part + 1) / it.parts);
+      it.begin = plan.n * part / it.parts;  // n < 2^23
+      it.end = plan.n * (part + 1) / it.parts;
       it.span[0] = make_span(it, q, 0);
       it.span[1] = make_span(it, q, 1);
       it.slot = (int32_t)(u * most_parts + part);
@@ -548,14 +549,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           const Span& span = it.span[t];
           if (!same(span.needs(i))) continue;
           if (same(i == span.start())) wait(q_full + 8 * t, q_turn >> t & 1);
-          const uint32_t of = S::kTwoS ? t : last;   // whose S was there before
-          wait(s_read + 8 * of, read_turn >> of & 1);
+          wait(s_read + 8 * last, read_turn >> last & 1);  // the S before has been read
           if (!ok) break;
           last = t;
           read_turn ^= 1u << t;
           const bool end = same(span.at_or_after(i + 1) >= to);
           if (end) q_turn ^= 1u << t;
-          const uint32_t a = same(q_desc + t * (S::kTileBytes >> 4)), d = same(tm + (S::kTwoS ? t * kTileKeys : 0));
+          const uint32_t a = same(q_desc + t * (S::kTileBytes >> 4)), d = tm;
           fence_after();
           if (elected()) {
 #pragma unroll
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       return others[turn * 512];
     };
     const uint32_t quadrant = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4) ..
-    const uint32_t s_at = tmem + (S::kTwoS ? t * kTileKeys : 0) + half * kHalfKeys + quadrant;
+    const uint32_t s_at = tmem + half * kHalfKeys + quadrant;
     const uint32_t o_at = tmem + S::kColO + t * DP + half * (DP / 2) + quadrant;  // each half rescales half of O
     const uint32_t p_at = tmem + S::kColP + t * (kTileKeys / 2) + half * (kHalfKeys / 2) + quadrant;
     const float c = q.scale_log2;
@@ -863,36 +863,43 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of 32 rows of a unit, in order.
+// Joins the parts of a unit, in order: a warp per row, eight rows a block.
 template <class T, int DP>
 __global__ void __launch_bounds__(256)
     k_kv_prompt_join(View kv, Batch bt, Query q, int32_t most_parts, const float* scratch) {
+  cudaGridDependencySynchronize();
+  constexpr int kPer = DP / 32;  // dims a lane
   const Unit un = find_unit<kBlockRows>(kv, bt, q, blockIdx.x);
   const int32_t parts = parts_of(make_plan(un).n, most_parts);
-  if (parts == 1) return;
+  const int32_t row = blockIdx.y * 8 + (threadIdx.x >> 5), d = (threadIdx.x & 31) * kPer;
+  if (parts == 1 || row >= un.rows || d >= kv.dim) return;
   const float* from = scratch + (int64_t)blockIdx.x * most_parts * kSlotFloats<DP>;
-  for (int32_t e = threadIdx.x * 4; e < 32 * DP; e += 256 * 4) {
-    const int32_t row = blockIdx.y * 32 + e / DP, d = e % DP;
-    if (row >= un.rows || d >= kv.dim) continue;
-    float top = -INFINITY;
-    for (int32_t p = 0; p < parts; ++p) top = fmaxf(top, from[p * kSlotFloats<DP> + kBlockRows * DP + row * 2]);
-    float sum = 0, v[4] = {0, 0, 0, 0};
-    for (int32_t p = 0; p < parts; ++p) {
-      const float* slot = from + p * kSlotFloats<DP>;
-      const float2 ml = *reinterpret_cast<const float2*>(slot + kBlockRows * DP + row * 2);
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // nothing seen: no O was stored
-      const float f = exp2_fast(ml.x - top);
-      const float4 x = *reinterpret_cast<const float4*>(slot + (int64_t)row * DP + d);
-      sum += f * ml.y;
-      v[0] += f * x.x;
-      v[1] += f * x.y;
-      v[2] += f * x.z;
-      v[3] += f * x.w;
+  // all parts' numbers asked for together
+  float2 ml[kMaxParts];
+  float top = -INFINITY, sum = 0, v[kPer] = {};
+#pragma unroll
+  for (int p = 0; p < kMaxParts; ++p)
+    if (p < parts) ml[p] = *reinterpret_cast<const float2*>(from + p * kSlotFloats<DP> + kBlockRows * DP + row * 2);
+#pragma unroll
+  for (int p = 0; p < kMaxParts; ++p)
+    if (p < parts) top = fmaxf(top, ml[p].x);
+#pragma unroll
+  for (int p = 0; p < kMaxParts; ++p) {
+    if (p >= parts || (ml[p].x == -INFINITY && ml[p].y == 0.f)) continue;  // nothing seen: no O was stored
+    const float f = exp2_fast(ml[p].x - top);
+    const float* o = from + p * kSlotFloats<DP> + (int64_t)row * DP + d;
+    sum += f * ml[p].y;
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(o + e);
+      v[e] += f * x.x;
+      v[e + 1] += f * x.y;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint2*>(un.result(kv, q, row) + d) =
-        make_uint2(T::pack(v[0] * inv, v[1] * inv), T::pack(v[2] * inv, v[3] * inv));
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* out = un.result(kv, q, row) + d;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(out + e) = T::pack(v[e] * inv, v[e + 1] * inv);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -963,7 +970,18 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, c
                                                                                            sp.parts, scratch, q_tokens);
   *launches += 1;
   if (sp.parts > 1) {
-    k_kv_prompt_join<T, DP><<<dim3((unsigned)sp.units, kBlockRows / 32), 256, 0, st>>>(kv, bt, q, sp.parts, scratch);
+    // its blocks may start while the last ones above are still running, and wait for them there
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at{};
+    cfg.gridDim = dim3((unsigned)sp.units, kBlockRows / 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, k_kv_prompt_join<T, DP>, kv, bt, q, sp.parts, (const float*)scratch);
+    if (e != cudaSuccess) return e;
     *launches += 1;
   }
   return cudaGetLastError();

@@ -100,17 +100,16 @@ __global__ void __launch_bounds__(kThreads)
   using R = Ring<DP>;
   extern __shared__ __align__(1024) uint8_t ring[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int32_t rank = (int32_t)(blockIdx.x % cluster);
-  const int64_t at_part = blockIdx.x / cluster;
-  const int32_t part = (int32_t)(at_part % parts);
-  const int64_t u = at_part / parts;
+  const uint32_t at_part = blockIdx.x / (uint32_t)cluster, u = at_part / (uint32_t)parts;
+  const int32_t rank = (int32_t)(blockIdx.x - at_part * cluster), part = (int32_t)(at_part - u * parts);
   const Unit un = find_unit<kRows>(kv, bt, q, u);
   const int32_t quad = lane >> 2, pair = (lane & 3) * 2;
 
   // stages of the unit -> this block's run of them
   const int32_t stages = (un.n + kKeys - 1) / kKeys;
   const int32_t shares = cluster * parts, share = part * cluster + rank;
-  const int32_t s0 = (int32_t)((int64_t)stages * share / shares), s1 = (int32_t)((int64_t)stages * (share + 1) / shares);
+  const int32_t per = stages / shares, more = stages - per * shares;
+  const int32_t s0 = share * per + min(share, more), s1 = s0 + per + (share < more);
 
   // query fragments (rows past the unit's and dims past the head's are 0)
   uint32_t qa[DP / 16][4];
@@ -353,7 +352,7 @@ __global__ void __launch_bounds__(kThreads)
         *reinterpret_cast<uint32_t*>(un.result(kv, q, row) + d) = T::pack(v0 * inv, v1 * inv);
       }
     } else {
-      float* to = scratch + (u * parts + part) * (kRows * (DP + 2));
+      float* to = scratch + ((int64_t)u * parts + part) * (kRows * (DP + 2));
       *reinterpret_cast<float2*>(to + e) = make_float2(v0, v1);
       if (d == 0) *reinterpret_cast<float2*>(to + kRows * DP + row * 2) = make_float2(top, sum);
     }
@@ -372,11 +371,11 @@ __global__ void __launch_bounds__(kThreads)
     k_kv_rows_join(View kv, Batch bt, Query q, int32_t parts, const float* scratch) {
   cudaGridDependencySynchronize();
   constexpr int kPer = DP / 32;  // dims a lane
-  const int64_t u = blockIdx.x / (kRows / kWarps);
+  const uint32_t u = blockIdx.x / (kRows / kWarps);
   const int32_t row = (blockIdx.x % (kRows / kWarps)) * kWarps + (threadIdx.x >> 5), d = (threadIdx.x & 31) * kPer;
   const Unit un = find_unit<kRows>(kv, bt, q, u);
   if (row >= un.rows || d >= kv.dim) return;
-  const float* from = scratch + u * parts * (kRows * (DP + 2));
+  const float* from = scratch + (int64_t)u * parts * (kRows * (DP + 2));
   float top = -INFINITY, sum = 0, v[kPer] = {};
   constexpr int kTogether = 8;  // parts whose numbers are asked for together
   for (int32_t c0 = 0; c0 < parts; c0 += kTogether) {

@@ -39,21 +39,22 @@ struct Unit {
 };
 
 // Units are numbered [block of ROWS rows of the batch][key head]; surplus numbers find no rows.  Every
-// warp of a block finds its unit by itself.
+// warp of a block finds its unit by itself.  In 32 bits (the entry points keep rows and units below
+// 2^31): this runs once, before anything else of its block can, and 64-bit divisions would be most of it.
 template <int ROWS>
-__device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const Query& q, int64_t u) {
+__device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const Query& q, uint32_t u) {
   Unit un;
-  un.g = (int32_t)(u % kv.heads);
-  const int64_t block = u / kv.heads;
+  const uint32_t block = u / (uint32_t)kv.heads;
+  un.g = (int32_t)(u - block * kv.heads);
   int32_t first = 0, tokens = 1, length = 0;
-  int64_t at = 0;  // the block of rows within the sequence
+  uint32_t at = 0;  // the block of rows within the sequence
   if (bt.starts) {
     // blocks of the sequences before this one, 32 sequences a step
     const int lane = threadIdx.x & 31;
-    int64_t before = 0;
+    uint32_t before = 0;
     bool found = false;
     for (int32_t b0 = 0; b0 < bt.seqs && !found; b0 += 32) {
-      int64_t mine = 0;
+      uint32_t mine = 0;
       int32_t s = 0, e = 0, held = 0;
       if (b0 + lane < bt.seqs) {
         held = bt.lengths[b0 + lane];  // in one round trip with the starts
@@ -63,15 +64,15 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
           flag_error(bt.err, kErrTable);
           s = e = 0;
         }
-        mine = ((int64_t)(e - s) * q.group + ROWS - 1) / ROWS;
+        mine = ((uint32_t)(e - s) * q.group + ROWS - 1) / ROWS;
       }
-      int64_t upto = mine;
+      uint32_t upto = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
+        const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += o;
       }
-      const uint32_t hit = __ballot_sync(0xffffffffu, block < before + upto);
+      const uint32_t hit = __ballot_sync(0xffffffffu, block - before < upto);
       if (hit) {
         const int from = __ffs(hit) - 1;
         un.b = b0 + from;
@@ -86,17 +87,18 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
     }
     if (!found) return un;
   } else {
-    const int32_t per = (q.group + ROWS - 1) / ROWS;
+    const uint32_t per = (q.group + ROWS - 1) / ROWS;
     un.b = (int32_t)(block / per);
-    at = block % per;
+    at = block - un.b * per;
     first = un.b;
     if (un.b >= bt.seqs) return un;
     length = bt.lengths[un.b];
   }
-  const int64_t all = (int64_t)tokens * q.group, row0 = at * ROWS;
-  un.rows = (int32_t)(all - row0 < ROWS ? all - row0 : ROWS);
-  const int32_t before = (int32_t)(row0 / q.group);
-  un.head0 = (int32_t)(row0 - (int64_t)before * q.group);
+  const uint32_t all = (uint32_t)tokens * q.group, row0 = at * ROWS;
+  if (at >= (all + ROWS - 1) / ROWS) return un;  // numbers that wrapped, of starts that overlap
+  un.rows = (int32_t)min(all - row0, (uint32_t)ROWS);
+  const int32_t before = (int32_t)(row0 / (uint32_t)q.group);
+  un.head0 = (int32_t)(row0 - (uint32_t)before * q.group);
   un.token0 = first + before;
   un.pos0 = checked_length(bt, kv, length) - tokens + before;
   // positions of the unit's first and last row

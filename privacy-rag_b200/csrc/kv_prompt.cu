@@ -19,7 +19,7 @@
 // K and V arrive by TMA page by page as the table names them, in the 128-byte swizzle (K as K-major,
 // V as MN-major operand).  Only visible tokens of V are loaded: what no row of the block sees may
 // hold NaN (unwritten rest of a page, pages given up), and 0 x NaN would reach every row.  Such
-// pages are read row by row, the other rows filled with zeros.
+// pages are read in rows, the others filled with zeros.
 //
 // Where there are too few rows to fill the GPU, the key tiles of a block's rows are dealt to several
 // blocks, which leave (m, sum, O) in 32 bits for a second kernel to join in a fixed order.
@@ -118,7 +118,8 @@ struct Maps {
   CUtensorMap q;         // 64 dims of a token's heads that share a key head; of 128 rows where they fill them
   CUtensorMap q_row;     // 64 dims of one row
   CUtensorMap k, v;      // one page (or 128 tokens of it) x 64 dims
-  CUtensorMap v_row;     // one token x 64 dims
+  CUtensorMap v_rows;    // eight tokens x 64 dims
+  CUtensorMap v_row;     // one
 };
 
 // ---- tcgen05, mbarrier and TMA ------------------------------------------------------------------
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kLoadWarp && lane < 5)
+  if (warp == kLoadWarp && lane < sizeof(Maps) / sizeof(CUtensorMap))
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.q) + lane * sizeof(CUtensorMap)) : "memory");
   if (warp == kScoreWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
@@ -485,17 +486,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h)
               tma_box(vb + h * S::kHalfBytes + lane * box * 128, &maps.v, h * 64, at, un.g, page, v_full + 8 * st);
+          // pages that are seen in part: eight rows at a time where those are all seen or all not, else one
           for (uint32_t left = __ballot_sync(0xffffffffu, !whole); left; left &= left - 1) {
             const int j = __ffs(left) - 1;
             const int32_t pj = __shfl_sync(0xffffffffu, page, j), tj = __shfl_sync(0xffffffffu, t0, j);
             const int32_t aj = __shfl_sync(0xffffffffu, at, j);
-            for (int32_t r = lane; r < box; r += 32) {
-              const int32_t tok = tj + r;
-              const bool seen = tok < un.sinks || (tok >= un.begin && tok < plan.end);
+            auto v_box = [&](const CUtensorMap* map, int32_t r, bool in) {
 #pragma unroll
               for (int h = 0; h < S::kHalves; ++h)
-                tma_box(vb + h * S::kHalfBytes + (j * box + r) * 128, &maps.v_row, h * 64, aj + r, un.g,
-                        seen ? pj : kv.pages, v_full + 8 * st);
+                tma_box(vb + h * S::kHalfBytes + (j * box + r) * 128, map, h * 64, aj + r, un.g, in ? pj : kv.pages,
+                        v_full + 8 * st);
+            };
+            auto row_seen = [&](int32_t k) { return k < un.sinks || (k >= un.begin && k < plan.end); };
+            const int32_t r8 = lane * 8, k8 = tj + r8;
+            const bool some = r8 < box && (k8 < un.sinks || (k8 < plan.end && k8 + 8 > un.begin));
+            const bool all = r8 < box && (k8 + 8 <= un.sinks || (k8 >= un.begin && k8 + 8 <= plan.end));
+            if (r8 < box && some == all) v_box(&maps.v_rows, r8, all);
+            for (uint32_t mixed = __ballot_sync(0xffffffffu, some != all); mixed; mixed &= mixed - 1) {
+              const int32_t r = (__ffs(mixed) - 1) * 8 + lane;
+              if (lane < 8) v_box(&maps.v_row, r, row_seen(tj + r));
             }
           }
           v_issued = turn + 1;
@@ -964,7 +973,7 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, c
       !encode_q(&maps.q_row, kv, q, dtype, 1, 1))
     return cudaErrorInvalidValue;
   if (!encode(&maps.k, kv, dtype, kv.k, box) || !encode(&maps.v, kv, dtype, kv.v, box) ||
-      !encode(&maps.v_row, kv, dtype, kv.v, 1))
+      !encode(&maps.v_rows, kv, dtype, kv.v, 8) || !encode(&maps.v_row, kv, dtype, kv.v, 1))
     return cudaErrorInvalidValue;
   k_kv_prompt<T, DP><<<(unsigned)(sp.units * sp.parts), kThreads, Smem<DP>::kLaunch, st>>>(maps, kv, bt, q, sp.units,
                                                                                            sp.parts, scratch, q_tokens);

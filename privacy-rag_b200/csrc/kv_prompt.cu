@@ -872,43 +872,54 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of a unit, in order: a warp per row, eight rows a block.
+// Joins the parts of a unit, in order: 32 rows a block, four a warp, whose numbers are asked for together
+// (finding the unit takes longer than a row: with eight rows a block the join took 25 us where this
+// takes 8).
+constexpr int kJoinRows = 32, kJoinThreads = 256;
 template <class T, int DP>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kJoinThreads)
     k_kv_prompt_join(View kv, Batch bt, Query q, int32_t most_parts, const float* scratch) {
   cudaGridDependencySynchronize();
-  constexpr int kPer = DP / 32;  // dims a lane
+  constexpr int kLanes = DP / 4, kAtOnce = 32 / kLanes;             // lanes a row, rows an access
+  constexpr int kPasses = kJoinRows / (kJoinThreads / 32) / kAtOnce;  // of a warp
   const Unit un = find_unit<kBlockRows>(kv, bt, q, blockIdx.x);
   const int32_t parts = parts_of(make_plan(un).n, most_parts);
-  const int32_t row = blockIdx.y * 8 + (threadIdx.x >> 5), d = (threadIdx.x & 31) * kPer;
-  if (parts == 1 || row >= un.rows || d >= kv.dim) return;
+  const int lane = threadIdx.x & 31, d = lane % kLanes * 4;
+  const int32_t row0 = blockIdx.y * kJoinRows + (threadIdx.x >> 5) * kAtOnce * kPasses + lane / kLanes;
+  if (parts == 1 || row0 >= un.rows || d >= kv.dim) return;
   const float* from = scratch + (int64_t)blockIdx.x * most_parts * kSlotFloats<DP>;
-  // all parts' numbers asked for together
-  float2 ml[kMaxParts];
-  float top = -INFINITY, sum = 0, v[kPer] = {};
+  float top[kPasses], sum[kPasses] = {}, v[kPasses][4] = {};
 #pragma unroll
-  for (int p = 0; p < kMaxParts; ++p)
-    if (p < parts) ml[p] = *reinterpret_cast<const float2*>(from + p * kSlotFloats<DP> + kBlockRows * DP + row * 2);
+  for (int i = 0; i < kPasses; ++i) top[i] = -INFINITY;
+  for (int32_t p = 0; p < parts; ++p)
 #pragma unroll
-  for (int p = 0; p < kMaxParts; ++p)
-    if (p < parts) top = fmaxf(top, ml[p].x);
+    for (int i = 0; i < kPasses; ++i)
+      top[i] = fmaxf(top[i], from[p * kSlotFloats<DP> + kBlockRows * DP + (row0 + i * kAtOnce) * 2]);
+#pragma unroll 2
+  for (int32_t p = 0; p < parts; ++p) {
+    const float* slot = from + p * kSlotFloats<DP>;
 #pragma unroll
-  for (int p = 0; p < kMaxParts; ++p) {
-    if (p >= parts || (ml[p].x == -INFINITY && ml[p].y == 0.f)) continue;  // nothing seen: no O was stored
-    const float f = exp2_fast(ml[p].x - top);
-    const float* o = from + p * kSlotFloats<DP> + (int64_t)row * DP + d;
-    sum += f * ml[p].y;
-#pragma unroll
-    for (int e = 0; e < kPer; e += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(o + e);
-      v[e] += f * x.x;
-      v[e + 1] += f * x.y;
+    for (int i = 0; i < kPasses; ++i) {
+      const int32_t row = row0 + i * kAtOnce;  // rows past the unit's read its slot's rest, and are not stored
+      const float2 ml = *reinterpret_cast<const float2*>(slot + kBlockRows * DP + row * 2);
+      const float4 x = *reinterpret_cast<const float4*>(slot + (int64_t)row * DP + d);
+      const bool some = ml.x != -INFINITY || ml.y != 0.f;  // else nothing was seen, and no O stored
+      const float f = some ? exp2_fast(ml.x - top[i]) : 0.f;
+      sum[i] += some ? f * ml.y : 0.f;
+      v[i][0] += some ? f * x.x : 0.f;
+      v[i][1] += some ? f * x.y : 0.f;
+      v[i][2] += some ? f * x.z : 0.f;
+      v[i][3] += some ? f * x.w : 0.f;
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint16_t* out = un.result(kv, q, row) + d;
 #pragma unroll
-  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(out + e) = T::pack(v[e] * inv, v[e + 1] * inv);
+  for (int i = 0; i < kPasses; ++i) {
+    const int32_t row = row0 + i * kAtOnce;
+    if (row >= un.rows) break;
+    const float inv = sum[i] == 0.f ? 0.f : 1.f / sum[i];
+    *reinterpret_cast<uint2*>(un.result(kv, q, row) + d) =
+        make_uint2(T::pack(v[i][0] * inv, v[i][1] * inv), T::pack(v[i][2] * inv, v[i][3] * inv));
+  }
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -982,8 +993,8 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, c
     // its blocks may start while the last ones above are still running, and wait for them there
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
-    cfg.gridDim = dim3((unsigned)sp.units, kBlockRows / 8);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3((unsigned)sp.units, kBlockRows / kJoinRows);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
@@ -1015,8 +1026,12 @@ PromptSplit plan_prompt(const View& kv, const Batch& bt, const Query& q, int sms
   sp.units = ((int64_t)q.tokens * q.group / kBlockRows + bt.seqs) * kv.heads;
   int64_t keys = (int64_t)bt.width << kv.page_log;
   if (q.window) keys = std::min<int64_t>(keys, (int64_t)q.window + q.sinks + 2 * kTileKeys + kBlockRows);
+  // As many parts as bring the blocks near the number of processors, where that leaves each some key tiles: more
+  // of them balance better, but each leaves its results in 32 bits for the join.  8192 keys, 8 key heads, 256,
+  // 1024 and 2048 rows: 36, 50 and 79 us so, 131, 129 and 128 in one part, 36, 61 and 84 in twice as many.
   const int64_t most = std::min<int64_t>(kMaxParts, keys / (kPartTiles * kTileKeys));
-  sp.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(most, 3 * sms / std::max<int64_t>(1, sp.units)));
+  const int64_t near = (2 * sms + sp.units) / std::max<int64_t>(1, 2 * sp.units);
+  sp.parts = (int32_t)std::max<int64_t>(1, std::min(most, near));
   return sp;
 }
 

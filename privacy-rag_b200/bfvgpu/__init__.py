@@ -10,4 +10,5 @@ from .backend import (ART002_PRIMES, Context, Matrix, NttBatch, PublicZero, Rota
 from .layout import (MatrixPacking, matrix_packing, matrix_packing_qk_reverse64,  # noqa: F401
                      pack_inputs, pack_weights, packed_bfv_rows_per_ciphertext, targets)
 from .kvcache import KvCache, PageBook, PagedKv  # noqa: F401
+from .attend import RingAttention  # noqa: F401
 from . import engine  # noqa: F401,E402

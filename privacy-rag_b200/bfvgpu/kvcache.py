@@ -3,7 +3,7 @@
 The protocol runs a decoder layer's linear calls; between the q/k/v call and the o call the party
 that holds the decrypted projections (a client that computes the non-linear steps itself, or a
 plaintext check of the protocol) needs a cache and its attention.  The reference has neither: its
-attention is a two-party integer protocol (IV1/compute/model.hpp:126-172).
+attention is a two-party integer protocol.
 
 * ``PagedKv``: the pages and the device calls on them (bfvgpu_kv_* of include/bfvgpu.h);
 * ``KvCache``: the book-keeping of a set of sequences over them: pages handed out, shared by forks,

@@ -132,6 +132,14 @@ PROMPT = [
     (BF, [(300, 150)], 1, 17, 64, 16, 50, 2, "hnd"),
     (FP, [(140, 140)], 1, 40, 8, 16, 0, 0, "hnd"),
     (BF, [(2100, 2100), (1, 1), (130, 40)], 1, 1, 128, 128, 0, 0, "nhd"),
+    # few rows, many keys: the keys in parts
+    (BF, [(5000, 300)], 1, 2, 64, 16, 0, 0, "hnd"),
+    (FP, [(9000, 200), (3000, 500)], 1, 1, 128, 64, 0, 0, "gaps"),
+    (BF, [(6000, 400)], 1, 3, 72, 32, 2500, 140, "nhd"),
+    (FP, [(4500, 140), (30, 30)], 2, 2, 64, 128, 3000, 2, "hnd"),
+    # more sequences than a warp looks through at once
+    (FP, [(200 + 11 * i, 40 + i % 7) for i in range(70)], 1, 2, 64, 32, 0, 0, "hnd"),
+    (BF, [(1 + 3 * i % 50, 1) for i in range(100)], 1, 4, 64, 16, 0, 0, "hnd"),
 ]
 
 
@@ -139,6 +147,27 @@ PROMPT = [
 def test_prompt(bfv, ctx, case):
     dtype, lens, g, r, dim, page, window, sinks, layout = case
     run_attention(bfv, ctx, "prompt", dtype, lens, g, r, dim, page, window, sinks, layout)
+
+
+@pytest.mark.parametrize("new", [1, 6, 500])
+def test_broadcast_and_transposed_queries(bfv, ctx, new):
+    """Queries with a stride of 0 over the heads or the tokens (broadcast), and with the tokens inside the
+    heads."""
+    gen = torch.Generator().manual_seed(4)
+    cache = R.Cache(2, 64, 16, BF, [700])
+    k, v = randn(gen, 700, 2, 64, dtype=BF), randn(gen, 700, 2, 64, dtype=BF)
+    cache.put(0, k, v)
+    kv = bfv.PagedKv(ctx, cache.k, cache.v)
+    starts = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([700], dtype=torch.int32, device="cuda")
+    one = randn(gen, new, 1, 64, dtype=BF)
+    for q in (one.cuda().expand(new, 4, 64), one[:1].cuda().expand(new, 4, 64),
+              randn(gen, 4, new, 64, dtype=BF).cuda().transpose(0, 1)):
+        want, bound = R.attention(q.cpu(), k, v, 700, 0, 0, 0.125, two_terms=False)
+        check(kv.prompt(q, starts, cache.table.cuda(), lengths), want, bound)
+        if new == 1:
+            check(kv.decode(q, cache.table.cuda(), lengths), want, bound)
+    assert ctx.check() == 0
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])

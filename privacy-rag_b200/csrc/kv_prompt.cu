@@ -10,12 +10,12 @@
 // and the 32-bit sums, and O need not be rescaled.  The sum of the weights is kept in 32 bits, from
 // the weights before they are rounded to 16 bits for the product.
 //
-// Roles: warps 0-7 and 8-15 hold the rows of tile 0 and 1, the first four of each the first 64 keys' scores,
-// warp 16 issues the products, warp 17 the loads of K and V, warps 18 and 19 load the queries of tile 0
-// and 1.  While one tile's rows are in their
-// exponentials, the other tile's products run.  A block is resident on its SM for the whole launch and
-// takes over the blocks that have not started yet (cluster launch control), so that the loads of the
-// next rows and the results of the last ones run under the products in between.
+// Roles: warps 0-7 and 8-15 hold the rows of tile 0 and 1, the first four of each the first 64 keys' scores;
+// warp 16 issues S of both tiles in turn, warp 17 the products with V, warp 18 finds the rows and loads K and
+// V, warp 19 loads the queries.  While one tile's rows are in their exponentials, the other tile's products
+// run.  A block is resident on its SM for the whole launch and takes over the blocks that have not started
+// yet (cluster launch control), so that the loads of the next rows and the results of the last ones run under
+// the products in between.
 // K and V arrive by TMA page by page as the table names them, in the 128-byte swizzle (K as K-major,
 // V as MN-major operand).  Only visible tokens of V are loaded: what no row of the block sees may
 // hold NaN (unwritten rest of a page, pages given up), and 0 x NaN would reach every row.  Such
@@ -46,9 +46,9 @@ constexpr int kTileKeys = 128;
 constexpr int kThreads = 640;
 constexpr int kScoreWarp = 16, kValueWarp = 17, kLoadWarp = 18, kQueryWarp = 19;
 constexpr int kReaders = 19;          // warps that are told of the next rows: all but the loads' own
-// Registers a thread: launched with 96 (640 x 96 of the SM's 65536); the issuing warpgroup keeps 56 and the
-// rows take 104: 128 x 56 + 512 x 104 <= 640 x 96.
-constexpr int kIssueRegs = 56, kRowRegs = 104;
+// Registers a thread: launched with 96 (640 x 96 of the SM's 65536); the issuing warpgroup keeps 64 and the
+// rows take 104: 128 x 64 + 512 x 104 = 640 x 96.
+constexpr int kIssueRegs = 64, kRowRegs = 104;
 constexpr int kHalfKeys = kTileKeys / 2;  // of a thread
 constexpr float kLag = 8.f;           // how far m may stay behind the running maximum
 constexpr uint32_t kPolls = 1u << 20;     // of a wait for the next step before it gives up

@@ -108,7 +108,7 @@ struct Smem {
   static constexpr int kAnswer = kMax + 2 * 512 * 4;      // of the launch control, 16 bytes
   static constexpr int kItems = kAnswer + 16;             // two
   static constexpr int kBar = kItems + ((2 * (int)sizeof(Item) + 7) & ~7);
-  static constexpr int kBars = 4 + 4 * kStages + 2 + 2 + 4 + 4 + 2 + 2 + 4 + 1 + 2;
+  static constexpr int kBars = 4 + 4 * kStages + 2 + 2 + 4 + 4 + 2 + 8 + 4 + 1 + 2;
   static constexpr int kBytes = kBar + kBars * 8 + 16;    // + tensor memory address, abort flag
   static constexpr int kLaunch = kBytes + 1024;           // slack for the 1024-byte alignment
   static_assert(kLaunch > 115 * 1024 && kLaunch <= 227 * 1024, "one block, and its tensor memory, per SM");
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * S::kStages,
                  v_full = k_empty + 8 * S::kStages, v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages,
                  s_read = s_full + 16, p_half = s_read + 16, o_done = p_half + 32, o_empty = o_done + 32,
-                 met = o_empty + 16, item_full = met + 16,
+                 met = o_empty + 16, item_full = met + 64,
                  item_empty = item_full + 16, drain = item_empty + 16, answered = drain + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::kBar + S::kBars * 8);
   volatile uint32_t* abort = tmem_slot + 1;
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bar_init(o_done + 16 * t + 8 * b, 1);
       }
       bar_init(o_empty + 8 * t, 2 * kTileRows);
-      bar_init(met + 8 * t, 2 * kTileRows);
+      for (int w = 0; w < 4; ++w) bar_init(met + 32 * t + 8 * w, 64);
       bar_init(item_full + 8 * t, 1);
       bar_init(item_empty + 8 * t, kReaders);
       bar_init(drain + 8 * t, 1);
@@ -692,12 +692,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // a number for the thread that has the other half of the row, and that thread's
     float* mine = reinterpret_cast<float*>(sm + S::kMax) + threadIdx.x;
     const float* others = reinterpret_cast<float*>(sm + S::kMax) + (threadIdx.x ^ kTileRows);
+    const uint32_t meets = met + 32 * t + 8 * (warp & 3);
     uint32_t exchanges = 0;
     auto exchange = [&](float v) {
       const uint32_t turn = exchanges++ & 1;
       mine[turn * 512] = v;
-      bar_arrive(met + 8 * t);
-      ok = __all_sync(0xffffffffu, bar_wait(met + 8 * t, turn, abort, bt.err));
+      bar_arrive(meets);
+      ok = __all_sync(0xffffffffu, bar_wait(meets, turn, abort, bt.err));
       return others[turn * 512];
     };
     const uint32_t quadrant = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4) ..

@@ -43,6 +43,7 @@ cudaError_t launch_rows(const View& kv, const Batch& bt, const Query& q, int dty
 struct PromptSplit {
   int64_t units = 0;
   int32_t parts = 1, dim_padded = 128;
+  bool ranked = false;  // the units of all sequences in the order of their keys
   uint64_t scratch_floats() const;
 };
 // Whether the queries' strides suit the prompt kernel's loads (no broadcast, no reversed axis).

@@ -38,6 +38,27 @@ struct Unit {
   }
 };
 
+// The `at`-th ROWS rows of sequence un.b, which has the new tokens from `first` on.
+template <int ROWS>
+__device__ __forceinline__ void fill_unit(Unit& un, const View& kv, const Batch& bt, const Query& q, int32_t first,
+                                          int32_t tokens, int32_t length, uint32_t at) {
+  const uint32_t all = (uint32_t)tokens * q.group, row0 = at * ROWS;
+  if (at >= (all + ROWS - 1) / ROWS) return;  // numbers that wrapped, of starts that overlap
+  un.rows = (int32_t)min(all - row0, (uint32_t)ROWS);
+  const int32_t before = (int32_t)(row0 / (uint32_t)q.group);
+  un.head0 = (int32_t)(row0 - (uint32_t)before * q.group);
+  un.token0 = first + before;
+  un.pos0 = checked_length(bt, kv, length) - tokens + before;
+  // positions of the unit's first and last row
+  const int32_t lo = un.pos0, hi = un.position(q, un.rows - 1);
+  if (hi >= 0) {
+    un.begin = q.window && lo + 1 > q.window ? lo + 1 - q.window : 0;
+    un.sinks = q.sinks < un.begin ? q.sinks : un.begin;
+    if (un.sinks == un.begin) un.sinks = un.begin = 0;  // nothing is left out between them
+    un.n = un.sinks + hi + 1 - un.begin;
+  }
+}
+
 // Units are numbered [block of ROWS rows of the batch][key head]; surplus numbers find no rows.  Every
 // warp of a block finds its unit by itself.  In 32 bits (the entry points keep rows and units below
 // 2^31): this runs once, before anything else of its block can, and 64-bit divisions would be most of it.
@@ -94,21 +115,49 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
     if (un.b >= bt.seqs) return un;
     length = bt.lengths[un.b];
   }
-  const uint32_t all = (uint32_t)tokens * q.group, row0 = at * ROWS;
-  if (at >= (all + ROWS - 1) / ROWS) return un;  // numbers that wrapped, of starts that overlap
-  un.rows = (int32_t)min(all - row0, (uint32_t)ROWS);
-  const int32_t before = (int32_t)(row0 / (uint32_t)q.group);
-  un.head0 = (int32_t)(row0 - (uint32_t)before * q.group);
-  un.token0 = first + before;
-  un.pos0 = checked_length(bt, kv, length) - tokens + before;
-  // positions of the unit's first and last row
-  const int32_t lo = un.pos0, hi = un.position(q, un.rows - 1);
-  if (hi >= 0) {
-    un.begin = q.window && lo + 1 > q.window ? lo + 1 - q.window : 0;
-    un.sinks = q.sinks < un.begin ? q.sinks : un.begin;
-    if (un.sinks == un.begin) un.sinks = un.begin = 0;  // nothing is left out between them
-    un.n = un.sinks + hi + 1 - un.begin;
+  fill_unit<ROWS>(un, kv, bt, q, first, tokens, length, at);
+  return un;
+}
+
+// The same units of up to 32 sequences in the order of their rows' positions, the last first: those with the
+// most keys, whichever sequence they belong to.  A unit's level is its place in its sequence in steps of ROWS
+// rows; one lane a sequence counts its units of a level or above.
+template <int ROWS>
+__device__ __forceinline__ Unit find_unit_ranked(const View& kv, const Batch& bt, const Query& q, uint32_t u) {
+  Unit un;
+  const uint32_t rank = u / (uint32_t)kv.heads;
+  un.g = (int32_t)(u - rank * kv.heads);
+  const int lane = threadIdx.x & 31;
+  int32_t s = 0, tokens = 0, length = 0;
+  if (lane < bt.seqs) {
+    length = bt.lengths[lane];
+    s = bt.starts[lane];
+    const int32_t e = bt.starts[lane + 1];
+    if (s < 0 || e < s || e > q.tokens) flag_error(bt.err, kErrTable);
+    else tokens = e - s;
   }
+  const uint32_t mine = ((uint32_t)tokens * q.group + ROWS - 1) / ROWS;
+  const uint64_t rows_before = (uint64_t)max(min(length, bt.width << kv.page_log) - tokens, 0) * q.group;
+  const uint32_t first = (uint32_t)min(rows_before / ROWS, (uint64_t)1 << 30);
+  auto from = [&](uint32_t level) {  // units of this level or above
+    return __reduce_add_sync(0xffffffffu, first + mine > level ? first + mine - max(first, level) : 0);
+  };
+  // the highest level that `rank` units have not passed
+  uint32_t low = __reduce_min_sync(0xffffffffu, mine ? first : 0xffffffffu), high = __reduce_max_sync(0xffffffffu, mine ? first + mine : 0);
+  if (low >= high || from(low) <= rank) return un;
+  uint32_t above = 0;  // units of level `high` or above
+  while (high - low > 1) {
+    const uint32_t mid = low + (high - low) / 2, n = from(mid);
+    if (n > rank) low = mid;
+    else high = mid, above = n;
+  }
+  const uint32_t here = __ballot_sync(0xffffffffu, mine && first <= low && low < first + mine);
+  const uint32_t lower = __popc(here & ((1u << lane) - 1));
+  const int owner = __ffs(__ballot_sync(0xffffffffu, (here >> lane & 1) && lower == rank - above)) - 1;
+  un.b = owner;
+  const uint32_t at = low - __shfl_sync(0xffffffffu, first, owner);
+  fill_unit<ROWS>(un, kv, bt, q, __shfl_sync(0xffffffffu, s, owner), __shfl_sync(0xffffffffu, tokens, owner),
+                  __shfl_sync(0xffffffffu, length, owner), at);
   return un;
 }
 

@@ -64,6 +64,27 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// A launch that may begin while the kernel before it on the stream ends: its kernel calls
+// cudaGridDependencySynchronize before it touches memory, so that only the start of its blocks, and what they do
+// before that, runs under the other's last blocks (first token of a decode: 6.0 -> @ us a call, back to back).
+template <class... P, class... A>
+cudaError_t launch_next(void (*kernel)(P...), dim3 grid, int threads, size_t shared, cudaStream_t st, int cluster, A... args) {
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 __device__ __forceinline__ void flag_error(uint32_t* err, uint32_t bit) { atomicOr(err, bit); }
 
 // A sequence's length, held to what its row of the table can name.

@@ -34,6 +34,7 @@ __device__ __forceinline__ uint4 eight(const void* base, int64_t at) {
 // of every head.
 template <class T, int SRC>
 __global__ void __launch_bounds__(kThreads) k_kv_append(View kv, Batch bt, Source s) {
+  cudaGridDependencySynchronize();
   const int lane = threadIdx.x & 31;
   const int64_t t64 = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (t64 >= s.tokens) return;
@@ -127,27 +128,28 @@ struct Copies {
   PageShape shape;
   int64_t layer_stride = 0;
   int32_t layers = 0, parts = 0, count = 0;
+  __host__ __device__ uint32_t per() const { return 2u * layers * parts; }  // blocks of a copy
 };
 
-// Blocks [copy c][layer][K, V][part of the page], part fastest.
-__device__ __forceinline__ void copy_block(const View& kv, const Copies& cp, int64_t block, int32_t from, int32_t to) {
-  const int32_t part = (int32_t)(block % cp.parts);
-  const int64_t rest = block / cp.parts;
-  uint16_t* base = ((rest & 1) ? kv.v : kv.k) + ((rest >> 1) % cp.layers) * cp.layer_stride;
-  copy_share(base, kv.page_stride, from, to, cp.shape, part);
+// Share of a copy's blocks [layer][K, V][part of the page], part fastest.
+__device__ __forceinline__ void copy_block(const View& kv, const Copies& cp, uint32_t share, int32_t from, int32_t to) {
+  const uint32_t rest = share / (uint32_t)cp.parts, part = share - rest * cp.parts;
+  uint16_t* base = ((rest & 1) ? kv.v : kv.k) + (int64_t)(rest >> 1) * cp.layer_stride;
+  copy_share(base, kv.page_stride, from, to, cp.shape, (int32_t)part);
 }
 
 __global__ void __launch_bounds__(kThreads)
     k_kv_move(View kv, Copies cp, const int32_t* src, const int32_t* dst, int32_t* table, int64_t entries,
               int64_t copy_blocks, uint32_t* err) {
+  cudaGridDependencySynchronize();
   if (blockIdx.x < copy_blocks) {
-    const int64_t c = blockIdx.x / (2ll * cp.layers * cp.parts);
+    const uint32_t c = blockIdx.x / cp.per();
     const int32_t from = src[c], to = dst[c];
     if ((uint32_t)from >= (uint32_t)kv.pages || (uint32_t)to >= (uint32_t)kv.pages) {
       if (threadIdx.x == 0) flag_error(err, kErrTable);
       return;
     }
-    copy_block(kv, cp, blockIdx.x, from, to);
+    copy_block(kv, cp, blockIdx.x - c * cp.per(), from, to);
     return;
   }
   // table entries: a binary search in src, which is strictly increasing
@@ -167,8 +169,8 @@ __global__ void __launch_bounds__(kThreads)
 __global__ void __launch_bounds__(kThreads)
     k_kv_fork(View kv, Copies cp, const int32_t* parents, const int32_t* children, const int32_t* fresh,
               int32_t* table, int32_t rows, int32_t width, int32_t* lengths, uint32_t* err) {
-  const int64_t per = 2ll * cp.layers * cp.parts;
-  const int64_t c = blockIdx.x / per, share = blockIdx.x % per;
+  cudaGridDependencySynchronize();
+  const uint32_t c = blockIdx.x / cp.per(), share = blockIdx.x - c * cp.per();
   const int32_t p = parents[c], child = children[c];
   if ((uint32_t)p >= (uint32_t)rows || (uint32_t)child >= (uint32_t)rows || p == child) {
     if (threadIdx.x == 0) flag_error(err, kErrTable);
@@ -249,13 +251,10 @@ extern "C" int32_t bfvgpu_kv_append_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cac
     s.head_stride = head_stride;
     s.tokens = (int32_t)tokens;
     const unsigned grid = (unsigned)((tokens + kThreads / 32 - 1) / (kThreads / 32));
-    if (source_dtype != BFVGPU_KV_F32)
-      k_kv_append<Bf16, 0><<<grid, kThreads, 0, at.stream>>>(w, bt, s);
-    else if (cache->dtype == BFVGPU_KV_BF16)
-      k_kv_append<Bf16, 2><<<grid, kThreads, 0, at.stream>>>(w, bt, s);
-    else
-      k_kv_append<Fp16, 2><<<grid, kThreads, 0, at.stream>>>(w, bt, s);
-    cuda_need(cudaGetLastError(), "kv append");
+    const auto kernel = source_dtype != BFVGPU_KV_F32        ? k_kv_append<Bf16, 0>
+                        : cache->dtype == BFVGPU_KV_BF16 ? k_kv_append<Bf16, 2>
+                                                         : k_kv_append<Fp16, 2>;
+    cuda_need(launch_next(kernel, dim3(grid), kThreads, 0, at.stream, 1, w, bt, s), "kv append");
     internal_count_launch(1);
   });
 }
@@ -273,9 +272,9 @@ extern "C" int32_t bfvgpu_kv_fork_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache
     const int64_t blocks = (int64_t)count * 2 * cp.layers * cp.parts;
     need(blocks <= kMostBlocks, BFVGPU_E_SHAPE, "E_KV_SHAPE");
     OnDevice scope(at.device);
-    k_kv_fork<<<(unsigned)blocks, kThreads, 0, at.stream>>>(w, cp, parents, children, fresh, table, (int32_t)rows,
-                                                            (int32_t)width, lengths, at.err);
-    cuda_need(cudaGetLastError(), "kv fork");
+    cuda_need(launch_next(k_kv_fork, dim3((unsigned)blocks), kThreads, 0, at.stream, 1, w, cp, parents, children, fresh, table,
+                          (int32_t)rows, (int32_t)width, lengths, at.err),
+              "kv fork");
     internal_count_launch(1);
   });
 }
@@ -295,8 +294,9 @@ extern "C" int32_t bfvgpu_kv_move_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache
     const int64_t blocks = copy_blocks + (entries + kThreads - 1) / kThreads;
     need(blocks <= kMostBlocks, BFVGPU_E_SHAPE, "E_KV_SHAPE");
     OnDevice scope(at.device);
-    k_kv_move<<<(unsigned)blocks, kThreads, 0, at.stream>>>(w, cp, src, dst, table, entries, copy_blocks, at.err);
-    cuda_need(cudaGetLastError(), "kv move");
+    cuda_need(launch_next(k_kv_move, dim3((unsigned)blocks), kThreads, 0, at.stream, 1, w, cp, src, dst, table, entries, copy_blocks,
+                          at.err),
+              "kv move");
     internal_count_launch(1);
   });
 }

@@ -381,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
+  cudaGridDependencySynchronize();
 
   // the next item, for every warp but the loads'; false: no more (or given up).  It stays where it is until
   // the warp gives its place back.
@@ -987,21 +988,13 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, c
   if (!encode(&maps.k, kv, dtype, kv.k, box) || !encode(&maps.v, kv, dtype, kv.v, box) ||
       !encode(&maps.v_rows, kv, dtype, kv.v, 8) || !encode(&maps.v_row, kv, dtype, kv.v, 1))
     return cudaErrorInvalidValue;
-  k_kv_prompt<T, DP><<<(unsigned)(sp.units * sp.parts), kThreads, Smem<DP>::kLaunch, st>>>(maps, kv, bt, q, sp.units,
-                                                                                           sp.parts, scratch, q_tokens, sp.ranked);
+  e = launch_next(k_kv_prompt<T, DP>, dim3((unsigned)(sp.units * sp.parts)), kThreads, Smem<DP>::kLaunch, st, 1, maps, kv, bt, q,
+                  sp.units, sp.parts, scratch, q_tokens, sp.ranked);
+  if (e != cudaSuccess) return e;
   *launches += 1;
   if (sp.parts > 1) {
-    // its blocks may start while the last ones above are still running, and wait for them there
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at{};
-    cfg.gridDim = dim3((unsigned)sp.units, kBlockRows / kJoinRows);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = st;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, k_kv_prompt_join<T, DP>, kv, bt, q, sp.parts, (const float*)scratch);
+    e = launch_next(k_kv_prompt_join<T, DP>, dim3((unsigned)sp.units, kBlockRows / kJoinRows), kJoinThreads, 0, st, 1, kv, bt, q,
+                    sp.parts, scratch);
     if (e != cudaSuccess) return e;
     *launches += 1;
   }

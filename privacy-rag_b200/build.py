@@ -2,20 +2,24 @@
 
 Usage: python privacy-rag_b200/build.py [--verbose]
 The library lands in privacy-rag_b200/lib/libbfvgpu.so, next to the Python mirror,
-so it travels with the repository snapshot to a GPU host.
+so it travels with the repository snapshot to a GPU host; beside it the module of PagedKv's
+calls on torch tensors (bfvgpu_kv_calls.so), compiled against the installed torch and Python.
 """
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "lib", "libbfvgpu.so")
 SOURCES = ["kernels.cu", "bfvgpu.cu", "noalloc.cu", "peak.cu", "kv_pages.cu", "kv_rows.cu", "kv_prompt.cu", "kv_attention.cu"]
+CALLS = os.path.join(PKG, "lib", "bfvgpu_kv_calls.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -30,7 +34,7 @@ def dependencies() -> list[str]:
     """Every file the library is compiled from: the sources, every header beside them and
     the public headers (a new header is picked up without editing this list)."""
     deps = [os.path.join(CSRC, f) for f in SOURCES]
-    deps += [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cuh", ".h"))]
+    deps += [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cuh", ".h", ".cpp"))]
     inc = os.path.join(ROOT, "include")  # the C ABI headers (the C++ adapters are header-only users)
     deps += [os.path.join(inc, f) for f in sorted(os.listdir(inc)) if f.endswith(".h")]
     deps.append(os.path.abspath(__file__))
@@ -38,10 +42,22 @@ def dependencies() -> list[str]:
 
 
 def stale() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(CALLS):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(CALLS))
     return any(os.path.getmtime(d) > t for d in dependencies())
+
+
+def calls_command() -> list[str]:
+    """Compiles and links kv_torch.cpp; the library's own symbols come from the libbfvgpu.so beside it."""
+    torch = os.path.join(importlib.util.find_spec("torch").submodule_search_locations[0])
+    cuda = os.path.dirname(os.path.dirname(nvcc())) if os.path.isabs(nvcc()) else "/usr/local/cuda"
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            "-isystem", os.path.join(torch, "include"), "-isystem", os.path.join(torch, "include/torch/csrc/api/include"),
+            "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
+            "-I", os.path.join(ROOT, "include"), os.path.join(CSRC, "kv_torch.cpp"), "-o", CALLS,
+            "-L", os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+            "-L", os.path.dirname(LIB), "-lbfvgpu", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -66,6 +82,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     subprocess.run(cmd, check=True)
     for o in objs:
         os.remove(o)
+    subprocess.run(calls_command(), check=True)
     return LIB
 
 

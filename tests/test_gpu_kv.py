@@ -401,6 +401,46 @@ def test_move_and_fork_reject_bad_numbers(bfv, ctx):
     assert torch.equal(before, cache.k)
 
 
+def test_refused_tensors(bfv, ctx):
+    """What the calls refuse before any launch: types, shapes, strides, devices, numbers out of 32 bits."""
+    cache = R.Cache(2, 64, 16, BF, [40, 9])
+    kv = bfv.PagedKv(ctx, cache.k, cache.v)
+    dev = dict(device="cuda")
+    table, lengths = cache.table.cuda(), torch.tensor([40, 9], dtype=torch.int32, **dev)
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, **dev)
+    q, k = torch.zeros(2, 4, 64, dtype=BF, **dev), torch.zeros(2, 2, 64, dtype=BF, **dev)
+    ids = torch.tensor([0, 1], dtype=torch.int32, **dev)
+    wide = torch.zeros(2, 4, 128, dtype=BF, **dev)
+    refused = [
+        lambda: kv.decode(q[:1], table, lengths), lambda: kv.decode(q[0], table, lengths),
+        lambda: kv.decode(wide, table, lengths), lambda: kv.decode(wide[..., ::2], table, lengths),
+        lambda: kv.decode(q.cpu(), table, lengths), lambda: kv.decode(q.half(), table, lengths),
+        lambda: kv.decode(q, table.cpu(), lengths), lambda: kv.decode(q, table.long(), lengths),
+        lambda: kv.decode(q, table.t(), lengths), lambda: kv.decode(q, table[0], lengths),
+        lambda: kv.decode(q, table, lengths[:1]), lambda: kv.decode(q, table, lengths.float()),
+        lambda: kv.decode(q, table, lengths, layer=1), lambda: kv.decode(q, table, lengths, window=-1),
+        lambda: kv.decode(q, table, lengths, scale=-1.0), lambda: kv.decode(q[:, :3], table, lengths),
+        lambda: kv.decode(q, table, lengths, out=q[:1]), lambda: kv.decode(q, table, lengths, out=q.half()),
+        lambda: kv.decode(q, table, lengths, out=wide[..., :64]),
+        lambda: kv.prompt(q, starts[:2], table, lengths), lambda: kv.prompt(q, starts.cpu(), table, lengths),
+        lambda: kv.append(k, k.half(), starts, table, lengths), lambda: kv.append(k.half(), k.half(), starts, table, lengths),
+        lambda: kv.append(k, k[:1], starts, table, lengths), lambda: kv.append(q, q, starts, table, lengths),
+        lambda: kv.append(k, k, starts[:2], table, lengths),
+        lambda: kv.fork(ids, ids[:1], ids, table, lengths), lambda: kv.fork(ids, ids, ids.long(), table, lengths),
+        lambda: kv.fork(ids, ids, ids, table, lengths[:1]),
+        lambda: kv.move(ids, ids[:1], table), lambda: kv.move(ids.cpu(), ids, table), lambda: kv.move(ids, ids, lengths),
+    ]
+    for i, call in enumerate(refused):
+        with pytest.raises(ValueError, match="E_KV_"):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    with pytest.raises(OverflowError):
+        kv.decode(q, table, lengths, window=1 << 40)
+    assert ctx.check() == 0
+    out = torch.empty_like(q)
+    assert kv.decode(q, table, lengths, out=out) is out
+
+
 # ---- streams, graphs, the whole cache -------------------------------------------------------------
 def test_other_stream_and_graph(bfv, ctx):
     """The calls on a side stream, and captured in a graph and replayed on new values, give the bits of

@@ -251,3 +251,32 @@ def test_paged_kv_refuses_host_tensors(bfv, host):
                        (z[0, 0], z[0, 0], "SHAPE")):
         with pytest.raises(ValueError, match="E_KV_" + text):
             bfv.PagedKv(host, k, v)
+
+
+def test_calls_refuse_host_tensors(bfv):
+    """The module of PagedKv's calls, on a made-up cache: what lies in host memory is refused before any use."""
+    torch = pytest.importorskip("torch")
+    import ctypes
+
+    from bfvgpu import kvcache
+    from bfvgpu._lib import KvDesc
+    calls = kvcache._calls()
+    desc = KvDesc(0x10000, 0x20000, 0, 1, 4, 2, 16, 64, 0, 2048, 1024, 64)
+    cache = calls.open(ctypes.addressof(desc), 0)
+    rows, ints = torch.zeros(3, 2, 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)
+    table = torch.zeros(3, 2, dtype=torch.int32)
+    for call in (lambda: calls.append(cache, None, rows, rows, None, table, ints, 0, None),
+                 lambda: calls.fork(cache, None, ints, ints, ints, table, ints, None),
+                 lambda: calls.move(cache, None, ints, ints, table, None),
+                 lambda: calls.decode(cache, None, rows, table, ints, 0, 0, 0, None, None, None),
+                 lambda: calls.prompt(cache, None, rows, ints, table, ints, 0, 0, 0, None, None, None)):
+        with pytest.raises(ValueError, match="E_KV_SHAPE.*on the cache's device"):
+            call()
+    with pytest.raises(TypeError, match="a tensor is wanted"):
+        calls.decode(cache, None, [1.0], table, ints, 0, 0, 0, None, None, None)
+    with pytest.raises(TypeError, match="arguments"):
+        calls.decode(cache, None, rows)
+    with pytest.raises(ValueError):  # not a cache
+        calls.move(object(), None, ints, ints, table, None)
+    with pytest.raises(ValueError, match="E_KV_ARGUMENT"):
+        calls.open(0, 0)

@@ -4,7 +4,7 @@
 // 16 bytes per thread and access, four accesses in flight per thread, all layers in one launch.
 // Measured: 17349 new tokens of 8 heads of 128 from 32 to 16 bits (213 MB) 36.4 us, 5.9 TB/s; 256 pages of 28
 // layers moved (939 MB) 144 us, 6.5 TB/s, as fast as a plain copy; 16 forks of 28 layers (59 MB, half of it
-// reads of one page that stay in L2) 9.9 us.  One token of 64 sequences takes 3.1 us, which is the latency of a
+// reads of one page that stay in L2) 7.7 us.  One token of 64 sequences takes 3.1 us, which is the latency of a
 // launch and of four dependent reads (length, table, source, store).
 #include "kv_host.h"
 
@@ -107,13 +107,35 @@ PageShape page_shape(const View& w) {
   return s;
 }
 
+// Blocks of a copy kernel per processor.  A page without gaps (WHOLE) needs no divisions and few registers.
+template <bool WHOLE>
+constexpr int kPerSm = WHOLE ? 8 : 6;
+// How often the threads move kInFlight chunks of such a page: twice in a fork, so that 16 of 28 layers are one wave
+// (7.7 us; 9.8 in three waves of once); a move is long (256 pages of 28 layers: 144 us with once, 146 with twice).
+constexpr int kForkBatches = 2;
+
 // The block's share `part` of page `from` -> page `to` of one layer's K or V.
+template <bool WHOLE>
 __device__ __forceinline__ void copy_share(uint16_t* base, int64_t page_stride, int32_t from, int32_t to,
-                                           const PageShape& s, int32_t part) {
+                                           const PageShape& s, int32_t part, int32_t batches) {
   const uint16_t* src = base + from * page_stride;
   uint16_t* dst = base + to * page_stride;
-  const int32_t chunks = s.rows * s.row_chunks, c0 = part * (kThreads * kInFlight) + threadIdx.x;
   uint4 x[kInFlight];
+  if constexpr (WHOLE) {
+    const int32_t chunks = s.row_chunks;
+    int32_t c = part * (kThreads * kInFlight * batches) + threadIdx.x;
+#pragma unroll 1
+    for (int b = 0; b < batches; ++b, c += kThreads * kInFlight) {
+#pragma unroll
+      for (int i = 0; i < kInFlight; ++i)
+        if (c + i * kThreads < chunks) x[i] = reinterpret_cast<const uint4*>(src)[c + i * kThreads];
+#pragma unroll
+      for (int i = 0; i < kInFlight; ++i)
+        if (c + i * kThreads < chunks) reinterpret_cast<uint4*>(dst)[c + i * kThreads] = x[i];
+    }
+    return;
+  }
+  const int32_t chunks = s.rows * s.row_chunks, c0 = part * (kThreads * kInFlight) + threadIdx.x;
   int64_t at[kInFlight];
 #pragma unroll
   for (int i = 0; i < kInFlight; ++i) {
@@ -131,18 +153,20 @@ __device__ __forceinline__ void copy_share(uint16_t* base, int64_t page_stride, 
 struct Copies {
   PageShape shape;
   int64_t layer_stride = 0;
-  int32_t layers = 0, parts = 0, count = 0;
+  int32_t layers = 0, parts = 0, count = 0, batches = 1;
   __host__ __device__ uint32_t per() const { return 2u * layers * parts; }  // blocks of a copy
 };
 
 // Share of a copy's blocks [layer][K, V][part of the page], part fastest.
+template <bool WHOLE>
 __device__ __forceinline__ void copy_block(const View& kv, const Copies& cp, uint32_t share, int32_t from, int32_t to) {
   const uint32_t rest = share / (uint32_t)cp.parts, part = share - rest * cp.parts;
   uint16_t* base = ((rest & 1) ? kv.v : kv.k) + (int64_t)(rest >> 1) * cp.layer_stride;
-  copy_share(base, kv.page_stride, from, to, cp.shape, (int32_t)part);
+  copy_share<WHOLE>(base, kv.page_stride, from, to, cp.shape, (int32_t)part, cp.batches);
 }
 
-__global__ void __launch_bounds__(kThreads)
+template <bool WHOLE>
+__global__ void __launch_bounds__(kThreads, kPerSm<WHOLE>)
     k_kv_move(View kv, Copies cp, const int32_t* src, const int32_t* dst, int32_t* table, int64_t entries,
               int64_t copy_blocks, uint32_t* err) {
   cudaGridDependencySynchronize();
@@ -153,7 +177,7 @@ __global__ void __launch_bounds__(kThreads)
       if (threadIdx.x == 0) flag_error(err, kErrTable);
       return;
     }
-    copy_block(kv, cp, blockIdx.x - c * cp.per(), from, to);
+    copy_block<WHOLE>(kv, cp, blockIdx.x - c * cp.per(), from, to);
     return;
   }
   // table entries: a binary search in src, which is strictly increasing
@@ -170,7 +194,8 @@ __global__ void __launch_bounds__(kThreads)
   if (lo < cp.count && src[lo] == page && (uint32_t)dst[lo] < (uint32_t)kv.pages) table[e] = dst[lo];
 }
 
-__global__ void __launch_bounds__(kThreads)
+template <bool WHOLE>
+__global__ void __launch_bounds__(kThreads, kPerSm<WHOLE>)
     k_kv_fork(View kv, Copies cp, const int32_t* parents, const int32_t* children, const int32_t* fresh,
               int32_t* table, int32_t rows, int32_t width, int32_t* lengths, uint32_t* err) {
   cudaGridDependencySynchronize();
@@ -200,16 +225,17 @@ __global__ void __launch_bounds__(kThreads)
     for (int32_t i = threadIdx.x; i < width; i += kThreads) out[i] = part && i == last ? to : row[i];
     if (threadIdx.x == 0) lengths[child] = n;
   }
-  if (part && from != to) copy_block(kv, cp, share, from, to);
+  if (part && from != to) copy_block<WHOLE>(kv, cp, share, from, to);
 }
 
-Copies copies_of(const View& w, const bfvgpu_kv* c, uint64_t count) {
+Copies copies_of(const View& w, const bfvgpu_kv* c, uint64_t count, int32_t batches) {
   Copies cp;
   cp.shape = page_shape(w);
   cp.layers = c->layers;
   cp.layer_stride = c->layers > 1 ? c->layer_stride : 0;
   cp.count = (int32_t)count;
-  const int64_t per = (int64_t)kThreads * kInFlight;
+  cp.batches = cp.shape.rows == 1 ? batches : 1;
+  const int64_t per = (int64_t)kThreads * kInFlight * cp.batches;
   cp.parts = (int32_t)((cp.shape.chunks() + per - 1) / per);
   return cp;
 }
@@ -272,11 +298,11 @@ extern "C" int32_t bfvgpu_kv_fork_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache
     const Place at = checked_place(ctx, stream);
     if (!count) return;
     need(parents && children && fresh && table && width && lengths, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
-    const Copies cp = copies_of(w, cache, count);
+    const Copies cp = copies_of(w, cache, count, kForkBatches);
     const int64_t blocks = (int64_t)count * 2 * cp.layers * cp.parts;
     need(blocks <= kMostBlocks, BFVGPU_E_SHAPE, "E_KV_SHAPE");
     OnDevice scope(at.device);
-    cuda_need(launch_next(k_kv_fork, dim3((unsigned)blocks), kThreads, 0, at.stream, 1, w, cp, parents, children, fresh, table,
+    cuda_need(launch_next(cp.shape.rows == 1 ? k_kv_fork<true> : k_kv_fork<false>, dim3((unsigned)blocks), kThreads, 0, at.stream, 1, w, cp, parents, children, fresh, table,
                           (int32_t)rows, (int32_t)width, lengths, at.err),
               "kv fork");
     internal_count_launch(1);
@@ -292,13 +318,13 @@ extern "C" int32_t bfvgpu_kv_move_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache
     const Place at = checked_place(ctx, stream);
     if (!count) return;
     need(src && dst && (table || !rows || !width), BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
-    const Copies cp = copies_of(w, cache, count);
+    const Copies cp = copies_of(w, cache, count, 1);
     const int64_t entries = table ? (int64_t)rows * (int64_t)width : 0;
     const int64_t copy_blocks = (int64_t)count * 2 * cp.layers * cp.parts;
     const int64_t blocks = copy_blocks + (entries + kThreads - 1) / kThreads;
     need(blocks <= kMostBlocks, BFVGPU_E_SHAPE, "E_KV_SHAPE");
     OnDevice scope(at.device);
-    cuda_need(launch_next(k_kv_move, dim3((unsigned)blocks), kThreads, 0, at.stream, 1, w, cp, src, dst, table, entries, copy_blocks,
+    cuda_need(launch_next(cp.shape.rows == 1 ? k_kv_move<true> : k_kv_move<false>, dim3((unsigned)blocks), kThreads, 0, at.stream, 1, w, cp, src, dst, table, entries, copy_blocks,
                           at.err),
               "kv move");
     internal_count_launch(1);

@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // takes many cycles, so the rows must not have to wait for them: S of the next key tile follows as
     // soon as its columns have been read, not when this tile's weights are used up. ----
     const uint32_t tm = same(tmem);
-    const uint32_t q_desc = same(operand(base + S::kQ, 16)), k_desc = operand(base + S::kK, 16);
+    const uint32_t q_desc = same(operand(base + S::kQ, 16)), q_desc1 = same(operand(base + S::kQ + S::kTileBytes, 16)), k_desc = operand(base + S::kK, 16);
     uint32_t turn = 0, q_turn = 0;                 // key tiles so far; bit t: turns of tile t's queries
     uint32_t read_turn = 0x3, last = 0;            // bit t: parity of the last phase of s_read[t]; tile of the last S
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -561,18 +561,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t st = turn % S::kStages;
         wait(k_full + 8 * st, (turn / S::kStages) & 1);
         const uint32_t b = same(k_desc + st * (S::kTileBytes >> 4));
-#pragma unroll 1
+#pragma unroll
         for (uint32_t t = 0; t < 2; ++t) {
           const Span& span = it.span[t];
           if (!same(span.needs(i))) continue;
           if (same(i == span.start())) wait(q_full + 8 * t, q_turn >> t & 1);
+          // all that can be is worked out before the wait: the rows wait for what stands behind it
+          const bool early = span.at_or_after(i + 1) >= to;
           wait(s_read + 8 * last, read_turn >> last & 1);  // the S before has been read
           if (!ok) break;
           last = t;
           read_turn ^= 1u << t;
-          const bool end = same(span.at_or_after(i + 1) >= to);
+          const bool end = same(early);
           if (end) q_turn ^= 1u << t;
-          const uint32_t a = same(q_desc + t * (S::kTileBytes >> 4)), d = tm;
+          const uint32_t a = t ? q_desc1 : q_desc, d = tm;
           fence_after();
           if (elected()) {
 #pragma unroll

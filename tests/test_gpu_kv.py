@@ -540,3 +540,25 @@ def test_cache_of_forked_sequences(bfv, ctx, window, sinks):
     step({r: 1 for r in history})  # every row one token: the single-token form
     assert torch.equal(cache.table.cpu(), torch.from_numpy(cache.book.table))
     assert torch.equal(cache.lengths.cpu(), torch.from_numpy(cache.book.lengths))
+
+
+@pytest.mark.parametrize("layout", ["hnd", "nhd", "gaps"])
+@pytest.mark.parametrize("heads,dim", [(3, 40), (1, 8), (5, 128)])
+def test_fork_and_move_of_large_pages(bfv, ctx, layout, heads, dim):
+    """Pages of several shares of the copy kernels, the last one partly filled, and of less than one."""
+    cache = R.Cache(heads, dim, 256, BF, [300, 0], layers=2, layout=layout, spare=3, width=2)
+    _fill(cache, torch.Generator().manual_seed(9))
+    want_k, want_v = cache.k.clone(), cache.v.clone()
+    fresh, to = cache.spare[:1].clone(), cache.spare[1:2].clone()
+    first, last = cache.table[0, :1].clone(), cache.table[0, 1:2].clone()
+    for x in (want_k, want_v):
+        x[:, fresh.long()] = x[:, last.long()]
+        x[:, to.long()] = x[:, first.long()]
+    table, lengths = cache.table.cuda(), torch.tensor([300, 0], dtype=torch.int32, device="cuda")
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    kv = bfv.PagedKv(ctx, cache.k, cache.v)
+    kv.fork(ints([0]), ints([1]), fresh.cuda(), table, lengths)
+    kv.move(first.cuda(), to.cuda(), table)
+    assert ctx.check() == 0
+    assert table.tolist() == [[int(to), int(last)], [int(to), int(fresh)]] and lengths.tolist() == [300, 300]
+    assert torch.equal(cache.k, want_k) and torch.equal(cache.v, want_v)

@@ -22,6 +22,12 @@
 // hold NaN (unwritten rest of a page, pages given up), and 0 x NaN would reach every row.  Such
 // pages are read in rows, the others filled with zeros.
 //
+// What bounds it: of a pair of row tiles and 128 keys the exponentials take 2048 cycles of the special-function pipe,
+// with 128 dims the products as many of the tensor pipe; measured 2500 cycles with 64 dims, 3000 with 128.  16384
+// tokens, 16 query heads on 8 of 128: 835 us, 1320 TFLOP/s (950 us once the power limit lowers the clock); of 64: 615
+// us; 8191 tokens with a window of 1024: 85 us; eight prompts of 512: 23 us, most of it the start of the blocks
+// (first S 3.3 us after it) and the results (2 us after the last product).
+//
 // Where there are too few rows to fill the GPU, the key tiles of a block's rows are dealt to several
 // blocks, which leave (m, sum, O) in 32 bits for a second kernel to join in a fixed order.
 #include <cuda.h>
@@ -381,6 +387,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kLoadWarp && lane < sizeof(Maps) / sizeof(CUtensorMap))
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.q) + lane * sizeof(CUtensorMap)) : "memory");
   if (warp == kScoreWarp) {
+    // not before the kernel ahead has ended: a block of it on this SM might still want tensor memory
+    cudaGridDependencySynchronize();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -567,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!same(span.needs(i))) continue;
           if (same(i == span.start())) wait(q_full + 8 * t, q_turn >> t & 1);
           // all that can be is worked out before the wait: the rows wait for what stands behind it
-          const bool early = span.at_or_after(i + 1) >= to;
+          const bool early = span.at_or_after(i + 1) >= to;  // before the wait: the rows wait for what stands behind it
           wait(s_read + 8 * last, read_turn >> last & 1);  // the S before has been read
           if (!ok) break;
           last = t;

@@ -26,19 +26,25 @@ int sm_count(int device) {
   return n;
 }
 
-// Single tokens go to the row kernel, which reads a sequence's keys once per 16 query rows; so do prompts of
-// up to 16 rows per sequence and key head on average (64 sequences of 4096 tokens, 2 to 16 rows each: 184 to
-// 205 us, the prompt kernel 218 to 221), and those whose rows times keys are few, where the prompt kernel's
-// start counts.  At 512 keys, 32, 64, 128 and 256 rows: 9, 10, 13 and 15 us against 13, 13, 13 and 16; at 8192
-// keys, 16 and 32 rows: 23 and 33 against 26 and 30; with 64 dims, 64 rows: 24 against 24.
-constexpr int64_t kFewRows = 16;
-constexpr double kFewProducts = 20e6;  // 16-row blocks x keys x padded dims
+// Single tokens go to the row kernel, which reads a sequence's keys once per 16 query rows.  Prompts go there
+// * where 16-row blocks x (keys + 200) x dims are few, that is, where the start of the prompt kernel counts more than
+//   what its tiles save (at 512 keys of 128 dims and 8 key heads, 32, 64 and 128 rows: 9, 10 and 13 us against 13, 13
+//   and 13; 4 sequences of 198 tokens with a window of 14, 4 key heads of 8 query heads: 42 us against 12), and
+// * up to 16 rows per sequence and key head on average with up to 64 dims, where its blocks stream the keys (64
+//   sequences of 5384 tokens, 16 rows: 98 us against 133), and up to 4 with more, where they multiply for longer
+//   (128 sequences of 3469 tokens, 32 rows: 350 us against 171; 100 of 7585, 16 rows: 208 against 164).
+// Over 130 prompts of 1 to 128 sequences, 2 to 1000 tokens and up to 16384 keys the choice cost 0.8 % of the time on
+// average, always the prompt kernel 13 %, always the row kernel 43 %.
+constexpr int64_t kFewRows = 16, kFewRowsWide = 4;
+constexpr double kFewProducts = 8e6;
+constexpr int64_t kStartKeys = 200;
 bool few_rows(const View& kv, const Batch& bt, const Query& q, bool ragged) {
-  if (!ragged || (int64_t)q.tokens * q.group <= kFewRows * bt.seqs) return true;
+  const bool wide = kv.dim > 64;
+  if (!ragged || (int64_t)q.tokens * q.group <= (wide ? kFewRowsWide : kFewRows) * bt.seqs) return true;
   int64_t keys = (int64_t)bt.width << kv.page_log;
   if (q.window) keys = std::min<int64_t>(keys, (int64_t)q.window + q.sinks);
   const int64_t blocks = ((int64_t)q.tokens * q.group / 16 + bt.seqs) * kv.heads;
-  return (double)blocks * (double)keys * (kv.dim <= 64 ? 64 : 128) <= kFewProducts;
+  return (double)blocks * (double)(keys + kStartKeys) * (wide ? 128 : 64) <= kFewProducts;
 }
 
 struct Call {

@@ -133,11 +133,6 @@ __global__ void __launch_bounds__(kThreads)
   }
 
   const uint32_t base = smem_addr(ring) + warp * R::kWarpBytes;
-  if (kv.dim != DP) {  // the chunks past the head's dims are never copied: zeros
-    for (int i = lane; i < R::kWarpBytes / 16; i += 32)
-      *reinterpret_cast<uint4*>(ring + warp * R::kWarpBytes + i * 16) = make_uint4(0, 0, 0, 0);
-    __syncwarp();
-  }
 
   // lane l looks up the page of key l % 16 of a stage, one stage ahead of its copies
   const int32_t* row_of_table = bt.table + (int64_t)un.b * bt.width;
@@ -188,6 +183,11 @@ __global__ void __launch_bounds__(kThreads)
 
 #pragma unroll
   for (int i = 0; i < R::kStages - 1; ++i) issue(s0 + warp + i * kWarps, i);
+  if (kv.dim != DP) {  // the chunks past the head's dims are never copied: zeros, while the first copies are on their way
+    for (int r = lane; r < R::kStages * 2 * kKeys; r += 32)
+      for (int c = kv.dim / 8; c < DP / 8; ++c)
+        *reinterpret_cast<uint4*>(ring + warp * R::kWarpBytes + r * R::kRowBytes + ((c ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+  }
   int slot = 0;
   for (int32_t s = s0 + warp; s < s1; s += kWarps) {
     // the slot filled next was read in the last step

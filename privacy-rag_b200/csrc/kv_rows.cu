@@ -97,9 +97,11 @@ __device__ __forceinline__ uint32_t pack_rest(float x, float y, uint32_t hi) {
   return T::pack(x - h.x, y - h.y);
 }
 
+// NK: 16-dim steps of the products, of a ring whose rows have DP dims (256 sequences of 2048 tokens of 72 and 96 dims:
+// 157 and 155 us with the eight steps of 128, 140 both with six).
 // PAIR: at most 8 rows.  The upper 8 rows of the products then carry what p loses in 16 bits (p = hi
 // + lo), so o keeps about 16 bits of p at no cost; with more rows a second product does the same.
-template <class T, int DP, bool PAIR>
+template <class T, int DP, bool PAIR, int NK>
 __global__ void __launch_bounds__(kThreads)
     k_kv_rows(View kv, Batch bt, Query q, int32_t cluster, int32_t parts, float* scratch) {
   using R = Ring<DP>;
@@ -118,13 +120,13 @@ __global__ void __launch_bounds__(kThreads)
   const int32_t s0 = share * per + min(share, more), s1 = s0 + per + (share < more);
 
   // query fragments (rows past the unit's and dims past the head's are 0)
-  uint32_t qa[DP / 16][4];
+  uint32_t qa[NK][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const bool in = quad + 8 * h < un.rows;
     const uint16_t* p = un.query(q, quad + 8 * h);
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks)
+    for (int ks = 0; ks < NK; ++ks)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int32_t d = ks * 16 + c * 8 + pair;
@@ -169,9 +171,9 @@ __global__ void __launch_bounds__(kThreads)
     copies_commit();
   };
 
-  float o[DP / 8][4];
+  float o[NK * 2][4];
 #pragma unroll
-  for (int i = 0; i < DP / 8; ++i)
+  for (int i = 0; i < NK * 2; ++i)
 #pragma unroll
     for (int c = 0; c < 4; ++c) o[i][c] = 0;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
@@ -183,9 +185,9 @@ __global__ void __launch_bounds__(kThreads)
 
 #pragma unroll
   for (int i = 0; i < R::kStages - 1; ++i) issue(s0 + warp + i * kWarps, i);
-  if (kv.dim != DP) {  // the chunks past the head's dims are never copied: zeros, while the first copies are on their way
+  if (kv.dim != NK * 16) {  // the chunks past the head's dims are never copied: zeros, while the first copies are on their way
     for (int r = lane; r < R::kStages * 2 * kKeys; r += 32)
-      for (int c = kv.dim / 8; c < DP / 8; ++c)
+      for (int c = kv.dim / 8; c < NK * 2; ++c)
         *reinterpret_cast<uint4*>(ring + warp * R::kWarpBytes + r * R::kRowBytes + ((c ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
   }
   int slot = 0;
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int i = 0; i < 4; ++i) c[t][i] = 0;
     const int mat = lane >> 3, r8 = lane & 7;
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
+    for (int ks = 0; ks < NK; ++ks) {
       uint32_t b[4];
       ldsm4(b, kt + ((mat >> 1) * 8 + r8) * R::kRowBytes + (((ks * 2 + (mat & 1)) ^ r8) << 4));
       mma<T>(c[0], qa[ks], b[0], b[1]);
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(kThreads)
       }
       if (PAIR) f[1] = f[0];
 #pragma unroll
-      for (int i = 0; i < DP / 8; ++i) {
+      for (int i = 0; i < NK * 2; ++i) {
         o[i][0] *= f[0];
         o[i][1] *= f[0];
         o[i][2] *= f[1];
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(kThreads)
         if (PAIR) hi[2 * t + 1] = lo[2 * t];
       }
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
+    for (int ks = 0; ks < NK; ++ks) {
       uint32_t b[4];
       ldsm4t(b, vt + ((mat & 1) * 8 + r8) * R::kRowBytes + (((ks * 2 + (mat >> 1)) ^ r8) << 4));
       mma<T>(o[2 * ks], hi, b[0], b[1]);
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(kThreads)
     const int row = quad + 8 * h;
     float* to = res + (warp * kRows + row) * DP;
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i) {
+    for (int i = 0; i < NK * 2; ++i) {
       const float a = PAIR ? o[i][0] + o[i][2] : o[i][2 * h], b = PAIR ? o[i][1] + o[i][3] : o[i][2 * h + 1];
       *reinterpret_cast<float2*>(to + i * 8 + pair) = make_float2(a, b);
     }
@@ -425,11 +427,11 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kDevices = 64;
 
 // The shared-memory limit is an attribute of the function on a device.
-template <class T, int DP, bool PAIR>
+template <class T, int DP, bool PAIR, int NK>
 cudaError_t allow_ring(int device) {
   static std::atomic<uint64_t> allowed{0};
   if (device < kDevices && (allowed.load() >> device & 1)) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(k_kv_rows<T, DP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DP>::kBytes);
+  const cudaError_t e = cudaFuncSetAttribute(k_kv_rows<T, DP, PAIR, NK>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DP>::kBytes);
   if (e == cudaSuccess && device < kDevices) allowed.fetch_or(uint64_t(1) << device);
   return e;
 }
@@ -447,14 +449,14 @@ void configure(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* at, int64_t blocks,
   cfg->numAttrs = 1;
 }
 
-template <class T, int DP, bool PAIR>
+template <class T, int DP, bool PAIR, int NK>
 cudaError_t launch(const View& kv, const Batch& bt, const Query& q, const RowSplit& sp, float* scratch, cudaStream_t st,
                    int* launches) {
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = allow_ring<T, DP, PAIR>(device);
+  if (e == cudaSuccess) e = allow_ring<T, DP, PAIR, NK>(device);
   if (e != cudaSuccess) return e;
-  e = launch_next(k_kv_rows<T, DP, PAIR>, dim3((unsigned)(sp.blocks16 * sp.parts * sp.cluster)), kThreads, Ring<DP>::kBytes, st,
+  e = launch_next(k_kv_rows<T, DP, PAIR, NK>, dim3((unsigned)(sp.blocks16 * sp.parts * sp.cluster)), kThreads, Ring<DP>::kBytes, st,
                   sp.cluster, kv, bt, q, sp.cluster, sp.parts, scratch);
   if (e != cudaSuccess) return e;
   *launches += 1;
@@ -480,8 +482,8 @@ int64_t resident_clusters(int device, int log) {
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
     configure<DP>(&cfg, &at, 1 << log, 1 << log, nullptr);
-    if (allow_ring<Bf16, DP, true>(device) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, k_kv_rows<Bf16, DP, true>, &cfg) != cudaSuccess || n < 1) {
+    if (allow_ring<Bf16, DP, true, DP / 16>(device) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_kv_rows<Bf16, DP, true, DP / 16>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = given[log];
     }
@@ -495,10 +497,13 @@ cudaError_t launch_typed(const View& kv, const Batch& bt, const Query& q, const 
                          cudaStream_t st, int* launches) {
   const bool pair = !bt.starts && q.group <= 8;
   if (sp.dim_padded == 64)
-    return pair ? launch<T, 64, true>(kv, bt, q, sp, scratch, st, launches)
-                : launch<T, 64, false>(kv, bt, q, sp, scratch, st, launches);
-  return pair ? launch<T, 128, true>(kv, bt, q, sp, scratch, st, launches)
-              : launch<T, 128, false>(kv, bt, q, sp, scratch, st, launches);
+    return pair ? launch<T, 64, true, 4>(kv, bt, q, sp, scratch, st, launches)
+                : launch<T, 64, false, 4>(kv, bt, q, sp, scratch, st, launches);
+  if (kv.dim <= 96)
+    return pair ? launch<T, 128, true, 6>(kv, bt, q, sp, scratch, st, launches)
+                : launch<T, 128, false, 6>(kv, bt, q, sp, scratch, st, launches);
+  return pair ? launch<T, 128, true, 8>(kv, bt, q, sp, scratch, st, launches)
+              : launch<T, 128, false, 8>(kv, bt, q, sp, scratch, st, launches);
 }
 
 }  // namespace

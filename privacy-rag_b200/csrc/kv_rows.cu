@@ -515,7 +515,9 @@ uint64_t RowSplit::scratch_floats() const {
 // Shares of the keys, by an estimate in keys that one block streams while all are busy: a block costs its
 // share plus kStart (start, first loads, joins: 6 us against 23 ns a key, measured with 2048 units of
 // 2048 keys in 1 to 8 shares: 167, 195, 269, 444 us), and blocks run in waves of what is resident
-// (whole waves up to two, after that they mix).  One unit's further parts cost a second kernel, kJoin.
+// (up to two waves they mix in part, after that wholly: lengths differ, and where they do not the blocks of a part-filled
+// wave are the faster for it; 12 sequences of up to 16000 keys, 4 key heads: 68 us in 4 shares, one wave, 46 in 8; 119 of up
+// to 8670, one key head: 74 in 2, 61 in 4).  One unit's further parts cost a second kernel, kJoin.
 // 16 sequences of 1024 keys and 8 key heads: 20, 17, 22 us in 1, 2, 4 shares; 131071 keys and 4 key heads:
 // 55 us in 8 x 8 shares, which are resident together, 82 us in 8 x 9, which are not.
 RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int device) {
@@ -535,7 +537,7 @@ RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int device) 
   double best = 0;
   for (int log = 0; 1 << log <= kMaxCluster; ++log) {
     const double fill = (double)sp.blocks16 / resident(log);
-    const double time = (fill < 2 ? std::ceil(fill) : fill) * ((double)keys / (1 << log) + kStart);
+    const double time = (fill > 1 && fill < 2 ? (fill + 2) / 2 : std::max(fill, 1.0)) * ((double)keys / (1 << log) + kStart);
     if (log && time >= best) continue;
     best = time;
     sp.cluster = 1 << log;

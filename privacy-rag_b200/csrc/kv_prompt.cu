@@ -771,7 +771,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float b = j + 1 < 16 ? x[(j + 1) / 8 & 1][(j + 1) % 8 * 4 + 2 * r + e] : -INFINITY;
               top[e] = fmaxf(fmaxf(top[e], a), b);
             }
-          now[r] = fmaxf(top[0], top[1]) * c;
+          // rows past the last hold the scores of whatever query lay there before: they must not move the others' m
+          now[r] = t * kTileRows + row0 + 8 * r < un.rows ? fmaxf(top[0], top[1]) * c : -INFINITY;
         }
         // of the thread's scores; those of the whole rows are of interest only where some exceed m by too much
         if (__any_sync(0xffffffffu, fresh || now[0] > m[0] + kLag || now[1] > m[1] + kLag)) {

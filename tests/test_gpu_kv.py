@@ -441,6 +441,16 @@ def test_refused_tensors(bfv, ctx):
     assert kv.decode(q, table, lengths, out=out) is out
 
 
+@pytest.mark.parametrize("dim,window,sinks", [(112, 0, 0), (64, 0, 0), (128, 3, 2)])
+def test_rows_past_the_last_change_nothing(bfv, ctx, dim, window, sinks):
+    """Many prompts of odd lengths whose query heads do not fill a block's rows, with scores that move the reference
+    exponent often: what the unused rows held before must not show in the others, not even in the last bit."""
+    lens = [(17, 16), (257, 257), (127, 1), (200, 200), (256, 1), (17, 17), (128, 16), (255, 255), (0, 0), (1, 1), (511, 128),
+            (300, 33), (640, 2), (63, 0), (31, 31), (257, 3), (128, 100), (127, 127), (127, 64), (64, 64), (257, 128),
+            (256, 256), (16, 16), (129, 0), (255, 16), (300, 100), (31, 31), (129, 64), (127, 33)]
+    run_attention(bfv, ctx, "prompt", BF, lens, 3, 9, dim, 16, window, sinks, spread=4.0)
+
+
 # ---- streams, graphs, the whole cache -------------------------------------------------------------
 def test_other_stream_and_graph(bfv, ctx):
     """The calls on a side stream, and captured in a graph and replayed on new values, give the bits of

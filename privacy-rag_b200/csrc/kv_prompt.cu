@@ -25,7 +25,7 @@
 // What bounds it: of a pair of row tiles and 128 keys the exponentials take 2048 cycles of the special-function pipe,
 // with 128 dims the products as many of the tensor pipe; measured 2500 cycles with 64 dims, 3000 with 128.  16384
 // tokens, 16 query heads on 8 of 128: 835 us, 1320 TFLOP/s (950 us once the power limit lowers the clock); of 64: 615
-// us; 8191 tokens with a window of 1024: 85 us; eight prompts of 512: 23 us, most of it the start of the blocks
+// us; 8191 tokens with a window of 1024: 87 us; eight prompts of 512: 23 us, most of it the start of the blocks
 // (first S 3.3 us after it) and the results (2 us after the last product).
 //
 // Where there are too few rows to fill the GPU, the key tiles of a block's rows are dealt to several
@@ -728,6 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int32_t pos[2];
       for (int r = 0; r < 2; ++r) pos[r] = un.position(q, min(t * kTileRows + row0 + 8 * r, un.rows - 1));
       const int32_t lo = __shfl_sync(0xffffffffu, pos[0], 0), hi = __shfl_sync(0xffffffffu, pos[1], 31);
+      const int32_t alive = un.rows - t * kTileRows;  // rows of the tile
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
       bool fresh = true;
       for (int32_t i = span.start(); i < span.end; i = span.at_or_after(i + 1)) {
@@ -772,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               top[e] = fmaxf(fmaxf(top[e], a), b);
             }
           // rows past the last hold the scores of whatever query lay there before: they must not move the others' m
-          now[r] = t * kTileRows + row0 + 8 * r < un.rows ? fmaxf(top[0], top[1]) * c : -INFINITY;
+          now[r] = row0 + 8 * r < alive ? fmaxf(top[0], top[1]) * c : -INFINITY;
         }
         // of the thread's scores; those of the whole rows are of interest only where some exceed m by too much
         if (__any_sync(0xffffffffu, fresh || now[0] > m[0] + kLag || now[1] > m[1] + kLag)) {

@@ -63,8 +63,14 @@ class PagedKv:
         st = k.stride()
         desc = KvDesc(k.data_ptr(), v.data_ptr(), 0 if k.dtype == torch.bfloat16 else 1, self.layers, self.pages, self.heads,
                       self.page_tokens, self.dim, st[0], st[1], st[2], st[3])
-        self._calls, self._handle = _calls(), ctx.handle.value
+        self._calls = _calls()
         self._cache = self._calls.open(ctypes.addressof(desc), ctx.device)
+
+    @property
+    def _handle(self) -> int | None:
+        """The context as it is now: None once it is closed, which the calls refuse."""
+        h = self.ctx.handle
+        return h.value if h is not None else None
 
     # ---- device calls ----
     def append(self, k_new, v_new, starts, table, lengths, layer: int = 0, stream: int | None = None) -> None:

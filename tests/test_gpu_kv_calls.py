@@ -1,0 +1,59 @@
+"""The calls of PagedKv on the GPU: contexts, streams, strides and starts that need care."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import kv_reference as R  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+@pytest.fixture
+def ctx(bfv):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    c = bfv.Context(4096, bfv.find_primes(4096, [36, 36, 37]), 2, 1, 65537, device=0)
+    yield c
+    c.close()
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def randn(gen, *shape, dtype=BF):
+    return torch.randn(*shape, generator=gen).to(dtype)
+
+
+def filled(bfv, ctx, lengths, heads=2, dim=64, page=16, dtype=BF, seed=3, **kw):
+    """(PagedKv, its pages, table, lengths, [(k, v)] on the CPU)."""
+    gen = torch.Generator().manual_seed(seed)
+    cache = R.Cache(heads, dim, page, dtype, lengths, **kw)
+    held = [(randn(gen, n, heads, dim, dtype=dtype), randn(gen, n, heads, dim, dtype=dtype)) for n in lengths]
+    for s, (k, v) in enumerate(held):
+        cache.put(s, k, v)
+    return bfv.PagedKv(ctx, cache.k, cache.v), cache, cache.table.cuda(), ints(lengths), held
+
+
+def check(got, want, bound):
+    got = got.double().cpu()
+    assert torch.isfinite(got).all()
+    over = ((got - want).abs() / bound).max().item()
+    assert over <= 1.0, f"error is {over:.3f} of the bound"
+
+
+def test_a_closed_context_is_refused(bfv, ctx):
+    kv, cache, table, lengths, _ = filled(bfv, ctx, [40, 9])
+    q = torch.zeros(2, 4, 64, dtype=BF, device="cuda")
+    one = ints([0])
+    kv.decode(q, table, lengths)
+    assert ctx.check() == 0
+    ctx.close()
+    for call in (lambda: kv.append(q[:, :2], q[:, 2:], None, table, lengths), lambda: kv.decode(q, table, lengths),
+                 lambda: kv.prompt(q, ints([0, 1, 2]), table, lengths), lambda: kv.fork(one, one, one, table, lengths),
+                 lambda: kv.move(one, one, table)):
+        with pytest.raises(bfv.BfvGpuInvalidArgument, match="E_BFVGPU_ARGUMENT"):
+            call()

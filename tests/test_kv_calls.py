@@ -1,0 +1,61 @@
+"""What PagedKv hands to its calls, without a GPU."""
+from __future__ import annotations
+
+import types
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+ARGUMENT = 1
+
+
+class Pages:
+    """What PagedKv asks of a tensor of pages."""
+
+    shape, dtype = (1, 4, 2, 16, 64), torch.bfloat16
+    device = types.SimpleNamespace(type="cuda", index=-1)
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, axis=None):
+        strides = 8192, 2048, 1024, 64, 1
+        return strides if axis is None else strides[axis]
+
+    def data_ptr(self):
+        return 0x10000
+
+
+def test_a_closed_context_is_not_used(bfv, monkeypatch):
+    """Every call hands over the context as it is then: none once it is closed, which the C ABI refuses."""
+    from bfvgpu import kvcache
+    given = []
+
+    class Calls:
+        def open(self, *a):
+            return "cache"
+
+        def __getattr__(self, name):
+            def call(cache, ctx, *rest):
+                given.append(ctx)
+                return 0 if ctx else bfv.lib().bfvgpu_kv_append_device(None, bfv._lib.KvDesc(
+                    0x10000, 0x10000, 0, 1, 4, 2, 16, 64, 8192, 2048, 1024, 64), 0, None, None, 0, 0, 0, 0, None, None, 0,
+                    None, 0, None)
+            return call
+
+    monkeypatch.setattr(kvcache, "_module", Calls())
+    ctx = bfv.Context(4096, bfv.find_primes(4096, [36, 36, 37]), 2, 1, 65537, device=-1)
+    kv = bfv.PagedKv(ctx, Pages(), Pages())
+    calls = [lambda: kv.append(1, 2, 3, 4, 5), lambda: kv.fork(1, 2, 3, 4, 5), lambda: kv.move(1, 2),
+             lambda: kv.decode(1, 2, 3), lambda: kv.prompt(1, 2, 3, 4)]
+    for call in calls:
+        call()
+    assert given == [ctx.handle.value] * len(calls)
+    ctx.close()
+    given.clear()
+    for call in calls:
+        with pytest.raises(bfv.BfvGpuInvalidArgument, match="E_BFVGPU_ARGUMENT") as refused:
+            call()
+        assert refused.value.code == ARGUMENT
+    assert given == [None] * len(calls)

@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(kThreads)
   else __syncthreads();
   for (int32_t e = (rank * kThreads + threadIdx.x) * 2; e < live; e += cluster * kThreads * 2) {
     const int32_t row = e / DP, d = e % DP;
+    if (d >= kv.dim) continue;  // padding: nobody reads it
     // all blocks' numbers asked for together: each is a round trip to another processor
     float2 mlc[kMaxCluster], vc[kMaxCluster];
 #pragma unroll
@@ -355,22 +356,17 @@ __global__ void __launch_bounds__(kThreads)
       v1 += f * vc[c].y;
     }
     if (parts == 1) {
-      if (d < kv.dim) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key seen: zeros
-        *reinterpret_cast<uint32_t*>(un.result(kv, q, row) + d) = T::pack(v0 * inv, v1 * inv);
-      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key seen: zeros
+      *reinterpret_cast<uint32_t*>(un.result(kv, q, row) + d) = T::pack(v0 * inv, v1 * inv);
     } else {
       float* to = scratch + ((int64_t)u * parts + part) * (kRows * (DP + 2));
       *reinterpret_cast<float2*>(to + e) = make_float2(v0, v1);
       if (d == 0) *reinterpret_cast<float2*>(to + kRows * DP + row * 2) = make_float2(top, sum);
     }
   }
-  if (cluster > 1) {
-    // No block leaves while another reads its shared memory.  What was read has been used in the stores
-    // above; relaxed, because the barrier need not wait for the stores themselves.
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-  }
+  // No block leaves while another reads its shared memory: every read is released by this arrival.  (A relaxed arrival,
+  // which orders no read, saved 0.25 us: one of 513 tokens 5.7 us against 5.95, 64 of up to 4096 101 against 102.)
+  if (cluster > 1) cl.sync();
 }
 
 // Joins the parts of a unit's rows, in order: a warp per row, four rows a block.

@@ -57,3 +57,33 @@ def test_a_closed_context_is_refused(bfv, ctx):
                  lambda: kv.move(one, one, table)):
         with pytest.raises(bfv.BfvGpuInvalidArgument, match="E_BFVGPU_ARGUMENT"):
             call()
+
+
+@pytest.mark.parametrize("dim", [8, 40, 56, 64, 72, 88, 104, 120, 128])
+@pytest.mark.parametrize("seqs,group", [(1, 1), (1, 16), (5, 2), (12, 9), (40, 3)])
+def test_blocks_that_share_keys(bfv, ctx, dim, seqs, group):
+    """Eight, four, two blocks and one for a key head, with dims that fill the padded rows and dims that do not: every block
+    is there until the others have read its part.  Many calls in a row give the same bits."""
+    heads, length = 8, 300
+    lens = [length - 7 * s % 290 for s in range(seqs)]
+    kv, cache, table, lengths, held = filled(bfv, ctx, lens, heads, dim)
+    q = randn(torch.Generator().manual_seed(5), seqs, heads * group, dim)
+    first = kv.decode(q.cuda(), table, lengths)
+    rest = [kv.decode(q.cuda(), table, lengths) for _ in range(20)]
+    assert ctx.check() == 0
+    assert all(torch.equal(first, x) for x in rest)
+    for s in range(0, seqs, 4):
+        want, bound = R.attention(q[s:s + 1], *held[s], lens[s], 0, 0, dim ** -0.5, two_terms=True)
+        check(first[s:s + 1], want, bound)
+
+
+@pytest.mark.parametrize("dim", [24, 72, 128])
+def test_blocks_that_share_keys_in_parts(bfv, ctx, dim):
+    """One sequence long enough for several groups of eight blocks, whose parts another kernel joins."""
+    kv, cache, table, lengths, held = filled(bfv, ctx, [9000], 1, dim, page=64)
+    q = randn(torch.Generator().manual_seed(5), 1, 12, dim)
+    first = kv.decode(q.cuda(), table, lengths)
+    assert all(torch.equal(first, kv.decode(q.cuda(), table, lengths)) for _ in range(20))
+    assert ctx.check() == 0
+    want, bound = R.attention(q, *held[0], 9000, 0, 0, dim ** -0.5, two_terms=True)
+    check(first, want, bound)

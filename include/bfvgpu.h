@@ -482,8 +482,9 @@ typedef struct bfvgpu_kv {
 /* Writes the keys and values of new tokens into their pages, one layer.  k_new, v_new
  * [tokens][heads][dim] with the given strides (elements; dim contiguous; rows 16-byte aligned), in
  * the cache's type or in 32 bits (rounded to nearest).  starts [seqs + 1]: sequence s has the new
- * tokens starts[s] .. starts[s + 1) - 1, the last ones of its lengths[s] tokens (lengths count
- * them already); NULL: one new token each (tokens == seqs). */
+ * tokens starts[s] .. starts[s + 1] - 1, the last ones of its lengths[s] tokens (lengths count
+ * them already); starts[0] = 0 and starts[seqs] = tokens (a token of no sequence is recorded like a
+ * page number outside the cache, and nothing is written for it); NULL: one new token each (tokens == seqs). */
 int32_t bfvgpu_kv_append_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t layer, const void *k_new,
                                 const void *v_new, int32_t source_dtype, int64_t token_stride, int64_t head_stride,
                                 uint64_t tokens, const int32_t *starts, const int32_t *table, uint64_t width,

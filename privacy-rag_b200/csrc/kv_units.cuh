@@ -59,6 +59,21 @@ __device__ __forceinline__ void fill_unit(Unit& un, const View& kv, const Batch&
   }
 }
 
+// The sequences' new tokens have to be all of the batch's: a token that belongs to none has no row, and nothing is
+// written for it.  Unit 0 records that; its two numbers are asked for before the search, in the same round trip.
+struct Covered {
+  int32_t first = 0, last;
+  __device__ __forceinline__ Covered(const Batch& bt, const Query& q, uint32_t u) : last(q.tokens) {
+    if (u == 0 && (threadIdx.x & 31) == 0) {
+      first = bt.starts[0];
+      last = bt.starts[bt.seqs];
+    }
+  }
+  __device__ __forceinline__ void record(const Batch& bt, const Query& q) const {
+    if (first != 0 || last != q.tokens) flag_error(bt.err, kErrTable);
+  }
+};
+
 // Units are numbered [block of ROWS rows of the batch][key head]; surplus numbers find no rows.  Every
 // warp of a block finds its unit by itself.  In 32 bits (the entry points keep rows and units below
 // 2^31): this runs once, before anything else of its block can, and 64-bit divisions would be most of it.
@@ -70,6 +85,7 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
   int32_t first = 0, tokens = 1, length = 0;
   uint32_t at = 0;  // the block of rows within the sequence
   if (bt.starts) {
+    const Covered all(bt, q, u);
     // blocks of the sequences before this one, 32 sequences a step
     const int lane = threadIdx.x & 31;
     uint32_t before = 0;
@@ -106,6 +122,7 @@ __device__ __forceinline__ Unit find_unit(const View& kv, const Batch& bt, const
         before += __shfl_sync(0xffffffffu, upto, 31);
       }
     }
+    all.record(bt, q);
     if (!found) return un;
   } else {
     const uint32_t per = (q.group + ROWS - 1) / ROWS;
@@ -128,6 +145,7 @@ __device__ __forceinline__ Unit find_unit_ranked(const View& kv, const Batch& bt
   const uint32_t rank = u / (uint32_t)kv.heads;
   un.g = (int32_t)(u - rank * kv.heads);
   const int lane = threadIdx.x & 31;
+  const Covered all(bt, q, u);
   int32_t s = 0, tokens = 0, length = 0;
   if (lane < bt.seqs) {
     length = bt.lengths[lane];
@@ -136,6 +154,7 @@ __device__ __forceinline__ Unit find_unit_ranked(const View& kv, const Batch& bt
     if (s < 0 || e < s || e > q.tokens) flag_error(bt.err, kErrTable);
     else tokens = e - s;
   }
+  all.record(bt, q);
   const uint32_t mine = ((uint32_t)tokens * q.group + ROWS - 1) / ROWS;
   const uint64_t rows_before = (uint64_t)max(min(length, bt.width << kv.page_log) - tokens, 0) * q.group;
   const uint32_t first = (uint32_t)min(rows_before / ROWS, (uint64_t)1 << 30);

@@ -87,3 +87,32 @@ def test_blocks_that_share_keys_in_parts(bfv, ctx, dim):
     assert ctx.check() == 0
     want, bound = R.attention(q, *held[0], 9000, 0, 0, dim ** -0.5, two_terms=True)
     check(first, want, bound)
+
+
+@pytest.mark.parametrize("tokens,seqs", [(9, 2), (600, 2), (600, 40)])
+def test_starts_that_leave_tokens_out_are_recorded(bfv, ctx, tokens, seqs):
+    """Tokens before the first sequence's or after the last one's: recorded by prompt as by append, whichever kernel it is;
+    the rows of the others are what they are anyway."""
+    heads, dim = 8, 128
+    kv, cache, table, lengths, held = filled(bfv, ctx, [tokens] * 2 + [16] * (seqs - 2), heads, dim)
+    q = randn(torch.Generator().manual_seed(5), tokens, 2 * heads, dim).cuda()
+    k = q[:, :heads].contiguous()
+    rest = [0] * (seqs - 2)
+    good = ints([0, tokens - 3, tokens] + [tokens for _ in rest])
+    want = kv.prompt(q, good, table, lengths)
+    assert ctx.check() == 0
+    some_left_out = ((0, tokens - 3, tokens - 1), (2, tokens - 3, tokens), (0, 0, 0), (0, tokens - 3, tokens - 3))
+    for a, b, c in some_left_out:
+        starts = ints([a, b, c] + [c for _ in rest])
+        out = torch.zeros_like(q)
+        kv.prompt(q, starts, table, lengths, out=out)
+        with pytest.raises(bfv.BfvGpuError, match="E_KV_TABLE"):
+            ctx.check()
+        assert (out[:a] == 0).all() and (out[c:] == 0).all()
+        if b == tokens - 3:
+            assert torch.equal(out[a:b], want[a:b])
+    for a, b, c in some_left_out:  # (these change the cache)
+        kv.append(k, k, ints([a, b, c] + [c for _ in rest]), table, lengths)
+        with pytest.raises(bfv.BfvGpuError, match="E_KV_TABLE"):
+            ctx.check()
+    assert ctx.check() == 0

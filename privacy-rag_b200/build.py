@@ -3,7 +3,8 @@
 Usage: python privacy-rag_b200/build.py [--verbose]
 The library lands in privacy-rag_b200/lib/libbfvgpu.so, next to the Python mirror,
 so it travels with the repository snapshot to a GPU host; beside it the module of PagedKv's
-calls on torch tensors (bfvgpu_kv_calls.so), compiled against the installed torch and Python.
+calls on torch tensors (bfvgpu_kv_calls.so), compiled against the installed torch and Python,
+where there is a torch with CUDA (the library itself needs none).
 """
 from __future__ import annotations
 
@@ -41,16 +42,26 @@ def dependencies() -> list[str]:
     return deps
 
 
+def torch_dir() -> str | None:
+    """The installed torch with CUDA; None: there is none, and the library is built without PagedKv's module."""
+    spec = importlib.util.find_spec("torch")
+    path = spec.submodule_search_locations[0] if spec is not None else None
+    return path if path and os.path.exists(os.path.join(path, "lib", "libc10_cuda.so")) else None
+
+
+def built() -> list[str]:
+    return [LIB, CALLS] if torch_dir() else [LIB]
+
+
 def stale() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(CALLS):
+    if not all(os.path.exists(f) for f in built()):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(CALLS))
+    t = min(os.path.getmtime(f) for f in built())
     return any(os.path.getmtime(d) > t for d in dependencies())
 
 
-def calls_command() -> list[str]:
+def calls_command(torch: str) -> list[str]:
     """Compiles and links kv_torch.cpp; the library's own symbols come from the libbfvgpu.so beside it."""
-    torch = os.path.join(importlib.util.find_spec("torch").submodule_search_locations[0])
     cuda = os.path.dirname(os.path.dirname(nvcc())) if os.path.isabs(nvcc()) else "/usr/local/cuda"
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
             "-isystem", os.path.join(torch, "include"), "-isystem", os.path.join(torch, "include/torch/csrc/api/include"),
@@ -82,7 +93,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     subprocess.run(cmd, check=True)
     for o in objs:
         os.remove(o)
-    subprocess.run(calls_command(), check=True)
+    if torch_dir():
+        subprocess.run(calls_command(torch_dir()), check=True)
     return LIB
 
 

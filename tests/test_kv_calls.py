@@ -59,3 +59,33 @@ def test_a_closed_context_is_not_used(bfv, monkeypatch):
             call()
         assert refused.value.code == ARGUMENT
     assert given == [None] * len(calls)
+
+
+def test_the_library_builds_without_torch(bfv, monkeypatch, tmp_path):
+    """The C library needs no torch: without it, only the module of the calls on torch tensors is left out, and what is
+    built is not called stale for the lack of it."""
+    import importlib.util
+
+    import build as B
+    ran = []
+    monkeypatch.setattr(B, "LIB", str(tmp_path / "libbfvgpu.so"))
+    monkeypatch.setattr(B, "CALLS", str(tmp_path / "bfvgpu_kv_calls.so"))
+    monkeypatch.setattr(B, "PKG", str(tmp_path))
+    (tmp_path / "lib").mkdir()
+
+    def run(command, check):
+        ran.append(command)
+        open(command[command.index("-o") + 1], "w").close()
+
+    monkeypatch.setattr(B.subprocess, "run", run)
+    find = importlib.util.find_spec
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else find(name, *a))
+    assert B.stale()
+    assert B.build() == B.LIB
+    assert ran and not any(B.CALLS in c for c in ran)
+    assert not B.stale()
+    monkeypatch.setattr(importlib.util, "find_spec", find)
+    assert B.stale()  # torch is there now, and the module is not
+    B.build()
+    assert any(B.CALLS in c for c in ran)
+    assert not B.stale()

@@ -10,7 +10,9 @@ attention is a two-party integer protocol.
   freed and compacted on the host, in step with the device's table and lengths.
 
 Torch provides device memory; the arithmetic is the library's kernels.  Calls run on torch's current
-stream unless ``stream`` names another (a raw handle, 0 or None: the current one).
+stream unless ``stream`` names another (a raw handle, 0 or None: the current one).  On a named stream the
+caller orders the call after what it reads; its tensors may be let go at once, as after
+``Tensor.record_stream``, and what it returns belongs to that stream.
 """
 from __future__ import annotations
 
@@ -64,7 +66,7 @@ class PagedKv:
         desc = KvDesc(k.data_ptr(), v.data_ptr(), 0 if k.dtype == torch.bfloat16 else 1, self.layers, self.pages, self.heads,
                       self.page_tokens, self.dim, st[0], st[1], st[2], st[3])
         self._calls = _calls()
-        self._cache = self._calls.open(ctypes.addressof(desc), ctx.device)
+        self._cache = self._calls.open(ctypes.addressof(desc), ctx.device, k, v)
 
     @property
     def _handle(self) -> int | None:

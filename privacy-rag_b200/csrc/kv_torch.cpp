@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -14,6 +15,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <new>
 #include <optional>
 #include <stdexcept>
@@ -30,6 +32,7 @@ struct Cache {
   bfvgpu_kv kv;
   int device;
   double scale;
+  at::Tensor k, v;  // the pages, where open was given them
   at::ScalarType type() const { return kv.dtype == BFVGPU_KV_BF16 ? at::kBFloat16 : at::kHalf; }
 };
 
@@ -97,7 +100,8 @@ const at::Tensor& rows_of(PyObject* o, const char* name, const Cache& c) {
 }
 
 // The stream of a call: the given handle, or torch's current one (whose null handle is the legacy stream: the C
-// ABI reads a null stream as the context's).  What is allocated meanwhile belongs to it.
+// ABI reads a null stream as the context's).  What is allocated meanwhile belongs to it, and a given one is recorded
+// with the tensors it uses, so that memory which the caller lets go is not given out again before the call's work is done.
 struct Stream {
   std::optional<c10::cuda::CUDAStreamGuard> guard;
   void* handle = nullptr;
@@ -111,6 +115,16 @@ struct Stream {
     else
       handle = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)c.device).stream();
     if (!handle) handle = cudaStreamLegacy;
+  }
+  void uses(const at::Tensor& t) const {
+    if (guard && t.defined()) c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), guard->current_stream());
+  }
+  void uses(const Cache& c, std::initializer_list<PyObject*> tensors) const {
+    if (!guard) return;
+    uses(c.k);
+    uses(c.v);
+    for (PyObject* o : tensors)
+      if (o && o != Py_None) uses(THPVariable_Unpack(o));
   }
 };
 
@@ -132,16 +146,18 @@ bool wants(Py_ssize_t n, Py_ssize_t want) {
 }
 
 // ---- calls ----
-// open(address of a bfvgpu_kv, device) -> cache
+// open(address of a bfvgpu_kv, device[, k, v]) -> cache, which keeps the pages k and v
 PyObject* open_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!wants(n, 2)) return nullptr;
+  if (n != 4 && !wants(n, 2)) return nullptr;
   return answered([&]() -> PyObject* {
     const void* from = PyLong_AsVoidPtr(a[0]);
     if (!from) {
       if (PyErr_Occurred()) throw python_error();
       refuse("E_KV_ARGUMENT");
     }
-    auto* c = new Cache{*static_cast<const bfvgpu_kv*>(from), int_of(a[1]), 0.0};
+    at::Tensor k, v;
+    if (n == 4) k = tensor_of(a[2], "k"), v = tensor_of(a[3], "v");
+    auto* c = new Cache{*static_cast<const bfvgpu_kv*>(from), int_of(a[1]), 0.0, k, v};
     c->scale = 1.0 / std::sqrt((double)c->kv.dim);
     PyObject* o = PyCapsule_New(c, kName, [](PyObject* o) { delete static_cast<Cache*>(PyCapsule_GetPointer(o, kName)); });
     if (!o) delete c;
@@ -164,6 +180,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t* starts = a[4] == Py_None ? nullptr : ints_of(a[4], "starts", t.rows + 1, c);
     const int32_t* lengths = ints_of(a[6], "lengths", t.rows, c);
     const Stream s(a[8], c);
+    s.uses(c, {a[2], a[3], a[4], a[5], a[6]});
     return PyLong_FromLong(bfvgpu_kv_append_device(context_of(a[1]), &c.kv, int_of(a[7]), k.data_ptr(), v.data_ptr(),
                                                    wide ? BFVGPU_KV_F32 : c.kv.dtype, k.stride(0), k.stride(1),
                                                    (uint64_t)k.size(0), starts, t.at, t.width, lengths, t.rows, s.handle));
@@ -181,6 +198,7 @@ PyObject* fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
                   *fresh = ints_of(a[4], "fresh", count, c);
     int32_t* lengths = ints_of(a[6], "lengths", t.rows, c);
     const Stream s(a[7], c);
+    s.uses(c, {a[2], a[3], a[4], a[5], a[6]});
     return PyLong_FromLong(bfvgpu_kv_fork_device(context_of(a[1]), &c.kv, parents, children, fresh, count, t.at, t.rows,
                                                  t.width, lengths, s.handle));
   });
@@ -195,6 +213,7 @@ PyObject* move(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const uint64_t count = count_of(a[2], "src");
     const int32_t *src = ints_of(a[2], "src", count, c), *dst = ints_of(a[3], "dst", count, c);
     const Stream s(a[5], c);
+    s.uses(c, {a[2], a[3], a[4]});
     return PyLong_FromLong(
         bfvgpu_kv_move_device(context_of(a[1]), &c.kv, src, dst, count, t.at, t.rows, t.width, s.handle));
   });
@@ -228,6 +247,7 @@ PyObject* attend(PyObject* const* a, PyObject* of_starts, PyObject* const* rest)
       if (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !there(given, c) || !given.is_contiguous())
         refuse("E_KV_SHAPE: out is dense, of q's shape and type");
     }
+    s.uses(c, {a[2], of_starts, rest[0], rest[1], rest[6]});
     const at::Tensor& out = made.defined() ? made : THPVariable_Unpack(rest[6]);
     const uint64_t words =
         of_starts ? bfvgpu_kv_prompt_scratch_words(ctx, &c.kv, heads, tokens, t.rows, t.width, window, sinks)

@@ -116,3 +116,84 @@ def test_starts_that_leave_tokens_out_are_recorded(bfv, ctx, tokens, seqs):
         with pytest.raises(bfv.BfvGpuError, match="E_KV_TABLE"):
             ctx.check()
     assert ctx.check() == 0
+
+
+def test_tensors_let_go_during_a_call_on_another_stream(bfv, ctx):
+    """What a call on a named stream reads and writes is not given out again before its work is done."""
+    gen = torch.Generator().manual_seed(5)
+    lens = [700, 90, 33]
+    kv, cache, table, lengths, held = filled(bfv, ctx, lens, 2, 64)
+    q, k, v = (randn(gen, 3, h, 64).cuda() for h in (4, 2, 2))
+    starts = ints([0, 1, 2, 3])
+    before = cache.k.clone(), cache.v.clone()
+    kv.append(k, v, starts, table, lengths)
+    want = kv.decode(q, table, lengths)
+    want_p = kv.prompt(q, starts, table, lengths)
+    cache.k.copy_(before[0])
+    cache.v.copy_(before[1])
+    page = int(table[1, 0])
+    src, dst = ints([page]), ints([int(cache.spare[0])])
+    fresh, rows = ints([int(cache.spare[1])]), ints([0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    handle = side.cuda_stream
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1_000_000_000)
+    out = torch.empty_like(q)
+    given = [[x.clone() for x in args] for args in (
+        (k, v, starts, table, lengths), (q, table, lengths, out), (q, starts, table, lengths, out), (src, dst, table),
+        (rows, ints([2]), fresh, table, lengths))]
+    torch.cuda.current_stream().synchronize()  # (the copies are there; the other stream still sleeps)
+    used = {x.data_ptr() for args in given for x in args}
+    kv.append(*given[0], stream=handle)
+    kv.decode(*given[1][:3], out=given[1][3], stream=handle)
+    kv.prompt(*given[2][:4], out=given[2][4], stream=handle)
+    kv.move(*given[3], stream=handle)
+    kv.fork(*given[4], stream=handle)
+    got, got_p = given[1][3], given[2][4]
+    shapes = [(x.shape, x.dtype) for args in given for x in args for _ in range(2)]
+    got_at = {got.data_ptr(), got_p.data_ptr()}
+    del given
+    others = [torch.zeros(shape, dtype=dtype, device="cuda") for shape, dtype in shapes]
+    assert not side.query()
+    assert not used & {x.data_ptr() for x in others} and not got_at & {x.data_ptr() for x in others}
+    side.synchronize()
+    assert ctx.check() == 0
+    assert torch.equal(got, want) and torch.equal(got_p, want_p)
+
+
+def test_pages_let_go_during_a_call_on_another_stream(bfv, ctx):
+    gen = torch.Generator().manual_seed(5)
+    kv, cache, table, lengths, held = filled(bfv, ctx, [50])
+    k = randn(gen, 1, 2, 64).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1_000_000_000)
+    kv.append(k, k, None, table, lengths, stream=side.cuda_stream)
+    pages = {cache.k.data_ptr(), cache.v.data_ptr()}
+    shape = cache.k.shape
+    del kv, cache
+    others = [torch.empty(shape, dtype=BF, device="cuda") for _ in range(4)]
+    assert not side.query()
+    assert not pages & {x.data_ptr() for x in others}
+    side.synchronize()
+    assert ctx.check() == 0
+
+
+def test_a_graph_of_calls_on_a_named_stream(bfv, ctx):
+    """Captured with the capturing stream's handle, tensors let go after the capture, replayed."""
+    kv, cache, table, lengths, held = filled(bfv, ctx, [700, 90, 33])
+    q = randn(torch.Generator().manual_seed(5), 3, 4, 64).cuda()
+    want = kv.decode(q, table, lengths)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = kv.decode(q, table, lengths, stream=side.cuda_stream)
+        kv.decode(q * 2, table, lengths, stream=side.cuda_stream)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    del graph
+    assert ctx.check() == 0

@@ -506,7 +506,7 @@ int32_t bfvgpu_kv_move_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, const int
  * reads key head h / (q_heads / heads).  The query of sequence s stands at p = lengths[s] - 1 and
  * sees key j if j <= p and (window == 0 or j > p - window or j < sinks):
  *   out = sum_j softmax_j(scale q.k_j) v_j;  a sequence of length 0 gets zeros.
- * scale > 0.  Sums and softmax statistics in 32 bits.  Keys that are not visible are not read, and the
+ * scale > 0, and scale log2(e) finite.  Sums and softmax statistics in 32 bits.  Keys that are not visible are not read, and the
  * pages that hold none that is visible may be given to others.
  * scratch: bfvgpu_kv_decode_scratch_words words (may be NULL when that is 0), free again when the
  * call's work on the stream is done. */

@@ -78,7 +78,8 @@ Call checked_call(const bfvgpu_kv* cache, int32_t layer, uint64_t q_heads, uint6
 void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int64_t token_stride, int64_t head_stride,
             const int32_t* starts, const int32_t* table, const int32_t* lengths, float scale, uint64_t* scratch,
             void* out, void* stream) {
-  need(std::isfinite(scale) && scale > 0, BFVGPU_E_ARGUMENT, "E_KV_SCALE");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  need(std::isfinite(scale_log2) && scale > 0, BFVGPU_E_ARGUMENT, "E_KV_SCALE");
   const Place at = checked_place(ctx, stream);
   if (!c.query.tokens) return;
   need(c.batch.seqs && q && table && c.batch.width && lengths && out, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
@@ -93,7 +94,7 @@ void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int
   c.query.token_stride = token_stride;
   c.query.head_stride = head_stride;
   c.query.out = static_cast<uint16_t*>(out);
-  c.query.scale_log2 = scale * 1.4426950408889634f;
+  c.query.scale_log2 = scale_log2;
   float* work = reinterpret_cast<float*>(scratch);
   auto need_scratch = [&](uint64_t floats) {
     need(floats == 0 || scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");

@@ -274,7 +274,7 @@ __device__ __forceinline__ void tmem_store_pairs(uint32_t at, const uint32_t (&r
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// ---- two floats at a time --------------------------------------------------------------------------
+// ---- two floats at a time (subnormal numbers kept: the scale may be one, and -inf times a flushed one is NaN) ----
 __device__ __forceinline__ uint64_t two(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -285,12 +285,12 @@ __device__ __forceinline__ void split(uint64_t v, float& a, float& b) {
 }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
-  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
-  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 // Bits first .. last of a word whose bits stand for the numbers from `base` on.

@@ -197,3 +197,13 @@ def test_a_graph_of_calls_on_a_named_stream(bfv, ctx):
         assert torch.equal(got, want)
     del graph
     assert ctx.check() == 0
+
+
+@pytest.mark.parametrize("scale", [1e-37, 1e-39, 2e-45])
+@pytest.mark.parametrize("dim,page", [(128, 16), (64, 64)])
+def test_scales_below_the_normal_range(bfv, ctx, scale, dim, page):
+    """Keys that a row does not see stay out of it for the smallest scales too, in both kernels."""
+    from test_gpu_kv import run_attention
+    for kind, lens in (("prompt", [(600, 600), (300, 40)]), ("prompt", [(60, 9)]), ("decode", [(600, 1), (9, 1)])):
+        run_attention(bfv, ctx, kind, BF, lens, 4, 2, dim, page, scale=scale)
+        run_attention(bfv, ctx, kind, BF, lens, 4, 2, dim, page, 50, 3, scale=scale)

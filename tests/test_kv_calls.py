@@ -89,3 +89,25 @@ def test_the_library_builds_without_torch(bfv, monkeypatch, tmp_path):
     B.build()
     assert any(B.CALLS in c for c in ran)
     assert not B.stale()
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38, 1e-50, -1e-39])
+def test_scales_that_32_bits_do_not_hold_are_refused(bfv, scale):
+    """The kernels work with scale log2(e): beyond 32 bits every score of 0 would be NaN."""
+    import ctypes
+
+    from bfvgpu._lib import KvDesc
+    host = bfv.Context(4096, bfv.find_primes(4096, [36, 36, 37]), 2, 1, 65537, device=-1)
+    cache = KvDesc(0x10000, 0x20000, 0, 1, 4, 2, 16, 64, 8192, 2048, 1024, 64)
+    at = 0x30000
+    L = bfv.lib()
+
+    def status(scale):
+        return (L.bfvgpu_kv_decode_device(host.handle, ctypes.byref(cache), 0, at, 256, 64, 4, at, 4, at, 2, 0, 0, scale, at, at,
+                                          None),
+                L.bfvgpu_kv_prompt_device(host.handle, ctypes.byref(cache), 0, at, 256, 64, 4, 9, at, at, 4, at, 2, 0, 0, scale,
+                                          at, at, None))
+
+    assert status(scale) == (ARGUMENT, ARGUMENT) and L.bfvgpu_last_error() == b"E_KV_SCALE"
+    for good in (2.3e38, 1.0, 1e-39, 2e-45):
+        assert status(good) == (10, 10) and L.bfvgpu_last_error() == b"E_BFVGPU_HOST_ONLY_CONTEXT"

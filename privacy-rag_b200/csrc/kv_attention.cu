@@ -53,8 +53,8 @@ struct Call {
   Query query;
 };
 
-Call checked_call(const bfvgpu_kv* cache, int32_t layer, uint64_t q_heads, uint64_t tokens, uint64_t seqs,
-                  uint64_t width, int32_t window, int32_t sinks) {
+Call checked_call(const bfvgpu_kv* cache, int32_t layer, int64_t token_stride, int64_t head_stride, uint64_t q_heads,
+                  uint64_t tokens, uint64_t seqs, uint64_t width, int32_t window, int32_t sinks) {
   Call c;
   need(layer >= 0, BFVGPU_E_SHAPE, "E_KV_LAYER");
   c.view = checked_view(cache, layer);
@@ -68,6 +68,9 @@ Call checked_call(const bfvgpu_kv* cache, int32_t layer, uint64_t q_heads, uint6
   c.query.group = (int32_t)(q_heads / c.view.heads);
   c.query.group_inverse = ((1u << kGroupShift) + c.query.group - 1) / c.query.group;
   c.query.tokens = (int32_t)tokens;
+  // an axis of one element has no stride
+  c.query.token_stride = tokens > 1 ? token_stride : c.view.dim;
+  c.query.head_stride = q_heads > 1 ? head_stride : c.view.dim;
   c.query.window = window < top ? window : 0;  // a window past every position hides nothing
   c.query.sinks = std::min(sinks, top);
   c.batch.seqs = (int32_t)seqs;
@@ -75,15 +78,14 @@ Call checked_call(const bfvgpu_kv* cache, int32_t layer, uint64_t q_heads, uint6
   return c;
 }
 
-void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int64_t token_stride, int64_t head_stride,
-            const int32_t* starts, const int32_t* table, const int32_t* lengths, float scale, uint64_t* scratch,
-            void* out, void* stream) {
+void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, const int32_t* starts, const int32_t* table,
+            const int32_t* lengths, float scale, uint64_t* scratch, void* out, void* stream) {
   const float scale_log2 = scale * 1.4426950408889634f;
   need(std::isfinite(scale_log2) && scale > 0, BFVGPU_E_ARGUMENT, "E_KV_SCALE");
   const Place at = checked_place(ctx, stream);
   if (!c.query.tokens) return;
   need(c.batch.seqs && q && table && c.batch.width && lengths && out, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
-  need(aligned16(q) && aligned16(out) && token_stride % 8 == 0 && head_stride % 8 == 0, BFVGPU_E_ARGUMENT,
+  need(aligned16(q) && aligned16(out) && c.query.token_stride % 8 == 0 && c.query.head_stride % 8 == 0, BFVGPU_E_ARGUMENT,
        "E_KV_ALIGNMENT");
   OnDevice scope(at.device);
   c.batch.table = table;
@@ -91,8 +93,6 @@ void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int
   c.batch.starts = starts;
   c.batch.err = at.err;
   c.query.q = static_cast<const uint16_t*>(q);
-  c.query.token_stride = token_stride;
-  c.query.head_stride = head_stride;
   c.query.out = static_cast<uint16_t*>(out);
   c.query.scale_log2 = scale_log2;
   float* work = reinterpret_cast<float*>(scratch);
@@ -101,7 +101,7 @@ void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, int
     need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
   };
   int launches = 0;
-  if (few_rows(c.view, c.batch, c.query, starts) || !prompt_strides(c.view, c.query)) {
+  if (few_rows(c.view, c.batch, c.query, starts) || !prompt_strides(c.query)) {
     const RowSplit sp = plan_rows(c.view, c.batch, c.query, at.device);
     need_scratch(sp.scratch_floats());
     need(sp.blocks16 * sp.parts <= (int64_t)(kMost / sp.cluster), BFVGPU_E_SHAPE, "E_KV_SHAPE");
@@ -120,7 +120,7 @@ uint64_t scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q
                        uint64_t seqs, uint64_t width, int32_t window, int32_t sinks) {
   uint64_t words = 0;
   guarded([&] {
-    Call c = checked_call(cache, 0, q_heads, tokens, seqs, width, window, sinks);
+    Call c = checked_call(cache, 0, 0, 0, q_heads, tokens, seqs, width, window, sinks);
     static const int32_t some = 0;
     if (ragged) c.batch.starts = &some;  // only asked whether there is one
     int device = -1;
@@ -154,8 +154,8 @@ extern "C" int32_t bfvgpu_kv_decode_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cac
                                            int32_t window, int32_t sinks, float scale, uint64_t* scratch, void* out,
                                            void* stream) {
   return guarded([&] {
-    Call c = checked_call(cache, layer, q_heads, seqs, seqs, width, window, sinks);
-    attend(ctx, cache, c, q, token_stride, head_stride, nullptr, table, lengths, scale, scratch, out, stream);
+    Call c = checked_call(cache, layer, token_stride, head_stride, q_heads, seqs, seqs, width, window, sinks);
+    attend(ctx, cache, c, q, nullptr, table, lengths, scale, scratch, out, stream);
   });
 }
 
@@ -172,7 +172,7 @@ extern "C" int32_t bfvgpu_kv_prompt_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cac
                                            int32_t sinks, float scale, uint64_t* scratch, void* out, void* stream) {
   return guarded([&] {
     need(starts || !tokens, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
-    Call c = checked_call(cache, layer, q_heads, tokens, seqs, width, window, sinks);
-    attend(ctx, cache, c, q, token_stride, head_stride, starts, table, lengths, scale, scratch, out, stream);
+    Call c = checked_call(cache, layer, token_stride, head_stride, q_heads, tokens, seqs, width, window, sinks);
+    attend(ctx, cache, c, q, starts, table, lengths, scale, scratch, out, stream);
   });
 }

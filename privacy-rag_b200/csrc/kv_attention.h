@@ -17,7 +17,7 @@ constexpr int kMaxGroup = 1024, kMaxRows = 256, kGroupShift = 21;
 // of the sequence's new token R / group: all rows of one key head read the same keys.
 struct Query {
   const uint16_t* q = nullptr;
-  int64_t token_stride = 0, head_stride = 0;  // elements
+  int64_t token_stride = 0, head_stride = 0;  // elements (of an axis of one element: the dims)
   uint16_t* out = nullptr;                    // [tokens][heads * group][dim]
   int32_t tokens = 0;                         // new tokens of the batch
   int32_t group = 1;                          // query heads per key head (at most kMaxGroup)
@@ -47,7 +47,7 @@ struct PromptSplit {
   uint64_t scratch_floats() const;
 };
 // Whether the queries' strides suit the prompt kernel's loads (no broadcast, no reversed axis).
-bool prompt_strides(const View& kv, const Query& q);
+bool prompt_strides(const Query& q);
 PromptSplit plan_prompt(const View& kv, const Batch& bt, const Query& q, int sms);
 cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& split,
                           float* scratch, cudaStream_t st, int* launches);

@@ -264,6 +264,9 @@ extern "C" int32_t bfvgpu_kv_append_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cac
     if (!tokens) return;
     need(seqs && k_new && v_new && table && width && lengths, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
     const int64_t unit = source_dtype == BFVGPU_KV_F32 ? 4 : 8;
+    // an axis of one element has no stride
+    if (tokens == 1) token_stride = 0;
+    if (w.heads == 1) head_stride = 0;
     need(aligned16(k_new) && aligned16(v_new) && token_stride % unit == 0 && head_stride % unit == 0, BFVGPU_E_ARGUMENT,
          "E_KV_ALIGNMENT");
     OnDevice scope(at.device);

@@ -984,8 +984,7 @@ bool encode_q(CUtensorMap* map, const View& kv, const Query& q, int dtype, uint3
   const auto enc = encoder();
   if (!enc) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)kv.dim, (cuuint64_t)kv.heads * q.group, (cuuint64_t)q.tokens};
-  const cuuint64_t strides[2] = {(cuuint64_t)std::max<int64_t>(q.head_stride, 8) * 2,
-                                 (cuuint64_t)std::max<int64_t>(q.token_stride, 8) * 2};
+  const cuuint64_t strides[2] = {(cuuint64_t)q.head_stride * 2, (cuuint64_t)q.token_stride * 2};
   const cuuint32_t box[3] = {64, heads, tokens}, ones[3] = {1, 1, 1};
   return enc(map, type_of(dtype), 3, const_cast<uint16_t*>(q.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1045,10 +1044,9 @@ uint64_t PromptSplit::scratch_floats() const {
   return parts > 1 ? (uint64_t)units * parts * kBlockRows * (dim_padded + 2) : 0;
 }
 
-bool prompt_strides(const View& kv, const Query& q) {
+bool prompt_strides(const Query& q) {
   const int64_t most = int64_t(1) << 38;
-  return (kv.heads * q.group == 1 || (q.head_stride >= 8 && q.head_stride < most)) &&
-         (q.tokens == 1 || (q.token_stride >= 8 && q.token_stride < most));
+  return q.head_stride >= 8 && q.head_stride < most && q.token_stride >= 8 && q.token_stride < most;
 }
 
 PromptSplit plan_prompt(const View& kv, const Batch& bt, const Query& q, int sms) {

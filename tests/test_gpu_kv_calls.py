@@ -207,3 +207,26 @@ def test_scales_below_the_normal_range(bfv, ctx, scale, dim, page):
     for kind, lens in (("prompt", [(600, 600), (300, 40)]), ("prompt", [(60, 9)]), ("decode", [(600, 1), (9, 1)])):
         run_attention(bfv, ctx, kind, BF, lens, 4, 2, dim, page, scale=scale)
         run_attention(bfv, ctx, kind, BF, lens, 4, 2, dim, page, 50, 3, scale=scale)
+
+
+@pytest.mark.parametrize("stride", [1001, 3, 0, 1 << 40])
+def test_the_stride_of_a_single_element_is_not_used(bfv, ctx, stride):
+    """One token, or one head: whatever the stride of that axis, as for the cache's own axes."""
+    gen = torch.Generator().manual_seed(5)
+    for heads, group, tokens, new in ((2, 2, 700, 1), (1, 1, 90, 90), (1, 1, 1500, 1500)):
+        kv, cache, table, lengths, held = filled(bfv, ctx, [tokens], heads, 64)
+        h = heads * group
+        dense = randn(gen, new, h, 64).cuda()
+        odd = dense.as_strided(dense.shape, (stride if new == 1 else h * 64, stride if h == 1 else 64, 1))
+        starts = ints([0, new])
+        assert torch.equal(kv.prompt(odd, starts, table, lengths), kv.prompt(dense, starts, table, lengths))
+        if new == 1:
+            assert torch.equal(kv.decode(odd, table, lengths), kv.decode(dense, table, lengths))
+        for dtype in (BF, torch.float32):
+            k = dense[:, :heads].to(dtype)
+            odd_k = k.as_strided(k.shape, (stride if new == 1 else heads * 64, stride if heads == 1 else 64, 1))
+            kv.append(odd_k, odd_k, starts, table, lengths)
+            p, r = cache.where(0)
+            assert torch.equal(cache.k[0, p[-new:].cuda(), :, r[-new:].cuda()], dense[:, :heads])
+            cache.put(0, *held[0])
+    assert ctx.check() == 0

@@ -528,6 +528,15 @@ int32_t bfvgpu_kv_prompt_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t
                                 const int32_t *starts, const int32_t *table, uint64_t width, const int32_t *lengths,
                                 uint64_t seqs, int32_t window, int32_t sinks, float scale, uint64_t *scratch,
                                 void *out, void *stream);
+/* Which kernel a prompt call with these arguments takes; it goes by sizes and strides alone, never by
+ * values on the device (-1: sizes that the call refuses).  BFVGPU_KV_ROWS, which every call of
+ * bfvgpu_kv_decode_device takes: the weights enter the product with the values as two 16-bit terms, so that
+ * results are rounded once.  BFVGPU_KV_TILES, the tensor-core kernel: as one, rounded to the cache's type
+ * (the error against 64 bits is a quarter to a third larger: 1.6e-3 -> 2.0e-3 in bfloat16, 2.0e-4 ->
+ * 2.5e-4 in float16, relative to the results' norm). */
+enum bfvgpu_kv_kernel { BFVGPU_KV_ROWS = 0, BFVGPU_KV_TILES = 1 };
+int32_t bfvgpu_kv_prompt_kernel(const bfvgpu_kv *cache, int64_t token_stride, int64_t head_stride, uint64_t q_heads,
+                                uint64_t tokens, uint64_t seqs, uint64_t width, int32_t window, int32_t sinks);
 
 #ifdef __cplusplus
 }

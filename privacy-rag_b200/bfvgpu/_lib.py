@@ -161,6 +161,7 @@ _SIGNATURES = {
     "bfvgpu_kv_decode_scratch_words": (U64, [VP, _KV, U64, U64, U64, I32, I32]),
     "bfvgpu_kv_decode_device": (I32, [VP, _KV, I32, VP, I64, I64, U64, VP, U64, VP, U64, I32, I32, F32, VP, VP, VP]),
     "bfvgpu_kv_prompt_scratch_words": (U64, [VP, _KV, U64, U64, U64, U64, I32, I32]),
+    "bfvgpu_kv_prompt_kernel": (I32, [_KV, I64, I64, U64, U64, U64, U64, I32, I32]),
     "bfvgpu_kv_prompt_device": (I32, [VP, _KV, I32, VP, I64, I64, U64, U64, VP, VP, U64, VP, U64, I32, I32, F32, VP,
                                       VP, VP]),
 }

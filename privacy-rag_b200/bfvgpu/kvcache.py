@@ -65,7 +65,7 @@ class PagedKv:
         st = k.stride()
         desc = KvDesc(k.data_ptr(), v.data_ptr(), 0 if k.dtype == torch.bfloat16 else 1, self.layers, self.pages, self.heads,
                       self.page_tokens, self.dim, st[0], st[1], st[2], st[3])
-        self._calls = _calls()
+        self._calls, self._desc = _calls(), desc
         self._cache = self._calls.open(ctypes.addressof(desc), ctx.device, k, v)
 
     @property
@@ -105,11 +105,23 @@ class PagedKv:
     def prompt(self, q, starts, table, lengths, layer: int = 0, window: int = 0, sinks: int = 0,
                scale: float | None = None, out=None, stream: int | None = None):
         """The same for the new tokens of every sequence: q [tokens][q_heads][dim], sequence s having
-        rows starts[s] .. starts[s+1] - 1, its last tokens.  bfvgpu_kv_prompt_device."""
+        rows starts[s] .. starts[s+1] - 1, its last tokens; every row belongs to a sequence.  The values of a
+        token that some rows of a block of 256 see have to be finite for the block's others too (0 x NaN);
+        what none of them sees may hold anything.  bfvgpu_kv_prompt_device."""
         r = self._calls.prompt(self._cache, self._handle, q, starts, table, lengths, layer, window, sinks, scale, out, stream)
         if type(r) is int:
             check(r, "kv_prompt_device")
         return r
+
+    def prompt_kernel(self, q, table, window: int = 0, sinks: int = 0) -> str:
+        """Which kernel ``prompt`` takes, by sizes and strides alone: "rows", as every ``decode``, whose weights
+        keep the remainder of their rounding to 16 bits, or "tiles", the tensor-core kernel, whose weights do
+        not.  bfvgpu_kv_prompt_kernel."""
+        kernel = lib().bfvgpu_kv_prompt_kernel(ctypes.byref(self._desc), q.stride(0), q.stride(1), q.shape[1], q.shape[0],
+                                               table.shape[0], table.shape[1], window, sinks)
+        if kernel < 0:
+            raise ValueError(lib().bfvgpu_last_error().decode())
+        return ("rows", "tiles")[kernel]
 
 
 class PageBook:

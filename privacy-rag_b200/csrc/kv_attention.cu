@@ -47,6 +47,11 @@ bool few_rows(const View& kv, const Batch& bt, const Query& q, bool ragged) {
   return (double)blocks * (double)(keys + kStartKeys) * (wide ? 128 : 64) <= kFewProducts;
 }
 
+// The kernel of a call: few rows, or queries whose strides the prompt kernel's loads cannot follow.
+bool takes_rows(const View& kv, const Batch& bt, const Query& q, bool ragged) {
+  return few_rows(kv, bt, q, ragged) || !prompt_strides(q);
+}
+
 struct Call {
   View view;
   Batch batch;
@@ -101,7 +106,7 @@ void attend(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, con
     need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
   };
   int launches = 0;
-  if (few_rows(c.view, c.batch, c.query, starts) || !prompt_strides(c.query)) {
+  if (takes_rows(c.view, c.batch, c.query, starts)) {
     const RowSplit sp = plan_rows(c.view, c.batch, c.query, at.device);
     need_scratch(sp.scratch_floats());
     need(sp.blocks16 * sp.parts <= (int64_t)(kMost / sp.cluster), BFVGPU_E_SHAPE, "E_KV_SHAPE");
@@ -175,4 +180,15 @@ extern "C" int32_t bfvgpu_kv_prompt_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cac
     Call c = checked_call(cache, layer, token_stride, head_stride, q_heads, tokens, seqs, width, window, sinks);
     attend(ctx, cache, c, q, starts, table, lengths, scale, scratch, out, stream);
   });
+}
+
+extern "C" int32_t bfvgpu_kv_prompt_kernel(const bfvgpu_kv* cache, int64_t token_stride, int64_t head_stride,
+                                           uint64_t q_heads, uint64_t tokens, uint64_t seqs, uint64_t width, int32_t window,
+                                           int32_t sinks) {
+  int32_t kernel = -1;
+  guarded([&] {
+    const Call c = checked_call(cache, 0, token_stride, head_stride, q_heads, tokens, seqs, width, window, sinks);
+    kernel = takes_rows(c.view, c.batch, c.query, true) ? BFVGPU_KV_ROWS : BFVGPU_KV_TILES;
+  });
+  return kernel;
 }

@@ -111,3 +111,29 @@ def test_scales_that_32_bits_do_not_hold_are_refused(bfv, scale):
     assert status(scale) == (ARGUMENT, ARGUMENT) and L.bfvgpu_last_error() == b"E_KV_SCALE"
     for good in (2.3e38, 1.0, 1e-39, 2e-45):
         assert status(good) == (10, 10) and L.bfvgpu_last_error() == b"E_BFVGPU_HOST_ONLY_CONTEXT"
+
+
+def test_the_choice_of_the_prompt_kernel(bfv):
+    """By sizes and strides; -1 and a message for sizes that the call refuses."""
+    import ctypes
+
+    from bfvgpu._lib import KvDesc
+    L = bfv.lib()
+
+    def kernel(tokens, seqs, keys, heads=8, group=2, dim=128, window=0, sinks=0, head_stride=None, token_stride=None, page=16):
+        cache = KvDesc(0x10000, 0x20000, 0, 1, 4, heads, page, dim, 0, heads * page * dim, page * dim, dim)
+        return L.bfvgpu_kv_prompt_kernel(ctypes.byref(cache), heads * group * dim if token_stride is None else token_stride,
+                                         dim if head_stride is None else head_stride, heads * group, tokens, seqs,
+                                         keys // page, window, sinks)
+
+    rows, tiles = 0, 1
+    assert [kernel(n, 1, 512) for n in (1, 16, 64, 128, 512)] == [rows, rows, rows, tiles, tiles]
+    assert kernel(4 * 198, 4, 208, heads=4, group=8, window=14) == tiles
+    assert kernel(64 * 16, 64, 5392, group=1, dim=64) == rows and kernel(64 * 17, 64, 5392, group=1, dim=64) == tiles
+    assert kernel(128 * 4, 128, 3472, group=1) == rows and kernel(128 * 5, 128, 3472, group=1) == tiles
+    for strides in (dict(head_stride=0), dict(token_stride=0), dict(head_stride=1 << 38), dict(token_stride=-8)):
+        assert kernel(512, 1, 512, **strides) == rows  # broadcast, reversed, too far for the loads
+    assert kernel(512, 1, 512, heads=1, group=1, dim=64, head_stride=0) == kernel(512, 1, 512, heads=1, group=1, dim=64)
+    assert kernel(512, 1, 512, window=-1) == -1 and L.bfvgpu_last_error() == b"E_KV_WINDOW"
+    assert kernel(512, 1, 512, dim=60) == -1 and L.bfvgpu_last_error() == b"E_KV_DIM"
+    assert L.bfvgpu_kv_prompt_kernel(None, 8, 8, 1, 1, 1, 1, 0, 0) == -1

@@ -156,7 +156,8 @@ __device__ __forceinline__ Unit find_unit_ranked(const View& kv, const Batch& bt
   }
   all.record(bt, q);
   const uint32_t mine = ((uint32_t)tokens * q.group + ROWS - 1) / ROWS;
-  const uint64_t rows_before = (uint64_t)max(min(length, bt.width << kv.page_log) - tokens, 0) * q.group;
+  // (a length outside its range is recorded by its units; here it only orders them)
+  const uint64_t rows_before = (uint64_t)max(max(min(length, bt.width << kv.page_log), 0) - tokens, 0) * q.group;
   const uint32_t first = (uint32_t)min(rows_before / ROWS, (uint64_t)1 << 30);
   auto from = [&](uint32_t level) {  // units of this level or above
     return __reduce_add_sync(0xffffffffu, first + mine > level ? first + mine - max(first, level) : 0);

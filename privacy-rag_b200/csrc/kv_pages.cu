@@ -4,7 +4,7 @@
 // 16 bytes per thread and access, four accesses in flight per thread, all layers in one launch.
 // Measured: 17349 new tokens of 8 heads of 128 from 32 to 16 bits (213 MB) 36.4 us, 5.9 TB/s; 256 pages of 28
 // layers moved (939 MB) 144 us, 6.5 TB/s, as fast as a plain copy; 16 forks of 28 layers (59 MB, half of it
-// reads of one page that stay in L2) 7.7 us.  One token of 64 sequences takes 3.1 us, which is the latency of a
+// reads of one page that stay in L2) 7.3 us.  One token of 64 sequences takes 3.1 us, which is the latency of a
 // launch and of four dependent reads (length, table, source, store).
 #include "kv_host.h"
 
@@ -110,29 +110,22 @@ PageShape page_shape(const View& w) {
 // Blocks of a copy kernel per processor.  A page without gaps (WHOLE) needs no divisions and few registers.
 template <bool WHOLE>
 constexpr int kPerSm = WHOLE ? 8 : 6;
-// How often the threads move kInFlight chunks of such a page: twice in a fork, so that 16 of 28 layers are one wave
-// (7.7 us; 9.8 in three waves of once); a move is long (256 pages of 28 layers: 144 us with once, 146 with twice).
-constexpr int kForkBatches = 2;
-
 // The block's share `part` of page `from` -> page `to` of one layer's K or V.
 template <bool WHOLE>
 __device__ __forceinline__ void copy_share(uint16_t* base, int64_t page_stride, int32_t from, int32_t to,
-                                           const PageShape& s, int32_t part, int32_t batches) {
+                                           const PageShape& s, int32_t part) {
   const uint16_t* src = base + from * page_stride;
   uint16_t* dst = base + to * page_stride;
   uint4 x[kInFlight];
   if constexpr (WHOLE) {
     const int32_t chunks = s.row_chunks;
-    int32_t c = part * (kThreads * kInFlight * batches) + threadIdx.x;
-#pragma unroll 1
-    for (int b = 0; b < batches; ++b, c += kThreads * kInFlight) {
+    const int32_t c = part * (kThreads * kInFlight) + threadIdx.x;
 #pragma unroll
-      for (int i = 0; i < kInFlight; ++i)
-        if (c + i * kThreads < chunks) x[i] = reinterpret_cast<const uint4*>(src)[c + i * kThreads];
+    for (int i = 0; i < kInFlight; ++i)
+      if (c + i * kThreads < chunks) x[i] = reinterpret_cast<const uint4*>(src)[c + i * kThreads];
 #pragma unroll
-      for (int i = 0; i < kInFlight; ++i)
-        if (c + i * kThreads < chunks) reinterpret_cast<uint4*>(dst)[c + i * kThreads] = x[i];
-    }
+    for (int i = 0; i < kInFlight; ++i)
+      if (c + i * kThreads < chunks) reinterpret_cast<uint4*>(dst)[c + i * kThreads] = x[i];
     return;
   }
   const int32_t chunks = s.rows * s.row_chunks, c0 = part * (kThreads * kInFlight) + threadIdx.x;
@@ -153,7 +146,7 @@ __device__ __forceinline__ void copy_share(uint16_t* base, int64_t page_stride, 
 struct Copies {
   PageShape shape;
   int64_t layer_stride = 0;
-  int32_t layers = 0, parts = 0, count = 0, batches = 1;
+  int32_t layers = 0, parts = 0, count = 0;
   __host__ __device__ uint32_t per() const { return 2u * layers * parts; }  // blocks of a copy
 };
 
@@ -162,7 +155,7 @@ template <bool WHOLE>
 __device__ __forceinline__ void copy_block(const View& kv, const Copies& cp, uint32_t share, int32_t from, int32_t to) {
   const uint32_t rest = share / (uint32_t)cp.parts, part = share - rest * cp.parts;
   uint16_t* base = ((rest & 1) ? kv.v : kv.k) + (int64_t)(rest >> 1) * cp.layer_stride;
-  copy_share<WHOLE>(base, kv.page_stride, from, to, cp.shape, (int32_t)part, cp.batches);
+  copy_share<WHOLE>(base, kv.page_stride, from, to, cp.shape, (int32_t)part);
 }
 
 template <bool WHOLE>
@@ -228,14 +221,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<WHOLE>)
   if (part && from != to) copy_block<WHOLE>(kv, cp, share, from, to);
 }
 
-Copies copies_of(const View& w, const bfvgpu_kv* c, uint64_t count, int32_t batches) {
+Copies copies_of(const View& w, const bfvgpu_kv* c, uint64_t count) {
   Copies cp;
   cp.shape = page_shape(w);
   cp.layers = c->layers;
   cp.layer_stride = c->layers > 1 ? c->layer_stride : 0;
   cp.count = (int32_t)count;
-  cp.batches = cp.shape.rows == 1 ? batches : 1;
-  const int64_t per = (int64_t)kThreads * kInFlight * cp.batches;
+  const int64_t per = (int64_t)kThreads * kInFlight;
   cp.parts = (int32_t)((cp.shape.chunks() + per - 1) / per);
   return cp;
 }
@@ -301,7 +293,7 @@ extern "C" int32_t bfvgpu_kv_fork_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache
     const Place at = checked_place(ctx, stream);
     if (!count) return;
     need(parents && children && fresh && table && width && lengths, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
-    const Copies cp = copies_of(w, cache, count, kForkBatches);
+    const Copies cp = copies_of(w, cache, count);
     const int64_t blocks = (int64_t)count * 2 * cp.layers * cp.parts;
     need(blocks <= kMostBlocks, BFVGPU_E_SHAPE, "E_KV_SHAPE");
     OnDevice scope(at.device);
@@ -321,7 +313,7 @@ extern "C" int32_t bfvgpu_kv_move_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache
     const Place at = checked_place(ctx, stream);
     if (!count) return;
     need(src && dst && (table || !rows || !width), BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
-    const Copies cp = copies_of(w, cache, count, 1);
+    const Copies cp = copies_of(w, cache, count);
     const int64_t entries = table ? (int64_t)rows * (int64_t)width : 0;
     const int64_t copy_blocks = (int64_t)count * 2 * cp.layers * cp.parts;
     const int64_t blocks = copy_blocks + (entries + kThreads - 1) / kThreads;

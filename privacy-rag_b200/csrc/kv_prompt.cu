@@ -1062,8 +1062,10 @@ PromptSplit plan_prompt(const View& kv, const Batch& bt, const Query& q, int sms
   const int64_t most = std::min<int64_t>(kMaxParts, keys / (kPartTiles * kTileKeys));
   const int64_t near = (2 * sms + sp.units) / std::max<int64_t>(1, 2 * sp.units);
   sp.parts = (int32_t)std::max<int64_t>(1, std::min(most, near));
-  // a few waves are balanced best with the longest units of all sequences first (8 prompts of 512 tokens: 26.5 us in
-  // the sequences' order, 24.0 so); with more waves a sequence's units follow one another, for its keys to stay in L2
+  // a few waves are balanced best with the longest units of all sequences first (8 prompts of 512 tokens: 26.9 us in
+  // the sequences' order, 24.2 so; 4 of 1024: 35.4 and 30.0; 8 of up to 2000, 2 key heads: 55.8 and 45.7; 32 of up to 256:
+  // 25.4 and 23.8; what it costs where there is nothing to balance: 2 of 1024 23.6 and 24.1, 6 of 700 with a window of 200
+  // 27.0 and 27.5); with more waves a sequence's units follow one another, for its keys to stay in L2
   sp.ranked = sp.parts == 1 && bt.seqs > 1 && bt.seqs <= 32 && sp.units <= 4 * (int64_t)sms;
   return sp;
 }

@@ -458,8 +458,9 @@ int32_t bfvgpu_token_close(bfvgpu_token *t, bfvgpu_cleanup *cleanup);
 int32_t bfvgpu_token_release(bfvgpu_token *t);
 
 /* ---- Paged key-value cache and its attention ----------------------------------------------
- * What runs between the q/k/v call and the o call of a decoder layer, for the party that holds
- * the decrypted projections.  No counterpart in the reference, whose attention is a two-party
+ * The cache and the attention between the q/k/v call and the o call of a decoder layer, for the
+ * party that holds the decrypted projections (head norms and positions, where the model has them,
+ * are that party's own).  No counterpart in the reference, whose attention is a two-party
  * integer protocol.  All pointers are device memory; stream as for the other device entry points
  * (NULL: the context stream; cudaStreamLegacy names the default stream).  Values on the device
  * (tables, lengths, starts, page lists) cannot be checked by the host: the kernels check every
@@ -507,7 +508,8 @@ int32_t bfvgpu_kv_move_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, const int
  * sees key j if j <= p and (window == 0 or j > p - window or j < sinks):
  *   out = sum_j softmax_j(scale q.k_j) v_j;  a sequence of length 0 gets zeros.
  * scale > 0, and scale log2(e) finite.  Sums and softmax statistics in 32 bits.  Keys that are not visible are not read, and the
- * pages that hold none that is visible may be given to others.
+ * pages that hold none that is visible may be given to others.  Visible values that are not finite give
+ * results that are not finite (an infinity may become a NaN).
  * scratch: bfvgpu_kv_decode_scratch_words words (may be NULL when that is 0), free again when the
  * call's work on the stream is done. */
 uint64_t bfvgpu_kv_decode_scratch_words(const bfvgpu_ctx *ctx, const bfvgpu_kv *cache, uint64_t q_heads,

@@ -8,6 +8,10 @@ the o call.  In between everything is 16-bit floating point with 32-bit sums: it
 reference's exact-integer attention, which runs as a two-party protocol and is out of this
 library's scope.
 
+It is the attention alone, on q and k as the call leaves them.  A model that changes them in between, as a Qwen3
+layer does by a norm of each head and rotary positions, takes the steps apart: ``words_to_floats``, its own norm
+and positions, ``KvCache.append`` and ``attend``, ``floats_to_words``.
+
     att = RingAttention(ctx, q_heads=16, kv_heads=8, dim=128, fraction=24, out_fraction=12, pages=4096)
     doc = att.open()
     att.extend({doc: 512})                      # a retrieved document

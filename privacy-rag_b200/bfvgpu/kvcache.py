@@ -2,7 +2,8 @@
 
 The protocol runs a decoder layer's linear calls; between the q/k/v call and the o call the party
 that holds the decrypted projections (a client that computes the non-linear steps itself, or a
-plaintext check of the protocol) needs a cache and its attention.  The reference has neither: its
+plaintext check of the protocol) needs a cache and its attention (head norms and positions, where
+the model has them, are its own).  The reference has neither: its
 attention is a two-party integer protocol.
 
 * ``PagedKv``: the pages and the device calls on them (bfvgpu_kv_* of include/bfvgpu.h);
@@ -48,7 +49,8 @@ class PagedKv:
     """Pages k, v [layers][pages][heads][page_tokens][dim] (or without the layers axis), bfloat16 or
     float16 CUDA tensors of the same shape and strides, dim contiguous; the outer axes may lie in
     any order (pass a transposed view).  table [rows][width], lengths, starts, page and row lists:
-    dense int32 CUDA tensors."""
+    dense int32 CUDA tensors.  For serving: no gradient passes through a call, what it returns or
+    writes is cut off from its arguments' graph."""
 
     def __init__(self, ctx: Context, k, v):
         import torch
@@ -301,7 +303,9 @@ class KvCache:
         self.kv.append(k_new, v_new, self.starts, self.table, self.lengths, layer=layer)
 
     def attend(self, q, layer: int = 0, window: int = 0, sinks: int = 0, scale: float | None = None, out=None):
-        """The attention of the step's tokens, after append: q [tokens][q_heads][dim]."""
+        """The attention of the step's tokens, after append: q [tokens][q_heads][dim].  A ``decode`` where
+        every row of the table gets one token, else a ``prompt`` of all rows, whose kernel goes by their number
+        and the table's width (``PagedKv.prompt_kernel``)."""
         if self._each:
             return self.kv.decode(q, self.table, self.lengths, layer, window, sinks, scale, out)
         return self.kv.prompt(q, self.starts, self.table, self.lengths, layer, window, sinks, scale, out)

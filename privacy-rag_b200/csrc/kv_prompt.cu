@@ -8,7 +8,11 @@
 // m is the row's reference exponent.  It starts as the running maximum and follows it only when the
 // maximum has grown by more than 8: until then weights of up to 2^8 stay far inside both 16-bit types
 // and the 32-bit sums, and O need not be rescaled.  The sum of the weights is kept in 32 bits, from
-// the weights before they are rounded to 16 bits for the product.
+// the weights before they are rounded to 16 bits for the product.  That rounding is a choice: the product takes 16-bit
+// operands, a second one for the remainder (as in the row kernel) would make half again as much work of the pipe that
+// bounds 128 dims, and there is no room in tensor memory for its operand beside S, P and O.  It costs a quarter to a
+// third of the error against 64 bits (eight prompts of 512 tokens: 1.6e-3 -> 2.0e-3 of the results' norm in bfloat16,
+// chunks of 1024 in float16: 2.0e-4 -> 2.5e-4); the results' own rounding is the rest.
 //
 // Roles: warps 0-7 and 8-15 hold the rows of tile 0 and 1, four threads a row, so that a row's maximum needs no
 // other warp (with a row's halves in two warps, which met for every key tile, 64 dims took 12 % longer);
@@ -24,9 +28,10 @@
 //
 // What bounds it: of a pair of row tiles and 128 keys the exponentials take 2048 cycles of the special-function pipe,
 // with 128 dims the products as many of the tensor pipe; measured 2500 cycles with 64 dims, 3000 with 128.  16384
-// tokens, 16 query heads on 8 of 128: 835 us, 1320 TFLOP/s (950 us once the power limit lowers the clock); of 64: 615
-// us; 8191 tokens with a window of 1024: 87 us; eight prompts of 512: 23 us, most of it the start of the blocks
-// (first S 3.3 us after it) and the results (2 us after the last product).
+// tokens, 16 query heads on 8 of 128: 835 us, 1320 TFLOP/s (950 us once the power limit lowers the clock); of 64: 630
+// us; 8191 tokens with a window of 1024: 86 us back to back (94 in a long run, at the power limit); eight prompts of 512:
+// 23 us, of which the start of the blocks (first S 3.3 us after it) and the results (2 us after the last product) are a
+// quarter.
 //
 // Where there are too few rows to fill the GPU, the key tiles of a block's rows are dealt to several
 // blocks, which leave (m, sum, O) in 32 bits for a second kernel to join in a fixed order.
@@ -114,8 +119,8 @@ struct Smem {
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
-  static constexpr int kMax = kV + kStages * kTileBytes;  // two turns: a number of each thread for the row's other
-  static constexpr int kAnswer = kMax + 2 * 512 * 4;      // of the launch control, 16 bytes
+  static constexpr int kStats = kV + kStages * kTileBytes;  // (m, sum) of the rows of both tiles, of two items in turn
+  static constexpr int kAnswer = kStats + 4 * kTileRows * 8;  // of the launch control, 16 bytes
   static constexpr int kItems = kAnswer + 16;             // two
   static constexpr int kBar = kItems + ((2 * (int)sizeof(Item) + 7) & ~7);
   static constexpr int kBars = 4 + 4 * kStages + 2 + 2 + 2 * kPieces + 4 + 2 + 8 + 4 + 1 + 2;
@@ -575,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!same(span.needs(i))) continue;
           if (same(i == span.start())) wait(q_full + 8 * t, q_turn >> t & 1);
           // all that can be is worked out before the wait: the rows wait for what stands behind it
-          const bool early = span.at_or_after(i + 1) >= to;  // before the wait: the rows wait for what stands behind it
+          const bool early = span.at_or_after(i + 1) >= to;
           wait(s_read + 8 * last, read_turn >> last & 1);  // the S before has been read
           if (!ok) break;
           last = t;
@@ -850,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // ---- results: a thread has a row, and half of its dims; m and l of it come through shared memory ----
-      float2* ml = reinterpret_cast<float2*>(sm + S::kMax) + ((results++ & 1) * 2 + t) * kTileRows;
+      float2* ml = reinterpret_cast<float2*>(sm + S::kStats) + ((results++ & 1) * 2 + t) * kTileRows;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);

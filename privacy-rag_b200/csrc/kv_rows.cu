@@ -21,7 +21,7 @@
 // the GPU (few sequences and key heads, long context) does a unit take several clusters, whose
 // partial results a second kernel joins, in order too: results do not depend on timing.
 //
-// Measured: 64 sequences of up to 4096 tokens, 8 key heads of 128: 101 us, 5.7 TB/s, of a copy's 6.5; 256 of 2048:
+// Measured: 64 sequences of up to 4096 tokens, 8 key heads of 128: 102 us, 5.6 TB/s, of a copy's 6.5; 256 of 2048:
 // 6.4 TB/s; one of 131071 tokens, 4 key heads, 8 query heads each: 49 us, 5.5 TB/s; 96 windows of 1024 keys, 2 key
 // heads of 64: 14.5 us, 3.4 TB/s; one of 513 tokens: 5.9 us.  The short ones spend their time in the chain of
 // launch, length, table, keys and join, whose 5 to 6 us no split makes shorter.

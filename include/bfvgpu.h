@@ -490,6 +490,38 @@ int32_t bfvgpu_kv_append_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t
                                 const void *v_new, int32_t source_dtype, int64_t token_stride, int64_t head_stride,
                                 uint64_t tokens, const int32_t *starts, const int32_t *table, uint64_t width,
                                 const int32_t *lengths, uint64_t seqs, void *stream);
+/* Rotary positions.  Pair i < dims / 2 of a head's first `dims` elements (a multiple of 4 in [4, 128], at most the
+ * head's) is (i, i + dims / 2) or (2 i, 2 i + 1); at position p
+ *   (a, b) -> scale (a cos p f_i - b sin p f_i, b cos p f_i + a sin p f_i),
+ * the other elements stay.  turns[i] is f_i modulo a turn, in 2^-64 turns: angles are exact to p 2^-64 turns at every
+ * position.  bfvgpu_rotary_set fills it from frequencies f_i in radians per position (finite); host only. */
+enum bfvgpu_rotary_layout { BFVGPU_ROTARY_HALF = 0, BFVGPU_ROTARY_INTERLEAVED = 1 };
+typedef struct bfvgpu_rotary {
+  int32_t dims, layout;
+  float scale;
+  uint64_t turns[64];
+} bfvgpu_rotary;
+int32_t bfvgpu_rotary_set(bfvgpu_rotary *r, int32_t dims, int32_t layout, const double *frequencies, double scale);
+/* out[t][h] = x[t][h] rotated at positions[t] (int32): x [tokens][heads][dim] of a type of enum bfvgpu_kv_dtype, out of
+ * the same type, both with dim contiguous and rows 16-byte aligned (strides in elements); dim a multiple of 8 in [8, 128].
+ * out may be x (with its strides), else they do not overlap.  norm (nullable): float32 weights [dim], 16-byte aligned; each
+ * head is first x rsqrt(mean(x^2) + eps) norm.  inverse: rotates back (with the scale, not divided by it), which
+ * takes the gradient of out to that of x; not with a norm.  Computed in 32 bits and rounded once. */
+int32_t bfvgpu_rotary_device(bfvgpu_ctx *ctx, const bfvgpu_rotary *rotary, const void *x, int32_t dtype,
+                             int64_t token_stride, int64_t head_stride, uint64_t tokens, uint64_t heads, int32_t dim,
+                             const int32_t *positions, const float *norm, float eps, int32_t inverse, void *out,
+                             int64_t out_token_stride, int64_t out_head_stride, void *stream);
+/* bfvgpu_kv_append_device with the keys normed (k_norm, nullable) and rotated at their tokens' positions in their
+ * sequences on the way, and the same tokens' queries q [tokens][q_heads][dim] (source_dtype; strides of their own) normed
+ * (q_norm, nullable) and rotated into q_out, dense, of the cache's type (q_heads 0: none).  Values are appended as they
+ * are.  q_out may be q, where q is dense and of the cache's type, else it overlaps nothing that the call reads.  A token
+ * whose sequence or page is outside its range is recorded, and nothing is written for it, nor its queries. */
+int32_t bfvgpu_kv_append_rotary_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t layer, const bfvgpu_rotary *rotary,
+                                       const void *k_new, const void *v_new, int32_t source_dtype, int64_t token_stride,
+                                       int64_t head_stride, const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                                       uint64_t q_heads, const float *q_norm, const float *k_norm, float eps,
+                                       uint64_t tokens, const int32_t *starts, const int32_t *table, uint64_t width,
+                                       const int32_t *lengths, uint64_t seqs, void *q_out, void *stream);
 /* Row children[i] of the table becomes a continuation of row parents[i]: the same length and
  * pages, but a partly filled last page is copied (all layers) to page fresh[i] (unread where the
  * parent's length is a multiple of page_tokens).  No row is a child twice, or both parent and

@@ -64,7 +64,14 @@ class KvDesc(ctypes.Structure):
                 ("head_stride", I64), ("token_stride", I64)]
 
 
+class RotaryDesc(ctypes.Structure):
+    """bfvgpu_rotary: angles per position."""
+
+    _fields_ = [("dims", I32), ("layout", I32), ("scale", F32), ("turns", U64 * 64)]
+
+
 _KV = ctypes.POINTER(KvDesc)
+_ROT = ctypes.POINTER(RotaryDesc)
 
 _SIGNATURES = {
     "bfvgpu_version": (I32, []),
@@ -156,6 +163,10 @@ _SIGNATURES = {
     "bfvgpu_token_close": (I32, [VP, ctypes.POINTER(Cleanup)]),
     "bfvgpu_token_release": (I32, [VP]),
     "bfvgpu_kv_append_device": (I32, [VP, _KV, I32, VP, VP, I32, I64, I64, U64, VP, VP, U64, VP, U64, VP]),
+    "bfvgpu_rotary_set": (I32, [_ROT, I32, I32, ctypes.POINTER(ctypes.c_double), ctypes.c_double]),
+    "bfvgpu_rotary_device": (I32, [VP, _ROT, VP, I32, I64, I64, U64, U64, I32, VP, VP, F32, I32, VP, I64, I64, VP]),
+    "bfvgpu_kv_append_rotary_device": (I32, [VP, _KV, I32, _ROT, VP, VP, I32, I64, I64, VP, I64, I64, U64, VP, VP, F32, U64,
+                                             VP, VP, U64, VP, U64, VP, VP]),
     "bfvgpu_kv_fork_device": (I32, [VP, _KV, VP, VP, VP, U64, VP, U64, U64, VP, VP]),
     "bfvgpu_kv_move_device": (I32, [VP, _KV, VP, VP, U64, VP, U64, U64, VP]),
     "bfvgpu_kv_decode_scratch_words": (U64, [VP, _KV, U64, U64, U64, I32, I32]),

@@ -84,6 +84,18 @@ class PagedKv:
         check(self._calls.append(self._cache, self._handle, k_new, v_new, starts, table, lengths, layer, stream),
               "kv_append_device")
 
+    def append_rotary(self, k_new, v_new, rotary, starts, table, lengths, q=None, q_norm=None, k_norm=None,
+                      eps: float = 1e-6, layer: int = 0, out=None, stream: int | None = None):
+        """``append`` with the keys rotated at their tokens' positions on the way (a ``Rotary``), and the same tokens'
+        queries q [tokens][q_heads][dim] (k_new's type) -> out [tokens][q_heads][dim] of the cache's type, rotated; None
+        without q.  q_norm, k_norm: float32 weights [dim] of a norm of each head before the rotation, x rsqrt(mean(x^2)
+        + eps) weight.  out may be q.  bfvgpu_kv_append_rotary_device."""
+        r = self._calls.append_rotary(self._cache, self._handle, rotary._address, k_new, v_new, starts, table, lengths, q, q_norm,
+                                      k_norm, eps, layer, out, stream)
+        if type(r) is int:
+            check(r, "kv_append_rotary_device")
+        return r
+
     def fork(self, parents, children, fresh, table, lengths, stream: int | None = None) -> None:
         """Rows children[i] of the table continue rows parents[i]; a partly filled last page is copied
         to page fresh[i].  bfvgpu_kv_fork_device."""

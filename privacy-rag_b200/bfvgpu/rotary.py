@@ -1,0 +1,88 @@
+"""Rotary positions: the rotation of pairs of a head's elements by angles that grow with a token's position.
+
+A ``Rotary`` holds the frequencies.  ``PagedKv.append_rotary`` applies it to keys and queries on the way into the
+cache, ``apply`` to any tensor of heads; with ``inverse`` that is the gradient's way back.  Angles are kept as
+64-bit fractions of a turn, so far positions lose nothing (bfvgpu_rotary of include/bfvgpu.h).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+from ._lib import RotaryDesc, check, lib
+from .backend import Context
+from .kvcache import _calls
+
+LAYOUTS = ("half", "interleaved")
+SCALINGS = ("none", "linear", "ntk", "yarn")
+
+
+def frequencies(dims: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, trained: int = 4096,
+                turns: tuple[float, float] = (1.0, 32.0)) -> tuple[list[float], float]:
+    """(radians per position of each pair, factor of the rotated values): base^(-2 i / dims), and for contexts `factor`
+    times the `trained` length
+
+    * "linear": positions divided by the factor;
+    * "ntk": the base times factor^(dims / (dims - 2)), which divides the slowest pair's frequency by the factor and
+      keeps the fastest's;
+    * "yarn": pairs that turn at least turns[1] times over the trained length keep their frequency, those that turn at most
+      turns[0] times are divided by the factor, and in between linearly by the pair's number; rotated values are multiplied
+      by 0.1 ln(factor) + 1."""
+    if scaling not in SCALINGS:
+        raise ValueError(f"E_ROTARY_SCALING: one of {SCALINGS}")
+    if dims < 2 or dims % 2 or not base > 1 or not math.isfinite(base) or not factor >= 1 or not math.isfinite(factor):
+        raise ValueError("E_ROTARY_FREQUENCIES: an even number of dims, base > 1, factor >= 1")
+    if scaling in ("ntk", "yarn") and dims < 4:
+        raise ValueError("E_ROTARY_DIMS")
+    if scaling == "ntk":
+        base = base * factor ** (dims / (dims - 2))
+    w = [base ** (-2 * i / dims) for i in range(dims // 2)]
+    if scaling == "linear":
+        return [x / factor for x in w], 1.0
+    if scaling != "yarn":
+        return w, 1.0
+    if not 0 < turns[0] < turns[1] or trained < 1:
+        raise ValueError("E_ROTARY_FREQUENCIES: 0 < turns[0] < turns[1], trained >= 1")
+    # the pair (a real number) that turns so often over the trained length
+    pair = lambda n: dims * math.log(trained / (2 * math.pi * n)) / (2 * math.log(base))  # noqa: E731
+    low, high = max(math.floor(pair(turns[1])), 0), min(math.ceil(pair(turns[0])), dims - 1)
+    span = max(high - low, 1e-3)
+    divided = [min(1.0, max(0.0, (i - low) / span)) for i in range(dims // 2)]
+    return [x * (1 - r) + x / factor * r for x, r in zip(w, divided)], 0.1 * math.log(factor) + 1
+
+
+class Rotary:
+    """The rotation of the first `dims` elements of a head (a multiple of 4, at most 128; the rest stays).  layout: pairs
+    (i, i + dims / 2), "half", or (2 i, 2 i + 1), "interleaved".  base, scaling, factor, trained and turns as for
+    ``frequencies``; `radians` (and `scale`) give the angles per position of a model that has others."""
+
+    def __init__(self, ctx: Context, dims: int, base: float = 10000.0, layout: str = "half", scaling: str = "none",
+                 factor: float = 1.0, trained: int = 4096, turns: tuple[float, float] = (1.0, 32.0), radians=None,
+                 scale: float | None = None):
+        if layout not in LAYOUTS:
+            raise ValueError(f"E_ROTARY_LAYOUT: one of {LAYOUTS}")
+        if dims < 4 or dims > 128 or dims % 4:
+            raise ValueError("E_ROTARY_DIMS: a multiple of 4 in [4, 128]")
+        gain = 1.0
+        if radians is None:
+            radians, gain = frequencies(dims, base, scaling, factor, trained, turns)
+        radians = [float(x) for x in radians]
+        if len(radians) != dims // 2:
+            raise ValueError("E_ROTARY_FREQUENCIES: one for each pair")
+        self.ctx, self.dims, self.layout, self.radians = ctx, dims, layout, tuple(radians)
+        self.scale = float(gain if scale is None else scale)
+        self._desc = RotaryDesc()
+        check(lib().bfvgpu_rotary_set(ctypes.byref(self._desc), dims, LAYOUTS.index(layout),
+                                      (ctypes.c_double * len(radians))(*radians), self.scale), "rotary_set")
+        self._address = ctypes.addressof(self._desc)
+
+    def apply(self, x, positions, norm=None, eps: float = 1e-6, inverse: bool = False, out=None, stream: int | None = None):
+        """x [tokens][heads][dim] (bfloat16, float16 or float32, dim contiguous, any other strides) rotated at positions
+        [tokens] (int32) -> out (may be x); with `norm` [dim] (float32) after x rsqrt(mean(x^2) + eps) norm of each
+        head.  inverse: the gradient of a rotation's result -> that of x; not with a norm.  bfvgpu_rotary_device."""
+        h = self.ctx.handle
+        r = _calls().rotate(h.value if h is not None else None, self.ctx.device, self._address, x, positions, norm, eps, inverse,
+                            out, stream)
+        if type(r) is int:
+            check(r, "rotary_device")
+        return r

@@ -279,25 +279,6 @@ __device__ __forceinline__ void tmem_store_pairs(uint32_t at, const uint32_t (&r
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// ---- two floats at a time (subnormal numbers kept: the scale may be one, and -inf times a flushed one is NaN) ----
-__device__ __forceinline__ uint64_t two(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void split(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // Bits first .. last of a word whose bits stand for the numbers from `base` on.
 __device__ __forceinline__ uint32_t bits_of(int32_t first, int32_t last, int32_t base) {
   const int32_t a = max(first - base, 0), b = min(last - base, 31);

@@ -1,0 +1,576 @@
+// Rotary positions: of queries and keys on their way from a joint product into the paged cache, and alone.
+//
+//   x' = x rsqrt(mean(x^2) + eps) w              (norm of each head, where there is one)
+//   (a, b) -> s (a cos p f_i - b sin p f_i, b cos p f_i + a sin p f_i)
+// for the pairs i of the first `dims` elements of a head: (i, i + dims / 2) or (2 i, 2 i + 1).  All in 32 bits, rounded
+// once.  The gradient is the rotation back: sin with its sign changed.
+//
+// Angles: f_i comes as a 64-bit fraction of a turn, so that p f_i modulo a turn is one 64-bit product whose carries out
+// are whole turns: exact to p 2^-64 of a turn at any position (in 32-bit floating point an angle of 131071 is off by up
+// to 2^-8).  The upper 32 bits are an angle of at most an eighth of a turn and a number of quarters, and the
+// sine and cosine of the former are Taylor polynomials of degrees 9 and 10 (error below 2^-28).
+//
+// Bound by HBM where there are many tokens, by latency where there are few.  A lane has W pairs of a head, as two runs of
+// W elements, so that no pair and no angle is shared between lanes and a norm is a sum over the lanes of a row.  A warp has
+// a token, whose angles it computes once for all its rows; few tokens are dealt to several warps each.  Instructions, not
+// only bytes, count here (16 elements a lane once took 360 of them), hence two pairs at a time, products kept, and rows
+// that arrive through a ring in shared memory (as loads into registers, which share six scoreboards, deeper prefetch
+// gained nothing: 16384 tokens of 32 heads, 52 us; 44 through the ring).
+// Measured: 17349 tokens of 16 + 2 x 8 heads of 128, 32 to 16 bits, with norms: 72 us, 5.9 TB/s; 16384 tokens of 32 heads in
+// bfloat16, with a norm: 44 us, 6.1 TB/s; 8191 of 12 heads of 96 in 32 bits: 15.1 us, 5.0 TB/s; 8191 of 32 + 2 x 4 heads,
+// 16 bits, appended: 32.8 us, 5.1 TB/s (three dependent look-ups come before a token's first result).  One decode step of
+// 64 sequences: 3.5 us; queries alone of 16 tokens: 2.6 us.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "kv_host.h"
+
+namespace bfvgpu {
+namespace kv {
+namespace {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMostPairs = 64;
+constexpr int kAhead = 4;  // tasks whose elements are in flight or in work
+// Blocks of a processor.
+template <int W>
+constexpr int kPerSm = W == 8 ? 3 : 4;
+
+struct Angles {
+  uint64_t turns[kMostPairs];  // 2^-64 turns per position
+  float scale = 1.f;
+  int32_t dims = 0;
+  int32_t back = 0;  // 1: rotates back
+};
+
+// A tensor [tokens][heads][dim]; strides in elements.
+struct Rows {
+  const void* from = nullptr;
+  int64_t token_stride = 0, head_stride = 0;
+  int32_t heads = 0;
+  const float* norm = nullptr;
+};
+
+struct Work {
+  Rows q, k, v;
+  void* out = nullptr;  // of q
+  int64_t out_token_stride = 0, out_head_stride = 0;
+  const int32_t* positions = nullptr;  // q alone: of each token
+  int32_t tokens = 0, dim = 0;
+  int32_t items = 0;        // lanes of a row that have elements
+  int32_t lanes_log = 0;    // log2(lanes of a row)
+  int32_t split = 1;        // warps of a token
+  float eps = 0, inverse_dim = 0;
+};
+
+// (cos, sin) of w 2^-64 turns times position.
+__device__ __forceinline__ float2 turned(uint64_t w, int32_t position) {
+  const uint32_t t = (uint32_t)((w * (uint64_t)(int64_t)position) >> 32);
+  const uint32_t quarter = (t + (1u << 29)) >> 30;
+  const float y = (float)(int32_t)(t - (quarter << 30)) * 1.4629180792671596e-9f;  // 2 pi 2^-32
+  const float z = y * y;
+  const float s = fmaf(y * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), y);
+  const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
+  const float a = quarter & 1 ? s : c, b = quarter & 1 ? c : s;
+  return make_float2((quarter + 1) & 2 ? -a : a, quarter & 2 ? -b : b);
+}
+
+// N elements of type KIND (0 bfloat16, 1 float16, 2 float32) <-> 32 bits, by accesses as wide as their alignment.
+template <int KIND>
+using Of = std::conditional_t<KIND == 0, Bf16, Fp16>;
+template <int KIND, int N>
+struct Run {
+  static constexpr int kWords = KIND == 2 ? N : N / 2;
+  uint32_t w[kWords];
+  static constexpr int kBytes = kWords * 4, kChunk = kBytes < 16 ? kBytes : 16, kChunks = kBytes / kChunk;
+  static __device__ __forceinline__ const void* place(const void* base, int64_t at) {
+    return static_cast<const char*>(base) + at * (KIND == 2 ? 4 : 2);
+  }
+  // A copy on its way to shared memory, where the chunks of a block's threads lie side by side, and what it brought.
+  static __device__ __forceinline__ void fetch(uint32_t to, const void* from) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const char* at = static_cast<const char*>(from) + i * kChunk;
+      if constexpr (kChunk == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * kThreads * 16), "l"(at) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(at), "n"(kChunk) : "memory");
+    }
+  }
+  __device__ __forceinline__ void take(const uint8_t* from) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) words(reinterpret_cast<const uint32_t*>(from + i * kThreads * kChunk), i * (kChunk / 4));
+  }
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+      words(static_cast<const uint32_t*>(place(base, at)) + i * (kChunk / 4), i * (kChunk / 4));
+  }
+  __device__ __forceinline__ void words(const uint32_t* p, int i) {
+    if constexpr (kChunk == 16) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p);
+      w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+    } else if constexpr (kChunk == 8) {
+      const uint2 x = *reinterpret_cast<const uint2*>(p);
+      w[0] = x.x, w[1] = x.y;
+    } else {
+      w[0] = *p;
+    }
+  }
+  __device__ __forceinline__ void store(void* base, int64_t at) const {
+    uint32_t* p = KIND == 2 ? static_cast<uint32_t*>(base) + at : reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(base) + at);
+    if constexpr (kWords >= 4) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) *reinterpret_cast<uint4*>(p + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    } else if constexpr (kWords == 2) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+      *p = w[0];
+    }
+  }
+  // two elements at a time
+  __device__ __forceinline__ void get(uint64_t* x) const {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (KIND == 2) {
+        x[i] = two(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+      } else {
+        const float2 f = Of<KIND>::unpack(w[i]);
+        x[i] = two(f.x, f.y);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(const uint64_t* x) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      float lo, hi;
+      split(x[i], lo, hi);
+      if constexpr (KIND == 2) w[2 * i] = __float_as_uint(lo), w[2 * i + 1] = __float_as_uint(hi);
+      else w[i] = Of<KIND>::pack(lo, hi);
+    }
+  }
+};
+
+// A task is 32 >> lanes_log rows of a token's queries, keys or values; a token's tasks are cut into an equal run for each
+// of its warps.  What a warp keeps from task to task are the products of angles and norm weights, so that the pairs of a
+// task take two products and two fused ones, two pairs at a time.
+// PAGES: keys and values go to their pages; else there are queries only, at given positions.
+template <int SRC, int DST, int W, bool HALF, bool PAGES>
+__global__ void __launch_bounds__(kThreads, kPerSm<W>)
+    k_rotary(View kv, Batch bt, const __grid_constant__ Work wk, const __grid_constant__ Angles an) {
+  cudaGridDependencySynchronize();
+  const int lane = threadIdx.x & 31, in_block = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const uint32_t warp = blockIdx.x * kWarps + in_block;
+  const int32_t t = (int32_t)(warp / (uint32_t)wk.split), share = (int32_t)(warp - (uint32_t)t * wk.split);
+  if (t >= wk.tokens) return;
+  const int32_t item = lane & ((1 << wk.lanes_log) - 1), sub = lane >> wk.lanes_log, per = 32 >> wk.lanes_log;
+  const bool mine = item < wk.items;
+  const int32_t q_tasks = (wk.q.heads + per - 1) >> (5 - wk.lanes_log);
+  const int32_t kv_tasks = PAGES ? (wk.k.heads + per - 1) >> (5 - wk.lanes_log) : 0;
+  const int32_t tasks = q_tasks + 2 * kv_tasks;
+  // the warp's tasks of token t: from `k` on, `left` of them
+  int32_t k = tasks * share / wk.split, left = tasks * (share + 1) / wk.split - k;
+
+  // The two runs of W elements, which lie so that neighbouring lanes have neighbouring runs: HALF: pairs of a run and the
+  // one half a rotation further, then the two halves of the elements that stay; else the two halves of a head, of which
+  // either may turn or stay.
+  const int32_t half = an.dims / 2;
+  const bool first_half = HALF && W * item < half;
+  const int32_t a0 = HALF && !first_half ? half + W * item : W * item;
+  const int32_t apart = !HALF ? wk.dim / 2 : first_half ? half : (wk.dim - an.dims) / 2;
+  const bool turns = HALF ? first_half : a0 < an.dims, turns_b = !HALF && a0 + apart < an.dims;
+
+  __shared__ __align__(16) float angles[kWarps][2][kMostPairs];
+  using In = Run<SRC, W>;
+  // a ring of tasks' elements on their way: each thread copies, and reads back, its own
+  constexpr int kRun = In::kBytes * kThreads;
+  __shared__ __align__(16) uint8_t ring[kAhead * 2 * kRun];
+  const uint8_t* ring_of = ring + threadIdx.x * In::kChunk;
+  const uint32_t ring_at = smem_addr(ring_of);
+  // The copies go through the tasks ahead of the arithmetic: task, end of the tensor's tasks, the lane's row.
+  int32_t ahead = left, at_task = k, at_end = 0, at_row = 0, at_heads = 0;
+  const char* from = nullptr;
+  int64_t from_step = 0;
+  auto source = [&](const Rows& r, int32_t before, int32_t count) {
+    at_end = before + count;
+    at_row = (at_task - before) * per + sub;
+    at_heads = mine ? r.heads : 0;
+    from = static_cast<const char*>(In::place(r.from, t * r.token_stride + at_row * r.head_stride + a0));
+    from_step = (int64_t)per * r.head_stride * (SRC == 2 ? 4 : 2);
+  };
+  auto fetch = [&](uint32_t slot) {
+    if (ahead > 0) {
+      if (at_task >= at_end) {
+        if (!PAGES || at_task < q_tasks) source(wk.q, 0, q_tasks);
+        else if (at_task < q_tasks + kv_tasks) source(wk.k, q_tasks, kv_tasks);
+        else source(wk.v, q_tasks + kv_tasks, kv_tasks);
+      }
+      if (at_row < at_heads) {
+        In::fetch(ring_at + slot, from);
+        In::fetch(ring_at + slot + kRun, from + apart * (SRC == 2 ? 4 : 2));
+      }
+      from += from_step;
+      at_row += per;
+      ++at_task;
+      --ahead;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int n = 0; n < kAhead - 1; ++n) fetch(2 * n * kRun);  // under the search for the token's place
+  Run<2, W> na, nb;  // a tensor's norm weights
+  const float* weighed = nullptr;
+  auto weights = [&](const Rows& r) {
+    if (r.norm == weighed) return;
+    weighed = r.norm;
+    if (r.norm && mine) {
+      na.load(r.norm, a0);
+      nb.load(r.norm, a0 + apart);
+    }
+  };
+  weights(k < q_tasks ? wk.q : wk.k);
+
+  int32_t position;
+  int64_t to = 0;  // the token's row in its page
+  if constexpr (!PAGES) {
+    position = __ldg(wk.positions + t);
+  } else {
+    int32_t b = t, first = t, next = t + 1;
+    if (bt.starts) {
+      b = sequence_of_token(bt, t);
+      first = bt.starts[b];
+      next = bt.starts[b + 1];
+    }
+    const int64_t pos = (int64_t)checked_length(bt, kv, bt.lengths[b]) - next + t;
+    const int64_t slot = pos >> kv.page_log;
+    const int32_t page = t >= first && t < next && pos >= 0 && slot < bt.width ? bt.table[(int64_t)b * bt.width + slot] : -1;
+    if (page < 0 || page >= kv.pages) {
+      if (lane == 0) flag_error(bt.err, kErrTable);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");  // nothing is on its way to a block that has left
+      return;
+    }
+    to = page * kv.page_stride + (pos & ((1 << kv.page_log) - 1)) * kv.token_stride;
+    position = (int32_t)pos;
+  }
+  if (k < q_tasks + kv_tasks) {
+    for (int32_t i = lane; i < half; i += 32) {
+      const float2 cs = turned(an.turns[i], position);
+      angles[in_block][0][i] = cs.x * an.scale;
+      angles[in_block][1][i] = (an.back ? -cs.y : cs.y) * an.scale;
+    }
+    __syncwarp();
+  }
+
+  // HALF: of a pair of pairs j, keep[j] (a) and keep[W / 2 + j] (b) times the element itself, cross[] times the other;
+  // else of pair j both at once.  Elements that stay: the norm's weights alone.
+  uint64_t keep[W], cross[W];
+  auto prepare = [&](bool normed) {
+    float wa[W], wb[W], c[W], s[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      wa[e] = normed ? __uint_as_float(na.w[e]) : 1.f;
+      wb[e] = normed ? __uint_as_float(nb.w[e]) : 1.f;
+      c[e] = 1.f;
+      s[e] = 0.f;
+    }
+    // pairs [at, at + N) into c and s from `e` on
+    auto angles_of = [&](auto n, int32_t at, int e) {
+      constexpr int N = decltype(n)::value;
+      Run<2, N> rc, rs;
+      rc.load(angles[in_block][0], at);
+      rs.load(angles[in_block][1], at);
+#pragma unroll
+      for (int i = 0; i < N; ++i) c[e + i] = __uint_as_float(rc.w[i]), s[e + i] = __uint_as_float(rs.w[i]);
+    };
+    if constexpr (HALF) {
+      if (turns) angles_of(std::integral_constant<int, W>(), a0, 0);
+    } else {
+      if (turns) angles_of(std::integral_constant<int, W / 2>(), a0 / 2, 0);
+      if (turns_b) angles_of(std::integral_constant<int, W / 2>(), (a0 + apart) / 2, W / 2);
+    }
+    if constexpr (HALF) {
+#pragma unroll
+      for (int j = 0; j < W / 2; ++j) {
+        keep[j] = two(wa[2 * j] * c[2 * j], wa[2 * j + 1] * c[2 * j + 1]);
+        cross[j] = two(-wb[2 * j] * s[2 * j], -wb[2 * j + 1] * s[2 * j + 1]);
+        keep[W / 2 + j] = two(wb[2 * j] * c[2 * j], wb[2 * j + 1] * c[2 * j + 1]);
+        cross[W / 2 + j] = two(wa[2 * j] * s[2 * j], wa[2 * j + 1] * s[2 * j + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float wx = j < W / 2 ? wa[2 * j % W] : wb[2 * j % W], wy = j < W / 2 ? wa[2 * j % W + 1] : wb[2 * j % W + 1];
+        keep[j] = two(wx * c[j], wy * c[j]);
+        cross[j] = two(-wy * s[j], wx * s[j]);
+      }
+    }
+  };
+  auto rotate = [&](uint64_t (&x)[W], bool normed) {
+    float f = 1.f;
+    if (normed) {
+      uint64_t sums = 0;
+#pragma unroll
+      for (int e = 0; e < W; ++e) sums = fma2(x[e], x[e], sums);
+      float sum, odd;
+      split(sums, sum, odd);
+      sum = mine ? sum + odd : 0.f;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1)
+        if (d < 1 << wk.lanes_log) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      f = rsqrtf(sum * wk.inverse_dim + wk.eps);
+    }
+    if constexpr (HALF) {
+      if (turns) {
+#pragma unroll
+        for (int j = 0; j < W / 2; ++j) {
+          const uint64_t a = x[j], b = x[W / 2 + j];
+          x[j] = fma2(a, keep[j], mul2(b, cross[j]));
+          x[W / 2 + j] = fma2(b, keep[W / 2 + j], mul2(a, cross[W / 2 + j]));
+        }
+      } else if (normed) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) x[e] = mul2(x[e], keep[e]);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h ? turns_b : turns) {
+#pragma unroll
+          for (int j = h * W / 2; j < (h + 1) * W / 2; ++j) {
+            float a, b;
+            split(x[j], a, b);
+            x[j] = fma2(x[j], keep[j], mul2(two(b, a), cross[j]));
+          }
+        } else if (normed) {
+#pragma unroll
+          for (int j = h * W / 2; j < (h + 1) * W / 2; ++j) x[j] = mul2(x[j], keep[j]);
+        }
+      }
+    }
+    if (normed) {
+#pragma unroll
+      for (int e = 0; e < W; ++e) x[e] = mul2(x[e], two(f, f));
+    }
+  };
+  using Out = Run<DST, W>;
+  uint32_t slot = 0;
+  // The warp's tasks of the token's rows of one tensor, whose tasks come after `before` others.
+  auto through = [&](const Rows& r, int32_t before, int32_t count, void* base, int64_t out_at, int64_t out_stride,
+                     auto turned_too) {
+    int32_t n = min(left, before + count - k);
+    if (n <= 0) return;
+    left -= n;
+    int32_t row = (k - before) * per + sub;
+    k += n;
+    char* out = const_cast<char*>(static_cast<const char*>(Out::place(base, out_at + row * out_stride + a0)));
+    const int64_t out_step = (int64_t)per * out_stride * (DST == 2 ? 4 : 2);
+    const int32_t heads = mine ? r.heads : 0;
+    const bool normed = turned_too && r.norm;
+    if constexpr (turned_too) {
+      weights(r);
+      prepare(normed);
+    }
+    for (; n > 0; --n) {
+      // the slot filled next was read in the last step
+      fetch(slot == 0 ? 2 * (kAhead - 1) * kRun : slot - 2 * kRun);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+      uint64_t x[W];
+      In in;
+      in.take(ring_of + slot);
+      in.get(x);
+      in.take(ring_of + slot + kRun);
+      in.get(x + W / 2);
+      slot = slot == 2 * (kAhead - 1) * kRun ? 0 : slot + 2 * kRun;
+      if constexpr (turned_too) rotate(x, normed);
+      if (row < heads) {
+        Out oa, ob;
+        oa.put(x);
+        ob.put(x + W / 2);
+        oa.store(out, 0);
+        ob.store(out, apart);
+      }
+      out += out_step;
+      row += per;
+    }
+  };
+
+  through(wk.q, 0, q_tasks, wk.out, t * wk.out_token_stride, wk.out_head_stride, std::true_type());
+  if constexpr (PAGES) {
+    through(wk.k, q_tasks, kv_tasks, kv.k, to, kv.head_stride, std::true_type());
+    through(wk.v, q_tasks + kv_tasks, kv_tasks, kv.v, to, kv.head_stride, std::false_type());
+  }
+}
+
+// The widest runs that the halves of a rotation, of what stays, or of a head consist of.
+int run_of(const bfvgpu_rotary& r, int32_t dim, int most) {
+  for (int w = most; w > 2; w /= 2)
+    if (r.layout == BFVGPU_ROTARY_HALF ? r.dims % (2 * w) == 0 && (dim - r.dims) % (2 * w) == 0 : dim % (2 * w) == 0 && r.dims % w == 0)
+      return w;
+  return 2;
+}
+
+template <int SRC, int DST, bool PAGES>
+auto kernel_of(int w, bool half) {
+  if constexpr (SRC != 2)
+    if (w == 8) return half ? k_rotary<SRC, DST, 8, true, PAGES> : k_rotary<SRC, DST, 8, false, PAGES>;
+  if (w >= 4) return half ? k_rotary<SRC, DST, 4, true, PAGES> : k_rotary<SRC, DST, 4, false, PAGES>;
+  return half ? k_rotary<SRC, DST, 2, true, PAGES> : k_rotary<SRC, DST, 2, false, PAGES>;
+}
+
+// An angle as a fraction of a turn in 2^-64; the division is exact to 2^-63 of its result, below 2^-64 of a turn for
+// frequencies below 1.
+uint64_t turns_of(double radians) {
+  const long double turn = 6.283185307179586476925286766559005768L;
+  long double x = radians / turn;
+  x -= std::floor(x);
+  x = std::floor(x * 0x1p64L + 0.5L);  // [0, 2^64]
+  return x >= 0x1p64L ? 0 : (uint64_t)x;
+}
+
+void checked_rotary(const bfvgpu_rotary* r, int32_t dim) {
+  need(r != nullptr, BFVGPU_E_ARGUMENT, "E_ROTARY_ARGUMENT");
+  need(r->layout == BFVGPU_ROTARY_HALF || r->layout == BFVGPU_ROTARY_INTERLEAVED, BFVGPU_E_ARGUMENT, "E_ROTARY_LAYOUT");
+  need(r->dims >= 4 && r->dims <= 2 * kMostPairs && r->dims % 4 == 0, BFVGPU_E_SHAPE, "E_ROTARY_DIMS");
+  need(r->dims <= dim, BFVGPU_E_SHAPE, "E_ROTARY_DIMS");
+  need(std::isfinite(r->scale), BFVGPU_E_ARGUMENT, "E_ROTARY_SCALE");
+}
+
+void launch(const View& kv, const Batch& bt, Work& wk, const bfvgpu_rotary& r, bool back, int src, int dst, cudaStream_t st) {
+  Angles an;
+  for (int i = 0; i < kMostPairs; ++i) an.turns[i] = i < r.dims / 2 ? r.turns[i] : 0;
+  an.scale = r.scale;
+  an.dims = r.dims;
+  an.back = back;
+  // Runs of 16 bytes; 8 of 16-bit types on the way into pages, where the registers of a fourth block count more
+  // (8191 tokens of 32 + 2 x 4 heads: 32.8 us against 38.1; rotated alone, 16384 tokens of 32 heads: 46.5 against 43.9).
+  const int w = run_of(r, wk.dim, src == 2 || !wk.positions ? 4 : 8);
+  wk.items = wk.dim / (2 * w);
+  wk.inverse_dim = 1.f / (float)wk.dim;
+  while (1 << wk.lanes_log < wk.items) ++wk.lanes_log;
+  const int32_t per = 32 >> wk.lanes_log, tasks = (wk.q.heads + per - 1) / per + 2 * ((wk.k.heads + per - 1) / per);
+  // a warp a token, and where they are few several (500 tokens of 32 heads: 4.25 us with this many warps, 5.1 with half
+  // as many again; 2000: 7.6 both)
+  constexpr int64_t kWarpsAtOnce = 148 * 2 * kWarps;
+  wk.split = (int32_t)std::clamp<int64_t>(kWarpsAtOnce / wk.tokens, 1, tasks);
+  const int64_t blocks = ((int64_t)wk.tokens * wk.split + kWarps - 1) / kWarps;
+  const bool half = r.layout == BFVGPU_ROTARY_HALF;
+  const auto kernel = wk.positions ? (src == 2   ? kernel_of<2, 2, false>(w, half)
+                                      : src == 0 ? kernel_of<0, 0, false>(w, half)
+                                                 : kernel_of<1, 1, false>(w, half))
+                      : src == 2   ? (dst == 0 ? kernel_of<2, 0, true>(w, half) : kernel_of<2, 1, true>(w, half))
+                                   : (src == 0 ? kernel_of<0, 0, true>(w, half) : kernel_of<1, 1, true>(w, half));
+  cuda_need(launch_next(kernel, dim3((unsigned)blocks), kThreads, 0, st, 1, kv, bt, wk, an), "rotary");
+  internal_count_launch(1);
+}
+
+bool aligned_strides(int dtype, int64_t a, int64_t b) {
+  const int64_t unit = dtype == BFVGPU_KV_F32 ? 4 : 8;
+  return a % unit == 0 && b % unit == 0;
+}
+
+}  // namespace
+}  // namespace kv
+}  // namespace bfvgpu
+
+using namespace bfvgpu;
+using namespace bfvgpu::kv;
+
+extern "C" int32_t bfvgpu_rotary_set(bfvgpu_rotary* r, int32_t dims, int32_t layout, const double* frequencies, double scale) {
+  return guarded([&] {
+    need(r && frequencies, BFVGPU_E_ARGUMENT, "E_ROTARY_ARGUMENT");
+    bfvgpu_rotary made{};
+    made.dims = dims;
+    made.layout = layout;
+    made.scale = (float)scale;
+    checked_rotary(&made, 2 * kMostPairs);
+    for (int i = 0; i < dims / 2; ++i) {
+      need(std::isfinite(frequencies[i]), BFVGPU_E_ARGUMENT, "E_ROTARY_FREQUENCIES");
+      made.turns[i] = turns_of(frequencies[i]);
+    }
+    *r = made;
+  });
+}
+
+extern "C" int32_t bfvgpu_rotary_device(bfvgpu_ctx* ctx, const bfvgpu_rotary* rotary, const void* x, int32_t dtype,
+                                        int64_t token_stride, int64_t head_stride, uint64_t tokens, uint64_t heads, int32_t dim,
+                                        const int32_t* positions, const float* norm, float eps, int32_t inverse, void* out,
+                                        int64_t out_token_stride, int64_t out_head_stride, void* stream) {
+  return guarded([&] {
+    need(dtype >= BFVGPU_KV_BF16 && dtype <= BFVGPU_KV_F32, BFVGPU_E_ARGUMENT, "E_ROTARY_DTYPE");
+    need(dim >= 8 && dim <= 2 * kMostPairs && dim % 8 == 0, BFVGPU_E_SHAPE, "E_ROTARY_DIM");
+    checked_rotary(rotary, dim);
+    need(tokens <= 0x7fffffff && heads <= 0xffff, BFVGPU_E_SHAPE, "E_ROTARY_SHAPE");
+    need(!(norm && inverse), BFVGPU_E_ARGUMENT, "E_ROTARY_NORM");  // the norm has no way back
+    need(std::isfinite(eps) && eps >= 0, BFVGPU_E_ARGUMENT, "E_ROTARY_EPS");
+    const Place at = checked_place(ctx, stream);
+    if (!tokens || !heads) return;
+    need(x && positions && out, BFVGPU_E_ARGUMENT, "E_ROTARY_ARGUMENT");
+    if (tokens == 1) token_stride = out_token_stride = 0;
+    if (heads == 1) head_stride = out_head_stride = 0;
+    need(aligned16(x) && aligned16(out) && aligned16(norm) && aligned_strides(dtype, token_stride, head_stride) &&
+             aligned_strides(dtype, out_token_stride, out_head_stride),
+         BFVGPU_E_ARGUMENT, "E_ROTARY_ALIGNMENT");
+    OnDevice scope(at.device);
+    Work wk;
+    wk.q = {x, token_stride, head_stride, (int32_t)heads, norm};
+    wk.out = out;
+    wk.out_token_stride = out_token_stride;
+    wk.out_head_stride = out_head_stride;
+    wk.positions = positions;
+    wk.tokens = (int32_t)tokens;
+    wk.dim = dim;
+    wk.eps = eps;
+    launch(View{}, Batch{}, wk, *rotary, inverse != 0, dtype, dtype, at.stream);
+  });
+}
+
+extern "C" int32_t bfvgpu_kv_append_rotary_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, int32_t layer,
+                                                  const bfvgpu_rotary* rotary, const void* k_new, const void* v_new,
+                                                  int32_t source_dtype, int64_t token_stride, int64_t head_stride,
+                                                  const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                                  uint64_t q_heads, const float* q_norm, const float* k_norm, float eps,
+                                                  uint64_t tokens, const int32_t* starts, const int32_t* table,
+                                                  uint64_t width, const int32_t* lengths, uint64_t seqs, void* q_out,
+                                                  void* stream) {
+  return guarded([&] {
+    need(layer >= 0, BFVGPU_E_SHAPE, "E_KV_LAYER");
+    const View w = checked_view(cache, layer);
+    checked_rotary(rotary, w.dim);
+    need(source_dtype == cache->dtype || source_dtype == BFVGPU_KV_F32, BFVGPU_E_ARGUMENT, "E_KV_SOURCE_DTYPE");
+    need(tokens <= 0x7fffffff && seqs <= 0x7ffffffe && width <= 0x7fffffff && q_heads <= 0xffff, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    need((width << w.page_log) <= (uint64_t(1) << 30), BFVGPU_E_SHAPE, "E_KV_WIDTH");  // positions are 32-bit numbers
+    need(starts || tokens == seqs, BFVGPU_E_SHAPE, "E_KV_STARTS");
+    need(std::isfinite(eps) && eps >= 0, BFVGPU_E_ARGUMENT, "E_ROTARY_EPS");
+    const Place at = checked_place(ctx, stream);
+    if (!tokens) return;
+    need(seqs && k_new && v_new && table && width && lengths && (!q_heads || (q && q_out)), BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
+    if (tokens == 1) token_stride = q_token_stride = 0;
+    if (w.heads == 1) head_stride = 0;
+    if (q_heads <= 1) q_head_stride = 0;
+    need(aligned16(k_new) && aligned16(v_new) && aligned_strides(source_dtype, token_stride, head_stride), BFVGPU_E_ARGUMENT,
+         "E_KV_ALIGNMENT");
+    need(!q_heads || (aligned16(q) && aligned16(q_out) && aligned_strides(source_dtype, q_token_stride, q_head_stride)),
+         BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
+    need(aligned16(q_norm) && aligned16(k_norm), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
+    OnDevice scope(at.device);
+    Batch bt;
+    bt.table = table;
+    bt.lengths = lengths;
+    bt.starts = starts;
+    bt.seqs = (int32_t)seqs;
+    bt.width = (int32_t)width;
+    bt.err = at.err;
+    Work wk;
+    if (q_heads) wk.q = {q, q_token_stride, q_head_stride, (int32_t)q_heads, q_norm};
+    wk.k = {k_new, token_stride, head_stride, w.heads, k_norm};
+    wk.v = {v_new, token_stride, head_stride, w.heads, nullptr};
+    wk.out = q_out;
+    wk.out_token_stride = (int64_t)q_heads * w.dim;
+    wk.out_head_stride = w.dim;
+    wk.tokens = (int32_t)tokens;
+    wk.dim = w.dim;
+    wk.eps = eps;
+    launch(w, bt, wk, *rotary, false, source_dtype, cache->dtype, at.stream);
+  });
+}

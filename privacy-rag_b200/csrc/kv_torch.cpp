@@ -1,4 +1,4 @@
-// The calls of PagedKv on torch tensors: checks, results and scratch, then the C ABI.
+// The calls of PagedKv and Rotary on torch tensors: checks, results and scratch, then the C ABI.
 //
 // A CPython module rather than ctypes, because these calls are a handful a layer and last microseconds on the
 // GPU: checking the tensors in Python and converting 17 arguments took 9.0 us a decode call, 4.4 us of it the
@@ -20,6 +20,7 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <utility>
 
 #include "bfvgpu.h"
 
@@ -81,10 +82,11 @@ Table table_of(PyObject* o, const Cache& c) {
     refuse(std::string("E_KV_SHAPE: the table is a dense int32 tensor [rows][width]") + kWhere);
   return {static_cast<int32_t*>(t.data_ptr()), (uint64_t)t.size(0), (uint64_t)t.size(1)};
 }
-int32_t* ints_of(PyObject* o, const char* name, uint64_t count, const Cache& c) {
+int32_t* ints_of(PyObject* o, const char* name, uint64_t count, const Cache& c, const char* error = "E_KV_SHAPE",
+                 const char* where = kWhere) {
   const at::Tensor& t = tensor_of(o, name);
   if (t.scalar_type() != at::kInt || !there(t, c) || t.dim() != 1 || (uint64_t)t.size(0) != count || !t.is_contiguous())
-    refuse(std::string("E_KV_SHAPE: ") + name + " is a dense int32 tensor [" + std::to_string(count) + "]" + kWhere);
+    refuse(std::string(error) + ": " + name + " is a dense int32 tensor [" + std::to_string(count) + "]" + where);
   return static_cast<int32_t*>(t.data_ptr());
 }
 uint64_t count_of(PyObject* o, const char* name) {
@@ -187,6 +189,147 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- rotary positions ----
+constexpr const char* kHere = " on the context's device";
+const bfvgpu_rotary* rotary_of(PyObject* o) {
+  const void* p = PyLong_AsVoidPtr(o);
+  if (!p && PyErr_Occurred()) throw python_error();
+  return static_cast<const bfvgpu_rotary*>(p);
+}
+// float32 weights of a head's norm, or none
+const float* norm_of(PyObject* o, const char* name, int64_t dim, const Cache& c) {
+  if (o == Py_None) return nullptr;
+  const at::Tensor& t = tensor_of(o, name);
+  if (t.scalar_type() != at::kFloat || !there(t, c) || t.dim() != 1 || t.size(0) != dim || !t.is_contiguous())
+    refuse(std::string("E_ROTARY_SHAPE: ") + name + " is a dense float32 tensor [" + std::to_string(dim) + "]" + kHere);
+  return static_cast<const float*>(t.data_ptr());
+}
+float float_of(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return (float)v;
+}
+// The bytes that a tensor's elements lie in.
+std::pair<const char*, const char*> bytes_of(const at::Tensor& t) {
+  int64_t lo = 0, hi = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (!t.size(i)) return {nullptr, nullptr};
+    (t.stride(i) < 0 ? lo : hi) += (t.size(i) - 1) * t.stride(i);
+  }
+  const char* at = static_cast<const char*>(t.data_ptr());
+  return {at + lo * t.element_size(), at + (hi + 1) * t.element_size()};
+}
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const auto x = bytes_of(a), y = bytes_of(b);
+  return x.first < y.second && y.first < x.second;
+}
+// Whether two tensors are the same elements in the same places.
+bool same_place(const at::Tensor& a, const at::Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.scalar_type() != b.scalar_type()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
+// append_rotary(cache, ctx, address of a bfvgpu_rotary, k_new, v_new, starts | None, table, lengths, q | None, q_norm | None,
+// k_norm | None, eps, layer, out | None, stream | None) -> out | None | status
+PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!wants(n, 15)) return nullptr;
+  return answered([&]() -> PyObject* {
+    const Cache& c = cache_of(a[0]);
+    const at::Tensor &k = rows_of(a[3], "k_new", c), &v = tensor_of(a[4], "v_new");
+    const bool wide = k.scalar_type() == at::kFloat;
+    if (k.size(1) != c.kv.heads || !(wide || k.scalar_type() == c.type()))
+      refuse("E_KV_SHAPE: k_new has the cache's heads, and its type or float32");
+    if (v.sizes() != k.sizes() || v.strides() != k.strides() || v.scalar_type() != k.scalar_type() || !there(v, c))
+      refuse("E_KV_SHAPE: k_new and v_new need one shape, type and layout");
+    const Table t = table_of(a[6], c);
+    const int32_t* starts = a[5] == Py_None ? nullptr : ints_of(a[5], "starts", t.rows + 1, c);
+    const int32_t* lengths = ints_of(a[7], "lengths", t.rows, c);
+    const float *q_norm = norm_of(a[9], "q_norm", c.kv.dim, c), *k_norm = norm_of(a[10], "k_norm", c.kv.dim, c);
+    const float eps = float_of(a[11]);
+    const int32_t layer = int_of(a[12]);
+    const bool with_q = a[8] != Py_None;
+    if (!with_q && (q_norm || a[13] != Py_None)) refuse("E_KV_SHAPE: q_norm and out are those of q");
+    const Stream s(a[14], c);
+    at::Tensor made;
+    if (with_q) {
+      const at::Tensor& q = rows_of(a[8], "q", c);
+      if (q.size(0) != k.size(0) || q.scalar_type() != k.scalar_type()) refuse("E_KV_SHAPE: q has the tokens and the type of k_new");
+      if (a[13] == Py_None) {
+        made = at::empty(q.sizes(), q.options().dtype(c.type()));
+      } else {
+        const at::Tensor& given = tensor_of(a[13], "out");
+        if (given.sizes() != q.sizes() || given.scalar_type() != c.type() || !there(given, c) || !given.is_contiguous())
+          refuse("E_KV_SHAPE: out is dense, of q's shape and the cache's type");
+        if (overlap(given, k) || overlap(given, v) || (overlap(given, q) && !same_place(given, q)))
+          refuse("E_KV_OVERLAP: out is q itself, or overlaps no argument");
+      }
+    }
+    s.uses(c, {a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[13]});
+    const at::Tensor none;
+    const at::Tensor& q = with_q ? THPVariable_Unpack(a[8]) : none;
+    const at::Tensor& out = made.defined() ? made : with_q ? THPVariable_Unpack(a[13]) : none;
+    const int32_t rc = bfvgpu_kv_append_rotary_device(
+        context_of(a[1]), &c.kv, layer, rotary_of(a[2]), k.data_ptr(), v.data_ptr(), wide ? BFVGPU_KV_F32 : c.kv.dtype, k.stride(0),
+        k.stride(1), with_q ? q.data_ptr() : nullptr, with_q ? q.stride(0) : 0, with_q ? q.stride(1) : 0,
+        with_q ? (uint64_t)q.size(1) : 0, q_norm, k_norm, eps, (uint64_t)k.size(0), starts, t.at, t.width, lengths, t.rows,
+        with_q ? out.data_ptr() : nullptr, s.handle);
+    if (rc) return PyLong_FromLong(rc);
+    if (made.defined()) return THPVariable_Wrap(made);
+    PyObject* back = with_q ? a[13] : Py_None;
+    Py_INCREF(back);
+    return back;
+  });
+}
+
+// rotate(ctx, device, address of a bfvgpu_rotary, x, positions, norm | None, eps, inverse, out | None, stream | None) -> out | status
+PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!wants(n, 10)) return nullptr;
+  return answered([&]() -> PyObject* {
+    Cache c{};
+    c.device = int_of(a[1]);
+    const at::Tensor& x = tensor_of(a[3], "x");
+    if (!there(x, c) || x.dim() != 3 || x.stride(2) != 1)
+      refuse(std::string("E_ROTARY_SHAPE: x is [tokens][heads][dim], dim contiguous,") + kHere);
+    const int32_t dtype = x.scalar_type() == at::kBFloat16 ? BFVGPU_KV_BF16
+                          : x.scalar_type() == at::kHalf   ? BFVGPU_KV_FP16
+                          : x.scalar_type() == at::kFloat  ? BFVGPU_KV_F32
+                                                           : -1;
+    if (dtype < 0) refuse("E_ROTARY_DTYPE: bfloat16, float16 or float32");
+    const int32_t* positions = ints_of(a[4], "positions", (uint64_t)x.size(0), c, "E_ROTARY_SHAPE", kHere);
+    const float* norm = norm_of(a[5], "norm", x.size(2), c);
+    const float eps = float_of(a[6]);
+    const int inverse = PyObject_IsTrue(a[7]);
+    if (inverse < 0) throw python_error();
+    const Stream s(a[9], c);
+    at::Tensor made;
+    if (a[8] == Py_None) {
+      made = at::empty(x.sizes(), x.options());
+    } else {
+      const at::Tensor& given = tensor_of(a[8], "out");
+      if (given.sizes() != x.sizes() || given.scalar_type() != x.scalar_type() || !there(given, c) || given.stride(2) != 1)
+        refuse(std::string("E_ROTARY_SHAPE: out has x's shape and type, dim contiguous,") + kHere);
+      // rows that do not overlap: one axis inside the other
+      const bool outer = given.stride(0) >= given.stride(1);
+      const int64_t in = given.size(outer ? 1 : 0), out = given.size(outer ? 0 : 1);
+      const int64_t small = given.stride(outer ? 1 : 0), large = given.stride(outer ? 0 : 1), dim = given.size(2);
+      if ((in > 1 && small < dim) || (out > 1 && large < (in > 1 ? (in - 1) * small : 0) + dim))
+        refuse("E_ROTARY_OVERLAP: the rows of out overlap");
+      if (overlap(given, x) && !same_place(given, x)) refuse("E_ROTARY_OVERLAP: out is x itself, or does not overlap it");
+    }
+    s.uses(c, {a[3], a[4], a[5], a[8]});
+    const at::Tensor& out = made.defined() ? made : THPVariable_Unpack(a[8]);
+    const int32_t rc = bfvgpu_rotary_device(context_of(a[0]), rotary_of(a[2]), x.data_ptr(), dtype, x.stride(0), x.stride(1),
+                                            (uint64_t)x.size(0), (uint64_t)x.size(1), (int32_t)x.size(2), positions, norm, eps,
+                                            inverse, out.data_ptr(), out.stride(0), out.stride(1), s.handle);
+    if (rc) return PyLong_FromLong(rc);
+    if (made.defined()) return THPVariable_Wrap(made);
+    Py_INCREF(a[8]);
+    return a[8];
+  });
+}
+
 // fork(cache, ctx, parents, children, fresh, table, lengths, stream | None) -> status
 PyObject* fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!wants(n, 8)) return nullptr;
@@ -281,7 +424,8 @@ PyMethodDef method(const char* name) {
 
 PyMODINIT_FUNC PyInit_bfvgpu_kv_calls() {
   static PyMethodDef methods[] = {method<open_cache>("open"), method<append>("append"), method<fork>("fork"), method<move>("move"),
-                                  method<decode>("decode"),   method<prompt>("prompt"), {nullptr, nullptr, 0, nullptr}};
+                                  method<decode>("decode"),   method<prompt>("prompt"), method<append_rotary>("append_rotary"),
+                                  method<rotate>("rotate"),   {nullptr, nullptr, 0, nullptr}};
   static PyModuleDef module = {PyModuleDef_HEAD_INIT, "bfvgpu_kv_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
   return PyModule_Create(&module);
 }

@@ -571,6 +571,26 @@ int32_t bfvgpu_kv_prompt_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t
 enum bfvgpu_kv_kernel { BFVGPU_KV_ROWS = 0, BFVGPU_KV_TILES = 1 };
 int32_t bfvgpu_kv_prompt_kernel(const bfvgpu_kv *cache, int64_t token_stride, int64_t head_stride, uint64_t q_heads,
                                 uint64_t tokens, uint64_t seqs, uint64_t width, int32_t window, int32_t sinks);
+/* The same two calls, without a window, where groups of sequences share their first tokens (answers forked from one
+ * document, questions on one document): what is shared is read once for a group.  groups [count + 1] (int32): group i has
+ * the sequences groups[i] .. groups[i + 1] - 1, groups[0] = 0, groups[count] = seqs; shared [count] (int32): how many
+ * first tokens its sequences share, any number from 0 to the position of their first new token plus one.  Shared tokens
+ * are read through the table's row of the group's first sequence; the other rows' entries of pages that only they lie in
+ * are not read.  Groups, like lengths, are read on the device and recorded where they are outside their range; the
+ * results are then unspecified.  Results are those of bfvgpu_kv_decode_device and bfvgpu_kv_prompt_device on the
+ * same keys up to the order of 32-bit sums.  scratch: bfvgpu_kv_shared_scratch_words words (decode: tokens = seqs). */
+uint64_t bfvgpu_kv_shared_scratch_words(const bfvgpu_ctx *ctx, const bfvgpu_kv *cache, uint64_t q_heads, uint64_t tokens,
+                                        uint64_t seqs, uint64_t width, uint64_t groups);
+int32_t bfvgpu_kv_decode_shared_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t layer, const void *q,
+                                       int64_t token_stride, int64_t head_stride, uint64_t q_heads, const int32_t *table,
+                                       uint64_t width, const int32_t *lengths, uint64_t seqs, const int32_t *groups,
+                                       const int32_t *shared, uint64_t count, float scale, uint64_t *scratch, void *out,
+                                       void *stream);
+int32_t bfvgpu_kv_prompt_shared_device(bfvgpu_ctx *ctx, const bfvgpu_kv *cache, int32_t layer, const void *q,
+                                       int64_t token_stride, int64_t head_stride, uint64_t q_heads, uint64_t tokens,
+                                       const int32_t *starts, const int32_t *table, uint64_t width, const int32_t *lengths,
+                                       uint64_t seqs, const int32_t *groups, const int32_t *shared, uint64_t count,
+                                       float scale, uint64_t *scratch, void *out, void *stream);
 
 #ifdef __cplusplus
 }

@@ -127,6 +127,26 @@ class PagedKv:
             check(r, "kv_prompt_device")
         return r
 
+    def decode_shared(self, q, table, lengths, groups, shared, layer: int = 0, scale: float | None = None, out=None,
+                      stream: int | None = None):
+        """``decode`` without a window, where the sequences groups[i] .. groups[i + 1] - 1 (groups [count + 1], int32, from 0 to
+        the number of rows) share their first shared[i] tokens ([count], int32; 0: nothing), which are read once for all
+        of them, through the table's row of the group's first.  bfvgpu_kv_decode_shared_device."""
+        r = self._calls.decode_shared(self._cache, self._handle, q, table, lengths, groups, shared, layer, scale, out, stream)
+        if type(r) is int:
+            check(r, "kv_decode_shared_device")
+        return r
+
+    def prompt_shared(self, q, starts, table, lengths, groups, shared, layer: int = 0, scale: float | None = None, out=None,
+                      stream: int | None = None):
+        """``prompt`` in the same way: no sequence's new tokens lie among those that it shares, but for the last.
+        bfvgpu_kv_prompt_shared_device."""
+        r = self._calls.prompt_shared(self._cache, self._handle, q, starts, table, lengths, groups, shared, layer, scale, out,
+                                      stream)
+        if type(r) is int:
+            check(r, "kv_prompt_shared_device")
+        return r
+
     def prompt_kernel(self, q, table, window: int = 0, sinks: int = 0) -> str:
         """Which kernel ``prompt`` takes, by sizes and strides alone: "rows", as every ``decode``, whose weights
         keep the remainder of their rounding to 16 bits, or "tiles", the tensor-core kernel, whose weights do

@@ -20,7 +20,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "lib", "libbfvgpu.so")
 SOURCES = ["kernels.cu", "bfvgpu.cu", "noalloc.cu", "peak.cu", "kv_pages.cu", "kv_rows.cu", "kv_prompt.cu", "kv_attention.cu",
-           "kv_rotary.cu"]
+           "kv_rotary.cu", "kv_shared.cu"]
 CALLS = os.path.join(PKG, "lib", "bfvgpu_kv_calls.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

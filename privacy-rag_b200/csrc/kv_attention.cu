@@ -6,6 +6,7 @@
 #include <optional>
 
 #include "kv_host.h"
+#include "kv_shared.h"
 
 namespace bfvgpu {
 namespace kv {
@@ -141,6 +142,48 @@ uint64_t scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q
   return words;
 }
 
+// ---- groups that share their first tokens ----
+SharedQuery shared_query(const Query& q, const int32_t* groups, const int32_t* shared, uint64_t count) {
+  SharedQuery sq;
+  static_cast<Query&>(sq) = q;
+  sq.groups = groups;
+  sq.shared = shared;
+  sq.count = (int32_t)count;
+  return sq;
+}
+
+void check_groups(const Call& c, uint64_t count) { need(count <= (uint64_t)c.batch.seqs, BFVGPU_E_SHAPE, "E_KV_GROUPS"); }
+
+void attend_shared(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, const int32_t* starts, const int32_t* table,
+                   const int32_t* lengths, const int32_t* groups, const int32_t* shared, uint64_t count, float scale,
+                   uint64_t* scratch, void* out, void* stream) {
+  const float scale_log2 = scale * 1.4426950408889634f;
+  need(std::isfinite(scale_log2) && scale > 0, BFVGPU_E_ARGUMENT, "E_KV_SCALE");
+  check_groups(c, count);
+  const Place at = checked_place(ctx, stream);
+  if (!c.query.tokens) return;
+  need(c.batch.seqs && q && table && c.batch.width && lengths && out && count && groups && shared, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
+  need(aligned16(q) && aligned16(out) && c.query.token_stride % 8 == 0 && c.query.head_stride % 8 == 0, BFVGPU_E_ARGUMENT,
+       "E_KV_ALIGNMENT");
+  OnDevice scope(at.device);
+  c.batch.table = table;
+  c.batch.lengths = lengths;
+  c.batch.starts = starts;
+  c.batch.err = at.err;
+  c.query.q = static_cast<const uint16_t*>(q);
+  c.query.out = static_cast<uint16_t*>(out);
+  c.query.scale_log2 = scale_log2;
+  const SharedQuery sq = shared_query(c.query, groups, shared, count);
+  const SharedPlan sp = plan_shared(c.view, c.batch, sq, sm_count(at.device));
+  need(scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
+  need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
+  need(sp.slots <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+  int launches = 0;
+  cuda_need(launch_shared(c.view, c.batch, sq, cache->dtype, sp, reinterpret_cast<float*>(scratch), at.stream, &launches),
+            "kv shared attention");
+  internal_count_launch(launches);
+}
+
 }  // namespace
 }  // namespace kv
 }  // namespace bfvgpu
@@ -191,4 +234,41 @@ extern "C" int32_t bfvgpu_kv_prompt_kernel(const bfvgpu_kv* cache, int64_t token
     kernel = takes_rows(c.view, c.batch, c.query, true) ? BFVGPU_KV_ROWS : BFVGPU_KV_TILES;
   });
   return kernel;
+}
+
+extern "C" uint64_t bfvgpu_kv_shared_scratch_words(const bfvgpu_ctx* ctx, const bfvgpu_kv* cache, uint64_t q_heads, uint64_t tokens,
+                                                   uint64_t seqs, uint64_t width, uint64_t groups) {
+  uint64_t words = 0;
+  guarded([&] {
+    Call c = checked_call(cache, 0, 0, 0, q_heads, tokens, seqs, width, 0, 0);
+    check_groups(c, groups);
+    int device = -1;
+    internal_params(ctx, &device, nullptr);
+    words = (plan_shared(c.view, c.batch, shared_query(c.query, nullptr, nullptr, groups), sm_count(device)).scratch_floats() + 1) / 2;
+  });
+  return words;
+}
+
+extern "C" int32_t bfvgpu_kv_decode_shared_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, int32_t layer, const void* q,
+                                                  int64_t token_stride, int64_t head_stride, uint64_t q_heads,
+                                                  const int32_t* table, uint64_t width, const int32_t* lengths, uint64_t seqs,
+                                                  const int32_t* groups, const int32_t* shared, uint64_t count, float scale,
+                                                  uint64_t* scratch, void* out, void* stream) {
+  return guarded([&] {
+    Call c = checked_call(cache, layer, token_stride, head_stride, q_heads, seqs, seqs, width, 0, 0);
+    attend_shared(ctx, cache, c, q, nullptr, table, lengths, groups, shared, count, scale, scratch, out, stream);
+  });
+}
+
+extern "C" int32_t bfvgpu_kv_prompt_shared_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, int32_t layer, const void* q,
+                                                  int64_t token_stride, int64_t head_stride, uint64_t q_heads, uint64_t tokens,
+                                                  const int32_t* starts, const int32_t* table, uint64_t width,
+                                                  const int32_t* lengths, uint64_t seqs, const int32_t* groups,
+                                                  const int32_t* shared, uint64_t count, float scale, uint64_t* scratch,
+                                                  void* out, void* stream) {
+  return guarded([&] {
+    need(starts || !tokens, BFVGPU_E_ARGUMENT, "E_KV_ARGUMENT");
+    Call c = checked_call(cache, layer, token_stride, head_stride, q_heads, tokens, seqs, width, 0, 0);
+    attend_shared(ctx, cache, c, q, starts, table, lengths, groups, shared, count, scale, scratch, out, stream);
+  });
 }

@@ -415,6 +415,64 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) { return wants(n, 
 // prompt(cache, ctx, q, starts, table, ...) -> out | status
 PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t n) { return wants(n, 12) ? attend(a, a[3], a + 4) : nullptr; }
 
+// The attention of q over tokens that groups of sequences share: of single tokens where starts is null.
+PyObject* attend_shared(PyObject* const* a, PyObject* of_starts, PyObject* const* rest) {
+  // a: cache, ctx, q; rest: table, lengths, groups, shared, layer, scale | None, out | None, stream | None
+  return answered([&]() -> PyObject* {
+    const Cache& c = cache_of(a[0]);
+    bfvgpu_ctx* ctx = context_of(a[1]);
+    const at::Tensor& q = rows_of(a[2], "q", c);
+    const uint64_t tokens = (uint64_t)q.size(0), heads = (uint64_t)q.size(1);
+    const Table t = table_of(rest[0], c);
+    if (!of_starts && tokens != t.rows) refuse("E_KV_SHAPE: one query per row of the table");
+    const int32_t* starts = of_starts ? ints_of(of_starts, "starts", t.rows + 1, c) : nullptr;
+    const int32_t* lengths = ints_of(rest[1], "lengths", t.rows, c);
+    const uint64_t count = count_of(rest[3], "shared");
+    const int32_t *groups = ints_of(rest[2], "groups", count + 1, c), *shared = ints_of(rest[3], "shared", count, c);
+    const int32_t layer = int_of(rest[4]);
+    double scale = c.scale;
+    if (rest[5] != Py_None) {
+      scale = PyFloat_AsDouble(rest[5]);
+      if (scale == -1.0 && PyErr_Occurred()) throw python_error();
+    }
+    if (q.scalar_type() != c.type()) refuse("E_KV_DTYPE: q has the cache's type");
+    const Stream s(rest[7], c);
+    at::Tensor made;
+    if (rest[6] == Py_None) {
+      made = at::empty(q.sizes(), q.options());
+    } else {
+      const at::Tensor& given = tensor_of(rest[6], "out");
+      if (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !there(given, c) || !given.is_contiguous())
+        refuse("E_KV_SHAPE: out is dense, of q's shape and type");
+    }
+    s.uses(c, {a[2], of_starts, rest[0], rest[1], rest[2], rest[3], rest[6]});
+    const at::Tensor& out = made.defined() ? made : THPVariable_Unpack(rest[6]);
+    const uint64_t words = bfvgpu_kv_shared_scratch_words(ctx, &c.kv, heads, tokens, t.rows, t.width, count);
+    at::Tensor scratch;
+    if (words) scratch = at::empty({(int64_t)words}, q.options().dtype(at::kLong));
+    auto* space = words ? static_cast<uint64_t*>(scratch.data_ptr()) : nullptr;
+    const int32_t rc =
+        of_starts ? bfvgpu_kv_prompt_shared_device(ctx, &c.kv, layer, q.data_ptr(), q.stride(0), q.stride(1), heads, tokens, starts,
+                                                   t.at, t.width, lengths, t.rows, groups, shared, count, (float)scale, space,
+                                                   out.data_ptr(), s.handle)
+                  : bfvgpu_kv_decode_shared_device(ctx, &c.kv, layer, q.data_ptr(), q.stride(0), q.stride(1), heads, t.at, t.width,
+                                                   lengths, t.rows, groups, shared, count, (float)scale, space, out.data_ptr(),
+                                                   s.handle);
+    if (rc) return PyLong_FromLong(rc);
+    if (made.defined()) return THPVariable_Wrap(made);
+    Py_INCREF(rest[6]);
+    return rest[6];
+  });
+}
+// decode_shared(cache, ctx, q, table, lengths, groups, shared, layer, scale | None, out | None, stream | None) -> out | status
+PyObject* decode_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return wants(n, 11) ? attend_shared(a, nullptr, a + 3) : nullptr;
+}
+// prompt_shared(cache, ctx, q, starts, table, ...) -> out | status
+PyObject* prompt_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return wants(n, 12) ? attend_shared(a, a[3], a + 4) : nullptr;
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyMethodDef method(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(F)), METH_FASTCALL, nullptr};
@@ -425,7 +483,8 @@ PyMethodDef method(const char* name) {
 PyMODINIT_FUNC PyInit_bfvgpu_kv_calls() {
   static PyMethodDef methods[] = {method<open_cache>("open"), method<append>("append"), method<fork>("fork"), method<move>("move"),
                                   method<decode>("decode"),   method<prompt>("prompt"), method<append_rotary>("append_rotary"),
-                                  method<rotate>("rotate"),   {nullptr, nullptr, 0, nullptr}};
+                                  method<rotate>("rotate"),   method<decode_shared>("decode_shared"),
+                                  method<prompt_shared>("prompt_shared"), {nullptr, nullptr, 0, nullptr}};
   static PyModuleDef module = {PyModuleDef_HEAD_INIT, "bfvgpu_kv_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
   return PyModule_Create(&module);
 }

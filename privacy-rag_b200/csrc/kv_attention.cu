@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 #include <optional>
 
 #include "kv_host.h"
@@ -174,10 +175,10 @@ void attend_shared(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void*
   c.query.out = static_cast<uint16_t*>(out);
   c.query.scale_log2 = scale_log2;
   const SharedQuery sq = shared_query(c.query, groups, shared, count);
-  const SharedPlan sp = plan_shared(c.view, c.batch, sq, sm_count(at.device));
+  const SharedPlan sp = plan_shared(c.view, c.batch, sq, sm_count(at.device), prompt_strides(sq));
   need(scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
   need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
-  need(sp.slots <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+  need(std::max(sp.slots[0], sp.slots[1]) <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
   int launches = 0;
   cuda_need(launch_shared(c.view, c.batch, sq, cache->dtype, sp, reinterpret_cast<float*>(scratch), at.stream, &launches),
             "kv shared attention");
@@ -244,9 +245,25 @@ extern "C" uint64_t bfvgpu_kv_shared_scratch_words(const bfvgpu_ctx* ctx, const 
     check_groups(c, groups);
     int device = -1;
     internal_params(ctx, &device, nullptr);
-    words = (plan_shared(c.view, c.batch, shared_query(c.query, nullptr, nullptr, groups), sm_count(device)).scratch_floats() + 1) / 2;
+    const SharedQuery q = shared_query(c.query, nullptr, nullptr, groups);
+    // the strides of the queries, which are not known here, may rule out the tensor-core kernel
+    for (const bool tiles : {false, true})
+      words = std::max(words, (plan_shared(c.view, c.batch, q, sm_count(device), tiles).scratch_floats() + 1) / 2);
   });
   return words;
+}
+
+extern "C" int32_t bfvgpu_kv_shared_kernel(const bfvgpu_kv* cache, int64_t token_stride, int64_t head_stride, uint64_t q_heads,
+                                           uint64_t tokens, uint64_t seqs, uint64_t width, uint64_t groups, int32_t own) {
+  int32_t kernel = -1;
+  guarded([&] {
+    const Call c = checked_call(cache, 0, token_stride, head_stride, q_heads, tokens, seqs, width, 0, 0);
+    check_groups(c, groups);
+    const SharedQuery q = shared_query(c.query, nullptr, nullptr, groups);
+    const SharedPlan p = plan_shared(c.view, c.batch, q, sm_count(-1), prompt_strides(q));
+    kernel = p.tiles[own != 0] ? BFVGPU_KV_TILES : BFVGPU_KV_ROWS;
+  });
+  return kernel;
 }
 
 extern "C" int32_t bfvgpu_kv_decode_shared_device(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, int32_t layer, const void* q,

@@ -43,6 +43,7 @@
 #include <type_traits>
 
 #include "kv_attention.h"
+#include "kv_shared.h"
 #include "kv_units.cuh"
 
 namespace bfvgpu {
@@ -296,21 +297,30 @@ __device__ __forceinline__ Plan make_plan(const Unit& un) {
   }
   return p;
 }
-__device__ __forceinline__ Span make_span(const Item& it, const Query& q, int t) {
+// The position of row r of a unit's.
+__device__ __forceinline__ int32_t stands_at(const Unit& un, const Query& q, int32_t r) { return un.position(q, r); }
+__device__ __forceinline__ int32_t stands_at(const Unit& un, const SharedQuery& q, int32_t r) {
+  return un.flat ? un.pos0 : un.position(q, r);
+}
+template <class Q>
+constexpr bool kSharing = std::is_same_v<Q, SharedQuery>;
+
+template <class Q>
+__device__ __forceinline__ Span make_span(const Item& it, const Q& q, int t) {
   const Unit& un = it.un;
   const Plan& p = it.plan;
   Span s;
   s.from = it.begin;
   s.to = it.end;
   if (t * kTileRows >= un.rows) return s;
-  s.lo = un.position(q, t * kTileRows);
-  s.hi = un.position(q, min(un.rows, (t + 1) * kTileRows) - 1);
-  if (s.hi < 0) return s;
+  s.lo = stands_at(un, q, t * kTileRows);
+  s.hi = stands_at(un, q, min(un.rows, (t + 1) * kTileRows) - 1);
+  if (s.hi < (kSharing<Q> ? un.begin : 0)) return s;
   s.first = p.first;
   s.end = min(it.end, p.first + s.hi / kTileKeys - p.from + 1);
   s.begin = p.first;
   // the window tiles before the row tile's own, unless first tokens reach into them
-  if (un.begin > 0 && un.sinks <= p.from * kTileKeys) s.begin += max(0, (s.lo + 1 - q.window) / kTileKeys - p.from);
+  if (!kSharing<Q> && un.begin > 0 && un.sinks <= p.from * kTileKeys) s.begin += max(0, (s.lo + 1 - q.window) / kTileKeys - p.from);
   return s;
 }
 // Parts of a unit of n key tiles where the launch has `most`.
@@ -332,10 +342,12 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* w, bool whole,
   }
 }
 
-template <class T, int DP>
+// Q: SharedQuery for tokens that groups of sequences share: shared and own keys are units of their own, whose key tiles are
+// cut into one equal run for each block (Runs; there is no launch control then), and all results are partial ones.
+template <class T, int DP, class Q = Query>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_kv_prompt(const __grid_constant__ Maps maps, View kv, Batch bt, Query q, int64_t units, int32_t most_parts,
-                float* scratch, uint32_t q_tokens, bool ranked) {
+    k_kv_prompt(const __grid_constant__ Maps maps, View kv, Batch bt, Q q, int64_t units, int32_t most_parts,
+                float* scratch, uint32_t q_tokens, bool ranked, Slots slots) {
   using S = Smem<DP>;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
@@ -427,21 +439,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     };
+    Runs<kBlockRows, kTileKeys> runs;
+    if constexpr (kSharing<Q>) {
+      if (block == 0) record_uncovered(bt, q);
+      runs.start(kv, bt, q, slots, (int32_t)block, kPartTiles / 2);
+    }
     while (ok && block >= 0) {
-      // the blocks with the most keys come first
-      const uint32_t from_end = (uint32_t)block / (uint32_t)most_parts, u = (uint32_t)units - 1 - from_end;
-      const int32_t part = (int32_t)((uint32_t)block - from_end * most_parts);
       Item it;
-      it.un = ranked ? find_unit_ranked<kBlockRows>(kv, bt, q, from_end) : find_unit<kBlockRows>(kv, bt, q, u);
       const Unit& un = it.un;
       const Plan& plan = it.plan;
-      it.plan = make_plan(un);
-      it.parts = parts_of(plan.n, most_parts);
-      it.begin = plan.n * part / it.parts;  // n < 2^23
-      it.end = plan.n * (part + 1) / it.parts;
+      int32_t part = 0;
+      if constexpr (kSharing<Q>) {
+        Piece piece;
+        if (!runs.next(kv, bt, q, slots, &piece)) break;
+        it.un = piece.un;
+        it.plan = make_plan(un);
+        it.begin = piece.from;
+        it.end = piece.to;
+        it.slot = piece.slot;
+        if (it.begin >= it.end) {  // a part of less than a tile: nothing is seen
+          for (int32_t r = lane; r < un.rows; r += 32)
+            *reinterpret_cast<float2*>(slots.floats + it.slot * kSlotFloats<DP> + kBlockRows * DP + r * 2) = make_float2(-INFINITY, 0.f);
+          continue;
+        }
+      } else {
+        // the blocks with the most keys come first
+        const uint32_t from_end = (uint32_t)block / (uint32_t)most_parts, u = (uint32_t)units - 1 - from_end;
+        part = (int32_t)((uint32_t)block - from_end * most_parts);
+        it.un = ranked ? find_unit_ranked<kBlockRows>(kv, bt, q, from_end) : find_unit<kBlockRows>(kv, bt, q, u);
+        it.plan = make_plan(un);
+        it.parts = parts_of(plan.n, most_parts);
+        it.begin = plan.n * part / it.parts;  // n < 2^23
+        it.end = plan.n * (part + 1) / it.parts;
+        it.slot = (int32_t)(u * most_parts + part);
+      }
       it.span[0] = make_span(it, q, 0);
       it.span[1] = make_span(it, q, 1);
-      it.slot = (int32_t)(u * most_parts + part);
       it.more = 1;
       if (un.rows > 0 && part < it.parts) {
         tell(it);
@@ -479,7 +512,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int h = 0; h < S::kHalves; ++h)
               tma_box(kb + h * S::kHalfBytes + lane * box * 128, &maps.k, h * 64, at, un.g, page, k_full + 8 * st);
           k_issued = turn + 1;
-          if (i + 1 == it.end) ask();
+          if constexpr (!kSharing<Q>)
+            if (i + 1 == it.end) ask();
           ok = __all_sync(0xffffffffu, bar_wait(v_empty + 8 * st, parity, abort, bt.err));
           if (!ok) break;
           if (lane == 0) bar_expect(v_full + 8 * st, S::kTileBytes);
@@ -513,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!ok) break;
+      if constexpr (kSharing<Q>) continue;
       ask();
       ok = __all_sync(0xffffffffu, bar_wait(answered, answers & 1, abort, bt.err));
       if (!ok) break;
@@ -712,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Span span = it.span[t];
       // positions of the thread's rows, and of the warp's first and last (rows past the last do its work again)
       int32_t pos[2];
-      for (int r = 0; r < 2; ++r) pos[r] = un.position(q, min(t * kTileRows + row0 + 8 * r, un.rows - 1));
+      for (int r = 0; r < 2; ++r) pos[r] = stands_at(un, q, min(t * kTileRows + row0 + 8 * r, un.rows - 1));
       const int32_t lo = __shfl_sync(0xffffffffu, pos[0], 0), hi = __shfl_sync(0xffffffffu, pos[1], 31);
       const int32_t alive = un.rows - t * kTileRows;  // rows of the tile
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
@@ -730,15 +765,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         bar_arrive(s_read + 8 * t);
         // which of the four 32 keys any row of the warp sees; not all rows may see them all
         uint32_t live = 0xf;
-        if (key0 + kTileKeys - 1 > lo || (q.window && key0 <= hi - q.window && key0 + kTileKeys > q.sinks)) {
+        const int32_t from_key = kSharing<Q> ? un.begin : 0;  // own keys begin behind the shared ones
+        if (key0 + kTileKeys - 1 > lo || (q.window && key0 <= hi - q.window && key0 + kTileKeys > q.sinks) || key0 < from_key) {
           live = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int32_t k = key0 + 32 * j;
-            if (k <= hi && (!q.window || k + 31 > lo - q.window || k < q.sinks)) live |= 1u << j;
+            if (k <= hi && k + 31 >= from_key && (!q.window || k + 31 > lo - q.window || k < q.sinks)) live |= 1u << j;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const int32_t last = pos[r] - k, first = q.window ? last - q.window + 1 : 0, sk = min(q.sinks - 1 - k, last);
+              const int32_t last = pos[r] - k, first = kSharing<Q> ? from_key - k : q.window ? last - q.window + 1 : 0, sk = min(q.sinks - 1 - k, last);
               const uint32_t in = (bits_of(first, last, 0) | bits_of(0, sk, 0)) >> pair;
 #pragma unroll
               for (int e = 0; e < 8; ++e)
@@ -849,10 +885,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int32_t row = (warp & 3) * 32 + lane, at_row = t * kTileRows + row;
       const bool mine_live = at_row < un.rows;
       const float sum = ml[row].y;
-      float* slot = scratch + it.slot * kSlotFloats<DP>;
-      if (it.parts > 1 && half == 0 && mine_live) *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = ml[row];
+      const bool partial = kSharing<Q> || it.parts > 1;
+      float* slot = (kSharing<Q> ? slots.floats : scratch) + it.slot * kSlotFloats<DP>;
+      if (partial && half == 0 && mine_live) *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = ml[row];
       if (fresh) {  // no row of the tile sees a key of the item
-        if (it.parts == 1 && half == 0 && mine_live)
+        if (!partial && half == 0 && mine_live)
           for (int32_t d = 0; d < kv.dim; d += 8) *reinterpret_cast<uint4*>(un.result(kv, q, at_row) + d) = make_uint4(0, 0, 0, 0);
         continue;
       }
@@ -875,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           bar_arrive(o_empty + 8 * t);
         }
         if (!mine_live) continue;
-        if (it.parts == 1) {
+        if (!partial) {
           uint32_t w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = sum == 0.f ? 0 : T::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
@@ -989,30 +1026,39 @@ bool encode(CUtensorMap* map, const View& kv, int dtype, uint16_t* pages, uint32
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int DP>
-cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& sp, float* scratch,
-                   cudaStream_t st, int* launches) {
+// The kernel's shared memory, which is an attribute of the function on a device, and the maps of its loads.
+template <class T, int DP, class Q>
+cudaError_t prepare(const View& kv, const Q& q, int dtype, Maps* maps, uint32_t* q_tokens) {
   static std::atomic<uint64_t> allowed{0};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
   if (device >= 64 || !(allowed.load() >> device & 1)) {
-    e = cudaFuncSetAttribute(k_kv_prompt<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<DP>::kLaunch);
+    e = cudaFuncSetAttribute(k_kv_prompt<T, DP, Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<DP>::kLaunch);
     if (e != cudaSuccess) return e;
     if (device < 64) allowed.fetch_or(uint64_t(1) << device);
   }
-  Maps maps;
   const uint32_t box = (uint32_t)std::min(1 << kv.page_log, kTileKeys);
   // whole tokens fill a row tile where the group divides it (units begin at multiples of 256 rows)
-  const uint32_t q_tokens = q.group <= kTileRows && kTileRows % q.group == 0 ? kTileRows / q.group : 0;
-  if (!encode_q(&maps.q, kv, q, dtype, q.group <= kTileRows ? q.group : 1, std::max(q_tokens, 1u)) ||
-      !encode_q(&maps.q_row, kv, q, dtype, 1, 1))
+  *q_tokens = q.group <= kTileRows && kTileRows % q.group == 0 ? kTileRows / q.group : 0;
+  if (!encode_q(&maps->q, kv, q, dtype, q.group <= kTileRows ? q.group : 1, std::max(*q_tokens, 1u)) ||
+      !encode_q(&maps->q_row, kv, q, dtype, 1, 1))
     return cudaErrorInvalidValue;
-  if (!encode(&maps.k, kv, dtype, kv.k, box) || !encode(&maps.v, kv, dtype, kv.v, box) ||
-      !encode(&maps.v_rows, kv, dtype, kv.v, 8) || !encode(&maps.v_row, kv, dtype, kv.v, 1))
+  if (!encode(&maps->k, kv, dtype, kv.k, box) || !encode(&maps->v, kv, dtype, kv.v, box) ||
+      !encode(&maps->v_rows, kv, dtype, kv.v, 8) || !encode(&maps->v_row, kv, dtype, kv.v, 1))
     return cudaErrorInvalidValue;
+  return cudaSuccess;
+}
+
+template <class T, int DP>
+cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& sp, float* scratch,
+                   cudaStream_t st, int* launches) {
+  Maps maps;
+  uint32_t q_tokens;
+  cudaError_t e = prepare<T, DP>(kv, q, dtype, &maps, &q_tokens);
+  if (e != cudaSuccess) return e;
   e = launch_next(k_kv_prompt<T, DP>, dim3((unsigned)(sp.units * sp.parts)), kThreads, Smem<DP>::kLaunch, st, 1, maps, kv, bt, q,
-                  sp.units, sp.parts, scratch, q_tokens, sp.ranked);
+                  sp.units, sp.parts, scratch, q_tokens, sp.ranked, Slots{});
   if (e != cudaSuccess) return e;
   *launches += 1;
   if (sp.parts > 1) {
@@ -1022,6 +1068,16 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, c
     *launches += 1;
   }
   return cudaGetLastError();
+}
+
+template <class T, int DP>
+cudaError_t launch_sharing(const View& kv, const Batch& bt, const SharedQuery& q, int dtype, const Slots& slots, cudaStream_t st) {
+  Maps maps;
+  uint32_t q_tokens;
+  const cudaError_t e = prepare<T, DP>(kv, q, dtype, &maps, &q_tokens);
+  if (e != cudaSuccess) return e;
+  return launch_next(k_kv_prompt<T, DP, SharedQuery>, dim3((unsigned)slots.workers), kThreads, Smem<DP>::kLaunch, st, 1, maps, kv, bt,
+                     q, int64_t(0), 1, static_cast<float*>(nullptr), q_tokens, false, slots);
 }
 
 }  // namespace
@@ -1064,6 +1120,14 @@ cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int d
                  : launch<Bf16, 128>(kv, bt, q, dtype, sp, scratch, st, launches);
   return small ? launch<Fp16, 64>(kv, bt, q, dtype, sp, scratch, st, launches)
                : launch<Fp16, 128>(kv, bt, q, dtype, sp, scratch, st, launches);
+}
+
+static_assert(kBlockRows == kSharedTileRows && kTileKeys == 128, "the units and key tiles of Runs");
+cudaError_t launch_shared_tiles(const View& kv, const Batch& bt, const SharedQuery& q, int dtype, const Slots& slots, cudaStream_t st) {
+  const bool small = kv.dim <= 64;
+  if (dtype == 0)
+    return small ? launch_sharing<Bf16, 64>(kv, bt, q, dtype, slots, st) : launch_sharing<Bf16, 128>(kv, bt, q, dtype, slots, st);
+  return small ? launch_sharing<Fp16, 64>(kv, bt, q, dtype, slots, st) : launch_sharing<Fp16, 128>(kv, bt, q, dtype, slots, st);
 }
 
 }  // namespace kv

@@ -7,8 +7,7 @@
 // a table may be wide, the shared part nearly all of it or nothing.  So the work is cut on the device.  The stages of 16
 // keys of all units (16 rows of a group, or of a sequence, and one key head) lie in a row; each warp takes an equal run
 // of them, finds its first unit by a scan over the groups and sequences, and leaves m, l and o of the units that it had a
-// part of in slots of its own; a second kernel joins them in order.  A unit's parts lie side by side: the slot of warp w
-// and unit u is w + u, which rises from part to part in the order of the row.
+// part of in slots of its own; a second kernel joins them in order.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -22,23 +21,17 @@ namespace kv {
 namespace {
 
 constexpr int kRunStages = 4;  // a warp has at least, where the row has them
+#ifndef TRS
+#define TRS 64
+#endif
+#ifndef TRO
+#define TRO 64
+#endif
+constexpr int kTileRowsShared = TRS, kTileRowsOwn = TRO;
 
-struct Slots {
-  int2* index[2] = {};          // of the units over shared and over own keys: first slot, slots
-  float* slots = nullptr;
-  int32_t most = 0;             // slots
-  int32_t warps = 0;
-  bool has[2] = {true, true};   // which keys
-};
 template <int DP>
 constexpr int64_t kSlotFloats = kRows * (DP + 2);
-
-struct Row {
-  int64_t total = 0;      // stages
-  int32_t runs = 0;       // warps that have some
-  __device__ __forceinline__ int64_t begin_of(int32_t w) const { return total * w / runs; }
-  __device__ __forceinline__ int32_t warp_of(int64_t stage) const { return (int32_t)(((stage + 1) * runs - 1) / total); }
-};
+static_assert(kRows == kSharedRows);
 
 template <class T, int DP, int NK>
 __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, SharedQuery q, Slots sl) {
@@ -48,28 +41,9 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, 
   const int32_t me = blockIdx.x * kWarps + warp;
   cudaGridDependencySynchronize();
   if (me == 0) record_uncovered(bt, q);
-  // 32 elements of a list (0 shared keys, 1 own keys), a lane each: what they are, their units and stages a unit
-  Element el;
-  int32_t units = 0, stages = 0;
-  auto load = [&](int list, int32_t e0) {
-    int32_t group;
-    el = list == 0 ? shared_element(kv, bt, q, e0 + lane) : own_element(kv, bt, q, e0 + lane, &group);
-    stages = (max(0, el.end - el.begin) + kKeys - 1) / kKeys;
-    units = stages ? (int32_t)(((uint32_t)el.tokens * q.group + kRows - 1) / kRows) * kv.heads : 0;
-  };
-  const int32_t length[2] = {sl.has[0] ? q.count : 0, sl.has[1] ? bt.seqs : 0};
-  Row row;
-  for (int list = 0; list < 2; ++list)
-    for (int32_t e0 = 0; e0 < length[list]; e0 += 32) {
-      load(list, e0);
-      row.total += (int64_t)units * stages;
-    }
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) row.total += __shfl_xor_sync(0xffffffffu, row.total, d);
-  row.runs = (int32_t)max((int64_t)1, min((int64_t)sl.warps, row.total / kRunStages));
-  if (me >= row.runs) return;
-  int64_t x = row.begin_of(me);
-  const int64_t x1 = row.begin_of(me + 1);
+  Runs<kRows, kKeys> runs;
+  runs.start(kv, bt, q, sl, me, kRunStages);
+  if (me >= runs.runs) return;
 
   const uint32_t base = smem_addr(ring) + warp * R::kWarpBytes;
   if (kv.dim != NK * 16) {  // the chunks past the head's dims are never copied
@@ -79,60 +53,10 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, 
   }
   const int32_t quad = lane >> 2, pair = (lane & 3) * 2, page_mask = (1 << kv.page_log) - 1;
 
-  int list = 0;
-  int32_t e0 = -32, units_before = 0, units_upto = 0;  // of the 32 elements; up to a lane's
-  int64_t before = 0, upto = 0;                        // stages
-  bool loaded = false;
-  while (x < x1) {
-    const uint32_t hit = loaded ? __ballot_sync(0xffffffffu, x < upto) : 0;
-    if (!hit) {  // the next 32 elements
-      before = loaded ? __shfl_sync(0xffffffffu, upto, 31) : 0;
-      units_before = loaded ? __shfl_sync(0xffffffffu, units_upto, 31) : 0;
-      e0 += 32;
-      while (list < 2 && e0 >= length[list]) ++list, e0 = 0;
-      if (list == 2) return;
-      load(list, e0);
-      loaded = true;
-      upto = (int64_t)units * stages;
-      units_upto = units;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t a = __shfl_up_sync(0xffffffffu, upto, d);
-        const int32_t b = __shfl_up_sync(0xffffffffu, units_upto, d);
-        if (lane >= d) upto += a, units_upto += b;
-      }
-      upto += before;
-      units_upto += units_before;
-      continue;
-    }
-    const int from = __ffs(hit) - 1;
-    Element e;
-    e.row = __shfl_sync(0xffffffffu, el.row, from);
-    e.first = __shfl_sync(0xffffffffu, el.first, from);
-    e.tokens = __shfl_sync(0xffffffffu, el.tokens, from);
-    e.begin = __shfl_sync(0xffffffffu, el.begin, from);
-    e.end = __shfl_sync(0xffffffffu, el.end, from);
-    const int32_t per = __shfl_sync(0xffffffffu, stages, from);
-    const int64_t first_stage = __shfl_sync(0xffffffffu, upto - (int64_t)units * stages, from);
-    const int32_t first_unit = __shfl_sync(0xffffffffu, units_upto - units, from);
-    const int32_t in = (int32_t)((uint64_t)(x - first_stage) / (uint32_t)per);
-    const int64_t unit_stage = first_stage + (int64_t)in * per;
-    const int32_t s0 = (int32_t)(x - unit_stage), s1 = (int32_t)min((int64_t)per, s0 + (x1 - x));
-    const int32_t block = in / kv.heads, g = in - block * kv.heads;
-    const bool flat = list == 0;
-    Unit un = element_unit<kRows>(q, e, block, g, flat);
-    un.n = e.end - e.begin;  // (whichever of its rows see them)
-    const int32_t slot = me + first_unit + in;
-    if (slot >= sl.most) {  // sequences that overlap have more units than there are
-      if (lane == 0) flag_error(bt.err, kErrTable);
-      return;
-    }
-    if (s0 == 0 && lane == 0) {
-      const int32_t last = row.warp_of(unit_stage + per - 1);
-      sl.index[list][place_of<kRows>(kv, q, e, e0 + from, block, g)] = make_int2(slot, last - me + 1);
-    }
-    x += s1 - s0;
-
+  for (Piece p; runs.next(kv, bt, q, sl, &p);) {
+    const Unit& un = p.un;
+    const int32_t s0 = p.from, s1 = p.to;
+    const bool flat = p.list == 0;
     uint32_t qa[NK][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -206,7 +130,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, 
     }
     copies_wait<0>();
     __syncwarp();
-    float* to = sl.slots + (int64_t)slot * kSlotFloats<DP>;
+    float* to = sl.floats + (int64_t)p.slot * kSlotFloats<DP>;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -221,9 +145,15 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, 
   }
 }
 
+// Where the two lists' partial results are.
+struct Sources {
+  Slots slots[2];
+  bool tiles[2];
+};
+
 // A warp a row (query head of a token): its parts over shared keys, then those over its own, in order.
 template <class T, int DP>
-__global__ void __launch_bounds__(kThreads) k_kv_shared_join(View kv, Batch bt, SharedQuery q, Slots sl) {
+__global__ void __launch_bounds__(kThreads) k_kv_shared_join(View kv, Batch bt, SharedQuery q, Sources src) {
   cudaGridDependencySynchronize();
   constexpr int kPer = DP / 32;  // dims a lane
   const int lane = threadIdx.x & 31, d = lane * kPer;
@@ -232,40 +162,43 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_join(View kv, Batch bt, 
   if (row >= rows) return;
   const int32_t t = (int32_t)(row / heads), head = (int32_t)(row - (int64_t)t * heads), g = head / q.group, in_group = head - g * q.group;
   const int32_t s = bt.starts ? sequence_of_token(bt, t) : t;
-  Element e[2];
-  int32_t number[2];
-  number[1] = s;
-  e[1] = own_element(kv, bt, q, s, &number[0]);
-  if (t < e[1].first || t >= e[1].first + e[1].tokens) {  // of no sequence
+  int32_t group;
+  const Element own = own_element(kv, bt, q, s, &group);
+  if (t < own.first || t >= own.first + own.tokens) {  // of no sequence
     if (lane == 0) flag_error(bt.err, kErrTable);
     return;
   }
-  if (number[0] >= 0) e[0] = shared_element(kv, bt, q, number[0]);
   float top = -INFINITY, sum = 0, v[kPer] = {};
 #pragma unroll
   for (int list = 0; list < 2; ++list) {
-    const Element& el = e[list];
+    if (list == 0 && group < 0) continue;
+    const Element el = list == 0 ? shared_element(kv, bt, q, group) : own;
     if (el.end <= el.begin || t < el.first || t >= el.first + el.tokens) continue;
-    const int32_t r = (t - el.first) * q.group + in_group, block = r / kRows, in = r - block * kRows;
-    const int2 parts = sl.index[list][place_of<kRows>(kv, q, el, number[list], block, g)];
+    const Slots& sl = src.slots[list];
+    const int32_t r = (t - el.first) * q.group + in_group, of = list == 0 ? group : s;
+    const int32_t unit_rows = src.tiles[list] ? kSharedTileRows : kSharedRows, block = r / unit_rows, in = r - block * unit_rows;
+    const int64_t place = src.tiles[list] ? place_of<kSharedTileRows>(kv, q, el, of, block, g) : place_of<kSharedRows>(kv, q, el, of, block, g);
+    const int2 parts = sl.index[list][place];
     if (parts.x < 0 || parts.y < 0 || parts.y > sl.most - parts.x) {  // sequences that overlap
       if (lane == 0) flag_error(bt.err, kErrTable);
       continue;
     }
-    const float* from = sl.slots + (int64_t)parts.x * kSlotFloats<DP>;
+    const int64_t slot_floats = (int64_t)unit_rows * (DP + 2);
+    const float* from = sl.floats + parts.x * slot_floats + in * DP;
+    const int64_t to_ml = (int64_t)unit_rows * DP + in * 2 - in * DP;
     constexpr int kTogether = 8;  // parts whose numbers are asked for together
     for (int32_t c0 = 0; c0 < parts.y; c0 += kTogether) {
       float2 mlc[kTogether];
       float vc[kTogether][kPer];
 #pragma unroll
       for (int c = 0; c < kTogether; ++c) {
-        const float* other = from + (c0 + c) * kSlotFloats<DP>;
+        const float* other = from + (c0 + c) * slot_floats;
         mlc[c] = make_float2(-INFINITY, 0.f);
-        if (c0 + c < parts.y) mlc[c] = *reinterpret_cast<const float2*>(other + kRows * DP + in * 2);
+        if (c0 + c < parts.y) mlc[c] = *reinterpret_cast<const float2*>(other + to_ml);
 #pragma unroll
         for (int i = 0; i < kPer; i += 2) {
           float2 y = make_float2(0.f, 0.f);
-          if (c0 + c < parts.y) y = *reinterpret_cast<const float2*>(other + in * DP + d + i);
+          if (c0 + c < parts.y) y = *reinterpret_cast<const float2*>(other + d + i);
           vc[c][i] = y.x;
           vc[c][i + 1] = y.y;
         }
@@ -279,10 +212,11 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_join(View kv, Batch bt, 
       for (int i = 0; i < kPer; ++i) v[i] *= fo;
 #pragma unroll
       for (int c = 0; c < kTogether; ++c) {
-        const float f = exp2_fast(mlc[c].x - ref);
+        const bool some = mlc[c].x != -INFINITY || mlc[c].y != 0.f;  // else nothing was seen, and values may not be there
+        const float f = some ? exp2_fast(mlc[c].x - ref) : 0.f;
         sum += f * mlc[c].y;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) v[i] += f * vc[c][i];
+        for (int i = 0; i < kPer; ++i) v[i] += some ? f * vc[c][i] : 0.f;
       }
       top = now;
     }
@@ -295,7 +229,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_join(View kv, Batch bt, 
 }
 
 template <class T, int DP, int NK>
-cudaError_t launch(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, cudaStream_t st, int* launches) {
+cudaError_t launch_rows_of(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, cudaStream_t st) {
   static std::atomic<uint64_t> allowed{0};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -305,50 +239,84 @@ cudaError_t launch(const View& kv, const Batch& bt, const SharedQuery& q, const 
     if (e != cudaSuccess) return e;
     if (device < 64) allowed.fetch_or(uint64_t(1) << device);
   }
-  e = launch_next(k_kv_shared_rows<T, DP, NK>, dim3((unsigned)(sl.warps / kWarps)), kThreads, Ring<DP>::kBytes, st, 1, kv, bt, q, sl);
-  if (e != cudaSuccess) return e;
-  *launches += 1;
-  const int64_t rows = (int64_t)q.tokens * kv.heads * q.group;
-  e = launch_next(k_kv_shared_join<T, DP>, dim3((unsigned)((rows + kWarps - 1) / kWarps)), kThreads, 0, st, 1, kv, bt, q, sl);
-  if (e != cudaSuccess) return e;
-  *launches += 1;
-  return cudaGetLastError();
+  return launch_next(k_kv_shared_rows<T, DP, NK>, dim3((unsigned)(sl.workers / kWarps)), kThreads, Ring<DP>::kBytes, st, 1, kv, bt, q, sl);
 }
 
 template <class T>
-cudaError_t launch_typed(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, cudaStream_t st, int* launches) {
-  if (kv.dim <= 64) return launch<T, 64, 4>(kv, bt, q, sl, st, launches);
-  if (kv.dim <= 96) return launch<T, 128, 6>(kv, bt, q, sl, st, launches);
-  return launch<T, 128, 8>(kv, bt, q, sl, st, launches);
+cudaError_t launch_rows_typed(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, cudaStream_t st) {
+  if (kv.dim <= 64) return launch_rows_of<T, 64, 4>(kv, bt, q, sl, st);
+  if (kv.dim <= 96) return launch_rows_of<T, 128, 6>(kv, bt, q, sl, st);
+  return launch_rows_of<T, 128, 8>(kv, bt, q, sl, st);
+}
+
+template <class T>
+cudaError_t launch_join(const View& kv, const Batch& bt, const SharedQuery& q, const Sources& src, cudaStream_t st) {
+  const int64_t rows = (int64_t)q.tokens * kv.heads * q.group;
+  return launch_next(kv.dim <= 64 ? k_kv_shared_join<T, 64> : k_kv_shared_join<T, 128>, dim3((unsigned)((rows + kWarps - 1) / kWarps)),
+                     kThreads, 0, st, 1, kv, bt, q, src);
 }
 
 }  // namespace
 
-SharedPlan plan_shared(const View& kv, const Batch& bt, const SharedQuery& q, int sms) {
+SharedPlan plan_shared(const View& kv, const Batch& bt, const SharedQuery& q, int sms, bool tiles) {
   SharedPlan p;
   const bool narrow = kv.dim <= 64;
   p.dim_padded = narrow ? 64 : 128;
-  p.warps = sms * (narrow ? 4 : 2) * kWarps;
-  p.places[0] = places(kv, q, q.count, kRows);
-  p.places[1] = places(kv, q, bt.seqs, kRows);
-  p.slots = p.warps + p.places[0] + p.places[1];
+  const int64_t rows = (int64_t)q.tokens * q.group;
+  p.tiles[0] = tiles && rows >= (int64_t)kTileRowsShared * q.count;
+  p.tiles[1] = tiles && rows >= (int64_t)kTileRowsOwn * bt.seqs;
+  const int32_t elements[2] = {q.count, bt.seqs};
+  p.workers[0] = sms * (narrow ? 3 : 2) * kWarps;
+  p.workers[1] = sms;
+  for (int list = 0; list < 2; ++list) {
+    p.places[list] = places(kv, q, elements[list], p.tiles[list] ? kSharedTileRows : kSharedRows);
+    p.slots[p.tiles[list]] += p.places[list];
+  }
+  for (int kernel = 0; kernel < 2; ++kernel)
+    if (p.slots[kernel]) p.slots[kernel] += p.workers[kernel];
   return p;
 }
 
+// [first slots and parts of the units][slots of few rows][slots of tiles], each 32-byte aligned
 uint64_t SharedPlan::scratch_floats() const {
-  return (uint64_t)2 * (places[0] + places[1]) + 4 + (uint64_t)slots * kRows * (dim_padded + 2);
+  auto up = [](int64_t n) { return (n + 7) & ~int64_t(7); };
+  return up(2 * (places[0] + places[1])) + up(slots[0] * kSharedRows * (dim_padded + 2)) + slots[1] * kSharedTileRows * (dim_padded + 2);
 }
 
 cudaError_t launch_shared(const View& kv, const Batch& bt, const SharedQuery& q, int dtype, const SharedPlan& p, float* scratch,
                           cudaStream_t st, int* launches) {
-  Slots sl;
-  sl.index[0] = reinterpret_cast<int2*>(scratch);
-  sl.index[1] = sl.index[0] + p.places[0];
-  // (16-byte aligned)
-  sl.slots = scratch + ((2 * (p.places[0] + p.places[1]) + 3) & ~int64_t(3));
-  sl.most = (int32_t)p.slots;
-  sl.warps = p.warps;
-  return dtype == 0 ? launch_typed<Bf16>(kv, bt, q, sl, st, launches) : launch_typed<Fp16>(kv, bt, q, sl, st, launches);
+  auto up = [](int64_t n) { return (n + 7) & ~int64_t(7); };
+  Slots kernel[2];
+  float* at = scratch + up(2 * (p.places[0] + p.places[1]));
+  for (int k = 0; k < 2; ++k) {
+    kernel[k].index[0] = reinterpret_cast<int2*>(scratch);
+    kernel[k].index[1] = kernel[k].index[0] + p.places[0];
+    kernel[k].floats = at;
+    kernel[k].most = (int32_t)p.slots[k];
+    kernel[k].workers = p.workers[k];
+    for (int list = 0; list < 2; ++list) kernel[k].has[list] = p.tiles[list] == (k == 1);
+    at += up(p.slots[k] * (k ? kSharedTileRows : kSharedRows) * (p.dim_padded + 2));
+  }
+  Sources src;
+  for (int list = 0; list < 2; ++list) {
+    src.tiles[list] = p.tiles[list];
+    src.slots[list] = kernel[p.tiles[list]];
+  }
+  cudaError_t e = cudaSuccess;
+  if (p.slots[1]) {
+    e = launch_shared_tiles(kv, bt, q, dtype, kernel[1], st);
+    if (e != cudaSuccess) return e;
+    *launches += 1;
+  }
+  if (p.slots[0]) {
+    e = dtype == 0 ? launch_rows_typed<Bf16>(kv, bt, q, kernel[0], st) : launch_rows_typed<Fp16>(kv, bt, q, kernel[0], st);
+    if (e != cudaSuccess) return e;
+    *launches += 1;
+  }
+  e = dtype == 0 ? launch_join<Bf16>(kv, bt, q, src, st) : launch_join<Fp16>(kv, bt, q, src, st);
+  if (e != cudaSuccess) return e;
+  *launches += 1;
+  return cudaGetLastError();
 }
 
 }  // namespace kv

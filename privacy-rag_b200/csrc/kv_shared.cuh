@@ -129,5 +129,139 @@ __device__ __forceinline__ Unit element_unit(const Query& q, const Element& e, i
   return un;
 }
 
+// What all workers leave: a unit's parts lie side by side in slots.  The slot of worker w and unit u (counted through the
+// row of all units) is w + u, which rises from part to part in the order of the row.
+struct Slots {
+  int2* index[2] = {};  // at the places of the units over shared and over own keys: first slot, parts
+  float* floats = nullptr;
+  int32_t most = 0;     // slots
+  int32_t workers = 0;
+  bool has[2] = {};     // which keys
+};
+
+// A worker's part of a unit: its tiles of KEYS keys [from, to) of n.
+struct Piece {
+  Unit un;
+  int list = 0;
+  int32_t from = 0, to = 0, n = 0;
+  int32_t slot = 0;
+};
+
+// The work of all units in a row, cut into one equal run for each worker.  A unit's work is its number of key tiles, for
+// own keys as if it rose evenly from block to block of its element's rows: ROWS / KEYS tiles each `group` blocks, so that
+// sums have a closed form.  Work counts in 1 / group of a tile.  Whole warps; the elements are 32 at a time, a lane each.
+template <int ROWS, int KEYS>
+struct Runs {
+  static constexpr int32_t kRise = ROWS / KEYS;
+  Element el;
+  int32_t blocks = 0, rise = 0;               // of the lane's element: blocks of rows; rise of the units' work from block to block
+  int64_t base = 0;                           // and work of the first block's units
+  int64_t upto = 0;                           // work up to and with the lane's element
+  int32_t units_upto = 0;
+  int64_t total = 0, x = 0, end = 0;          // work; the worker's run
+  int32_t runs = 0, worker = 0, list = 0, e0 = -32;
+
+  __device__ __forceinline__ static int32_t tiles(int32_t begin, int32_t end) {
+    if (end <= begin) return 0;
+    return KEYS == 16 ? (end - begin + KEYS - 1) / KEYS : (end - 1) / KEYS - begin / KEYS + 1;
+  }
+  __device__ __forceinline__ int64_t before(int32_t b, int64_t of_base, int32_t of_rise) const {  // work of b blocks of one key head
+    return b * of_base + (int64_t)b * (b - 1) / 2 * of_rise;
+  }
+  __device__ __forceinline__ int64_t load(const View& kv, const Batch& bt, const SharedQuery& q, int of, int32_t at) {
+    const int lane = threadIdx.x & 31;
+    int32_t group;
+    el = of == 0 ? shared_element(kv, bt, q, at + lane) : own_element(kv, bt, q, at + lane, &group);
+    const uint32_t rows = (uint32_t)el.tokens * q.group;
+    blocks = el.end > el.begin ? (int32_t)((rows + ROWS - 1) / ROWS) : 0;
+    // the last key of the first block's rows
+    const int32_t seen = of == 0 ? el.end : el.end - el.tokens + (int32_t)((min(rows, (uint32_t)ROWS) - 1) / (uint32_t)q.group) + 1;
+    base = (int64_t)max(1, tiles(el.begin, min(seen, el.end))) * q.group;
+    rise = of == 0 ? 0 : kRise;
+    return before(blocks, base, rise) * kv.heads;
+  }
+  __device__ __forceinline__ int32_t length(const Batch& bt, const SharedQuery& q, const Slots& sl, int of) const {
+    return sl.has[of] ? (of == 0 ? q.count : bt.seqs) : 0;
+  }
+  __device__ __forceinline__ int64_t cut(int32_t w) const { return total * w / runs; }
+  // least: tiles that a run has at least
+  __device__ __forceinline__ void start(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, int32_t me, int32_t least) {
+#pragma unroll 1
+    for (int of = 0; of < 2; ++of)
+#pragma unroll 1
+      for (int32_t at = 0; at < length(bt, q, sl, of); at += 32) total += load(kv, bt, q, of, at);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    runs = (int32_t)max((int64_t)1, min((int64_t)sl.workers, total / ((int64_t)least * q.group)));
+    worker = me;
+    if (me < runs) {
+      x = cut(me);
+      end = cut(me + 1);
+    }
+  }
+  // The next piece of the run; false: none is left.
+  __device__ __forceinline__ bool next(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, Piece* piece) {
+    const int lane = threadIdx.x & 31;
+    if (x >= end) return false;
+    uint32_t hit;
+#pragma unroll 1
+    while (!(hit = __ballot_sync(0xffffffffu, x < upto))) {  // the next 32 elements
+      const int64_t so_far = __shfl_sync(0xffffffffu, upto, 31);
+      const int32_t units_so_far = __shfl_sync(0xffffffffu, units_upto, 31);
+      e0 += 32;
+      while (list < 2 && e0 >= length(bt, q, sl, list)) ++list, e0 = 0;
+      if (list == 2) return false;
+      upto = load(kv, bt, q, list, e0);
+      units_upto = blocks * kv.heads;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t a = __shfl_up_sync(0xffffffffu, upto, d);
+        const int32_t b = __shfl_up_sync(0xffffffffu, units_upto, d);
+        if (lane >= d) upto += a, units_upto += b;
+      }
+      upto += so_far;
+      units_upto += units_so_far;
+    }
+    const int at = __ffs(hit) - 1;
+    Element e;
+    e.row = __shfl_sync(0xffffffffu, el.row, at);
+    e.first = __shfl_sync(0xffffffffu, el.first, at);
+    e.tokens = __shfl_sync(0xffffffffu, el.tokens, at);
+    e.begin = __shfl_sync(0xffffffffu, el.begin, at);
+    e.end = __shfl_sync(0xffffffffu, el.end, at);
+    const int64_t of_base = __shfl_sync(0xffffffffu, base, at);
+    const int32_t of_rise = __shfl_sync(0xffffffffu, rise, at), of_blocks = __shfl_sync(0xffffffffu, blocks, at);
+    const int64_t first = __shfl_sync(0xffffffffu, upto, at) - before(of_blocks, of_base, of_rise) * kv.heads;
+    const int32_t first_unit = __shfl_sync(0xffffffffu, units_upto, at) - of_blocks * kv.heads;
+    // the block: the last that begins at or before x
+    int32_t low = 0, high = of_blocks;
+    while (high - low > 1) {
+      const int32_t mid = low + (high - low) / 2;
+      if (first + before(mid, of_base, of_rise) * kv.heads <= x) low = mid;
+      else high = mid;
+    }
+    const int64_t work = of_base + (int64_t)low * of_rise, into = x - first - before(low, of_base, of_rise) * kv.heads;
+    const int32_t g = (int32_t)(into / work);
+    const int64_t unit_x = x - (into - g * work), to = min(end, unit_x + work);
+    piece->list = list;
+    piece->un = element_unit<ROWS>(q, e, low, g, list == 0);
+    piece->n = tiles(e.begin, e.begin + piece->un.n);
+    piece->from = (int32_t)((x - unit_x) * piece->n / work);
+    piece->to = (int32_t)((to - unit_x) * piece->n / work);
+    piece->slot = worker + first_unit + low * kv.heads + g;
+    if (piece->slot >= sl.most) {  // sequences that overlap have more units than there are
+      if (lane == 0) flag_error(bt.err, kErrTable);
+      x = end;
+      return false;
+    }
+    if (x == unit_x && lane == 0) {
+      const int32_t last = (int32_t)(((unit_x + work) * runs - 1) / total);  // the worker of the unit's last work
+      sl.index[list][place_of<ROWS>(kv, q, e, e0 + at, low, g)] = make_int2(piece->slot, last - worker + 1);
+    }
+    x = to;
+    return true;
+  }
+};
+
 }  // namespace kv
 }  // namespace bfvgpu

@@ -6,14 +6,22 @@
 namespace bfvgpu {
 namespace kv {
 
+constexpr int kSharedRows = 16, kSharedTileRows = 256;  // of a unit of the kernel of few rows, and of the tensor-core kernel
+
 struct SharedPlan {
-  int32_t warps = 0, dim_padded = 128;
-  int64_t places[2] = {}, slots = 0;  // units over shared and over own keys; partial results
+  bool tiles[2] = {};         // which kernel works on shared and on own keys
+  int32_t dim_padded = 128;
+  int32_t workers[2] = {};    // warps of the kernel of few rows, blocks of the tensor-core kernel
+  int64_t places[2] = {};     // units over shared and over own keys
+  int64_t slots[2] = {};      // partial results of the two kernels
   uint64_t scratch_floats() const;
 };
-SharedPlan plan_shared(const View& kv, const Batch& bt, const SharedQuery& q, int sms);
+// tiles: whether the queries' strides suit the tensor-core kernel's loads.
+SharedPlan plan_shared(const View& kv, const Batch& bt, const SharedQuery& q, int sms, bool tiles);
 cudaError_t launch_shared(const View& kv, const Batch& bt, const SharedQuery& q, int dtype, const SharedPlan& plan, float* scratch,
                           cudaStream_t st, int* launches);
+// The tensor-core kernel's part (kv_prompt.cu).
+cudaError_t launch_shared_tiles(const View& kv, const Batch& bt, const SharedQuery& q, int dtype, const Slots& slots, cudaStream_t st);
 
 }  // namespace kv
 }  // namespace bfvgpu

@@ -81,8 +81,12 @@ class Shared:
         return [torch.cat(x) for x in zip(*out)]
 
 
-def run(bfv, ctx, *a, two_terms=True, scale=None, **kw):
+def run(bfv, ctx, *a, kernels=None, scale=None, **kw):
+    """kernels: those that the call has to take."""
     case = Shared(bfv, ctx, *a, **kw)
+    taken = case.kv.shared_kernels(case.q, case.table, len(case.shared))
+    assert kernels is None or taken == kernels
+    two_terms = taken == ("rows", "rows")
     call = {} if scale is None else dict(scale=scale)
     got = case.run(**call)
     assert ctx.check() == 0
@@ -126,3 +130,28 @@ def test_decode_shared(bfv, ctx, case):
 def test_prompt_shared(bfv, ctx, case):
     groups, g, r, dim, page, dtype, layout = case
     run(bfv, ctx, groups, g, r, dim, page, dtype, layout)
+
+
+def repeated(own, new, count):
+    return [(own, new)] * count
+
+
+TILES = [
+    # groups, kv_heads, group, dim, page, dtype, layout, kernels
+    ([(300, one(*range(1, 131)))], 1, 2, 64, 16, BF, "nhd", ("tiles", "rows")),        # 260 rows: two units
+    ([(1000, one(*range(40))), (129, one(*range(1, 40)))], 2, 8, 128, 16, BF, "hnd", ("tiles", "rows")),
+    ([(17, one(*range(1, 100)))], 1, 5, 72, 32, FP, "gaps", ("tiles", "rows")),         # tokens cut between the row tiles
+    ([(3000, one(*[3] * 64)), (1, one(*[1] * 64)), (128, one(*[2] * 64))], 3, 3, 128, 64, FP, "nhd", ("tiles", "rows")),
+    ([(2000, one(1, 1, 1))], 1, 200, 96, 128, BF, "hnd", ("tiles", "tiles")),          # a group of 200 query heads
+    ([(500, [(64, 64), (100, 80), (0, 1), (70, 70)])], 2, 2, 64, 16, BF, "hnd", ("tiles", "tiles")),
+    ([(700, [(1300, 1000)]), (0, [(257, 257)]), (127, [(200, 3), (400, 333)])], 2, 3, 72, 32, FP, "gaps", ("tiles", "tiles")),
+    ([(129, repeated(150, 130, 5)), (4000, repeated(129, 129, 2))], 1, 4, 128, 64, BF, "hnd", ("tiles", "tiles")),
+    ([(64, [(900, 900)]), (1, repeated(300, 256, 3))], 4, 1, 128, 16, FP, "nhd", ("tiles", "tiles")),
+    ([(0, [(500, 500)]), (0, [(0, 0), (300, 300)])], 1, 2, 64, 256, BF, "hnd", ("tiles", "tiles")),  # nothing shared
+]
+
+
+@pytest.mark.parametrize("case", TILES, ids=name)
+def test_tiles(bfv, ctx, case):
+    groups, g, r, dim, page, dtype, layout, kernels = case
+    run(bfv, ctx, groups, g, r, dim, page, dtype, layout, kernels=kernels)

@@ -137,3 +137,23 @@ def test_the_choice_of_the_prompt_kernel(bfv):
     assert kernel(512, 1, 512, window=-1) == -1 and L.bfvgpu_last_error() == b"E_KV_WINDOW"
     assert kernel(512, 1, 512, dim=60) == -1 and L.bfvgpu_last_error() == b"E_KV_DIM"
     assert L.bfvgpu_kv_prompt_kernel(None, 8, 8, 1, 1, 1, 1, 0, 0) == -1
+
+
+def test_the_scratch_of_shared_attention_holds_what_either_kernel_leaves(bfv):
+    """The words do not know the queries' strides, which may rule the tensor-core kernel out: they are enough for it."""
+    import ctypes
+
+    from bfvgpu._lib import KvDesc
+    L = bfv.lib()
+    host = bfv.Context(4096, bfv.find_primes(4096, [36, 36, 37]), 2, 1, 65537, device=-1)
+    for heads, group, dim, tokens, seqs, count in ((4, 8, 128, 128, 128, 1), (1, 2, 64, 300, 2, 2), (8, 2, 72, 4000, 16, 3)):
+        cache = KvDesc(0x10000, 0x20000, 0, 1, 4, heads, 16, dim, 0, heads * 16 * dim, 16 * dim, dim)
+        words = L.bfvgpu_kv_shared_scratch_words(host.handle, ctypes.byref(cache), heads * group, tokens, seqs, 100, count)
+        kernels = [L.bfvgpu_kv_shared_kernel(ctypes.byref(cache), heads * group * dim, dim, heads * group, tokens, seqs, 100, count,
+                                             own) for own in (0, 1)]
+        assert kernels[0] == 1
+        padded = 64 if dim <= 64 else 128
+        # a slot of 256 rows for each of 148 blocks and each unit over shared keys
+        slots = 148 + (tokens * group // 256 + count) * heads
+        assert 2 * words >= slots * 256 * (padded + 2)
+        assert L.bfvgpu_kv_shared_scratch_words(host.handle, ctypes.byref(cache), heads * group, tokens, seqs, 100, seqs + 1) == 0

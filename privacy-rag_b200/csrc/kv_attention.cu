@@ -178,7 +178,8 @@ void attend_shared(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void*
   const SharedPlan sp = plan_shared(c.view, c.batch, sq, sm_count(at.device), prompt_strides(sq));
   need(scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
   need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
-  need(std::max(sp.slots[0], sp.slots[1]) <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+  // (rows of slots are numbered in 32 bits)
+  need(sp.slots[0] * kSharedRows <= (int64_t)kMost && sp.slots[1] * kSharedTileRows <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
   int launches = 0;
   cuda_need(launch_shared(c.view, c.batch, sq, cache->dtype, sp, reinterpret_cast<float*>(scratch), at.stream, &launches),
             "kv shared attention");

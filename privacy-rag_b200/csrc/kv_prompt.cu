@@ -67,6 +67,13 @@ constexpr uint32_t kPolls = 1u << 20;     // of a wait for the next step before 
 constexpr uint32_t kLongPolls = 1u << 27; // of a wait that may span all keys of other rows
 constexpr int kPartTiles = 8;         // key tiles that a part has at least
 constexpr int kMaxParts = 16;
+#ifndef TLD
+#define TLD 2
+#endif
+#ifndef TRT
+#define TRT 3
+#endif
+constexpr int kLeadTiles = TLD, kRunTiles = TRT;
 
 // A row tile's part of an item.
 struct Span {
@@ -395,6 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = *tmem_slot;
   cudaGridDependencySynchronize();
+  if constexpr (kSharing<Q>)  // the kernel of few rows needs nothing of this one, only what came before both
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // the next item, for every warp but the loads'; false: no more (or given up).  It stays where it is until
   // the warp gives its place back.
@@ -439,10 +448,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     };
-    Runs<kBlockRows, kTileKeys> runs;
+    Runs<kBlockRows, kTileKeys, kLeadTiles> runs;
     if constexpr (kSharing<Q>) {
       if (block == 0) record_uncovered(bt, q);
-      runs.start(kv, bt, q, slots, (int32_t)block, kPartTiles / 2);
+      runs.start(kv, bt, q, slots, (int32_t)block, kRunTiles);
     }
     while (ok && block >= 0) {
       Item it;
@@ -459,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         it.slot = piece.slot;
         if (it.begin >= it.end) {  // a part of less than a tile: nothing is seen
           for (int32_t r = lane; r < un.rows; r += 32)
-            *reinterpret_cast<float2*>(slots.floats + it.slot * kSlotFloats<DP> + kBlockRows * DP + r * 2) = make_float2(-INFINITY, 0.f);
+            slots.sums[(int64_t)it.slot * kBlockRows + r] = make_float2(-INFINITY, 0.f);
           continue;
         }
       } else {
@@ -886,8 +895,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mine_live = at_row < un.rows;
       const float sum = ml[row].y;
       const bool partial = kSharing<Q> || it.parts > 1;
-      float* slot = (kSharing<Q> ? slots.floats : scratch) + it.slot * kSlotFloats<DP>;
-      if (partial && half == 0 && mine_live) *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = ml[row];
+      float* slot = kSharing<Q> ? slots.values + (int64_t)it.slot * (kBlockRows * DP) : scratch + it.slot * kSlotFloats<DP>;
+      if (partial && half == 0 && mine_live) {
+        if constexpr (kSharing<Q>) slots.sums[(int64_t)it.slot * kBlockRows + at_row] = ml[row];
+        else *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = ml[row];
+      }
       if (fresh) {  // no row of the tile sees a key of the item
         if (!partial && half == 0 && mine_live)
           for (int32_t d = 0; d < kv.dim; d += 8) *reinterpret_cast<uint4*>(un.result(kv, q, at_row) + d) = make_uint4(0, 0, 0, 0);

@@ -20,7 +20,14 @@ namespace bfvgpu {
 namespace kv {
 namespace {
 
-constexpr int kRunStages = 4;  // a warp has at least, where the row has them
+#ifndef RST
+#define RST 6
+#endif
+#ifndef RLD
+#define RLD 3
+#endif
+constexpr int kRunStages = RST;  // a warp has at least, where the row has them
+constexpr int kLead = RLD;
 #ifndef TRS
 #define TRS 64
 #endif
@@ -29,21 +36,17 @@ constexpr int kRunStages = 4;  // a warp has at least, where the row has them
 #endif
 constexpr int kTileRowsShared = TRS, kTileRowsOwn = TRO;
 
-template <int DP>
-constexpr int64_t kSlotFloats = kRows * (DP + 2);
-static_assert(kRows == kSharedRows);
-
 template <class T, int DP, int NK>
-__global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, SharedQuery q, Slots sl) {
+__global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, SharedQuery q, Slots sl, bool beside) {
   using R = Ring<DP>;
   extern __shared__ __align__(1024) uint8_t ring[];
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int32_t me = blockIdx.x * kWarps + warp;
-  cudaGridDependencySynchronize();
+  // Beside the tensor-core kernel, which lets this one start once what came before it is done, the wait for it is at the end.
+  if (!beside) cudaGridDependencySynchronize();
   if (me == 0) record_uncovered(bt, q);
-  Runs<kRows, kKeys> runs;
+  Runs<kRows, kKeys, kLead> runs;
   runs.start(kv, bt, q, sl, me, kRunStages);
-  if (me >= runs.runs) return;
 
   const uint32_t base = smem_addr(ring) + warp * R::kWarpBytes;
   if (kv.dim != NK * 16) {  // the chunks past the head's dims are never copied
@@ -56,18 +59,18 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, 
   for (Piece p; runs.next(kv, bt, q, sl, &p);) {
     const Unit& un = p.un;
     const int32_t s0 = p.from, s1 = p.to;
-    const bool flat = p.list == 0;
+    const bool flat = un.flat;
     uint32_t qa[NK][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const bool some = quad + 8 * h < un.rows;
-      const uint16_t* p = un.query(q, quad + 8 * h);
+      const uint16_t* of_row = un.query(q, quad + 8 * h);
 #pragma unroll
       for (int ks = 0; ks < NK; ++ks)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int32_t d = ks * 16 + c * 8 + pair;
-          qa[ks][h + 2 * c] = some && d < kv.dim ? __ldg(reinterpret_cast<const uint32_t*>(p + d)) : 0;
+          qa[ks][h + 2 * c] = some && d < kv.dim ? __ldg(reinterpret_cast<const uint32_t*>(of_row + d)) : 0;
         }
     }
     // lane l looks up the page of key l % 16 of a stage, one stage ahead of its copies
@@ -130,7 +133,8 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, 
     }
     copies_wait<0>();
     __syncwarp();
-    float* to = sl.floats + (int64_t)p.slot * kSlotFloats<DP>;
+    float* to = sl.values + (int64_t)p.slot * (kRows * DP);
+    float2* sums = sl.sums + (int64_t)p.slot * kRows;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -140,96 +144,82 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, 
 #pragma unroll
       for (int i = 0; i < NK * 2; ++i)
         *reinterpret_cast<float2*>(to + r * DP + i * 8 + pair) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
-      if (pair == 0) *reinterpret_cast<float2*>(to + kRows * DP + r * 2) = make_float2(m[h], l[h]);
+      if (pair == 0) sums[r] = make_float2(m[h], l[h]);
     }
   }
+  if (beside) cudaGridDependencySynchronize();
 }
 
-// Where the two lists' partial results are.
+// Where the rows' partial results over shared and over own keys are.
 struct Sources {
-  Slots slots[2];
-  bool tiles[2];
+  const int2* parts[2];
+  const float* values[2];
+  const float2* sums[2];
+  int32_t unit_rows[2], most[2];  // rows of a unit, slots
+  int64_t rows;                   // [tokens][query heads]
+  int32_t dim;
+  uint16_t* out;
+  uint32_t* err;
 };
 
-// A warp a row (query head of a token): its parts over shared keys, then those over its own, in order.
+// kLanes a row (query head of a token): its parts over shared keys, then those over its own, in order.
 template <class T, int DP>
-__global__ void __launch_bounds__(kThreads) k_kv_shared_join(View kv, Batch bt, SharedQuery q, Sources src) {
+__global__ void __launch_bounds__(kThreads) k_kv_shared_join(const __grid_constant__ Sources src) {
   cudaGridDependencySynchronize();
-  constexpr int kPer = DP / 32;  // dims a lane
-  const int lane = threadIdx.x & 31, d = lane * kPer;
-  const int32_t heads = kv.heads * q.group;
-  const int64_t rows = (int64_t)q.tokens * heads, row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int32_t t = (int32_t)(row / heads), head = (int32_t)(row - (int64_t)t * heads), g = head / q.group, in_group = head - g * q.group;
-  const int32_t s = bt.starts ? sequence_of_token(bt, t) : t;
-  int32_t group;
-  const Element own = own_element(kv, bt, q, s, &group);
-  if (t < own.first || t >= own.first + own.tokens) {  // of no sequence
-    if (lane == 0) flag_error(bt.err, kErrTable);
-    return;
-  }
-  float top = -INFINITY, sum = 0, v[kPer] = {};
+  constexpr int kLanes = DP / 4, kTogether = 8;  // parts whose numbers are asked for together
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const int d = threadIdx.x % kLanes * 4;
+  if (row >= src.rows || d >= src.dim) return;
+  float top = -INFINITY, sum = 0, v[4] = {};
+  const int2 all[2] = {src.parts[0][row], src.parts[1][row]};
 #pragma unroll
   for (int list = 0; list < 2; ++list) {
-    if (list == 0 && group < 0) continue;
-    const Element el = list == 0 ? shared_element(kv, bt, q, group) : own;
-    if (el.end <= el.begin || t < el.first || t >= el.first + el.tokens) continue;
-    const Slots& sl = src.slots[list];
-    const int32_t r = (t - el.first) * q.group + in_group, of = list == 0 ? group : s;
-    const int32_t unit_rows = src.tiles[list] ? kSharedTileRows : kSharedRows, block = r / unit_rows, in = r - block * unit_rows;
-    const int64_t place = src.tiles[list] ? place_of<kSharedTileRows>(kv, q, el, of, block, g) : place_of<kSharedRows>(kv, q, el, of, block, g);
-    const int2 parts = sl.index[list][place];
-    if (parts.x < 0 || parts.y < 0 || parts.y > sl.most - parts.x) {  // sequences that overlap
-      if (lane == 0) flag_error(bt.err, kErrTable);
+    const int32_t unit_rows = src.unit_rows[list], slot = all[list].x / unit_rows;
+    if (all[list].x < 0 || all[list].y < 0 || all[list].y > src.most[list] - slot) {  // of tokens outside all sequences
+      flag_error(src.err, kErrTable);
       continue;
     }
-    const int64_t slot_floats = (int64_t)unit_rows * (DP + 2);
-    const float* from = sl.floats + parts.x * slot_floats + in * DP;
-    const int64_t to_ml = (int64_t)unit_rows * DP + in * 2 - in * DP;
-    constexpr int kTogether = 8;  // parts whose numbers are asked for together
-    for (int32_t c0 = 0; c0 < parts.y; c0 += kTogether) {
-      float2 mlc[kTogether];
-      float vc[kTogether][kPer];
-#pragma unroll
-      for (int c = 0; c < kTogether; ++c) {
-        const float* other = from + (c0 + c) * slot_floats;
-        mlc[c] = make_float2(-INFINITY, 0.f);
-        if (c0 + c < parts.y) mlc[c] = *reinterpret_cast<const float2*>(other + to_ml);
-#pragma unroll
-        for (int i = 0; i < kPer; i += 2) {
-          float2 y = make_float2(0.f, 0.f);
-          if (c0 + c < parts.y) y = *reinterpret_cast<const float2*>(other + d + i);
-          vc[c][i] = y.x;
-          vc[c][i + 1] = y.y;
-        }
-      }
+    const float* from = src.values[list] + (int64_t)all[list].x * DP + d;
+    const float2* sums = src.sums[list] + all[list].x;
+#pragma unroll 1
+    for (int32_t c0 = 0; c0 < all[list].y; c0 += kTogether) {
+      float2 ml[kTogether];
+      float4 x[kTogether];
       float now = top;
 #pragma unroll
-      for (int c = 0; c < kTogether; ++c) now = fmaxf(now, mlc[c].x);
+      for (int c = 0; c < kTogether; ++c) {
+        ml[c] = make_float2(-INFINITY, 0.f);
+        x[c] = make_float4(0, 0, 0, 0);
+        if (c0 + c < all[list].y) {
+          ml[c] = sums[(int64_t)(c0 + c) * unit_rows];
+          x[c] = *reinterpret_cast<const float4*>(from + (int64_t)(c0 + c) * unit_rows * DP);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kTogether; ++c) now = fmaxf(now, ml[c].x);
       const float ref = now == -INFINITY ? 0.f : now, fo = exp2_fast(top - ref);
       sum *= fo;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) v[i] *= fo;
+      for (int i = 0; i < 4; ++i) v[i] *= fo;
 #pragma unroll
       for (int c = 0; c < kTogether; ++c) {
-        const bool some = mlc[c].x != -INFINITY || mlc[c].y != 0.f;  // else nothing was seen, and values may not be there
-        const float f = some ? exp2_fast(mlc[c].x - ref) : 0.f;
-        sum += f * mlc[c].y;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) v[i] += some ? f * vc[c][i] : 0.f;
+        const bool some = ml[c].x != -INFINITY || ml[c].y != 0.f;  // else nothing was seen, and values may not be there
+        const float f = some ? exp2_fast(ml[c].x - ref) : 0.f;
+        sum += f * ml[c].y;
+        v[0] += some ? f * x[c].x : 0.f;
+        v[1] += some ? f * x[c].y : 0.f;
+        v[2] += some ? f * x[c].z : 0.f;
+        v[3] += some ? f * x[c].w : 0.f;
       }
       top = now;
     }
   }
-  if (d >= kv.dim) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key seen: zeros
-  uint16_t* out = q.out + row * kv.dim + d;
-#pragma unroll
-  for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(out + i) = T::pack(v[i] * inv, v[i + 1] * inv);
+  *reinterpret_cast<uint2*>(src.out + row * src.dim + d) = make_uint2(T::pack(v[0] * inv, v[1] * inv), T::pack(v[2] * inv, v[3] * inv));
 }
 
 template <class T, int DP, int NK>
-cudaError_t launch_rows_of(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, cudaStream_t st) {
+cudaError_t launch_rows_of(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, bool beside, cudaStream_t st) {
   static std::atomic<uint64_t> allowed{0};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -239,21 +229,22 @@ cudaError_t launch_rows_of(const View& kv, const Batch& bt, const SharedQuery& q
     if (e != cudaSuccess) return e;
     if (device < 64) allowed.fetch_or(uint64_t(1) << device);
   }
-  return launch_next(k_kv_shared_rows<T, DP, NK>, dim3((unsigned)(sl.workers / kWarps)), kThreads, Ring<DP>::kBytes, st, 1, kv, bt, q, sl);
+  return launch_next(k_kv_shared_rows<T, DP, NK>, dim3((unsigned)(sl.workers / kWarps)), kThreads, Ring<DP>::kBytes, st, 1, kv, bt, q, sl,
+                     beside);
 }
 
 template <class T>
-cudaError_t launch_rows_typed(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, cudaStream_t st) {
-  if (kv.dim <= 64) return launch_rows_of<T, 64, 4>(kv, bt, q, sl, st);
-  if (kv.dim <= 96) return launch_rows_of<T, 128, 6>(kv, bt, q, sl, st);
-  return launch_rows_of<T, 128, 8>(kv, bt, q, sl, st);
+cudaError_t launch_rows_typed(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, bool beside, cudaStream_t st) {
+  if (kv.dim <= 64) return launch_rows_of<T, 64, 4>(kv, bt, q, sl, beside, st);
+  if (kv.dim <= 96) return launch_rows_of<T, 128, 6>(kv, bt, q, sl, beside, st);
+  return launch_rows_of<T, 128, 8>(kv, bt, q, sl, beside, st);
 }
 
 template <class T>
-cudaError_t launch_join(const View& kv, const Batch& bt, const SharedQuery& q, const Sources& src, cudaStream_t st) {
-  const int64_t rows = (int64_t)q.tokens * kv.heads * q.group;
-  return launch_next(kv.dim <= 64 ? k_kv_shared_join<T, 64> : k_kv_shared_join<T, 128>, dim3((unsigned)((rows + kWarps - 1) / kWarps)),
-                     kThreads, 0, st, 1, kv, bt, q, src);
+cudaError_t launch_join(int dim, const Sources& src, cudaStream_t st) {
+  const int per = kThreads / ((dim <= 64 ? 64 : 128) / 4);
+  return launch_next(dim <= 64 ? k_kv_shared_join<T, 64> : k_kv_shared_join<T, 128>, dim3((unsigned)((src.rows + per - 1) / per)),
+                     kThreads, 0, st, 1, src);
 }
 
 }  // namespace
@@ -265,55 +256,78 @@ SharedPlan plan_shared(const View& kv, const Batch& bt, const SharedQuery& q, in
   const int64_t rows = (int64_t)q.tokens * q.group;
   p.tiles[0] = tiles && rows >= (int64_t)kTileRowsShared * q.count;
   p.tiles[1] = tiles && rows >= (int64_t)kTileRowsOwn * bt.seqs;
-  const int32_t elements[2] = {q.count, bt.seqs};
+  p.rows = rows * kv.heads;
+  const int64_t elements[2] = {q.count, bt.seqs};
   p.workers[0] = sms * (narrow ? 3 : 2) * kWarps;
   p.workers[1] = sms;
-  for (int list = 0; list < 2; ++list) {
-    p.places[list] = places(kv, q, elements[list], p.tiles[list] ? kSharedTileRows : kSharedRows);
-    p.slots[p.tiles[list]] += p.places[list];
+  for (int list = 0; list < 2; ++list)
+    p.slots[p.tiles[list]] += most_units(kv, q, elements[list], p.tiles[list] ? kSharedTileRows : kSharedRows);
+  for (int kernel = 0; kernel < 2; ++kernel) {
+    if (!p.slots[kernel]) continue;
+    // the work in tiles is below the number of units times the tiles of the longest sequence, and has to fit 32 bits
+    const int64_t tiles_of_all = (((int64_t)bt.width << kv.page_log) / (kernel ? 128 : 16) + 2) * 2;
+    while (((tiles_of_all >> p.coarse[kernel]) + 2) * p.slots[kernel] >= int64_t(1) << 31) ++p.coarse[kernel];
+    p.slots[kernel] += p.workers[kernel];
   }
-  for (int kernel = 0; kernel < 2; ++kernel)
-    if (p.slots[kernel]) p.slots[kernel] += p.workers[kernel];
   return p;
 }
 
-// [first slots and parts of the units][slots of few rows][slots of tiles], each 32-byte aligned
+namespace {
+// [parts of the rows, twice][sums][values] of both kernels, each 32-byte aligned
+int64_t up8(int64_t floats) { return (floats + 7) & ~int64_t(7); }
+int64_t slot_rows(const SharedPlan& p, int kernel) { return p.slots[kernel] * (kernel ? kSharedTileRows : kSharedRows); }
+}  // namespace
+
 uint64_t SharedPlan::scratch_floats() const {
-  auto up = [](int64_t n) { return (n + 7) & ~int64_t(7); };
-  return up(2 * (places[0] + places[1])) + up(slots[0] * kSharedRows * (dim_padded + 2)) + slots[1] * kSharedTileRows * (dim_padded + 2);
+  int64_t n = 2 * up8(2 * rows);
+  for (int kernel = 0; kernel < 2; ++kernel) n += up8(2 * slot_rows(*this, kernel)) + slot_rows(*this, kernel) * dim_padded;
+  return n;
 }
 
 cudaError_t launch_shared(const View& kv, const Batch& bt, const SharedQuery& q, int dtype, const SharedPlan& p, float* scratch,
                           cudaStream_t st, int* launches) {
-  auto up = [](int64_t n) { return (n + 7) & ~int64_t(7); };
-  Slots kernel[2];
-  float* at = scratch + up(2 * (p.places[0] + p.places[1]));
-  for (int k = 0; k < 2; ++k) {
-    kernel[k].index[0] = reinterpret_cast<int2*>(scratch);
-    kernel[k].index[1] = kernel[k].index[0] + p.places[0];
-    kernel[k].floats = at;
-    kernel[k].most = (int32_t)p.slots[k];
-    kernel[k].workers = p.workers[k];
-    for (int list = 0; list < 2; ++list) kernel[k].has[list] = p.tiles[list] == (k == 1);
-    at += up(p.slots[k] * (k ? kSharedTileRows : kSharedRows) * (p.dim_padded + 2));
+  Slots of[2];
+  float* at = scratch + 2 * up8(2 * p.rows);
+  for (int kernel = 0; kernel < 2; ++kernel) {
+    Slots& sl = of[kernel];
+    for (int list = 0; list < 2; ++list) {
+      sl.parts[list] = reinterpret_cast<int2*>(scratch + list * up8(2 * p.rows));
+      sl.has[list] = p.tiles[list] == (kernel == 1);
+    }
+    sl.sums = reinterpret_cast<float2*>(at);
+    at += up8(2 * slot_rows(p, kernel));
+    sl.values = at;
+    at += slot_rows(p, kernel) * p.dim_padded;
+    sl.most = (int32_t)p.slots[kernel];
+    sl.workers = p.workers[kernel];
+    sl.coarse = p.coarse[kernel];
   }
   Sources src;
   for (int list = 0; list < 2; ++list) {
-    src.tiles[list] = p.tiles[list];
-    src.slots[list] = kernel[p.tiles[list]];
+    const Slots& sl = of[p.tiles[list]];
+    src.parts[list] = sl.parts[list];
+    src.values[list] = sl.values;
+    src.sums[list] = sl.sums;
+    src.unit_rows[list] = p.tiles[list] ? kSharedTileRows : kSharedRows;
+    src.most[list] = sl.most;
   }
+  src.rows = p.rows;
+  src.dim = kv.dim;
+  src.out = q.out;
+  src.err = bt.err;
   cudaError_t e = cudaSuccess;
   if (p.slots[1]) {
-    e = launch_shared_tiles(kv, bt, q, dtype, kernel[1], st);
+    e = launch_shared_tiles(kv, bt, q, dtype, of[1], st);
     if (e != cudaSuccess) return e;
     *launches += 1;
   }
   if (p.slots[0]) {
-    e = dtype == 0 ? launch_rows_typed<Bf16>(kv, bt, q, kernel[0], st) : launch_rows_typed<Fp16>(kv, bt, q, kernel[0], st);
+    const bool beside = p.slots[1] != 0;
+    e = dtype == 0 ? launch_rows_typed<Bf16>(kv, bt, q, of[0], beside, st) : launch_rows_typed<Fp16>(kv, bt, q, of[0], beside, st);
     if (e != cudaSuccess) return e;
     *launches += 1;
   }
-  e = dtype == 0 ? launch_join<Bf16>(kv, bt, q, src, st) : launch_join<Fp16>(kv, bt, q, src, st);
+  e = dtype == 0 ? launch_join<Bf16>(kv.dim, src, st) : launch_join<Fp16>(kv.dim, src, st);
   if (e != cudaSuccess) return e;
   *launches += 1;
   return cudaGetLastError();

@@ -28,6 +28,7 @@ __device__ __forceinline__ int32_t start_of(const Batch& bt, int32_t s) { return
 __device__ __forceinline__ int32_t ends_up_to(const int32_t* ends, int32_t count, int32_t x) {
   const int lane = threadIdx.x & 31;
   int32_t n = 0;
+#pragma unroll 1
   for (int32_t i0 = 0; i0 < count; i0 += 32) {
     const int32_t end = i0 + lane < count ? ends[i0 + lane] : 0x7fffffff;
     int32_t c = 0;
@@ -39,55 +40,31 @@ __device__ __forceinline__ int32_t ends_up_to(const int32_t* ends, int32_t count
   return n;
 }
 
-__device__ __forceinline__ int32_t checked_shared(const View& kv, const Batch& bt, int32_t n) {
-  return checked_length(bt, kv, n);
-}
-
-// The shared keys of group j (a lane each; none: from q.count on, or numbers outside their range, which are recorded).
-__device__ __forceinline__ Element shared_element(const View& kv, const Batch& bt, const SharedQuery& q, int32_t j) {
+// The shared keys of group `index` (OWN false), or the own keys of sequence `index`: an index a lane, whole warps; below
+// 0, or past the last: none.  What is outside its range is recorded, and has no rows.
+__device__ __forceinline__ Element element_at(const View& kv, const Batch& bt, const SharedQuery& q, int32_t index, bool own) {
   Element e;
-  if (j >= q.count) return e;
-  const int32_t a = q.groups[j], b = q.groups[j + 1], n = q.shared[j];
-  if (a < 0 || b < a || b > bt.seqs) {
+  int32_t j = ends_up_to(q.groups + 1, q.count, own ? index : -1);
+  if (index < 0 || index >= (own ? bt.seqs : q.count)) return e;
+  if (!own) j = index;
+  const bool in = j < q.count;
+  const int32_t a = q.groups[in ? j : 0], b = q.groups[in ? j + 1 : 0], shared = in ? q.shared[j] : 0;
+  bool good = in && a >= 0 && b >= a && b <= bt.seqs && (!own || a <= index);
+  const int32_t s = own || !good ? min(index, bt.seqs - 1) : min(a, bt.seqs - 1), t = own || !good ? s + 1 : b;
+  const int32_t first = start_of(bt, s), next = start_of(bt, t);
+  const int32_t most = bt.width << kv.page_log, length = own ? bt.lengths[s] : shared;
+  good = good && first >= 0 && next >= first && next <= q.tokens && shared >= 0 && shared <= most && length >= 0 && length <= most;
+  // every new token sees all that is shared
+  good = good && !(own && next > first && shared > max(0, length - (next - first) + 1));
+  if (!good) {
     flag_error(bt.err, kErrTable);
     return e;
-  }
-  if (a == b) return e;
-  const int32_t s = start_of(bt, a), t = start_of(bt, b);
-  if (s < 0 || t < s || t > q.tokens) {
-    flag_error(bt.err, kErrTable);
-    return e;
-  }
-  e.row = a;
-  e.first = s;
-  e.tokens = t - s;
-  e.end = checked_shared(kv, bt, n);
-  return e;
-}
-
-// The own keys of sequence s (a lane each; whole warps), and its group (-1: it is in none, which is recorded).
-__device__ __forceinline__ Element own_element(const View& kv, const Batch& bt, const SharedQuery& q, int32_t s, int32_t* group) {
-  Element e;
-  int32_t j = ends_up_to(q.groups + 1, q.count, s);
-  *group = -1;
-  if (s >= bt.seqs) return e;
-  const int32_t first = start_of(bt, s), next = start_of(bt, s + 1), length = bt.lengths[s];
-  if (j < q.count && q.groups[j] <= s) {
-    e.begin = checked_shared(kv, bt, q.shared[j]);
-    *group = j;
-  } else {
-    flag_error(bt.err, kErrTable);
-  }
-  if (first < 0 || next < first || next > q.tokens) {
-    flag_error(bt.err, kErrTable);
-    return Element{};
   }
   e.row = s;
   e.first = first;
   e.tokens = next - first;
-  e.end = checked_length(bt, kv, length);
-  // every new token sees all that is shared
-  if (e.tokens && e.begin > max(0, e.end - e.tokens + 1)) flag_error(bt.err, kErrTable);
+  e.begin = own ? shared : 0;
+  e.end = length;
   return e;
 }
 
@@ -97,17 +74,6 @@ __device__ __forceinline__ void record_uncovered(const Batch& bt, const SharedQu
   if (q.groups[0] != 0 || q.groups[q.count] != bt.seqs ||
       (bt.starts && (bt.starts[0] != 0 || bt.starts[bt.seqs] != q.tokens)))
     flag_error(bt.err, kErrTable);
-}
-
-// A unit (ROWS rows of an element's tokens and one key head) has a place in a table of all units that needs no sum over
-// the elements before it: the element's first unit of rows is at (first row) / ROWS + its number, which leaves room for
-// each element's last, partly filled one.
-template <int ROWS>
-__device__ __forceinline__ int64_t place_of(const View& kv, const Query& q, const Element& e, int32_t number, int32_t block, int32_t g) {
-  return ((int64_t)((uint32_t)e.first * (uint32_t)q.group / ROWS) + number + block) * kv.heads + g;
-}
-inline int64_t places(const View& kv, const Query& q, int32_t elements, int rows) {
-  return ((int64_t)q.tokens * q.group / rows + elements) * kv.heads;
 }
 
 // Block `block` of ROWS rows of an element, and key head g.  FLAT: shared keys, which every row sees.
@@ -129,98 +95,128 @@ __device__ __forceinline__ Unit element_unit(const Query& q, const Element& e, i
   return un;
 }
 
-// What all workers leave: a unit's parts lie side by side in slots.  The slot of worker w and unit u (counted through the
+// What all workers leave.  A unit's parts lie side by side in slots: the slot of worker w and unit u (counted through the
 // row of all units) is w + u, which rises from part to part in the order of the row.
 struct Slots {
-  int2* index[2] = {};  // at the places of the units over shared and over own keys: first slot, parts
-  float* floats = nullptr;
-  int32_t most = 0;     // slots
+  int2* parts[2] = {};      // [tokens][query heads] of the rows' shared and own keys: first slot times its rows + row, parts
+  float* values = nullptr;  // [slots][rows of a unit][padded dims]
+  float2* sums = nullptr;   // [slots][rows of a unit] maximum and sum
+  int32_t most = 0;         // slots
   int32_t workers = 0;
-  bool has[2] = {};     // which keys
+  int32_t coarse = 0;       // log2 of the tiles that work is counted in, for sums in 32 bits
+  bool has[2] = {};         // which keys
 };
 
-// A worker's part of a unit: its tiles of KEYS keys [from, to) of n.
+// A worker's part of a unit: its tiles of KEYS keys [from, to).
 struct Piece {
   Unit un;
-  int list = 0;
-  int32_t from = 0, to = 0, n = 0;
+  int32_t from = 0, to = 0;
   int32_t slot = 0;
 };
 
-// The work of all units in a row, cut into one equal run for each worker.  A unit's work is its number of key tiles, for
-// own keys as if it rose evenly from block to block of its element's rows: ROWS / KEYS tiles each `group` blocks, so that
-// sums have a closed form.  Work counts in 1 / group of a tile.  Whole warps; the elements are 32 at a time, a lane each.
-template <int ROWS, int KEYS>
+// The work of all units in a row, cut into one equal run for each worker.  Work is counted in key tiles, and a unit's start
+// as LEAD of them, so that runs of many short units are not longer than others; a run that ends in a unit's start leaves
+// it to the next.  Of an element's blocks of rows the later ones see more own keys, so they are taken in pairs, the last with the first and so
+// on, which have much the same work.  Whole warps; the elements are 32 at a time, a lane each.  Small code, in 32 bits: it
+// runs once, and its instructions come from memory (in 64 bits, with divisions for each unit, it took 20 us).
+template <int ROWS, int KEYS, int LEAD>
 struct Runs {
-  static constexpr int32_t kRise = ROWS / KEYS;
   Element el;
-  int32_t blocks = 0, rise = 0;               // of the lane's element: blocks of rows; rise of the units' work from block to block
-  int64_t base = 0;                           // and work of the first block's units
-  int64_t upto = 0;                           // work up to and with the lane's element
+  int32_t pairs = 0;                        // of the lane's element and one key head
+  uint32_t work = 0, upto = 0;              // of a pair, and up to and with the lane's element
   int32_t units_upto = 0;
-  int64_t total = 0, x = 0, end = 0;          // work; the worker's run
-  int32_t runs = 0, worker = 0, list = 0, e0 = -32;
+  uint32_t total = 0, length = 1, x = 0, end = 0;  // work; a run's, the worker's
+  int32_t worker = 0, e0 = -32;
 
   __device__ __forceinline__ static int32_t tiles(int32_t begin, int32_t end) {
     if (end <= begin) return 0;
     return KEYS == 16 ? (end - begin + KEYS - 1) / KEYS : (end - 1) / KEYS - begin / KEYS + 1;
   }
-  __device__ __forceinline__ int64_t before(int32_t b, int64_t of_base, int32_t of_rise) const {  // work of b blocks of one key head
-    return b * of_base + (int64_t)b * (b - 1) / 2 * of_rise;
+  // tiles of block b, and the work they are counted as
+  __device__ __forceinline__ static int32_t tiles_of(const SharedQuery& q, const Element& e, bool own, int32_t b) {
+    const uint32_t rows = min((uint32_t)e.tokens * q.group, (uint32_t)(b + 1) * ROWS);
+    const int32_t end = own ? e.end - e.tokens + (int32_t)((rows - 1) / (uint32_t)q.group) + 1 : e.end;
+    return tiles(e.begin, end);
   }
-  __device__ __forceinline__ int64_t load(const View& kv, const Batch& bt, const SharedQuery& q, int of, int32_t at) {
+  __device__ __forceinline__ static uint32_t lead(const Slots& sl) { return LEAD >> sl.coarse; }
+  __device__ __forceinline__ static uint32_t counted(const Slots& sl, int32_t tiles) {
+    return max(1u, ((uint32_t)tiles + (1u << sl.coarse) - 1) >> sl.coarse) + lead(sl);
+  }
+  __device__ __forceinline__ static int32_t blocks_of(const SharedQuery& q, const Element& e) {
+    return e.end > e.begin ? (int32_t)(((uint32_t)e.tokens * q.group + ROWS - 1) / ROWS) : 0;
+  }
+  __device__ __forceinline__ void load(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl) {
+    const int32_t e = e0 + (threadIdx.x & 31), groups = sl.has[0] ? q.count : 0;
+    const bool own = e >= groups;
+    el = element_at(kv, bt, q, own && !sl.has[1] ? -1 : own ? e - groups : e, own);
+    const int32_t blocks = blocks_of(q, el);
+    // own keys of several blocks in pairs, else one by one
+    const bool paired = own && blocks > 1;
+    pairs = paired ? (blocks + 1) / 2 : blocks;
+    work = blocks ? counted(sl, tiles_of(q, el, own, blocks - 1)) + (paired ? counted(sl, tiles_of(q, el, own, 0)) : 0) : 0;
+  }
+  __device__ __forceinline__ int32_t elements(const Batch& bt, const SharedQuery& q, const Slots& sl) const {
+    return (sl.has[0] ? q.count : 0) + (sl.has[1] ? bt.seqs : 0);
+  }
+  // The next 32 elements.
+  __device__ __forceinline__ void advance(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl) {
     const int lane = threadIdx.x & 31;
-    int32_t group;
-    el = of == 0 ? shared_element(kv, bt, q, at + lane) : own_element(kv, bt, q, at + lane, &group);
-    const uint32_t rows = (uint32_t)el.tokens * q.group;
-    blocks = el.end > el.begin ? (int32_t)((rows + ROWS - 1) / ROWS) : 0;
-    // the last key of the first block's rows
-    const int32_t seen = of == 0 ? el.end : el.end - el.tokens + (int32_t)((min(rows, (uint32_t)ROWS) - 1) / (uint32_t)q.group) + 1;
-    base = (int64_t)max(1, tiles(el.begin, min(seen, el.end))) * q.group;
-    rise = of == 0 ? 0 : kRise;
-    return before(blocks, base, rise) * kv.heads;
-  }
-  __device__ __forceinline__ int32_t length(const Batch& bt, const SharedQuery& q, const Slots& sl, int of) const {
-    return sl.has[of] ? (of == 0 ? q.count : bt.seqs) : 0;
-  }
-  __device__ __forceinline__ int64_t cut(int32_t w) const { return total * w / runs; }
-  // least: tiles that a run has at least
-  __device__ __forceinline__ void start(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, int32_t me, int32_t least) {
-#pragma unroll 1
-    for (int of = 0; of < 2; ++of)
-#pragma unroll 1
-      for (int32_t at = 0; at < length(bt, q, sl, of); at += 32) total += load(kv, bt, q, of, at);
+    const uint32_t so_far = __shfl_sync(0xffffffffu, upto, 31);
+    const int32_t units_so_far = __shfl_sync(0xffffffffu, units_upto, 31);
+    e0 += 32;
+    load(kv, bt, q, sl);
+    upto = (uint32_t)(pairs * kv.heads) * work;
+    units_upto = 2 * pairs * kv.heads;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    runs = (int32_t)max((int64_t)1, min((int64_t)sl.workers, total / ((int64_t)least * q.group)));
-    worker = me;
-    if (me < runs) {
-      x = cut(me);
-      end = cut(me + 1);
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t a = __shfl_up_sync(0xffffffffu, upto, d);
+      const int32_t b = __shfl_up_sync(0xffffffffu, units_upto, d);
+      if (lane >= d) upto += a, units_upto += b;
+    }
+    upto += so_far;
+    units_upto += units_so_far;
+  }
+  // Elements without keys have no units: their rows have no parts.
+  __device__ __forceinline__ void record_none(const View& kv, const SharedQuery& q, const Slots& sl) const {
+    const int32_t e = e0 + (threadIdx.x & 31), list = e >= (sl.has[0] ? q.count : 0);
+    const int32_t heads = kv.heads * q.group;
+    for (uint32_t left = __ballot_sync(0xffffffffu, el.tokens && !pairs); left; left &= left - 1) {
+      const int from = __ffs(left) - 1;
+      const int64_t first = (int64_t)__shfl_sync(0xffffffffu, el.first, from) * heads;
+      const int64_t rows = (int64_t)__shfl_sync(0xffffffffu, el.tokens, from) * heads;
+      int2* to = sl.parts[__shfl_sync(0xffffffffu, list, from)] + first;
+      for (int64_t r = threadIdx.x & 31; r < rows; r += 32) to[r] = make_int2(0, 0);
     }
   }
-  // The next piece of the run; false: none is left.
+  // least: tiles that a run has at least
+  __device__ __forceinline__ void start(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, int32_t me, uint32_t least) {
+    const int32_t count = elements(bt, q, sl);
+#pragma unroll 1
+    do {
+      advance(kv, bt, q, sl);
+      if (me == 0) record_none(kv, q, sl);
+    } while (e0 + 32 < count);
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    least = max(1u, least >> sl.coarse);
+    length = max(least, (total + sl.workers - 1) / sl.workers);
+    worker = me;
+    x = min((uint64_t)me * length, (uint64_t)total);
+    end = min((uint64_t)x + length, (uint64_t)total);
+    if (count > 32) {  // from the first again
+      e0 = -32;
+      upto = 0;
+      units_upto = 0;
+    }
+  }
+  // The next piece of the run; false: none is left.  Pieces may be empty.
   __device__ __forceinline__ bool next(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl, Piece* piece) {
     const int lane = threadIdx.x & 31;
     if (x >= end) return false;
     uint32_t hit;
 #pragma unroll 1
-    while (!(hit = __ballot_sync(0xffffffffu, x < upto))) {  // the next 32 elements
-      const int64_t so_far = __shfl_sync(0xffffffffu, upto, 31);
-      const int32_t units_so_far = __shfl_sync(0xffffffffu, units_upto, 31);
-      e0 += 32;
-      while (list < 2 && e0 >= length(bt, q, sl, list)) ++list, e0 = 0;
-      if (list == 2) return false;
-      upto = load(kv, bt, q, list, e0);
-      units_upto = blocks * kv.heads;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t a = __shfl_up_sync(0xffffffffu, upto, d);
-        const int32_t b = __shfl_up_sync(0xffffffffu, units_upto, d);
-        if (lane >= d) upto += a, units_upto += b;
-      }
-      upto += so_far;
-      units_upto += units_so_far;
+    while (!(hit = __ballot_sync(0xffffffffu, x < upto))) {
+      if (e0 + 32 >= elements(bt, q, sl)) return false;  // (the numbers on the device have changed meanwhile)
+      advance(kv, bt, q, sl);
     }
     const int at = __ffs(hit) - 1;
     Element e;
@@ -229,39 +225,59 @@ struct Runs {
     e.tokens = __shfl_sync(0xffffffffu, el.tokens, at);
     e.begin = __shfl_sync(0xffffffffu, el.begin, at);
     e.end = __shfl_sync(0xffffffffu, el.end, at);
-    const int64_t of_base = __shfl_sync(0xffffffffu, base, at);
-    const int32_t of_rise = __shfl_sync(0xffffffffu, rise, at), of_blocks = __shfl_sync(0xffffffffu, blocks, at);
-    const int64_t first = __shfl_sync(0xffffffffu, upto, at) - before(of_blocks, of_base, of_rise) * kv.heads;
-    const int32_t first_unit = __shfl_sync(0xffffffffu, units_upto, at) - of_blocks * kv.heads;
-    // the block: the last that begins at or before x
-    int32_t low = 0, high = of_blocks;
-    while (high - low > 1) {
-      const int32_t mid = low + (high - low) / 2;
-      if (first + before(mid, of_base, of_rise) * kv.heads <= x) low = mid;
-      else high = mid;
+    const uint32_t each = __shfl_sync(0xffffffffu, work, at);
+    const int32_t units = __shfl_sync(0xffffffffu, pairs, at) * kv.heads;
+    const uint32_t into = x - (__shfl_sync(0xffffffffu, upto, at) - (uint32_t)units * each);
+    const int32_t first_unit = __shfl_sync(0xffffffffu, units_upto, at) - 2 * units;
+    const int32_t number = (int32_t)(into / each), pair = number / kv.heads, g = number - pair * kv.heads;
+    uint32_t off = into - (uint32_t)number * each;
+    const bool own = e0 + at >= (sl.has[0] ? q.count : 0);
+    // of a pair the later block first
+    const int32_t blocks = blocks_of(q, e);
+    int32_t block = own ? blocks - 1 - pair : pair;
+    int32_t n = tiles_of(q, e, own, block), which = 0;
+    uint32_t of_unit = own && blocks > 1 && block != pair ? min(counted(sl, n), each) : each;
+    if (off >= of_unit) {
+      off -= of_unit;
+      of_unit = each - of_unit;
+      block = pair;
+      n = tiles_of(q, e, own, block);
+      which = 1;
     }
-    const int64_t work = of_base + (int64_t)low * of_rise, into = x - first - before(low, of_base, of_rise) * kv.heads;
-    const int32_t g = (int32_t)(into / work);
-    const int64_t unit_x = x - (into - g * work), to = min(end, unit_x + work);
-    piece->list = list;
-    piece->un = element_unit<ROWS>(q, e, low, g, list == 0);
-    piece->n = tiles(e.begin, e.begin + piece->un.n);
-    piece->from = (int32_t)((x - unit_x) * piece->n / work);
-    piece->to = (int32_t)((to - unit_x) * piece->n / work);
-    piece->slot = worker + first_unit + low * kv.heads + g;
+    const uint32_t unit_x = x - off, key_x = unit_x + lead(sl), to = min(end, unit_x + of_unit);
+    if (to <= key_x) {  // the run ends in the unit's start
+      x = end;
+      return false;
+    }
+    const bool first = x <= key_x;
+    piece->un = element_unit<ROWS>(q, e, block, g, !own);
+    // all of a unit's tiles by the end of its work
+    piece->from = first ? 0 : (int32_t)min((uint64_t)(x - key_x) << sl.coarse, (uint64_t)n);
+    piece->to = to == unit_x + of_unit ? n : (int32_t)min((uint64_t)(to - key_x) << sl.coarse, (uint64_t)n);
+    piece->slot = worker + first_unit + 2 * number + which;
     if (piece->slot >= sl.most) {  // sequences that overlap have more units than there are
       if (lane == 0) flag_error(bt.err, kErrTable);
       x = end;
       return false;
     }
-    if (x == unit_x && lane == 0) {
-      const int32_t last = (int32_t)(((unit_x + work) * runs - 1) / total);  // the worker of the unit's last work
-      sl.index[list][place_of<ROWS>(kv, q, e, e0 + at, low, g)] = make_int2(piece->slot, last - worker + 1);
+    if (first) {
+      const int32_t last = (int32_t)((unit_x + of_unit - 1) / length);  // the worker of the unit's last work
+      const Unit& un = piece->un;
+      int2* parts = sl.parts[own];
+      for (int32_t r = lane; r < un.rows; r += 32) {
+        const int32_t t = un.token_of(q, r);
+        parts[((int64_t)(un.token0 + t) * kv.heads + g) * q.group + un.head0 + r - t * q.group] =
+            make_int2(piece->slot * ROWS + r, last - worker + 1);
+      }
     }
     x = to;
     return true;
   }
 };
+// Bounds on the host's side: of the units' numbers, and of the work in tiles.
+inline int64_t most_units(const View& kv, const Query& q, int64_t elements, int rows) {
+  return 2 * ((int64_t)q.tokens * q.group / rows + elements) * kv.heads;
+}
 
 }  // namespace kv
 }  // namespace bfvgpu

@@ -12,8 +12,9 @@ struct SharedPlan {
   bool tiles[2] = {};         // which kernel works on shared and on own keys
   int32_t dim_padded = 128;
   int32_t workers[2] = {};    // warps of the kernel of few rows, blocks of the tensor-core kernel
-  int64_t places[2] = {};     // units over shared and over own keys
-  int64_t slots[2] = {};      // partial results of the two kernels
+  int32_t coarse[2] = {};     // of the two kernels, as in Slots
+  int64_t slots[2] = {};      // partial results of the two kernels; 0: it has no work
+  int64_t rows = 0;
   uint64_t scratch_floats() const;
 };
 // tiles: whether the queries' strides suit the tensor-core kernel's loads.

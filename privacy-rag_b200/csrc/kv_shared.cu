@@ -20,21 +20,17 @@ namespace bfvgpu {
 namespace kv {
 namespace {
 
-#ifndef RST
-#define RST 6
-#endif
-#ifndef RLD
-#define RLD 3
-#endif
-constexpr int kRunStages = RST;  // a warp has at least, where the row has them
-constexpr int kLead = RLD;
-#ifndef TRS
-#define TRS 64
-#endif
-#ifndef TRO
-#define TRO 64
-#endif
-constexpr int kTileRowsShared = TRS, kTileRowsOwn = TRO;
+// Stages that a warp has at least, and that a unit's start (queries, table, first keys: 2 us against 0.6 a stage) counts
+// as.  16 answers on 992 tokens, 64 sequences in four groups, 24 answers on 30000: 11.8, 39.0, 43.9 us so; with 8 stages at
+// least 14.4, 39.0, 48.3; with a start as none 17.0, 54.1 (before other steps), as five 12.8, 39.9, 44.0.
+constexpr int kRunStages = 4, kLead = 3;
+// Which kernel: the tensor-core kernel's blocks take longer to start and to end, and read the keys once for 256 rows.  By the
+// average rows of a group (its tokens x query heads of a key head) x the keys that a table can name, since how many there
+// are is not known here: 16 answers, 32 rows, on 992 shared tokens 12.8 us with few rows, 16.1 with tiles; on 8000 25.2
+// and 22.1; 64 answers, 128 rows, on 992 tokens 17.8 and 19.3, on 8000 48.0 and 32.9; 4 x 32 rows on up to 4096 38.9 and
+// 42.6.  Own keys by the rows of a sequence: 16 questions of up to 30 tokens, 30 rows, with up to 2000 own tokens 64.8 and
+// 44.2, of up to 64 tokens 49.6 and 42.1.
+constexpr int64_t kTileWork = 200000, kTileRowsOwn = 24, kTileWorkOwn = 32000;
 
 template <class T, int DP, int NK>
 __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, SharedQuery q, Slots sl, bool beside) {
@@ -155,7 +151,7 @@ struct Sources {
   const int2* parts[2];
   const float* values[2];
   const float2* sums[2];
-  int32_t unit_rows[2], most[2];  // rows of a unit, slots
+  int32_t unit_log[2], most[2];  // log2(rows of a unit), slots
   int64_t rows;                   // [tokens][query heads]
   int32_t dim;
   uint16_t* out;
@@ -170,49 +166,54 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_join(const __grid_consta
   const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
   const int d = threadIdx.x % kLanes * 4;
   if (row >= src.rows || d >= src.dim) return;
-  float top = -INFINITY, sum = 0, v[4] = {};
-  const int2 all[2] = {src.parts[0][row], src.parts[1][row]};
+  int2 parts[2] = {src.parts[0][row], src.parts[1][row]};
 #pragma unroll
   for (int list = 0; list < 2; ++list) {
-    const int32_t unit_rows = src.unit_rows[list], slot = all[list].x / unit_rows;
-    if (all[list].x < 0 || all[list].y < 0 || all[list].y > src.most[list] - slot) {  // of tokens outside all sequences
+    const int2 p = parts[list];
+    if (p.x < 0 || p.y < 0 || p.y > src.most[list] - (p.x >> src.unit_log[list])) {  // of tokens outside all sequences
       flag_error(src.err, kErrTable);
-      continue;
+      parts[list] = make_int2(0, 0);
     }
-    const float* from = src.values[list] + (int64_t)all[list].x * DP + d;
-    const float2* sums = src.sums[list] + all[list].x;
+  }
+  // the i-th of all parts: i-th over shared keys, then those over its own
+  const float *shared = src.values[0] + (int64_t)parts[0].x * DP + d, *own = src.values[1] + (int64_t)parts[1].x * DP + d;
+  const float2 *shared_sums = src.sums[0] + parts[0].x, *own_sums = src.sums[1] + parts[1].x;
+  const int32_t some = parts[0].y, all = some + parts[1].y;
+  float top = -INFINITY, sum = 0, v[4] = {};
 #pragma unroll 1
-    for (int32_t c0 = 0; c0 < all[list].y; c0 += kTogether) {
-      float2 ml[kTogether];
-      float4 x[kTogether];
-      float now = top;
+  for (int32_t c0 = 0; c0 < all; c0 += kTogether) {
+    float2 ml[kTogether];
+    float4 x[kTogether];
+    float now = top;
 #pragma unroll
-      for (int c = 0; c < kTogether; ++c) {
-        ml[c] = make_float2(-INFINITY, 0.f);
-        x[c] = make_float4(0, 0, 0, 0);
-        if (c0 + c < all[list].y) {
-          ml[c] = sums[(int64_t)(c0 + c) * unit_rows];
-          x[c] = *reinterpret_cast<const float4*>(from + (int64_t)(c0 + c) * unit_rows * DP);
-        }
+    for (int c = 0; c < kTogether; ++c) {
+      const int32_t i = c0 + c;
+      const bool of_shared = i < some;
+      const int64_t rows = (int64_t)(of_shared ? i : i - some) << src.unit_log[of_shared ? 0 : 1];
+      ml[c] = make_float2(-INFINITY, 0.f);
+      x[c] = make_float4(0, 0, 0, 0);
+      if (i < all) {
+        ml[c] = (of_shared ? shared_sums : own_sums)[rows];
+        x[c] = *reinterpret_cast<const float4*>((of_shared ? shared : own) + rows * DP);
       }
-#pragma unroll
-      for (int c = 0; c < kTogether; ++c) now = fmaxf(now, ml[c].x);
-      const float ref = now == -INFINITY ? 0.f : now, fo = exp2_fast(top - ref);
-      sum *= fo;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] *= fo;
-#pragma unroll
-      for (int c = 0; c < kTogether; ++c) {
-        const bool some = ml[c].x != -INFINITY || ml[c].y != 0.f;  // else nothing was seen, and values may not be there
-        const float f = some ? exp2_fast(ml[c].x - ref) : 0.f;
-        sum += f * ml[c].y;
-        v[0] += some ? f * x[c].x : 0.f;
-        v[1] += some ? f * x[c].y : 0.f;
-        v[2] += some ? f * x[c].z : 0.f;
-        v[3] += some ? f * x[c].w : 0.f;
-      }
-      top = now;
     }
+#pragma unroll
+    for (int c = 0; c < kTogether; ++c) now = fmaxf(now, ml[c].x);
+    const float ref = now == -INFINITY ? 0.f : now, fo = exp2_fast(top - ref);
+    sum *= fo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= fo;
+#pragma unroll
+    for (int c = 0; c < kTogether; ++c) {
+      const bool seen = ml[c].x != -INFINITY || ml[c].y != 0.f;  // else values may not be there
+      const float f = seen ? exp2_fast(ml[c].x - ref) : 0.f;
+      sum += f * ml[c].y;
+      v[0] += seen ? f * x[c].x : 0.f;
+      v[1] += seen ? f * x[c].y : 0.f;
+      v[2] += seen ? f * x[c].z : 0.f;
+      v[3] += seen ? f * x[c].w : 0.f;
+    }
+    top = now;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key seen: zeros
   *reinterpret_cast<uint2*>(src.out + row * src.dim + d) = make_uint2(T::pack(v[0] * inv, v[1] * inv), T::pack(v[2] * inv, v[3] * inv));
@@ -254,8 +255,9 @@ SharedPlan plan_shared(const View& kv, const Batch& bt, const SharedQuery& q, in
   const bool narrow = kv.dim <= 64;
   p.dim_padded = narrow ? 64 : 128;
   const int64_t rows = (int64_t)q.tokens * q.group;
-  p.tiles[0] = tiles && rows >= (int64_t)kTileRowsShared * q.count;
-  p.tiles[1] = tiles && rows >= (int64_t)kTileRowsOwn * bt.seqs;
+  const int64_t keys = (int64_t)bt.width << kv.page_log;
+  p.tiles[0] = tiles && (double)rows * keys >= (double)kTileWork * q.count;
+  p.tiles[1] = tiles && rows >= kTileRowsOwn * bt.seqs && (double)rows * keys >= (double)kTileWorkOwn * bt.seqs;
   p.rows = rows * kv.heads;
   const int64_t elements[2] = {q.count, bt.seqs};
   p.workers[0] = sms * (narrow ? 3 : 2) * kWarps;
@@ -308,7 +310,8 @@ cudaError_t launch_shared(const View& kv, const Batch& bt, const SharedQuery& q,
     src.parts[list] = sl.parts[list];
     src.values[list] = sl.values;
     src.sums[list] = sl.sums;
-    src.unit_rows[list] = p.tiles[list] ? kSharedTileRows : kSharedRows;
+    src.unit_log[list] = p.tiles[list] ? 8 : 4;
+    static_assert(kSharedTileRows == 1 << 8 && kSharedRows == 1 << 4);
     src.most[list] = sl.most;
   }
   src.rows = p.rows;

@@ -8,15 +8,16 @@ the o call.  In between everything is 16-bit floating point with 32-bit sums: it
 reference's exact-integer attention, which runs as a two-party protocol and is out of this
 library's scope.
 
-It is the attention alone, on q and k as the call leaves them.  A model that changes them in between, as a Qwen3
-layer does by a norm of each head and rotary positions, takes the steps apart: ``words_to_floats``, its own norm
-and positions, ``KvCache.append`` and ``attend``, ``floats_to_words``.
+Norms of the heads and rotary positions, as a Qwen3 layer has them between the call and the attention, are applied on
+the way into the cache where ``rotary`` and the norms' weights are given; without them it is the attention alone, on q and
+k as the call leaves them.
 
-    att = RingAttention(ctx, q_heads=16, kv_heads=8, dim=128, fraction=24, out_fraction=12, pages=4096)
+    att = RingAttention(ctx, q_heads=16, kv_heads=8, dim=128, fraction=24, out_fraction=12, pages=4096,
+                        rotary=Rotary(ctx, 128, base=1e6), share=True)
     doc = att.open()
     att.extend({doc: 512})                      # a retrieved document
     o_words = att.layer(qkv_words)              # [512][4096] -> [512][2048]
-    answers = att.fork(doc, 4)                  # four answers share its pages
+    answers = att.fork(doc, 4)                  # four answers share its pages (and with share read them once)
     att.extend({a: 1 for a in answers})         # one token each
     o_words = att.layer(qkv_words_of_the_step)  # [4][4096] -> [4][2048], rows in the cache's order
 """
@@ -44,17 +45,25 @@ def floats_to_words(torch, x, fraction: int):
 class RingAttention:
     """Keys, values and attention of `layers` layers for a set of sequences.  qkv words of a call are
     [tokens][(q_heads + 2 kv_heads) dim], q first, with `fraction` fraction bits; the result has
-    `out_fraction`.  window and sinks as for ``PagedKv.decode``."""
+    `out_fraction`.  window and sinks as for ``PagedKv.decode``.  rotary: a ``Rotary`` for queries and keys; q_norm, k_norm:
+    float32 weights [dim], of each layer [layers][dim], of the norm of each head before it (eps).  share: rows that share
+    their first pages read them once together (``KvCache.attend``)."""
 
     def __init__(self, ctx: Context, q_heads: int, kv_heads: int, dim: int, fraction: int, out_fraction: int, pages: int,
                  layers: int = 1, page_tokens: int = 16, sequences: int = 64, tokens: int = 4096, dtype=None,
-                 window: int = 0, sinks: int = 0):
+                 window: int = 0, sinks: int = 0, rotary=None, q_norm=None, k_norm=None, eps: float = 1e-6, share: bool = False):
         import torch
+        if rotary is None and (q_norm is not None or k_norm is not None):
+            raise ValueError("E_ROTARY_NORM: norms of the heads come with a rotation")
+        for w in (q_norm, k_norm):
+            if w is not None and tuple(w.shape) not in ((dim,), (layers, dim)):
+                raise ValueError("E_ROTARY_SHAPE: a norm has weights [dim] or [layers][dim]")
         if not 0 <= fraction <= 58 or not 0 <= out_fraction <= 58:
             raise ValueError("E_SHAPE")
         self._torch = torch
         self.q_heads, self.kv_heads, self.dim = q_heads, kv_heads, dim
         self.fraction, self.out_fraction, self.window, self.sinks = fraction, out_fraction, window, sinks
+        self.rotary, self.q_norm, self.k_norm, self.eps, self.share = rotary, q_norm, k_norm, eps, share
         self.cache = KvCache(ctx, pages, kv_heads, dim, layers, page_tokens, sequences, tokens, dtype)
         self.open, self.free, self.fork, self.compact = (self.cache.open, self.cache.free, self.cache.fork,
                                                          self.cache.compact)
@@ -72,6 +81,12 @@ class RingAttention:
         if qkv_words.dim() != 2 or qkv_words.shape[1] != (h + 2 * g) * d:
             raise ValueError("E_SHAPE")
         x = words_to_floats(self._torch, qkv_words, self.fraction).unflatten(1, (h + 2 * g, d))
-        self.cache.append(x[:, h:h + g], x[:, h + g:], layer)
-        out = self.cache.attend(x[:, :h].to(self.cache.kv.k.dtype), layer, self.window, self.sinks)
+        if self.rotary is None:
+            self.cache.append(x[:, h:h + g], x[:, h + g:], layer)
+            q = x[:, :h].to(self.cache.kv.k.dtype)
+        else:
+            of_layer = lambda w: w if w is None or w.dim() == 1 else w[layer]  # noqa: E731
+            q = self.cache.append_rotary(x[:, h:h + g], x[:, h + g:], self.rotary, x[:, :h], of_layer(self.q_norm),
+                                         of_layer(self.k_norm), self.eps, layer)
+        out = self.cache.attend(q, layer, self.window, self.sinks, share=self.share)
         return floats_to_words(self._torch, out.flatten(1), self.out_fraction)

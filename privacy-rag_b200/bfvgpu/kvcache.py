@@ -256,6 +256,30 @@ class PageBook:
             fresh.append(int(self.table[c, last]) if part else -1)
         return children, fresh
 
+    def shared(self, new) -> tuple[list[int], list[int]]:
+        """Neighbouring rows that share their first pages, as groups and shared tokens of ``PagedKv.decode_shared``; new[row]:
+        the tokens of the step, which are among none's shared.  A row joins the group before it where that leaves the group
+        at least half of what it shares; rows without a sequence, or without new tokens, join the one before."""
+        new = np.asarray(new, dtype=np.int64)
+        full = (self.lengths - new) // self.page_tokens  # pages before the step's tokens
+        groups, shared = [0], []
+        first, now = -1, -1  # first row of the group that has tokens; pages that the group shares (-1: one row so far)
+        for row in np.flatnonzero((self.lengths > 0) & (new > 0)):
+            row = int(row)
+            if first >= 0:
+                top = int(min(full[first], full[row])) if now < 0 else int(min(now, full[row]))
+                apart = np.flatnonzero((self.table[first, :top] != self.table[row, :top]) | (self.table[first, :top] < 0))
+                common = int(apart[0]) if len(apart) else top
+                if common > 0 and 2 * common >= now:
+                    now = common
+                    continue
+            if row > groups[-1] or first >= 0:  # what is shared is read through the group's first row
+                shared.append(max(now, 0) * self.page_tokens)
+                groups.append(row)
+            first, now = row, -1
+        shared.append(max(now, 0) * self.page_tokens)
+        return groups + [len(self.lengths)], shared
+
     def free(self, row: int) -> None:
         """Ends a sequence."""
         self._row(row)
@@ -317,12 +341,15 @@ class KvCache:
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device=dev)
         self.starts = torch.zeros(sequences + 1, dtype=torch.int32, device=dev)
         self._each = 0  # 1: the step gives every row one token
+        self._new = np.zeros(sequences, dtype=np.int64)  # tokens of the step
+        self._groups = None  # the step's groups and shared tokens on the device, where they were asked for
 
     def _ints(self, values):
         return self._torch.tensor(values, dtype=self._torch.int32).pin_memory().to(self.table.device, non_blocking=True)
 
     def _push(self) -> None:
         """The host's table and lengths to the device, in the order of the current stream."""
+        self._groups = None
         self.table.copy_(self._torch.from_numpy(self.book.table.copy()).pin_memory(), non_blocking=True)
         self.lengths.copy_(self._torch.from_numpy(self.book.lengths.copy()).pin_memory(), non_blocking=True)
 
@@ -336,6 +363,7 @@ class KvCache:
         for row, n in counts.items():
             new[row] = n
         self._each = int((new == 1).all())
+        self._new = new
         self.starts.copy_(self._ints(np.concatenate([[0], np.cumsum(new)]).tolist()), non_blocking=True)
         self._push()
 
@@ -343,18 +371,38 @@ class KvCache:
         """The step's keys and values [tokens][heads][dim] of one layer."""
         self.kv.append(k_new, v_new, self.starts, self.table, self.lengths, layer=layer)
 
-    def attend(self, q, layer: int = 0, window: int = 0, sinks: int = 0, scale: float | None = None, out=None):
+    def append_rotary(self, k_new, v_new, rotary, q=None, q_norm=None, k_norm=None, eps: float = 1e-6, layer: int = 0):
+        """``append`` with norms of the heads and rotary positions on the way; the step's queries with theirs, or None
+        (``PagedKv.append_rotary``)."""
+        return self.kv.append_rotary(k_new, v_new, rotary, self.starts, self.table, self.lengths, q, q_norm, k_norm, eps, layer)
+
+    def attend(self, q, layer: int = 0, window: int = 0, sinks: int = 0, scale: float | None = None, out=None,
+               share: bool = False):
         """The attention of the step's tokens, after append: q [tokens][q_heads][dim].  A ``decode`` where
         every row of the table gets one token, else a ``prompt`` of all rows, whose kernel goes by their number
-        and the table's width (``PagedKv.prompt_kernel``)."""
+        and the table's width (``PagedKv.prompt_kernel``).  share: neighbouring rows that share their first pages, as
+        forks do, read them once together (``PageBook.shared``; without a window)."""
+        groups = self._shared() if share and not window else None
+        if groups is not None:
+            if self._each:
+                return self.kv.decode_shared(q, self.table, self.lengths, *groups, layer, scale, out)
+            return self.kv.prompt_shared(q, self.starts, self.table, self.lengths, *groups, layer, scale, out)
         if self._each:
             return self.kv.decode(q, self.table, self.lengths, layer, window, sinks, scale, out)
         return self.kv.prompt(q, self.starts, self.table, self.lengths, layer, window, sinks, scale, out)
+
+    def _shared(self):
+        """The step's groups and shared tokens on the device; None where no rows share any."""
+        if self._groups is None:
+            groups, shared = self.book.shared(self._new)
+            self._groups = (self._ints(groups), self._ints(shared)) if any(shared) else ()
+        return self._groups or None
 
     def fork(self, row: int, count: int = 1) -> list[int]:
         """count sequences that continue `row`, sharing its full pages."""
         children, fresh = self.book.fork(row, count)
         if children:
+            self._groups = None
             self.kv.fork(self._ints([row] * count), self._ints(children), self._ints(fresh), self.table, self.lengths)
         return children
 
@@ -373,5 +421,6 @@ class KvCache:
         """Moves the pages in use to the lowest numbers; how many moved."""
         src, dst = self.book.compact()
         if src:
+            self._groups = None
             self.kv.move(self._ints(src), self._ints(dst), self.table)
         return len(src)

@@ -1,0 +1,132 @@
+"""The steps between a layer's linear calls together: norms of the heads and rotary positions on the way into the cache,
+answers forked from one document, and attention that reads what they share once, against 64 bits."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import kv_reference as R  # noqa: E402
+import rotary_reference as RR  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+H, G, D = 8, 2, 64
+
+
+@pytest.fixture
+def ctx(bfv):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    c = bfv.Context(4096, bfv.find_primes(4096, [36, 36, 37]), 2, 1, 65537, device=0)
+    yield c
+    c.close()
+
+
+class Model:
+    """What the cache should hold: the kernels' own rotated keys and queries (tested for themselves), rounded to 16 bits, so
+    that the attention's bound is that of its own arithmetic; they are checked against the definition on the way."""
+
+    def __init__(self, rotary, q_norm, k_norm):
+        self.rotary, self.q_norm, self.k_norm, self.held = rotary, q_norm, k_norm, {}
+
+    def step(self, row, x, got_q):
+        k, v = self.held.get(row, (torch.zeros(0, G, D, dtype=BF),) * 2)
+        at = torch.arange(len(k), len(k) + len(x))
+        new, bound = RR.rotate(x[:, H:H + G], at, self.rotary.radians, self.rotary.scale, self.rotary.layout, self.k_norm, dtype=BF)
+        q, q_bound = RR.rotate(x[:, :H], at, self.rotary.radians, self.rotary.scale, self.rotary.layout, self.q_norm, dtype=BF)
+        assert ((got_q.double() - q).abs() <= q_bound).all()
+        return at, new, bound, k, v
+
+
+@pytest.mark.parametrize("share", [False, True])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_answers_of_a_document(bfv, ctx, share, layout):
+    gen = torch.Generator().manual_seed(21)
+    layers = 2
+    cache = bfv.KvCache(ctx, pages=200, heads=G, dim=D, layers=layers, page_tokens=16, sequences=6, tokens=512)
+    rotary = bfv.Rotary(ctx, D, base=1e6, layout=layout, scaling="yarn", factor=2.0)
+    q_norm, k_norm = (1 + 0.2 * torch.randn(D, generator=gen) for _ in range(2))
+    models = [Model(rotary, q_norm, k_norm) for _ in range(layers)]
+
+    def step(counts, joint):
+        cache.extend(counts)
+        for layer, model in enumerate(models):
+            x = torch.randn(sum(counts.values()), H + 2 * G, D, generator=gen)
+            dev = x.cuda()
+            q = cache.append_rotary(dev[:, H:H + G], dev[:, H + G:], rotary, dev[:, :H], q_norm.cuda(), k_norm.cuda(), layer=layer)
+            got = cache.attend(q, layer, share=share)
+            assert ctx.check() == 0
+            assert (cache._shared() is not None) == joint
+            table, pages, first = cache.table.cpu(), cache.kv.k[layer].cpu(), 0
+            for row in sorted(counts):
+                n = counts[row]
+                at, new, bound, k, v = model.step(row, x[first:first + n], q[first:first + n].cpu())
+                mine = pages[table[row, at // 16].long(), :, at % 16]
+                assert ((mine.double() - new).abs() <= bound).all()
+                k, v = torch.cat([k, mine]), torch.cat([v, x[first:first + n, H + G:].to(BF)])
+                model.held[row] = k, v
+                want, bound = R.attention(q[first:first + n].cpu(), k, v, len(k), 0, 0, D ** -0.5, two_terms=False)
+                assert ((got[first:first + n].double().cpu() - want).abs() <= bound).all()
+                first += n
+
+    doc = cache.open()
+    step({doc: 200}, False)
+    answers = cache.fork(doc, 4)
+    for m in models:
+        for a in answers:
+            m.held[a] = m.held[doc]
+    step({a: 1 for a in answers}, True)
+    step({a: 3 + a for a in answers}, True)
+    step({doc: 40, answers[0]: 1, answers[2]: 1}, True)       # the document goes on, too
+    more = cache.fork(answers[3], 1)
+    for m in models:
+        m.held[more[0]] = m.held[answers[3]]
+    step({r: 1 for r in [doc] + answers + more}, True)         # a token for every row of the table
+    cache.free(answers[1])
+    for m in models:
+        del m.held[answers[1]]
+    cache.compact()
+    step({answers[2]: 5, answers[3]: 5, more[0]: 5}, True)
+    cache.free(doc)
+    step({answers[0]: 2}, False)
+
+
+def test_ring_words_with_rotary_positions_and_sharing(bfv, ctx):
+    """RingAttention in words: the same as its parts one by one, with and without sharing within one result's bound."""
+    gen = torch.Generator().manual_seed(22)
+    rotary = bfv.Rotary(ctx, 32, base=1e4)
+    norms = [(1 + 0.2 * torch.randn(2, D, generator=gen)).cuda(), (1 + 0.2 * torch.randn(D, generator=gen)).cuda()]
+    make = lambda share: bfv.RingAttention(ctx, H, G, D, 20, 16, pages=100, layers=2, sequences=4, tokens=256,  # noqa: E731
+                                           rotary=rotary, q_norm=norms[0], k_norm=norms[1], eps=1e-5, share=share)
+    both = [make(False), make(True)]
+    kv = bfv.KvCache(ctx, 100, G, D, 2, 16, 4, 256)
+
+    def words(tokens):
+        x = torch.randn(tokens, (H + 2 * G) * D, generator=gen)
+        return (torch.round(x.double() * 2 ** 20).long() & ((1 << 59) - 1)).cuda()
+
+    def step(counts):
+        for a in both + [kv]:
+            a.extend(counts)
+        for layer in range(2):
+            w = words(sum(counts.values()))
+            plain, shared = (a.layer(w, layer) for a in both)
+            x = (((w + (1 << 58)) & ((1 << 59) - 1)) - (1 << 58)).double().mul(2.0 ** -20).float().unflatten(1, (H + 2 * G, D))
+            q = kv.append_rotary(x[:, H:H + G], x[:, H + G:], rotary, x[:, :H], norms[0][layer], norms[1], 1e-5, layer)
+            one = kv.attend(q, layer)
+            signed = [torch.where(o >= 1 << 58, o - (1 << 59), o).double() * 2.0 ** -16 for o in (plain, shared)]
+            assert torch.equal(signed[0], torch.round(one.flatten(1).double() * 2 ** 16) * 2.0 ** -16)
+            # values of +-4 at most, each side within 2 steps of bfloat16 of the exact result
+            assert (signed[0] - signed[1]).abs().max() <= 4 * 4 * 2.0 ** -8
+        assert ctx.check() == 0
+
+    doc = both[0].open()
+    assert both[1].open() == doc and kv.open() == doc
+    step({doc: 60})
+    answers = [a.fork(doc, 3) for a in both + [kv]][0]
+    step({a: 1 for a in answers})
+    step({r: 1 for r in [doc] + answers})
+    for bad in (dict(rotary=None, q_norm=norms[1]), dict(rotary=rotary, k_norm=norms[0][:, :8])):
+        with pytest.raises(ValueError, match="E_ROTARY"):
+            bfv.RingAttention(ctx, H, G, D, 20, 16, pages=4, layers=2, **bad)

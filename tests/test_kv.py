@@ -280,3 +280,52 @@ def test_calls_refuse_host_tensors(bfv):
         calls.move(object(), None, ints, ints, table, None)
     with pytest.raises(ValueError, match="E_KV_ARGUMENT"):
         calls.open(0, 0)
+
+
+def test_rows_that_share_their_pages(bfv):
+    """Groups are neighbours, cover all rows, and share full pages before the step's tokens, read through their first row."""
+    rng = random.Random(12)
+    found = 0
+    for trial in range(200):
+        page = 16
+        book = bfv.PageBook(400, page, 12, 20)
+        rows = []
+        for _ in range(rng.randint(1, 14)):
+            kind = rng.random()
+            try:
+                if kind < 0.35 or not rows:
+                    rows.append(book.open())
+                elif kind < 0.75:
+                    rows += book.fork(rng.choice(rows), rng.randint(1, 4))[0]
+                elif kind < 0.85:
+                    row = rng.choice(rows)
+                    book.free(row)
+                    rows.remove(row)
+                book.extend({r: rng.randint(0, 60) for r in rows if rng.random() < 0.6 and book.lengths[r] < 200})
+            except bfv.BfvGpuError:
+                pass  # no row is free
+        new = np.zeros(12, dtype=np.int64)
+        step = {r: rng.choice([0, 1, 1, 30]) for r in rows}
+        book.extend(step)
+        for r, n in step.items():
+            new[r] = n
+        groups, shared = book.shared(new)
+        assert groups[0] == 0 and groups[-1] == 12 and len(shared) == len(groups) - 1 and groups == sorted(set(groups))
+        for a, b, p in zip(groups, groups[1:], shared):
+            live = [r for r in range(a, b) if new[r]]
+            assert p % page == 0 and (p == 0 or live[0] == a)
+            for r in live:
+                assert p <= book.lengths[r] - new[r] and (book.table[r, :p // page] == book.table[a, :p // page]).all()
+                assert (book.table[r, :p // page] >= 0).all()
+            found += p > 0 and len(live) > 1
+            assert p == 0 or len(live) > 1
+    assert found > 50
+    book = bfv.PageBook(100, 16, 6, 10)
+    book.open(), book.open()
+    doc = book.open()
+    book.extend({doc: 40})
+    answers, _ = book.fork(doc, 3)
+    book.extend({a: 1 for a in answers})
+    assert book.shared([0, 0, 0, 1, 1, 1]) == ([0, 3, 6], [0, 32])  # not through rows 0 to 2, which have no token
+    assert book.shared([0, 0, 0, 1, 0, 0]) == ([0, 3, 6], [0, 0])
+    assert book.shared([0] * 6) == ([0, 6], [0])

@@ -157,3 +157,48 @@ def test_the_scratch_of_shared_attention_holds_what_either_kernel_leaves(bfv):
         slots = 148 + (tokens * group // 256 + count) * heads
         assert 2 * words >= slots * 256 * (padded + 2)
         assert L.bfvgpu_kv_shared_scratch_words(host.handle, ctypes.byref(cache), heads * group, tokens, seqs, 100, seqs + 1) == 0
+
+
+def test_shared_attention_refuses_on_the_host(bfv):
+    import ctypes
+
+    from bfvgpu._lib import KvDesc
+    L, at = bfv.lib(), 0x30000
+    host = bfv.Context(4096, bfv.find_primes(4096, [36, 36, 37]), 2, 1, 65537, device=-1)
+
+    def calls(cache=KvDesc(0x10000, 0x20000, 0, 1, 4, 2, 16, 64, 8192, 2048, 1024, 64), layer=0, heads=4, width=4, seqs=2, count=1,
+              scale=1.0, starts=at):
+        ref, got = ctypes.byref(cache), []
+        got.append((L.bfvgpu_kv_decode_shared_device(host.handle, ref, layer, at, 256, 64, heads, at, width, at, seqs, at, at, count,
+                                                     scale, at, at, None), L.bfvgpu_last_error()))
+        got.append((L.bfvgpu_kv_prompt_shared_device(host.handle, ref, layer, at, 256, 64, heads, 9, starts, at, width, at, seqs, at,
+                                                     at, count, scale, at, at, None), L.bfvgpu_last_error()))
+        return got
+
+    assert calls() == [(10, b"E_BFVGPU_HOST_ONLY_CONTEXT")] * 2
+    assert calls(count=3) == [(3, b"E_KV_GROUPS")] * 2
+    assert calls(scale=0.0) == [(1, b"E_KV_SCALE")] * 2
+    assert calls(layer=1) == [(3, b"E_KV_LAYER")] * 2 == calls(layer=-1)
+    assert calls(heads=3) == [(3, b"E_KV_HEADS")] * 2
+    assert calls(width=1 << 27) == [(3, b"E_KV_WIDTH")] * 2
+    assert calls(starts=None)[1] == (1, b"E_KV_ARGUMENT")
+    assert L.bfvgpu_kv_shared_kernel(None, 8, 8, 1, 1, 1, 1, 1, 0) == -1
+    assert L.bfvgpu_kv_shared_scratch_words(host.handle, None, 4, 9, 2, 4, 1) == 0
+
+
+def test_the_choice_of_the_shared_kernels(bfv):
+    import ctypes
+
+    from bfvgpu._lib import KvDesc
+    L = bfv.lib()
+
+    def kernels(tokens, seqs, count, keys, heads=8, group=2, dim=128, head_stride=None):
+        cache = KvDesc(0x10000, 0x20000, 0, 1, 4, heads, 16, dim, 0, heads * 16 * dim, 16 * dim, dim)
+        return [L.bfvgpu_kv_shared_kernel(ctypes.byref(cache), heads * group * dim, dim if head_stride is None else head_stride,
+                                          heads * group, tokens, seqs, keys // 16, count, own) for own in (0, 1)]
+
+    rows, tiles = 0, 1
+    assert kernels(16, 16, 1, 1040) == [rows, rows] and kernels(16, 16, 1, 8192) == [tiles, rows]
+    assert kernels(64, 64, 4, 4608) == [rows, rows] and kernels(64, 64, 1, 4608) == [tiles, rows]
+    assert kernels(500, 16, 1, 4176) == [tiles, tiles] and kernels(40, 2, 1, 144) == [rows, rows]
+    assert kernels(500, 16, 1, 4176, head_stride=0) == [rows, rows]

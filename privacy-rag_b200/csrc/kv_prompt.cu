@@ -94,8 +94,9 @@ struct Plan {
 };
 
 // What the loading warp tells the others: the rows, and which of their key tiles.
-struct Item {
-  Unit un;
+template <class U>
+struct ItemOf {
+  U un;
   Plan plan;
   int32_t begin = 0, end = 0;  // key tiles
   Span span[2];
@@ -126,7 +127,7 @@ struct Smem {
   static constexpr int kStats = kV + kStages * kTileBytes;  // (m, sum) of the rows of both tiles, of two items in turn
   static constexpr int kAnswer = kStats + 4 * kTileRows * 8;  // of the launch control, 16 bytes
   static constexpr int kItems = kAnswer + 16;             // two
-  static constexpr int kBar = kItems + ((2 * (int)sizeof(Item) + 7) & ~7);
+  static constexpr int kBar = kItems + ((2 * (int)sizeof(ItemOf<SharedUnit>) + 7) & ~7);
   static constexpr int kBars = 4 + 4 * kStages + 2 + 2 + 2 * kPieces + 4 + 2 + 8 + 4 + 1 + 2;
   static constexpr int kBytes = kBar + kBars * 8 + 16;    // + tensor memory address, abort flag
   static constexpr int kLaunch = kBytes + 1024;           // slack for the 1024-byte alignment
@@ -300,17 +301,22 @@ __device__ __forceinline__ Plan make_plan(const Unit& un) {
   }
   return p;
 }
-// The position of row r of a unit's.
-__device__ __forceinline__ int32_t stands_at(const Unit& un, const Query& q, int32_t r) { return un.position(q, r); }
-__device__ __forceinline__ int32_t stands_at(const Unit& un, const SharedQuery& q, int32_t r) {
-  return un.flat ? un.pos0 : un.position(q, r);
-}
 template <class Q>
 constexpr bool kSharing = std::is_same_v<Q, SharedQuery>;
+struct NoSlots {};
+template <class Q>
+using SlotsOf = std::conditional_t<kSharing<Q>, Slots, NoSlots>;
+template <class Q>
+using UnitOf = std::conditional_t<kSharing<Q>, SharedUnit, Unit>;
+// The position of row r of a unit's.
+__device__ __forceinline__ int32_t stands_at(const Unit& un, const Query& q, int32_t r) { return un.position(q, r); }
+__device__ __forceinline__ int32_t stands_at(const SharedUnit& un, const SharedQuery& q, int32_t r) {
+  return un.flat ? un.pos0 : un.position(q, r);
+}
 
 template <class Q>
-__device__ __forceinline__ Span make_span(const Item& it, const Q& q, int t) {
-  const Unit& un = it.un;
+__device__ __forceinline__ Span make_span(const ItemOf<UnitOf<Q>>& it, const Q& q, int t) {
+  const UnitOf<Q>& un = it.un;
   const Plan& p = it.plan;
   Span s;
   s.from = it.begin;
@@ -350,8 +356,9 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* w, bool whole,
 template <class T, int DP, class Q = Query>
 __global__ void __launch_bounds__(kThreads, 1)
     k_kv_prompt(const __grid_constant__ Maps maps, View kv, Batch bt, Q q, int64_t units, int32_t most_parts,
-                float* scratch, uint32_t q_tokens, bool ranked, Slots slots) {
+                float* scratch, uint32_t q_tokens, bool ranked, SlotsOf<Q> slots) {
   using S = Smem<DP>;
+  using Item = ItemOf<UnitOf<Q>>;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
   uint8_t* sm = raw + (base - smem_addr(raw));
@@ -444,14 +451,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     };
-    Runs<kBlockRows, kTileKeys, kLeadTiles> runs;
+    [[maybe_unused]] Runs<kBlockRows, kTileKeys, kLeadTiles> runs;
     if constexpr (kSharing<Q>) {
       if (block == 0) record_uncovered(bt, q);
       runs.start(kv, bt, q, slots, (int32_t)block, kRunTiles);
     }
     while (ok && block >= 0) {
       Item it;
-      const Unit& un = it.un;
+      const UnitOf<Q>& un = it.un;
       const Plan& plan = it.plan;
       int32_t part = 0;
       if constexpr (kSharing<Q>) {
@@ -692,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t turn = 0;  // bit t: of tile t
     for (; next_item(); end_item()) {
       const Item& it = items[item_turn & 1];
-      const Unit& un = it.un;
+      const UnitOf<Q>& un = it.un;
 #pragma unroll 1
       for (int t = 0; t < 2 && ok; ++t) {
         if (!it.span[t].active()) continue;
@@ -746,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto added = [&](uint32_t n) { return bar_wait(o_done + 16 * t + 8 * (n & 1), (n >> 1) & 1, abort, bt.err); };
     for (; next_item(); end_item()) {
       const Item& it = items[item_turn & 1];
-      const Unit& un = it.un;
+      const UnitOf<Q>& un = it.un;
       if (t * kTileRows >= un.rows) continue;
       const Plan plan = it.plan;
       const Span span = it.span[t];
@@ -771,12 +778,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         // which of the four 32 keys any row of the warp sees; not all rows may see them all
         uint32_t live = 0xf;
         const int32_t from_key = kSharing<Q> ? un.begin : 0;  // own keys begin behind the shared ones
-        if (key0 + kTileKeys - 1 > lo || (q.window && key0 <= hi - q.window && key0 + kTileKeys > q.sinks) || key0 < from_key) {
+        if (key0 + kTileKeys - 1 > lo || (q.window && key0 <= hi - q.window && key0 + kTileKeys > q.sinks) || (kSharing<Q> && key0 < from_key)) {
           live = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int32_t k = key0 + 32 * j;
-            if (k <= hi && k + 31 >= from_key && (!q.window || k + 31 > lo - q.window || k < q.sinks)) live |= 1u << j;
+            if (k <= hi && (!kSharing<Q> || k + 31 >= from_key) && (!q.window || k + 31 > lo - q.window || k < q.sinks)) live |= 1u << j;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const int32_t last = pos[r] - k, first = kSharing<Q> ? from_key - k : q.window ? last - q.window + 1 : 0, sk = min(q.sinks - 1 - k, last);
@@ -891,7 +898,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mine_live = at_row < un.rows;
       const float sum = ml[row].y;
       const bool partial = kSharing<Q> || it.parts > 1;
-      float* slot = kSharing<Q> ? slots.values + (int64_t)it.slot * (kBlockRows * DP) : scratch + it.slot * kSlotFloats<DP>;
+      float* slot;
+      if constexpr (kSharing<Q>) slot = slots.values + (int64_t)it.slot * (kBlockRows * DP);
+      else slot = scratch + it.slot * kSlotFloats<DP>;
       if (partial && half == 0 && mine_live) {
         if constexpr (kSharing<Q>) slots.sums[(int64_t)it.slot * kBlockRows + at_row] = ml[row];
         else *reinterpret_cast<float2*>(slot + kBlockRows * DP + at_row * 2) = ml[row];
@@ -1066,7 +1075,7 @@ cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, c
   cudaError_t e = prepare<T, DP>(kv, q, dtype, &maps, &q_tokens);
   if (e != cudaSuccess) return e;
   e = launch_next(k_kv_prompt<T, DP>, dim3((unsigned)(sp.units * sp.parts)), kThreads, Smem<DP>::kLaunch, st, 1, maps, kv, bt, q,
-                  sp.units, sp.parts, scratch, q_tokens, sp.ranked, Slots{});
+                  sp.units, sp.parts, scratch, q_tokens, sp.ranked, NoSlots{});
   if (e != cudaSuccess) return e;
   *launches += 1;
   if (sp.parts > 1) {

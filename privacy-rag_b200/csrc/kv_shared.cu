@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_shared_rows(View kv, Batch bt, 
   const int32_t quad = lane >> 2, pair = (lane & 3) * 2, page_mask = (1 << kv.page_log) - 1;
 
   for (Piece p; runs.next(kv, bt, q, sl, &p);) {
-    const Unit& un = p.un;
+    const SharedUnit& un = p.un;
     const int32_t s0 = p.from, s1 = p.to;
     const bool flat = un.flat;
     uint32_t qa[NK][4];

@@ -76,10 +76,14 @@ __device__ __forceinline__ void record_uncovered(const Batch& bt, const SharedQu
     flag_error(bt.err, kErrTable);
 }
 
+struct SharedUnit : Unit {
+  bool flat = false;  // every row stands at pos0, behind all of the keys
+};
+
 // Block `block` of ROWS rows of an element, and key head g.  FLAT: shared keys, which every row sees.
 template <int ROWS>
-__device__ __forceinline__ Unit element_unit(const Query& q, const Element& e, int32_t block, int32_t g, bool flat) {
-  Unit un;
+__device__ __forceinline__ SharedUnit element_unit(const Query& q, const Element& e, int32_t block, int32_t g, bool flat) {
+  SharedUnit un;
   un.b = e.row;
   un.g = g;
   const uint32_t all = (uint32_t)e.tokens * q.group, row0 = (uint32_t)block * ROWS;
@@ -109,7 +113,7 @@ struct Slots {
 
 // A worker's part of a unit: its tiles of KEYS keys [from, to).
 struct Piece {
-  Unit un;
+  SharedUnit un;
   int32_t from = 0, to = 0;
   int32_t slot = 0;
 };

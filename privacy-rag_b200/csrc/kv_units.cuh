@@ -14,7 +14,6 @@ struct Unit {
   int32_t head0 = 0;             // and the first row's query head within the group
   int32_t sinks = 0, begin = 0;  // visible keys: [0, sinks) and [begin, begin + n - sinks)
   int32_t n = 0;
-  bool flat = false;             // every row stands at pos0 (attention over shared tokens)
   __device__ __forceinline__ int32_t token(int32_t i) const { return i < sinks ? i : i - sinks + begin; }
   // tokens from the first row's to row r's
   __device__ __forceinline__ int32_t token_of(const Query& q, int32_t r) const {

@@ -14,6 +14,16 @@ BF = torch.bfloat16
 H, G, D = 8, 2, 64
 
 
+@pytest.fixture(scope="module", autouse=True)
+def memory_given_back():
+    """What torch has cached goes back, so that the tests after these allocate as without them (calls on a context's own
+    stream are not ordered after torch's, which an allocation from the driver hides)."""
+    yield
+    if torch.cuda.is_available():
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+
+
 @pytest.fixture
 def ctx(bfv):
     if not torch.cuda.is_available():

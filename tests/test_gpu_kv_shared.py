@@ -13,6 +13,16 @@ pytestmark = pytest.mark.gpu
 BF, FP = torch.bfloat16, torch.float16
 
 
+@pytest.fixture(scope="module", autouse=True)
+def memory_given_back():
+    """What torch has cached goes back, so that the tests after these allocate as without them (calls on a context's own
+    stream are not ordered after torch's, which an allocation from the driver hides)."""
+    yield
+    if torch.cuda.is_available():
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+
+
 @pytest.fixture
 def ctx(bfv):
     if not torch.cuda.is_available():

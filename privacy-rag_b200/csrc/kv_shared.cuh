@@ -44,27 +44,41 @@ __device__ __forceinline__ int32_t ends_up_to(const int32_t* ends, int32_t count
 // 0, or past the last: none.  What is outside its range is recorded, and has no rows.
 __device__ __forceinline__ Element element_at(const View& kv, const Batch& bt, const SharedQuery& q, int32_t index, bool own) {
   Element e;
-  int32_t j = ends_up_to(q.groups + 1, q.count, own ? index : -1);
-  if (index < 0 || index >= (own ? bt.seqs : q.count)) return e;
-  if (!own) j = index;
-  const bool in = j < q.count;
-  const int32_t a = q.groups[in ? j : 0], b = q.groups[in ? j + 1 : 0], shared = in ? q.shared[j] : 0;
-  bool good = in && a >= 0 && b >= a && b <= bt.seqs && (!own || a <= index);
-  const int32_t s = own || !good ? min(index, bt.seqs - 1) : min(a, bt.seqs - 1), t = own || !good ? s + 1 : b;
-  const int32_t first = start_of(bt, s), next = start_of(bt, t);
-  const int32_t most = bt.width << kv.page_log, length = own ? bt.lengths[s] : shared;
-  good = good && first >= 0 && next >= first && next <= q.tokens && shared >= 0 && shared <= most && length >= 0 && length <= most;
+  const bool some = index >= 0 && index < (own ? bt.seqs : q.count);
+  // what needs no other number is asked for first, in one round trip
+  const int32_t at = some ? index : 0;
+  const int32_t* one = own ? bt.starts : q.groups;
+  int32_t x = own && !one ? at : one[at], y = own && !one ? at + 1 : one[at + 1], n = own ? bt.lengths[at] : q.shared[at];
+  int32_t a = x, b = y, shared = n;
+  bool good = true;
+  if (__any_sync(0xffffffffu, some && own)) {
+    const int32_t j = ends_up_to(q.groups + 1, q.count, own ? index : -1);
+    if (own) {
+      good = j < q.count;
+      a = q.groups[good ? j : 0];
+      b = q.groups[good ? j + 1 : 0];
+      shared = q.shared[good ? j : 0];
+    }
+  }
+  if (!some) return e;
+  good = good && a >= 0 && b >= a && b <= bt.seqs && (!own || a <= index);
+  e.row = own ? index : good ? min(a, bt.seqs - 1) : 0;
+  if (!own) {
+    x = start_of(bt, good ? a : 0);
+    y = start_of(bt, good ? b : 0);
+  }
+  const int32_t most = bt.width << kv.page_log;
+  good = good && x >= 0 && y >= x && y <= q.tokens && shared >= 0 && shared <= most && n >= 0 && n <= most;
   // every new token sees all that is shared
-  good = good && !(own && next > first && shared > max(0, length - (next - first) + 1));
+  good = good && !(own && y > x && shared > max(0, n - (y - x) + 1));
   if (!good) {
     flag_error(bt.err, kErrTable);
     return e;
   }
-  e.row = s;
-  e.first = first;
-  e.tokens = next - first;
+  e.first = x;
+  e.tokens = y - x;
   e.begin = own ? shared : 0;
-  e.end = length;
+  e.end = n;
   return e;
 }
 

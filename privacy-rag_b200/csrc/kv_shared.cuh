@@ -273,7 +273,7 @@ struct Runs {
     piece->from = first ? 0 : (int32_t)min((uint64_t)(x - key_x) << sl.coarse, (uint64_t)n);
     piece->to = to == unit_x + of_unit ? n : (int32_t)min((uint64_t)(to - key_x) << sl.coarse, (uint64_t)n);
     piece->slot = worker + first_unit + 2 * number + which;
-    if (piece->slot >= sl.most) {  // sequences that overlap have more units than there are
+    if ((uint32_t)piece->slot >= (uint32_t)sl.most) {  // sequences that overlap have more units than there are
       if (lane == 0) flag_error(bt.err, kErrTable);
       x = end;
       return false;

@@ -262,8 +262,9 @@ PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& given = tensor_of(a[13], "out");
         if (given.sizes() != q.sizes() || given.scalar_type() != c.type() || !there(given, c) || !given.is_contiguous())
           refuse("E_KV_SHAPE: out is dense, of q's shape and the cache's type");
-        if (overlap(given, k) || overlap(given, v) || (overlap(given, q) && !same_place(given, q)))
-          refuse("E_KV_OVERLAP: out is q itself, or overlaps no argument");
+        const bool pages = c.k.defined() && (overlap(given, c.k) || overlap(given, c.v));
+        if (pages || overlap(given, k) || overlap(given, v) || (overlap(given, q) && !same_place(given, q)))
+          refuse("E_KV_OVERLAP: out is q itself, or overlaps neither an argument nor the pages");
       }
     }
     s.uses(c, {a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[13]});

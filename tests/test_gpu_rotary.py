@@ -252,10 +252,13 @@ def test_queries_in_place(bfv, ctx):
     table, lengths = cache.table.cuda(), ints([30, 20])
     want = kv.append_rotary(k, v, rotary, None, table, lengths, q=q)
     assert kv.append_rotary(k, v, rotary, None, table, lengths, q=q, out=q) is q and torch.equal(q, want)
-    both = torch.zeros(4, 2, 64, dtype=BF, device="cuda")
-    for out, kw in ((both[1:3], dict(q=both[:2])), (k, dict(q=both[:2])), (v, dict(q=both[2:]))):
+    # out may be neither over the rows that are read nor over the pages
+    both, wide = torch.zeros(3, 4, 64, dtype=BF, device="cuda"), torch.zeros(2, 8, 64, dtype=BF, device="cuda")
+    over = wide.view(-1)[:512].view(2, 4, 64)
+    for kw in (dict(q=both[:2], out=both[1:]), dict(q=q, out=cache.k.view(-1)[:512].view(2, 4, 64)),
+               dict(q=q, k_new=wide[:, :2], v_new=wide[:, 6:], out=over), dict(q=q, k_new=wide[:, 6:], v_new=wide[:, 2:4], out=over)):
         with pytest.raises(ValueError, match="E_KV_OVERLAP"):
-            kv.append_rotary(k, v, rotary, None, table, lengths, out=out, **kw)
+            kv.append_rotary(**{**dict(k_new=k, v_new=v, rotary=rotary, starts=None, table=table, lengths=lengths), **kw})
 
 
 def test_bad_numbers_on_the_device_are_recorded(bfv, ctx):

@@ -75,14 +75,17 @@ class Rotary:
         check(lib().bfvgpu_rotary_set(ctypes.byref(self._desc), dims, LAYOUTS.index(layout),
                                       (ctypes.c_double * len(radians))(*radians), self.scale), "rotary_set")
         self._address = ctypes.addressof(self._desc)
+        self._rotate = None  # the call, from the first on
 
     def apply(self, x, positions, norm=None, eps: float = 1e-6, inverse: bool = False, out=None, stream: int | None = None):
         """x [tokens][heads][dim] (bfloat16, float16 or float32, dim contiguous, any other strides) rotated at positions
         [tokens] (int32) -> out (may be x); with `norm` [dim] (float32) after x rsqrt(mean(x^2) + eps) norm of each
         head.  inverse: the gradient of a rotation's result -> that of x; not with a norm.  bfvgpu_rotary_device."""
+        if self._rotate is None:
+            self._rotate = _calls().rotate
         h = self.ctx.handle
-        r = _calls().rotate(h.value if h is not None else None, self.ctx.device, self._address, x, positions, norm, eps, inverse,
-                            out, stream)
+        r = self._rotate(h.value if h is not None else None, self.ctx.device, self._address, x, positions, norm, eps, inverse, out,
+                         stream)
         if type(r) is int:
             check(r, "rotary_device")
         return r

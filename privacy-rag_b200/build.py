@@ -68,7 +68,7 @@ def calls_command(torch: str) -> list[str]:
             "-isystem", os.path.join(torch, "include"), "-isystem", os.path.join(torch, "include/torch/csrc/api/include"),
             "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
             "-I", os.path.join(ROOT, "include"), os.path.join(CSRC, "kv_torch.cpp"), "-o", CALLS,
-            "-L", os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+            "-L", os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
             "-L", os.path.dirname(LIB), "-lbfvgpu", "-Wl,-rpath,$ORIGIN"]
 
 

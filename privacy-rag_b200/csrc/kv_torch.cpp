@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -99,6 +100,12 @@ const at::Tensor& rows_of(PyObject* o, const char* name, const Cache& c) {
   if (!there(t, c) || t.dim() != 3 || t.size(2) != c.kv.dim || t.stride(2) != 1)
     refuse(std::string("E_KV_SHAPE: ") + name + " is [tokens][heads][" + std::to_string(c.kv.dim) + "], dim contiguous," + kWhere);
   return t;
+}
+
+// A result or scratch on the cache's device, without the dispatcher's way to it (a result, with its Python object: 1.1 us of
+// the host a call; by at::empty 1.6).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Cache& c) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, (c10::DeviceIndex)c.device), std::nullopt));
 }
 
 // The stream of a call: the given handle, or torch's current one (whose null handle is the legacy stream: the C
@@ -257,7 +264,7 @@ PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const at::Tensor& q = rows_of(a[8], "q", c);
       if (q.size(0) != k.size(0) || q.scalar_type() != k.scalar_type()) refuse("E_KV_SHAPE: q has the tokens and the type of k_new");
       if (a[13] == Py_None) {
-        made = at::empty(q.sizes(), q.options().dtype(c.type()));
+        made = fresh(q.sizes(), c.type(), c);
       } else {
         const at::Tensor& given = tensor_of(a[13], "out");
         if (given.sizes() != q.sizes() || given.scalar_type() != c.type() || !there(given, c) || !given.is_contiguous())
@@ -306,7 +313,7 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Stream s(a[9], c);
     at::Tensor made;
     if (a[8] == Py_None) {
-      made = at::empty(x.sizes(), x.options());
+      made = fresh(x.sizes(), x.scalar_type(), c);
     } else {
       const at::Tensor& given = tensor_of(a[8], "out");
       if (given.sizes() != x.sizes() || given.scalar_type() != x.scalar_type() || !there(given, c) || given.stride(2) != 1)
@@ -385,7 +392,7 @@ PyObject* attend(PyObject* const* a, PyObject* of_starts, PyObject* const* rest)
     const Stream s(rest[7], c);
     at::Tensor made;
     if (rest[6] == Py_None) {
-      made = at::empty(q.sizes(), q.options());
+      made = fresh(q.sizes(), q.scalar_type(), c);
     } else {
       const at::Tensor& given = tensor_of(rest[6], "out");
       if (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !there(given, c) || !given.is_contiguous())
@@ -397,7 +404,7 @@ PyObject* attend(PyObject* const* a, PyObject* of_starts, PyObject* const* rest)
         of_starts ? bfvgpu_kv_prompt_scratch_words(ctx, &c.kv, heads, tokens, t.rows, t.width, window, sinks)
                   : bfvgpu_kv_decode_scratch_words(ctx, &c.kv, heads, t.rows, t.width, window, sinks);
     at::Tensor scratch;
-    if (words) scratch = at::empty({(int64_t)words}, q.options().dtype(at::kLong));
+    if (words) scratch = fresh({(int64_t)words}, at::kLong, c);
     auto* space = words ? static_cast<uint64_t*>(scratch.data_ptr()) : nullptr;
     const int32_t rc =
         of_starts ? bfvgpu_kv_prompt_device(ctx, &c.kv, layer, q.data_ptr(), q.stride(0), q.stride(1), heads, tokens, starts,
@@ -440,7 +447,7 @@ PyObject* attend_shared(PyObject* const* a, PyObject* of_starts, PyObject* const
     const Stream s(rest[7], c);
     at::Tensor made;
     if (rest[6] == Py_None) {
-      made = at::empty(q.sizes(), q.options());
+      made = fresh(q.sizes(), q.scalar_type(), c);
     } else {
       const at::Tensor& given = tensor_of(rest[6], "out");
       if (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !there(given, c) || !given.is_contiguous())
@@ -450,7 +457,7 @@ PyObject* attend_shared(PyObject* const* a, PyObject* of_starts, PyObject* const
     const at::Tensor& out = made.defined() ? made : THPVariable_Unpack(rest[6]);
     const uint64_t words = bfvgpu_kv_shared_scratch_words(ctx, &c.kv, heads, tokens, t.rows, t.width, count);
     at::Tensor scratch;
-    if (words) scratch = at::empty({(int64_t)words}, q.options().dtype(at::kLong));
+    if (words) scratch = fresh({(int64_t)words}, at::kLong, c);
     auto* space = words ? static_cast<uint64_t*>(scratch.data_ptr()) : nullptr;
     const int32_t rc =
         of_starts ? bfvgpu_kv_prompt_shared_device(ctx, &c.kv, layer, q.data_ptr(), q.stride(0), q.stride(1), heads, tokens, starts,

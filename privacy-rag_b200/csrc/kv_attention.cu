@@ -40,13 +40,14 @@ int sm_count(int device) {
 constexpr int64_t kFewRows = 16, kFewRowsWide = 4;
 constexpr double kFewProducts = 8e6;
 constexpr int64_t kStartKeys = 200;
-bool few_rows(const View& kv, const Batch& bt, const Query& q, bool ragged) {
-  const bool wide = kv.dim > 64;
-  if (!ragged || (int64_t)q.tokens * q.group <= (wide ? kFewRowsWide : kFewRows) * bt.seqs) return true;
+bool few_products(const View& kv, const Batch& bt, const Query& q, double few = kFewProducts) {
   int64_t keys = (int64_t)bt.width << kv.page_log;
   if (q.window) keys = std::min<int64_t>(keys, (int64_t)q.window + q.sinks);
   const int64_t blocks = ((int64_t)q.tokens * q.group / 16 + bt.seqs) * kv.heads;
-  return (double)blocks * (double)(keys + kStartKeys) * (wide ? 128 : 64) <= kFewProducts;
+  return (double)blocks * (double)(keys + kStartKeys) * (kv.dim > 64 ? 128 : 64) <= few;
+}
+bool few_rows(const View& kv, const Batch& bt, const Query& q, bool ragged) {
+  return !ragged || (int64_t)q.tokens * q.group <= (kv.dim > 64 ? kFewRowsWide : kFewRows) * bt.seqs || few_products(kv, bt, q);
 }
 
 // The kernel of a call: few rows, or queries whose strides the prompt kernel's loads cannot follow.
@@ -153,6 +154,12 @@ SharedQuery shared_query(const Query& q, const int32_t* groups, const int32_t* s
   return sq;
 }
 
+// Where there is little to read, each sequence by itself, as without sharing: one launch, and no parts to join.  16 query
+// heads on 8 of 128, 1, 4, 8 and 16 sequences on 992 shared tokens: 6.5, 8.0, 10.0 and 14.0 us each by itself, 9.4, 10.1,
+// 10.7 and 10.6 together; 32 and 64 on 200: 8.6 and 15.9, 12.2 and 13.2; 64 with one key head on 992: 10.9 and 21.7.
+constexpr double kEachProducts = 17e6;
+bool takes_each(const View& kv, const Batch& bt, const Query& q) { return few_products(kv, bt, q, kEachProducts); }
+
 void check_groups(const Call& c, uint64_t count) { need(count <= (uint64_t)c.batch.seqs, BFVGPU_E_SHAPE, "E_KV_GROUPS"); }
 
 void attend_shared(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, const int32_t* starts, const int32_t* table,
@@ -175,12 +182,22 @@ void attend_shared(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void*
   c.query.out = static_cast<uint16_t*>(out);
   c.query.scale_log2 = scale_log2;
   const SharedQuery sq = shared_query(c.query, groups, shared, count);
+  int launches = 0;
+  if (takes_each(c.view, c.batch, sq)) {
+    const RowSplit sp = plan_rows(c.view, c.batch, sq, at.device);
+    need(sp.scratch_floats() == 0 || scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
+    need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
+    need(sp.blocks16 * sp.parts <= (int64_t)(kMost / sp.cluster), BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    cuda_need(launch_rows(c.view, c.batch, sq, cache->dtype, sp, reinterpret_cast<float*>(scratch), at.stream, &launches),
+              "kv shared attention");
+    internal_count_launch(launches);
+    return;
+  }
   const SharedPlan sp = plan_shared(c.view, c.batch, sq, sm_count(at.device), prompt_strides(sq));
   need(scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
   need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
   // (rows of slots are numbered in 32 bits)
   need(sp.slots[0] * kSharedRows <= (int64_t)kMost && sp.slots[1] * kSharedTileRows <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
-  int launches = 0;
   cuda_need(launch_shared(c.view, c.batch, sq, cache->dtype, sp, reinterpret_cast<float*>(scratch), at.stream, &launches),
             "kv shared attention");
   internal_count_launch(launches);
@@ -248,6 +265,16 @@ extern "C" uint64_t bfvgpu_kv_shared_scratch_words(const bfvgpu_ctx* ctx, const 
     internal_params(ctx, &device, nullptr);
     const SharedQuery q = shared_query(c.query, nullptr, nullptr, groups);
     // the strides of the queries, which are not known here, may rule out the tensor-core kernel
+    if (takes_each(c.view, c.batch, q)) {
+      std::optional<OnDevice> scope;
+      if (device >= 0) scope.emplace(device);
+      static const int32_t some = 0;
+      for (const int32_t* starts : {static_cast<const int32_t*>(nullptr), &some}) {  // single tokens, or several
+        c.batch.starts = starts;
+        words = std::max(words, (plan_rows(c.view, c.batch, q, device).scratch_floats() + 1) / 2);
+      }
+      return;
+    }
     for (const bool tiles : {false, true})
       words = std::max(words, (plan_shared(c.view, c.batch, q, sm_count(device), tiles).scratch_floats() + 1) / 2);
   });
@@ -262,7 +289,7 @@ extern "C" int32_t bfvgpu_kv_shared_kernel(const bfvgpu_kv* cache, int64_t token
     check_groups(c, groups);
     const SharedQuery q = shared_query(c.query, nullptr, nullptr, groups);
     const SharedPlan p = plan_shared(c.view, c.batch, q, sm_count(-1), prompt_strides(q));
-    kernel = p.tiles[own != 0] ? BFVGPU_KV_TILES : BFVGPU_KV_ROWS;
+    kernel = takes_each(c.view, c.batch, q) ? BFVGPU_KV_EACH : p.tiles[own != 0] ? BFVGPU_KV_TILES : BFVGPU_KV_ROWS;
   });
   return kernel;
 }

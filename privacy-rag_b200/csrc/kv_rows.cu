@@ -33,9 +33,11 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "kv_attention.h"
 #include "kv_row_ops.cuh"
+#include "kv_shared.h"
 #include "kv_units.cuh"
 
 namespace cg = cooperative_groups;
@@ -48,10 +50,11 @@ constexpr int kMaxCluster = 8;
 
 // NK: 16-dim steps of the products, of a ring whose rows have DP dims (256 sequences of 2048 tokens of 72 and 96 dims:
 // 157 and 155 us with the eight steps of 128, 140 both with six).
-// PAIR: as in row_stage.
-template <class T, int DP, bool PAIR, int NK>
+// PAIR: as in row_stage.  Q: SharedQuery where little is shared: each sequence for itself, its shared keys through the
+// table's row of its group's first.
+template <class T, int DP, bool PAIR, int NK, class Q = Query>
 __global__ void __launch_bounds__(kThreads)
-    k_kv_rows(View kv, Batch bt, Query q, int32_t cluster, int32_t parts, float* scratch) {
+    k_kv_rows(View kv, Batch bt, Q q, int32_t cluster, int32_t parts, float* scratch) {
   using R = Ring<DP>;
   extern __shared__ __align__(1024) uint8_t ring[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -86,10 +89,21 @@ __global__ void __launch_bounds__(kThreads)
 
   // lane l looks up the page of key l % 16 of a stage, one stage ahead of its copies
   const int32_t* row_of_table = bt.table + (int64_t)un.b * bt.width;
+  constexpr bool kSharing = std::is_same_v<Q, SharedQuery>;
+  Prefix shared;
+  if constexpr (kSharing) {
+    if (blockIdx.x == 0 && warp == 0) record_uncovered(bt, q);
+    if (un.rows > 0) shared = prefix_of(kv, bt, q, un.b, un.pos0);
+  }
+  const int32_t* shared_row = bt.table + (int64_t)shared.row * bt.width;
   const int32_t page_mask = (1 << kv.page_log) - 1;
   const int64_t head_at = un.g * kv.head_stride;
   auto entry_of = [&](int32_t s) {
     const int32_t i = s * kKeys + (lane & 15);
+    if constexpr (kSharing) {
+      const int32_t token = un.token(i);
+      return s < s1 && i < un.n ? __ldg((token < shared.tokens ? shared_row : row_of_table) + (token >> kv.page_log)) : 0;
+    }
     return s < s1 && i < un.n ? __ldg(row_of_table + (un.token(i) >> kv.page_log)) : 0;
   };
   int32_t entry = entry_of(s0 + warp);
@@ -298,11 +312,11 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kDevices = 64;
 
 // The shared-memory limit is an attribute of the function on a device.
-template <class T, int DP, bool PAIR, int NK>
+template <class T, int DP, bool PAIR, int NK, class Q>
 cudaError_t allow_ring(int device) {
   static std::atomic<uint64_t> allowed{0};
   if (device < kDevices && (allowed.load() >> device & 1)) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(k_kv_rows<T, DP, PAIR, NK>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DP>::kBytes);
+  const cudaError_t e = cudaFuncSetAttribute(k_kv_rows<T, DP, PAIR, NK, Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DP>::kBytes);
   if (e == cudaSuccess && device < kDevices) allowed.fetch_or(uint64_t(1) << device);
   return e;
 }
@@ -320,20 +334,20 @@ void configure(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* at, int64_t blocks,
   cfg->numAttrs = 1;
 }
 
-template <class T, int DP, bool PAIR, int NK>
-cudaError_t launch(const View& kv, const Batch& bt, const Query& q, const RowSplit& sp, float* scratch, cudaStream_t st,
+template <class T, int DP, bool PAIR, int NK, class Q>
+cudaError_t launch(const View& kv, const Batch& bt, const Q& q, const RowSplit& sp, float* scratch, cudaStream_t st,
                    int* launches) {
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = allow_ring<T, DP, PAIR, NK>(device);
+  if (e == cudaSuccess) e = allow_ring<T, DP, PAIR, NK, Q>(device);
   if (e != cudaSuccess) return e;
-  e = launch_next(k_kv_rows<T, DP, PAIR, NK>, dim3((unsigned)(sp.blocks16 * sp.parts * sp.cluster)), kThreads, Ring<DP>::kBytes, st,
+  e = launch_next(k_kv_rows<T, DP, PAIR, NK, Q>, dim3((unsigned)(sp.blocks16 * sp.parts * sp.cluster)), kThreads, Ring<DP>::kBytes, st,
                   sp.cluster, kv, bt, q, sp.cluster, sp.parts, scratch);
   if (e != cudaSuccess) return e;
   *launches += 1;
   if (sp.parts > 1) {
-    e = launch_next(k_kv_rows_join<T, DP>, dim3((unsigned)(sp.blocks16 * (kRows / kWarps))), kThreads, 0, st, 1, kv, bt, q, sp.parts,
-                    scratch);
+    e = launch_next(k_kv_rows_join<T, DP>, dim3((unsigned)(sp.blocks16 * (kRows / kWarps))), kThreads, 0, st, 1, kv, bt,
+                    static_cast<const Query&>(q), sp.parts, scratch);
     if (e != cudaSuccess) return e;
     *launches += 1;
   }
@@ -353,7 +367,7 @@ int64_t resident_clusters(int device, int log) {
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
     configure<DP>(&cfg, &at, 1 << log, 1 << log, nullptr);
-    if (allow_ring<Bf16, DP, true, DP / 16>(device) != cudaSuccess ||
+    if (allow_ring<Bf16, DP, true, DP / 16, Query>(device) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&n, k_kv_rows<Bf16, DP, true, DP / 16>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = given[log];
@@ -363,18 +377,18 @@ int64_t resident_clusters(int device, int log) {
   return n;
 }
 
-template <class T>
-cudaError_t launch_typed(const View& kv, const Batch& bt, const Query& q, const RowSplit& sp, float* scratch,
+template <class T, class Q>
+cudaError_t launch_typed(const View& kv, const Batch& bt, const Q& q, const RowSplit& sp, float* scratch,
                          cudaStream_t st, int* launches) {
   const bool pair = !bt.starts && q.group <= 8;
   if (sp.dim_padded == 64)
-    return pair ? launch<T, 64, true, 4>(kv, bt, q, sp, scratch, st, launches)
-                : launch<T, 64, false, 4>(kv, bt, q, sp, scratch, st, launches);
+    return pair ? launch<T, 64, true, 4, Q>(kv, bt, q, sp, scratch, st, launches)
+                : launch<T, 64, false, 4, Q>(kv, bt, q, sp, scratch, st, launches);
   if (kv.dim <= 96)
-    return pair ? launch<T, 128, true, 6>(kv, bt, q, sp, scratch, st, launches)
-                : launch<T, 128, false, 6>(kv, bt, q, sp, scratch, st, launches);
-  return pair ? launch<T, 128, true, 8>(kv, bt, q, sp, scratch, st, launches)
-              : launch<T, 128, false, 8>(kv, bt, q, sp, scratch, st, launches);
+    return pair ? launch<T, 128, true, 6, Q>(kv, bt, q, sp, scratch, st, launches)
+                : launch<T, 128, false, 6, Q>(kv, bt, q, sp, scratch, st, launches);
+  return pair ? launch<T, 128, true, 8, Q>(kv, bt, q, sp, scratch, st, launches)
+              : launch<T, 128, false, 8, Q>(kv, bt, q, sp, scratch, st, launches);
 }
 
 }  // namespace
@@ -421,6 +435,11 @@ RowSplit plan_rows(const View& kv, const Batch& bt, const Query& q, int device) 
 }
 
 cudaError_t launch_rows(const View& kv, const Batch& bt, const Query& q, int dtype, const RowSplit& sp, float* scratch,
+                        cudaStream_t st, int* launches) {
+  return dtype == 0 ? launch_typed<Bf16>(kv, bt, q, sp, scratch, st, launches)
+                    : launch_typed<Fp16>(kv, bt, q, sp, scratch, st, launches);
+}
+cudaError_t launch_rows(const View& kv, const Batch& bt, const SharedQuery& q, int dtype, const RowSplit& sp, float* scratch,
                         cudaStream_t st, int* launches) {
   return dtype == 0 ? launch_typed<Bf16>(kv, bt, q, sp, scratch, st, launches)
                     : launch_typed<Fp16>(kv, bt, q, sp, scratch, st, launches);

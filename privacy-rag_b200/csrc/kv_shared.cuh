@@ -113,6 +113,24 @@ __device__ __forceinline__ SharedUnit element_unit(const Query& q, const Element
   return un;
 }
 
+// What sequence s shares (0: nothing, or numbers outside their range, which are recorded), and the row of the table
+// that it is read through.  first: the position of the sequence's first new token, or a later one.  Whole warps, s the same.
+struct Prefix {
+  int32_t tokens = 0, row = 0;
+};
+__device__ __forceinline__ Prefix prefix_of(const View& kv, const Batch& bt, const SharedQuery& q, int32_t s, int32_t first) {
+  Prefix p;
+  const int32_t j = ends_up_to(q.groups + 1, q.count, s), at = j < q.count ? j : 0;
+  const int32_t a = q.groups[at], b = q.groups[at + 1], n = q.shared[at];
+  if (j < q.count && a >= 0 && a <= s && b <= bt.seqs && n >= 0 && n <= bt.width << kv.page_log && n <= max(0, first + 1)) {
+    p.tokens = n;
+    p.row = a;
+  } else {
+    flag_error(bt.err, kErrTable);
+  }
+  return p;
+}
+
 // What all workers leave.  A unit's parts lie side by side in slots: the slot of worker w and unit u (counted through the
 // row of all units) is w + u, which rises from part to part in the order of the row.
 struct Slots {

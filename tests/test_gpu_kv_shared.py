@@ -96,7 +96,7 @@ def run(bfv, ctx, *a, kernels=None, scale=None, **kw):
     case = Shared(bfv, ctx, *a, **kw)
     taken = case.kv.shared_kernels(case.q, case.table, len(case.shared))
     assert kernels is None or taken == kernels
-    two_terms = taken == ("rows", "rows")
+    two_terms = "tiles" not in taken
     call = {} if scale is None else dict(scale=scale)
     got = case.run(**call)
     assert ctx.check() == 0
@@ -130,16 +130,32 @@ MORE = [
 name = lambda c: "-".join(str(x).replace("torch.", "") for x in c[1:]) + "-%d" % len(c[0])  # noqa: E731
 
 
+def width_for(groups, g, r, dim, page):
+    """A table so wide that what it can name is worth sharing, and no wider (the choice goes by it)."""
+    tokens, seqs = sum(n for _, s in groups for _, n in s), sum(len(s) for _, s in groups)
+    keys = 17e6 / ((tokens * r // 16 + seqs) * g * (64 if dim <= 64 else 128)) - 200
+    return max(2, int(keys) // page + 1, max(-(-(p + own) // page) for p, s in groups for own, _ in s) + 1)
+
+
+@pytest.mark.parametrize("each", [True, False])
 @pytest.mark.parametrize("case", DECODE, ids=name)
-def test_decode_shared(bfv, ctx, case):
+def test_decode_shared(bfv, ctx, case, each):
     groups, g, r, dim, page, dtype, layout = case
-    run(bfv, ctx, groups, g, r, dim, page, dtype, layout)
+    width = None if each else width_for(groups, g, r, dim, page)
+    c = run(bfv, ctx, groups, g, r, dim, page, dtype, layout, width=width)
+    kernels = c.kv.shared_kernels(c.q, c.table, len(groups))
+    assert each or "each" not in kernels
+    assert not each or kernels == ("each", "each") or sum(n for n, _ in c.lens) > 2000
 
 
+@pytest.mark.parametrize("each", [True, False])
 @pytest.mark.parametrize("case", MORE, ids=name)
-def test_prompt_shared(bfv, ctx, case):
+def test_prompt_shared(bfv, ctx, case, each):
     groups, g, r, dim, page, dtype, layout = case
-    run(bfv, ctx, groups, g, r, dim, page, dtype, layout)
+    width = None if each else width_for(groups, g, r, dim, page)
+    c = run(bfv, ctx, groups, g, r, dim, page, dtype, layout, width=width)
+    kernels = c.kv.shared_kernels(c.q, c.table, len(groups))
+    assert each or "each" not in kernels
 
 
 def repeated(own, new, count):
@@ -169,7 +185,7 @@ def test_tiles(bfv, ctx, case):
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
-@pytest.mark.parametrize("wide", [None, 5000])
+@pytest.mark.parametrize("wide", [None, 180, 9000])
 def test_large_scores(bfv, ctx, dtype, wide):
     """Scores to about +-200, whose maxima lie in one part or the other."""
     run(bfv, ctx, [(300, one(*range(40))), (20, one(300, 2))], 1, 3, 128, 16, dtype, spread=40.0, width=wide)
@@ -198,10 +214,9 @@ def test_the_same_as_without_sharing(bfv, ctx):
 def test_numbers_on_the_device_outside_their_range(bfv, ctx):
     """Recorded; nothing is read or written outside (the shapes here keep every wrong number within the tensors' ranges or
     refused by the kernel's checks), and the next call is as before."""
-    for wide in (None, 4000):  # both kernels
+    for wide in (None, 300, 4000):  # all kernels
         case = Shared(bfv, ctx, [(100, one(*[3] * 20)), (40, one(1, 2, 3, 4))], 2, 2, 64, 16, BF, width=wide)
-        if wide:
-            assert case.kv.shared_kernels(case.q, case.table, 2)[0] == "tiles"
+        assert case.kv.shared_kernels(case.q, case.table, 2)[0] == {None: "each", 300: "rows", 4000: "tiles"}[wide]
         want = case.run()
         assert ctx.check() == 0
         good = {n: getattr(case, n) for n in ("groups", "shared", "lengths", "table")}
@@ -232,7 +247,7 @@ def test_numbers_on_the_device_outside_their_range(bfv, ctx):
 
 
 def test_starts_outside_their_range(bfv, ctx):
-    for wide in (None, 4000):
+    for wide in (None, 300, 4000):
         case = Shared(bfv, ctx, [(100, [(30, 20), (40, 31)]), (0, [(50, 50), (9, 1)])], 2, 2, 64, 16, BF, width=wide)
         want, starts = case.run(), case.starts
         assert ctx.check() == 0
@@ -249,7 +264,7 @@ def test_starts_outside_their_range(bfv, ctx):
 
 def test_values_that_are_not_finite(bfv, ctx):
     """An own value that is not finite reaches its own sequence alone; a shared one all of its group."""
-    for wide in (None, 4000):
+    for wide in (None, 300, 4000):
         case = Shared(bfv, ctx, [(64, one(*[5] * 24)), (32, one(*[5] * 24))], 1, 2, 64, 16, BF, width=wide)
         want = case.run()
         pages, rows = case.cache.where(7)
@@ -264,7 +279,7 @@ def test_values_that_are_not_finite(bfv, ctx):
 
 def test_graphs_and_streams(bfv, ctx):
     """A captured step replays with other lengths, groups and tables; a named stream keeps what it uses."""
-    for wide in (None, 4000):
+    for wide in (None, 300, 4000):
         case = Shared(bfv, ctx, [(100, one(*[9] * 30)), (48, one(*[9] * 2))], 2, 2, 64, 16, BF, width=wide)
         case.run()
         side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
@@ -298,7 +313,7 @@ def test_strides_that_rule_out_the_tensor_cores(bfv, ctx):
     case = Shared(bfv, ctx, [(100, one(*[3] * 50))], 2, 2, 64, 16, BF, width=4000)
     assert case.kv.shared_kernels(case.q, case.table, 1)[0] == "tiles"
     case.q, case.cpu_q = case.q[:1].expand(case.q.shape), case.cpu_q[:1].expand(case.cpu_q.shape)
-    assert case.kv.shared_kernels(case.q, case.table, 1) == ("rows", "rows")
+    assert case.kv.shared_kernels(case.q, case.table, 1) == ("rows", "rows")  # 50 x 64000 keys
     got = case.run()
     assert ctx.check() == 0
     check(got, *case.want())

@@ -148,15 +148,15 @@ def test_the_scratch_of_shared_attention_holds_what_either_kernel_leaves(bfv):
     host = bfv.Context(4096, bfv.find_primes(4096, [36, 36, 37]), 2, 1, 65537, device=-1)
     for heads, group, dim, tokens, seqs, count in ((4, 8, 128, 128, 128, 1), (1, 2, 64, 300, 2, 2), (8, 2, 72, 4000, 16, 3)):
         cache = KvDesc(0x10000, 0x20000, 0, 1, 4, heads, 16, dim, 0, heads * 16 * dim, 16 * dim, dim)
-        words = L.bfvgpu_kv_shared_scratch_words(host.handle, ctypes.byref(cache), heads * group, tokens, seqs, 100, count)
-        kernels = [L.bfvgpu_kv_shared_kernel(ctypes.byref(cache), heads * group * dim, dim, heads * group, tokens, seqs, 100, count,
+        words = L.bfvgpu_kv_shared_scratch_words(host.handle, ctypes.byref(cache), heads * group, tokens, seqs, 4000, count)
+        kernels = [L.bfvgpu_kv_shared_kernel(ctypes.byref(cache), heads * group * dim, dim, heads * group, tokens, seqs, 4000, count,
                                              own) for own in (0, 1)]
         assert kernels[0] == 1
         padded = 64 if dim <= 64 else 128
         # a slot of 256 rows for each of 148 blocks and each unit over shared keys
         slots = 148 + (tokens * group // 256 + count) * heads
         assert 2 * words >= slots * 256 * (padded + 2)
-        assert L.bfvgpu_kv_shared_scratch_words(host.handle, ctypes.byref(cache), heads * group, tokens, seqs, 100, seqs + 1) == 0
+        assert L.bfvgpu_kv_shared_scratch_words(host.handle, ctypes.byref(cache), heads * group, tokens, seqs, 4000, seqs + 1) == 0
 
 
 def test_shared_attention_refuses_on_the_host(bfv):
@@ -197,8 +197,9 @@ def test_the_choice_of_the_shared_kernels(bfv):
         return [L.bfvgpu_kv_shared_kernel(ctypes.byref(cache), heads * group * dim, dim if head_stride is None else head_stride,
                                           heads * group, tokens, seqs, keys // 16, count, own) for own in (0, 1)]
 
-    rows, tiles = 0, 1
+    rows, tiles, each = 0, 1, 2
+    assert kernels(1, 1, 1, 1040) == [each, each] and kernels(16, 16, 1, 208) == [each, each]
     assert kernels(16, 16, 1, 1040) == [rows, rows] and kernels(16, 16, 1, 8192) == [tiles, rows]
     assert kernels(64, 64, 4, 4608) == [rows, rows] and kernels(64, 64, 1, 4608) == [tiles, rows]
-    assert kernels(500, 16, 1, 4176) == [tiles, tiles] and kernels(40, 2, 1, 144) == [rows, rows]
+    assert kernels(500, 16, 1, 4176) == [tiles, tiles] and kernels(40, 2, 1, 144) == [each, each]
     assert kernels(500, 16, 1, 4176, head_stride=0) == [rows, rows]

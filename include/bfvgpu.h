@@ -459,8 +459,8 @@ int32_t bfvgpu_token_release(bfvgpu_token *t);
 
 /* ---- Paged key-value cache and its attention ----------------------------------------------
  * The cache and the attention between the q/k/v call and the o call of a decoder layer, for the
- * party that holds the decrypted projections (head norms and positions, where the model has them,
- * are that party's own).  No counterpart in the reference, whose attention is a two-party
+ * party that holds the decrypted projections; norms of the heads and rotary positions, where the model has
+ * them, on the way into the cache.  No counterpart in the reference, whose attention is a two-party
  * integer protocol.  All pointers are device memory; stream as for the other device entry points
  * (NULL: the context stream; cudaStreamLegacy names the default stream).  Values on the device
  * (tables, lengths, starts, page lists) cannot be checked by the host: the kernels check every

@@ -2,9 +2,9 @@
 
 The protocol runs a decoder layer's linear calls; between the q/k/v call and the o call the party
 that holds the decrypted projections (a client that computes the non-linear steps itself, or a
-plaintext check of the protocol) needs a cache and its attention (head norms and positions, where
-the model has them, are its own).  The reference has neither: its
-attention is a two-party integer protocol.
+plaintext check of the protocol) needs a cache and its attention; norms of the heads and rotary
+positions, where the model has them, are applied on the way into the cache (``Rotary``).  The
+reference has neither: its attention is a two-party integer protocol.
 
 * ``PagedKv``: the pages and the device calls on them (bfvgpu_kv_* of include/bfvgpu.h);
 * ``KvCache``: the book-keeping of a set of sequences over them: pages handed out, shared by forks,

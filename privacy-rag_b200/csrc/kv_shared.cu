@@ -9,16 +9,17 @@
 // each warp takes an equal run of them, finds its first unit by a scan over the groups and sequences, and leaves m, l and o
 // of the units that it had a part of in slots of its own; a second kernel joins them in order, so that results do not
 // depend on timing.  Groups of many rows go to the tensor-core kernel (kv_prompt.cu), whose blocks cut their key tiles in
-// the same way; own keys of single tokens run here beside it.
+// the same way; own keys of single tokens run here beside it.  Where there is little to read, the kernel of single tokens
+// (kv_rows.cu) takes each sequence by itself.
 //
 // Bound by latency where there is little (16 answers on 992 tokens: first keys 4 us after the start, the longest run 8, the
-// join 3.5 behind it), by what arrives from L2 and HBM where there is much: a unit's keys come once for 16 rows, 58 GB a
-// second and processor in 64 sequences on four times up to 4096 tokens (main kernel 27 of 39 us, of which 17 are the floor).
+// join 2.5 behind it), by what arrives from L2 and HBM where there is much: a unit's keys come once for 16 rows, 150 MB in
+// 26 of the 39 us of 64 sequences on four times up to 4096 tokens, whose floor is 17.
 // Four warps that share each stage for 64 rows read less and took longer (71 us): two teams a processor go through the
 // many short own units one by one, where eight warps have eight at once.
-// Measured: 16 answers 11.7 us (decode without sharing of 16 x 1024 keys: 17 to 20), 64 sequences 39, 128 on 65536 tokens 167
-// (tensor-core kernel 125, own keys 33), 16 questions of up to 64 tokens on 4096 43, six chunks of up to 1024 on two
-// documents of up to 8192 tokens 111.
+// Measured, and the same without sharing (bfvgpu_kv_decode_device, _prompt_device): 16 answers 10.6 us and 13.0, 64 sequences
+// 38.7 and 124, 128 on 65536 tokens 171 and 2067 (tensor-core kernel 125, own keys 33), 16 questions of up to 64 tokens on
+// 4096 43 and 57, six chunks of up to 1024 on two documents of up to 8192 tokens 111.5 and 116.5.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

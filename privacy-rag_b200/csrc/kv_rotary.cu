@@ -307,7 +307,6 @@ __global__ void __launch_bounds__(kThreads, kPerSm<W>)
     }
   };
   auto rotate = [&](uint64_t (&x)[W], bool normed) {
-    float f = 1.f;
     if (normed) {
       uint64_t sums = 0;
 #pragma unroll
@@ -318,7 +317,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm<W>)
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1)
         if (d < 1 << wk.lanes_log) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      f = rsqrtf(sum * wk.inverse_dim + wk.eps);
+      const float f = rsqrtf(sum * wk.inverse_dim + wk.eps);
+#pragma unroll
+      for (int e = 0; e < W; ++e) x[e] = mul2(x[e], two(f, f));
     }
     if constexpr (HALF) {
       if (turns) {
@@ -347,10 +348,6 @@ __global__ void __launch_bounds__(kThreads, kPerSm<W>)
           for (int j = h * W / 2; j < (h + 1) * W / 2; ++j) x[j] = mul2(x[j], keep[j]);
         }
       }
-    }
-    if (normed) {
-#pragma unroll
-      for (int e = 0; e < W; ++e) x[e] = mul2(x[e], two(f, f));
     }
   };
   using Out = Run<DST, W>;

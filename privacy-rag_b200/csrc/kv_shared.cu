@@ -320,7 +320,7 @@ SharedPlan plan_shared(const View& kv, const Batch& bt, const SharedQuery& q, in
     if (!p.slots[kernel]) continue;
     // the work in tiles is below the number of units times the tiles of the longest sequence, and has to fit 32 bits
     const int64_t tiles_of_all = (((int64_t)bt.width << kv.page_log) / (kernel ? 128 : 16) + 2) * 2;
-    while (((tiles_of_all >> p.coarse[kernel]) + 2) * p.slots[kernel] >= int64_t(1) << 31) ++p.coarse[kernel];
+    while (((tiles_of_all >> p.coarse[kernel]) + 8) * p.slots[kernel] >= int64_t(1) << 31) ++p.coarse[kernel];
     p.slots[kernel] += p.workers[kernel];
   }
   return p;

@@ -181,6 +181,8 @@ struct Runs {
   __device__ __forceinline__ static int32_t blocks_of(const SharedQuery& q, const Element& e) {
     return e.end > e.begin ? (int32_t)(((uint32_t)e.tokens * q.group + ROWS - 1) / ROWS) : 0;
   }
+  // units of a pair, or of a block by itself
+  __device__ __forceinline__ static int32_t units_of(bool own, int32_t blocks) { return own && blocks > 1 ? 2 : 1; }
   __device__ __forceinline__ void load(const View& kv, const Batch& bt, const SharedQuery& q, const Slots& sl) {
     const int32_t e = e0 + (threadIdx.x & 31), groups = sl.has[0] ? q.count : 0;
     const bool own = e >= groups;
@@ -202,7 +204,7 @@ struct Runs {
     e0 += 32;
     load(kv, bt, q, sl);
     upto = (uint32_t)(pairs * kv.heads) * work;
-    units_upto = 2 * pairs * kv.heads;
+    units_upto = pairs * kv.heads * units_of(e0 + lane >= (sl.has[0] ? q.count : 0), blocks_of(q, el));
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const uint32_t a = __shfl_up_sync(0xffffffffu, upto, d);
@@ -264,12 +266,12 @@ struct Runs {
     const uint32_t each = __shfl_sync(0xffffffffu, work, at);
     const int32_t units = __shfl_sync(0xffffffffu, pairs, at) * kv.heads;
     const uint32_t into = x - (__shfl_sync(0xffffffffu, upto, at) - (uint32_t)units * each);
-    const int32_t first_unit = __shfl_sync(0xffffffffu, units_upto, at) - 2 * units;
     const int32_t number = (int32_t)(into / each), pair = number / kv.heads, g = number - pair * kv.heads;
     uint32_t off = into - (uint32_t)number * each;
     const bool own = e0 + at >= (sl.has[0] ? q.count : 0);
     // of a pair the later block first
-    const int32_t blocks = blocks_of(q, e);
+    const int32_t blocks = blocks_of(q, e), side = units_of(own, blocks);
+    const int32_t first_unit = __shfl_sync(0xffffffffu, units_upto, at) - side * units;
     int32_t block = own ? blocks - 1 - pair : pair;
     int32_t n = tiles_of(q, e, own, block), which = 0;
     uint32_t of_unit = own && blocks > 1 && block != pair ? min(counted(sl, n), each) : each;
@@ -290,7 +292,7 @@ struct Runs {
     // all of a unit's tiles by the end of its work
     piece->from = first ? 0 : (int32_t)min((uint64_t)(x - key_x) << sl.coarse, (uint64_t)n);
     piece->to = to == unit_x + of_unit ? n : (int32_t)min((uint64_t)(to - key_x) << sl.coarse, (uint64_t)n);
-    piece->slot = worker + first_unit + 2 * number + which;
+    piece->slot = worker + first_unit + side * number + which;
     if ((uint32_t)piece->slot >= (uint32_t)sl.most) {  // sequences that overlap have more units than there are
       if (lane == 0) flag_error(bt.err, kErrTable);
       x = end;
@@ -312,7 +314,7 @@ struct Runs {
 };
 // Bounds on the host's side: of the units' numbers, and of the work in tiles.
 inline int64_t most_units(const View& kv, const Query& q, int64_t elements, int rows) {
-  return 2 * ((int64_t)q.tokens * q.group / rows + elements) * kv.heads;
+  return ((int64_t)q.tokens * q.group / rows + 2 * elements) * kv.heads;  // (an odd block of an element has a pair's two numbers)
 }
 
 }  // namespace kv

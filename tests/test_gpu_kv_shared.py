@@ -174,6 +174,8 @@ TILES = [
     ([(129, repeated(150, 130, 5)), (4000, repeated(129, 129, 2))], 1, 4, 128, 64, BF, "hnd", ("tiles", "tiles")),
     ([(64, [(900, 900)]), (1, repeated(300, 256, 3))], 4, 1, 128, 16, FP, "nhd", ("tiles", "tiles")),
     ([(0, [(500, 500)]), (0, [(0, 0), (300, 300)])], 1, 2, 64, 256, BF, "hnd", ("tiles", "tiles")),  # nothing shared
+    ([(260, one(*range(1, 80)))], 2, 4, 8, 16, BF, "hnd", ("tiles", "rows")),
+    ([(140, [(90, 77), (33, 33)])], 2, 3, 104, 128, FP, "gaps", ("tiles", "tiles")),
 ]
 
 
@@ -339,3 +341,55 @@ def test_refusals(bfv, ctx):
     ctx.close()
     with pytest.raises(bfv.BfvGpuInvalidArgument, match="E_BFVGPU_ARGUMENT"):
         case.run()
+
+
+def test_many_sequences(bfv, ctx):
+    """1500 sequences in 400 groups: against decode over whole tables."""
+    gen = torch.Generator().manual_seed(5)
+    heads, dim, page, seqs = 2, 64, 16, 1500
+    cuts = sorted(torch.randperm(seqs - 1, generator=gen)[:399].add(1).tolist())
+    groups = [0] + cuts + [seqs]
+    shared = torch.randint(0, 4, (400,), generator=gen) * page
+    of = torch.repeat_interleave(shared, torch.tensor(groups).diff())
+    lengths = of + torch.randint(1, 40, (seqs,), generator=gen)
+    pages = int((-(-lengths // page)).sum())
+    table = torch.full((seqs, 8), -1, dtype=torch.int32)
+    at = 0
+    for s in range(seqs):
+        first = groups[max(i for i, g in enumerate(groups) if g <= s)] if of[s] else s
+        k, n = int(of[s]) // page, -(-int(lengths[s]) // page)
+        if first != s:
+            table[s, :k] = table[first, :k]
+        else:
+            k = 0
+        table[s, k:n] = torch.arange(at, at + n - k)
+        at += n - k
+    k, v = (randn(gen, pages, heads, page, dim, dtype=BF).cuda() for _ in range(2))
+    kv, q = bfv.PagedKv(ctx, k, v), randn(gen, seqs, 4, dim, dtype=BF).cuda()
+    for wide in (8, 2000):
+        t = torch.nn.functional.pad(table, (0, wide - 8), value=-1).cuda()
+        got = kv.decode_shared(q, t, lengths.int().cuda(), ints(groups), shared.int().cuda())
+        want = kv.decode(q, t, lengths.int().cuda())
+        assert ctx.check() == 0
+        # both within the bound of one result: at most (2^-8 + 2^-12) of the values, which are below 6
+        assert (got.double() - want.double()).abs().max() <= 6 * 2 * (2.0 ** -8 + 2.0 ** -12)
+
+
+def test_far_pages(bfv, ctx):
+    """Pages whose elements lie past 2^31: keys appended with a rotation, and read as shared and as own ones."""
+    dim, page, far = 64, 16, (1 << 31) + 4096
+    whole = [torch.empty(far + 4 * page * dim, dtype=BF, device="cuda") for _ in range(2)]
+    k, v = (w.as_strided((2, 1, page, dim), (far, page * dim, dim, 1)) for w in whole)
+    kv, rotary = bfv.PagedKv(ctx, k, v), bfv.Rotary(ctx, dim)
+    gen = torch.Generator().manual_seed(6)
+    x = randn(gen, 24, 3, dim, dtype=BF).cuda()
+    table, lengths = ints([[1, 0]]), ints([24])
+    q = kv.append_rotary(x[:, 1:2], x[:, 2:], rotary, ints([0, 24]), table, lengths, q=x[:, :1])
+    want = rotary.apply(x[:, 1:2], ints(list(range(24))))
+    assert torch.equal(k[1, 0], want[:16, 0]) and torch.equal(k[0, 0, :8], want[16:, 0]) and torch.equal(v[1, 0], x[:16, 2])
+    o, bound = R.attention(q[23:].cpu(), want.cpu(), x[:, 2:].cpu(), 24, 0, 0, dim ** -0.5, two_terms=False)
+    for wide in (2, 5000, 20000):
+        t = torch.nn.functional.pad(table, (0, wide - 2), value=-1)
+        for shared in (0, 16, 20, 24):
+            check(kv.decode_shared(q[23:], t, lengths, ints([0, 1]), ints([shared])), o, bound)
+    assert ctx.check() == 0

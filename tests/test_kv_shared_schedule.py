@@ -36,8 +36,9 @@ def runs(rows_of_unit, keys, lead, elements, group, heads, workers, least, coars
         pairs = (blocks + 1) // 2 if paired else blocks
         work = counted(tiles_of(e, blocks - 1)) + (counted(tiles_of(e, 0)) if paired else 0) if blocks else 0
         upto += pairs * heads * work
-        units_upto += 2 * pairs * heads
-        row.append((number, e, blocks, pairs, work, upto, units_upto))
+        side = 2 if paired else 1
+        units_upto += side * pairs * heads
+        row.append((number, e, blocks, pairs, work, upto, units_upto, side))
     length = max(max(1, least >> coarse), (upto + workers - 1) // workers)
     assert upto < 1 << 31
     covered, parts, slots = {}, {}, set()
@@ -45,7 +46,7 @@ def runs(rows_of_unit, keys, lead, elements, group, heads, workers, least, coars
         x = min(w * length, upto)
         end = min(x + length, upto)
         while x < end:
-            number, e, blocks, pairs, each, last, units_last = next(i for i in row if x < i[5])
+            number, e, blocks, pairs, each, last, units_last, side = next(i for i in row if x < i[5])
             units = pairs * heads
             into = x - (last - units * each)
             at, off = divmod(into, each)
@@ -65,7 +66,7 @@ def runs(rows_of_unit, keys, lead, elements, group, heads, workers, least, coars
             first = x <= key_x
             a = 0 if first else min((x - key_x) << coarse, n)
             b = n if to == unit_x + of_unit else min((to - key_x) << coarse, n)
-            slot = w + units_last - 2 * units + 2 * at + which
+            slot = w + units_last - side * units + side * at + which
             assert slot not in slots
             slots.add(slot)
             covered.setdefault((number, block, g), []).append((a, b, slot))
@@ -106,4 +107,4 @@ def test_runs(seed):
         assert not slots or max(slots) < workers + units
         # the host's bound on the units' numbers
         total = sum(e[1] for e in elements)
-        assert units <= 2 * (total * group // rows_of_unit + len(elements)) * heads
+        assert units <= (total * group // rows_of_unit + 2 * len(elements)) * heads

@@ -159,13 +159,13 @@ class PagedKv:
 
     def shared_kernels(self, q, table, count: int) -> tuple[str, str]:
         """Which kernels ``decode_shared`` and ``prompt_shared`` take for what `count` groups share and for the sequences' own
-        keys, as in ``prompt_kernel``; "each" for both: so little is read that each sequence is worked on by itself, as in
-        "rows".  bfvgpu_kv_shared_kernel."""
+        keys, as in ``prompt_kernel``; "each" or "each tiles" for both: sharing would spare so little that each sequence is worked
+        on by itself, as in "rows" or "tiles".  bfvgpu_kv_shared_kernel."""
         kernels = [lib().bfvgpu_kv_shared_kernel(ctypes.byref(self._desc), q.stride(0), q.stride(1), q.shape[1], q.shape[0],
                                                  table.shape[0], table.shape[1], count, own) for own in (0, 1)]
         if min(kernels) < 0:
             raise ValueError(lib().bfvgpu_last_error().decode())
-        return tuple(("rows", "tiles", "each")[k] for k in kernels)
+        return tuple(("rows", "tiles", "each", "each tiles")[k] for k in kernels)
 
 
 class PageBook:

@@ -160,6 +160,18 @@ SharedQuery shared_query(const Query& q, const int32_t* groups, const int32_t* s
 constexpr double kEachProducts = 17e6;
 bool takes_each(const View& kv, const Batch& bt, const Query& q) { return few_products(kv, bt, q, kEachProducts); }
 
+// Prompts on the tensor cores, each sequence by itself: where the key tiles that sharing spares take less than its parts, its
+// join and its starts, 13 us.  Tile steps of a processor, 2 us each of 256 rows and 1.3 of up to 128.  16 questions of up to
+// 64 tokens on 1000, 2000 and 4096 shared ones: 21, 33 and 57 us by themselves, 34, 34 and 43 together; of up to 300 on 1000
+// 44 and 77; six chunks of up to 1024 with 64 shared 33 and 67.
+bool takes_each_tiles(const View& kv, const Batch& bt, const SharedQuery& q, const SharedPlan& p, int sms) {
+  if (!p.tiles[1]) return false;
+  const double keys = (double)((int64_t)bt.width << kv.page_log) / 128, rows = (double)q.tokens * q.group;
+  auto steps = [&](double elements) { return elements * std::ceil(rows / elements / 256) * kv.heads * keys / sms; };
+  const double single = rows <= 128.0 * bt.seqs ? 1.3 : 2.0;
+  return single * steps(bt.seqs) <= 2.0 * steps(q.count) + 13;
+}
+
 void check_groups(const Call& c, uint64_t count) { need(count <= (uint64_t)c.batch.seqs, BFVGPU_E_SHAPE, "E_KV_GROUPS"); }
 
 void attend_shared(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void* q, const int32_t* starts, const int32_t* table,
@@ -194,6 +206,18 @@ void attend_shared(bfvgpu_ctx* ctx, const bfvgpu_kv* cache, Call& c, const void*
     return;
   }
   const SharedPlan sp = plan_shared(c.view, c.batch, sq, sm_count(at.device), prompt_strides(sq));
+  if (takes_each_tiles(c.view, c.batch, sq, sp, sm_count(at.device))) {
+    const PromptSplit each = plan_prompt(c.view, c.batch, sq, sm_count(at.device));
+    need(each.scratch_floats() == 0 || scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
+    need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
+    need(each.units * each.parts <= (int64_t)kMost, BFVGPU_E_SHAPE, "E_KV_SHAPE");
+    EachQuery eq;
+    static_cast<SharedQuery&>(eq) = sq;
+    cuda_need(launch_prompt(c.view, c.batch, eq, cache->dtype, each, reinterpret_cast<float*>(scratch), at.stream, &launches),
+              "kv shared attention");
+    internal_count_launch(launches);
+    return;
+  }
   need(scratch, BFVGPU_E_ARGUMENT, "E_KV_SCRATCH");
   need(aligned16(scratch), BFVGPU_E_ARGUMENT, "E_KV_ALIGNMENT");
   // (rows of slots are numbered in 32 bits)
@@ -275,8 +299,13 @@ extern "C" uint64_t bfvgpu_kv_shared_scratch_words(const bfvgpu_ctx* ctx, const 
       }
       return;
     }
-    for (const bool tiles : {false, true})
-      words = std::max(words, (plan_shared(c.view, c.batch, q, sm_count(device), tiles).scratch_floats() + 1) / 2);
+    const int sms = sm_count(device);
+    for (const bool tiles : {false, true}) {
+      const SharedPlan p = plan_shared(c.view, c.batch, q, sms, tiles);
+      const uint64_t floats = takes_each_tiles(c.view, c.batch, q, p, sms) ? plan_prompt(c.view, c.batch, q, sms).scratch_floats()
+                                                                           : p.scratch_floats();
+      words = std::max(words, (floats + 1) / 2);
+    }
   });
   return words;
 }
@@ -289,7 +318,9 @@ extern "C" int32_t bfvgpu_kv_shared_kernel(const bfvgpu_kv* cache, int64_t token
     check_groups(c, groups);
     const SharedQuery q = shared_query(c.query, nullptr, nullptr, groups);
     const SharedPlan p = plan_shared(c.view, c.batch, q, sm_count(-1), prompt_strides(q));
-    kernel = takes_each(c.view, c.batch, q) ? BFVGPU_KV_EACH : p.tiles[own != 0] ? BFVGPU_KV_TILES : BFVGPU_KV_ROWS;
+    kernel = takes_each(c.view, c.batch, q)                           ? BFVGPU_KV_EACH
+             : takes_each_tiles(c.view, c.batch, q, p, sm_count(-1)) ? BFVGPU_KV_EACH_TILES
+             : p.tiles[own != 0] ? BFVGPU_KV_TILES : BFVGPU_KV_ROWS;
   });
   return kernel;
 }

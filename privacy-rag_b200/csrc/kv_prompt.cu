@@ -146,6 +146,11 @@ struct Maps {
   CUtensorMap v_rows;    // eight tokens x 64 dims
   CUtensorMap v_row;     // one
 };
+// Of sequences whose first keys lie in another's pages: a page that holds the last of those and the first of their own is
+// loaded in rows from both.
+struct EachMaps : Maps {
+  CUtensorMap k_rows, k_row;  // as v_rows and v_row
+};
 
 // ---- tcgen05, mbarrier and TMA ------------------------------------------------------------------
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
@@ -308,6 +313,11 @@ __device__ __forceinline__ Plan make_plan(const Unit& un) {
 }
 template <class Q>
 constexpr bool kSharing = std::is_same_v<Q, SharedQuery>;
+// Each sequence by itself, its shared keys through the table's row of its group's first.
+template <class Q>
+constexpr bool kRedirected = std::is_same_v<Q, EachQuery>;
+template <class Q>
+using MapsOf = std::conditional_t<kRedirected<Q>, EachMaps, Maps>;
 struct NoSlots {};
 template <class Q>
 using SlotsOf = std::conditional_t<kSharing<Q>, Slots, NoSlots>;
@@ -360,7 +370,7 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* w, bool whole,
 // cut into one equal run for each block (Runs; there is no launch control then), and all results are partial ones.
 template <class T, int DP, class Q = Query>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_kv_prompt(const __grid_constant__ Maps maps, View kv, Batch bt, Q q, int64_t units, int32_t most_parts,
+    k_kv_prompt(const __grid_constant__ MapsOf<Q> maps, View kv, Batch bt, Q q, int64_t units, int32_t most_parts,
                 float* scratch, uint32_t q_tokens, bool ranked, SlotsOf<Q> slots) {
   using S = Smem<DP>;
   using Item = ItemOf<UnitOf<Q>>;
@@ -397,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kLoadWarp && lane < sizeof(Maps) / sizeof(CUtensorMap))
+  if (warp == kLoadWarp && lane < sizeof(maps) / sizeof(CUtensorMap))
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.q) + lane * sizeof(CUtensorMap)) : "memory");
   if (warp == kScoreWarp) {
     // not before the kernel ahead has ended: a block of it on this SM might still want tensor memory
@@ -480,6 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           continue;
         }
       } else {
+        if constexpr (kRedirected<Q>)
+          if (block == 0) record_uncovered(bt, q);
         // the blocks with the most keys come first
         const uint32_t from_end = (uint32_t)block / (uint32_t)most_parts, u = (uint32_t)units - 1 - from_end;
         part = (int32_t)((uint32_t)block - from_end * most_parts);
@@ -496,11 +508,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (un.rows > 0 && part < it.parts) {
         tell(it);
         const int32_t* row = bt.table + (int64_t)un.b * bt.width;
+        [[maybe_unused]] Prefix shared;
+        [[maybe_unused]] const int32_t* shared_row = row;
+        if constexpr (kRedirected<Q>) {
+          shared = prefix_of(kv, bt, q, un.b, un.pos0);
+          shared_row = bt.table + (int64_t)shared.row * bt.width;
+        }
         // lane j's box of a key tile; its page is looked up one tile ahead
         auto box_at = [&](int32_t i) { return plan.key0(i) + lane * box; };
         auto seen = [&](int32_t k) { return k < un.sinks || (k < plan.end && k + box > un.begin); };
+        // keys of a box that lie in the shared pages: none, all that are seen, or the first of them
+        auto in_shared = [&](int32_t k) { return k < shared.tokens && min(k + box, plan.end) <= shared.tokens; };
         auto look_up = [&](int32_t i) {
           const int32_t k = box_at(i);
+          if constexpr (kRedirected<Q>)
+            return i < it.end && lane < boxes && seen(k) ? __ldg((in_shared(k) ? shared_row : row) + (k >> kv.page_log)) : kv.pages;
           return i < it.end && lane < boxes && seen(k) ? __ldg(row + (k >> kv.page_log)) : kv.pages;
         };
         int32_t ahead = look_up(it.begin);
@@ -518,16 +540,44 @@ __global__ void __launch_bounds__(kThreads, 1)
               page = kv.pages;
             }
           }
+          [[maybe_unused]] bool both = false;  // the box lies in two pages
+          [[maybe_unused]] int32_t first_page = kv.pages;
+          if constexpr (kRedirected<Q>) {
+            both = lane < boxes && seen(t0) && t0 < shared.tokens && !in_shared(t0);
+            if (both) {
+              first_page = __ldg(shared_row + (t0 >> kv.page_log));
+              if ((uint32_t)first_page >= (uint32_t)kv.pages) {
+                flag_error(bt.err, kErrTable);
+                first_page = kv.pages;
+              }
+              whole = false;
+            }
+          }
           const int32_t at = t0 & (page_tokens - 1);
           const uint32_t kb = base + S::kK + st * S::kTileBytes, vb = base + S::kV + st * S::kTileBytes;
           ok = __all_sync(0xffffffffu, bar_wait(k_empty + 8 * st, parity, abort, bt.err));
           if (!ok) break;
           if (lane == 0) bar_expect(k_full + 8 * st, S::kTileBytes);
           __syncwarp();
-          if (lane < boxes)
+          if (lane < boxes && !both)
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h)
               tma_box(kb + h * S::kHalfBytes + lane * box * 128, &maps.k, h * 64, at, un.g, page, k_full + 8 * st);
+          if constexpr (kRedirected<Q>) {
+            for (uint32_t left = __ballot_sync(0xffffffffu, both); left; left &= left - 1) {
+              const int j = __ffs(left) - 1;
+              const int32_t pj = __shfl_sync(0xffffffffu, page, j), fj = __shfl_sync(0xffffffffu, first_page, j);
+              const int32_t edge = shared.tokens - __shfl_sync(0xffffffffu, t0, j), aj = __shfl_sync(0xffffffffu, at, j);
+              auto k_box = [&](const CUtensorMap* map, int32_t r) {
+#pragma unroll
+                for (int h = 0; h < S::kHalves; ++h)
+                  tma_box(kb + h * S::kHalfBytes + (j * box + r) * 128, map, h * 64, aj + r, un.g, r < edge ? fj : pj, k_full + 8 * st);
+              };
+              const int32_t r8 = lane * 8, edge8 = edge & ~7;
+              if (r8 < box && (r8 != edge8 || edge == edge8)) k_box(&maps.k_rows, r8);
+              if (edge != edge8 && lane < 8) k_box(&maps.k_row, edge8 + lane);
+            }
+          }
           k_issued = turn + 1;
           if constexpr (!kSharing<Q>)
             if (i + 1 == it.end) ask();
@@ -544,18 +594,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int j = __ffs(left) - 1;
             const int32_t pj = __shfl_sync(0xffffffffu, page, j), tj = __shfl_sync(0xffffffffu, t0, j);
             const int32_t aj = __shfl_sync(0xffffffffu, at, j);
+            // rows before `edge` lie in the first page
+            [[maybe_unused]] int32_t edge = 0, fj = pj;
+            if constexpr (kRedirected<Q>) {
+              fj = __shfl_sync(0xffffffffu, first_page, j);
+              if (__shfl_sync(0xffffffffu, both, j)) edge = shared.tokens - tj;
+            }
             auto v_box = [&](const CUtensorMap* map, int32_t r, bool in) {
+              int32_t of = pj;
+              if constexpr (kRedirected<Q>) of = r < edge ? fj : pj;
 #pragma unroll
               for (int h = 0; h < S::kHalves; ++h)
-                tma_box(vb + h * S::kHalfBytes + (j * box + r) * 128, map, h * 64, aj + r, un.g, in ? pj : kv.pages,
+                tma_box(vb + h * S::kHalfBytes + (j * box + r) * 128, map, h * 64, aj + r, un.g, in ? of : kv.pages,
                         v_full + 8 * st);
             };
             auto row_seen = [&](int32_t k) { return k < un.sinks || (k >= un.begin && k < plan.end); };
             const int32_t r8 = lane * 8, k8 = tj + r8;
             const bool some = r8 < box && (k8 < un.sinks || (k8 < plan.end && k8 + 8 > un.begin));
             const bool all = r8 < box && (k8 + 8 <= un.sinks || (k8 >= un.begin && k8 + 8 <= plan.end));
-            if (r8 < box && some == all) v_box(&maps.v_rows, r8, all);
-            for (uint32_t mixed = __ballot_sync(0xffffffffu, some != all); mixed; mixed &= mixed - 1) {
+            const bool cut = kRedirected<Q> && r8 < edge && edge < r8 + 8;  // in two pages
+            if (r8 < box && some == all && !cut) v_box(&maps.v_rows, r8, all);
+            for (uint32_t mixed = __ballot_sync(0xffffffffu, some != all || cut); mixed; mixed &= mixed - 1) {
               const int32_t r = (__ffs(mixed) - 1) * 8 + lane;
               if (lane < 8) v_box(&maps.v_row, r, row_seen(tj + r));
             }
@@ -1050,7 +1109,7 @@ bool encode(CUtensorMap* map, const View& kv, int dtype, uint16_t* pages, uint32
 
 // The kernel's shared memory, which is an attribute of the function on a device, and the maps of its loads.
 template <class T, int DP, class Q>
-cudaError_t prepare(const View& kv, const Q& q, int dtype, Maps* maps, uint32_t* q_tokens) {
+cudaError_t prepare(const View& kv, const Q& q, int dtype, MapsOf<Q>* maps, uint32_t* q_tokens) {
   static std::atomic<uint64_t> allowed{0};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -1069,23 +1128,25 @@ cudaError_t prepare(const View& kv, const Q& q, int dtype, Maps* maps, uint32_t*
   if (!encode(&maps->k, kv, dtype, kv.k, box) || !encode(&maps->v, kv, dtype, kv.v, box) ||
       !encode(&maps->v_rows, kv, dtype, kv.v, 8) || !encode(&maps->v_row, kv, dtype, kv.v, 1))
     return cudaErrorInvalidValue;
+  if constexpr (kRedirected<Q>)
+    if (!encode(&maps->k_rows, kv, dtype, kv.k, 8) || !encode(&maps->k_row, kv, dtype, kv.k, 1)) return cudaErrorInvalidValue;
   return cudaSuccess;
 }
 
-template <class T, int DP>
-cudaError_t launch(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& sp, float* scratch,
+template <class T, int DP, class Q>
+cudaError_t launch(const View& kv, const Batch& bt, const Q& q, int dtype, const PromptSplit& sp, float* scratch,
                    cudaStream_t st, int* launches) {
-  Maps maps;
+  MapsOf<Q> maps;
   uint32_t q_tokens;
   cudaError_t e = prepare<T, DP>(kv, q, dtype, &maps, &q_tokens);
   if (e != cudaSuccess) return e;
-  e = launch_next(k_kv_prompt<T, DP>, dim3((unsigned)(sp.units * sp.parts)), kThreads, Smem<DP>::kLaunch, st, 1, maps, kv, bt, q,
+  e = launch_next(k_kv_prompt<T, DP, Q>, dim3((unsigned)(sp.units * sp.parts)), kThreads, Smem<DP>::kLaunch, st, 1, maps, kv, bt, q,
                   sp.units, sp.parts, scratch, q_tokens, sp.ranked, NoSlots{});
   if (e != cudaSuccess) return e;
   *launches += 1;
   if (sp.parts > 1) {
-    e = launch_next(k_kv_prompt_join<T, DP>, dim3((unsigned)sp.units, kBlockRows / kJoinRows), kJoinThreads, 0, st, 1, kv, bt, q,
-                    sp.parts, scratch);
+    e = launch_next(k_kv_prompt_join<T, DP>, dim3((unsigned)sp.units, kBlockRows / kJoinRows), kJoinThreads, 0, st, 1, kv, bt,
+                    static_cast<const Query&>(q), sp.parts, scratch);
     if (e != cudaSuccess) return e;
     *launches += 1;
   }
@@ -1134,14 +1195,25 @@ PromptSplit plan_prompt(const View& kv, const Batch& bt, const Query& q, int sms
   return sp;
 }
 
-cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& sp,
-                          float* scratch, cudaStream_t st, int* launches) {
+namespace {
+template <class Q>
+cudaError_t launch_typed(const View& kv, const Batch& bt, const Q& q, int dtype, const PromptSplit& sp, float* scratch,
+                         cudaStream_t st, int* launches) {
   const bool small = sp.dim_padded == 64;
   if (dtype == 0)
     return small ? launch<Bf16, 64>(kv, bt, q, dtype, sp, scratch, st, launches)
                  : launch<Bf16, 128>(kv, bt, q, dtype, sp, scratch, st, launches);
   return small ? launch<Fp16, 64>(kv, bt, q, dtype, sp, scratch, st, launches)
                : launch<Fp16, 128>(kv, bt, q, dtype, sp, scratch, st, launches);
+}
+}  // namespace
+cudaError_t launch_prompt(const View& kv, const Batch& bt, const Query& q, int dtype, const PromptSplit& sp,
+                          float* scratch, cudaStream_t st, int* launches) {
+  return launch_typed(kv, bt, q, dtype, sp, scratch, st, launches);
+}
+cudaError_t launch_prompt(const View& kv, const Batch& bt, const EachQuery& q, int dtype, const PromptSplit& sp,
+                          float* scratch, cudaStream_t st, int* launches) {
+  return launch_typed(kv, bt, q, dtype, sp, scratch, st, launches);
 }
 
 static_assert(kBlockRows == kSharedTileRows && kTileKeys == 128, "the units and key tiles of Runs");

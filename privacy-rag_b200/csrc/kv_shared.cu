@@ -9,8 +9,8 @@
 // each warp takes an equal run of them, finds its first unit by a scan over the groups and sequences, and leaves m, l and o
 // of the units that it had a part of in slots of its own; a second kernel joins them in order, so that results do not
 // depend on timing.  Groups of many rows go to the tensor-core kernel (kv_prompt.cu), whose blocks cut their key tiles in
-// the same way; own keys of single tokens run here beside it.  Where there is little to read, the kernel of single tokens
-// (kv_rows.cu) takes each sequence by itself.
+// the same way; own keys of single tokens run here beside it.  Where sharing would spare less than its
+// parts and its join take, the kernels of single tokens and of prompts take each sequence by itself (kv_attention.cu).
 //
 // Bound by latency where there is little (16 answers on 992 tokens: first keys 4 us after the start, the longest run 8, the
 // join 2.5 behind it), by what arrives from L2 and HBM where there is much: a unit's keys come once for 16 rows, 150 MB in

@@ -16,6 +16,9 @@ struct SharedQuery : Query {
   int32_t count = 0;
 };
 
+// The same where each sequence is worked on by itself, its shared keys read through the row of its group's first.
+struct EachQuery : SharedQuery {};
+
 struct Element {
   int32_t row = 0;                // of the table
   int32_t first = 0, tokens = 0;  // the tokens whose rows see the keys

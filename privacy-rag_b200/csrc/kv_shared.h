@@ -21,7 +21,9 @@ struct SharedPlan {
 SharedPlan plan_shared(const View& kv, const Batch& bt, const SharedQuery& q, int sms, bool tiles);
 cudaError_t launch_shared(const View& kv, const Batch& bt, const SharedQuery& q, int dtype, const SharedPlan& plan, float* scratch,
                           cudaStream_t st, int* launches);
-// Each sequence for itself (kv_rows.cu).
+// Each sequence by itself (kv_rows.cu, kv_prompt.cu).
+cudaError_t launch_prompt(const View& kv, const Batch& bt, const EachQuery& q, int dtype, const PromptSplit& split, float* scratch,
+                          cudaStream_t st, int* launches);
 cudaError_t launch_rows(const View& kv, const Batch& bt, const SharedQuery& q, int dtype, const RowSplit& split, float* scratch,
                         cudaStream_t st, int* launches);
 // The tensor-core kernel's part (kv_prompt.cu).

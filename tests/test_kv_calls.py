@@ -146,7 +146,7 @@ def test_the_scratch_of_shared_attention_holds_what_either_kernel_leaves(bfv):
     from bfvgpu._lib import KvDesc
     L = bfv.lib()
     host = bfv.Context(4096, bfv.find_primes(4096, [36, 36, 37]), 2, 1, 65537, device=-1)
-    for heads, group, dim, tokens, seqs, count in ((4, 8, 128, 128, 128, 1), (1, 2, 64, 300, 2, 2), (8, 2, 72, 4000, 16, 3)):
+    for heads, group, dim, tokens, seqs, count in ((4, 8, 128, 128, 128, 1), (1, 2, 64, 1800, 60, 2), (8, 2, 72, 520, 16, 1)):
         cache = KvDesc(0x10000, 0x20000, 0, 1, 4, heads, 16, dim, 0, heads * 16 * dim, 16 * dim, dim)
         words = L.bfvgpu_kv_shared_scratch_words(host.handle, ctypes.byref(cache), heads * group, tokens, seqs, 4000, count)
         kernels = [L.bfvgpu_kv_shared_kernel(ctypes.byref(cache), heads * group * dim, dim, heads * group, tokens, seqs, 4000, count,
